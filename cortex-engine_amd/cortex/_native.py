@@ -141,6 +141,16 @@ _SIGNATURES = {
     "cortex_linear_residual_ln_splitk": (
         _int, [_i64, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr, _f32,
                _ptr, _i64, _i64, _ptr, _i64, _ptr]),
+    "cortex_kv_append": (
+        _int, [_ptr, _i64, _i64, _int, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr,
+               _ptr]),
+    "cortex_paged_attention_workspace_bytes": (_i64, [_ptr, _i64, _i64, _i64, _int]),
+    "cortex_paged_attention": (
+        _int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _f32, _int, _ptr, _i64, _i64, _ptr, _i64,
+               _ptr, _ptr]),
+    "cortex_kv_evict_plan": (
+        _int, [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr]),
+    "cortex_kv_evict_apply": (_int, [_ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _ptr, _ptr]),
     "cortex_page_table_create": (_int, [_i64, _ptr]),
     "cortex_page_table_destroy": (_int, [_ptr]),
     "cortex_page_table_write": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr]),
@@ -153,6 +163,15 @@ _SIGNATURES = {
 }
 
 EXPORTED = tuple(_SIGNATURES)
+
+
+class KvPagesStruct(ctypes.Structure):
+    """``cortex_kv_pages`` of include/cortex_hip.h."""
+
+    _fields_ = [(n, _i64) for n in ("num_pages", "kv_heads", "page_size", "head_dim", "dtype", "k_page", "k_head",
+                                    "k_slot", "v_page", "v_head", "v_slot")] + \
+               [(n, _ptr) for n in ("k", "v", "k_scale", "v_scale", "weight", "position")]
+
 
 _lib: ctypes.CDLL | None = None
 _fns: dict = {}  # entry points already looked up

@@ -501,7 +501,85 @@ int cortex_linear_residual_ln_splitk(int64_t M, int64_t N, int64_t K, const void
                                      const float* gamma, const float* beta, float eps, void* xn, int64_t ld_xn,
                                      int64_t splits, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
-/* Host page table of that cache (no device work; not thread-safe, one caller per
+/* ---- paged K/V cache: append, attention of one new token, eviction -------------
+ * No reference counterpart: StreamingKVCache (cortex/cache/streaming.py:79-236) pages embedding
+ * rows by (session, bin) and attends to none of them; these operators keep the keys and values
+ * of a sequence in pages and attend to them there.
+ *
+ * Slot j of sequence b is row j % page_size of page block_table[b * ld_table + j / page_size],
+ * j < max_pages * page_size.  A page holds page_size rows for each key/value head; element
+ * (page, head, row, d) of k is at page * k_page + head * k_head + row * k_slot + d (element
+ * strides; d contiguous), v likewise.  dtype 0 f32, 1 bf16, or 3 int8 with a scale per row
+ * (k_scale, v_scale; the row is code * scale).  weight (the softmax weight that a key received
+ * so far) and position (where in its sequence the token stood) are optional.  The four per-row
+ * arrays are contiguous (num_pages, kv_heads, page_size).
+ * page_size a power of two from 8 to 65536; head_dim a multiple of 16 up to 128; rows 16-byte
+ * aligned.  A page id outside [0, num_pages), a length outside [0, max_pages * page_size] or a
+ * slot without a page never reads or writes out of bounds: its rows are taken as absent and bit
+ * 2 (value 4) is OR-ed into *err (when given). */
+typedef struct cortex_kv_pages {
+  int64_t num_pages, kv_heads, page_size, head_dim, dtype;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  float* weight;
+  int32_t* position;
+} cortex_kv_pages;
+
+/* The rows of n_tokens new tokens into the pages of B sequences.  k, v (n_tokens, kv_heads, head_dim)
+ * f32 or bf16 (x_dtype), element (t, h, d) at t * st + h * sh + d, rows 16-byte aligned.
+ * Token t belongs to sequence b, offsets[b] <= t < offsets[b + 1] (CSR, B + 1 values; tokens outside
+ * [offsets[0], offsets[B]) are skipped), or to sequence t when offsets is NULL (n_tokens == B), and goes to
+ * slot lengths[b] + (t - offsets[b]).  Float pages take the value rounded to nearest even; int8
+ * pages s = max(max|x|, 1e-8) / 127 and clamp(rint(x / s), -127, 127), as cortex_quantize_int8
+ * does (a row with an infinity or a NaN gets a scale that makes all of it NaN).  The slot's
+ * weight becomes 0 and its position positions[t] (the slot number when NULL), where the pages have
+ * these.  new_lengths[b] (may be lengths itself) = lengths[b] + the tokens of b that have a slot. */
+int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t n_tokens, int x_dtype, const void* k,
+                     int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                     const int32_t* block_table, int64_t ld_table, int64_t max_pages, const int64_t* offsets,
+                     const int64_t* lengths, const int64_t* positions, int64_t* new_lengths, int32_t* err,
+                     hipStream_t stream);
+
+/* One query per sequence against its cached keys: q and out (B, heads, head_dim) in the pages'
+ * dtype (bf16 for int8 pages), element (b, h, d) at b * sb + h * sh + d; query head h reads key head
+ * h / (heads / kv_heads):
+ *   p[b,h,j] = softmax_{j < lengths[b]}(scale * q[b,h] . k_j),  out[b,h] = sum_j p[b,h,j] v_j
+ * A sequence without keys gives 0.  accumulate != 0: weight of slot j += sum over the query heads
+ * of its key head of p (no two sequences of the call may then share a page).  Lengths up to
+ * max_length (negative: max_pages * page_size) are expected; a longer one is cut to it, as a
+ * malformed length.  out may not overlap q.  B up to 4096.  workspace: cortex_paged_attention_workspace_bytes(...) bytes (0: none is
+ * needed), 16-byte aligned, written before it is read. */
+int64_t cortex_paged_attention_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t heads,
+                                               int64_t max_length, int accumulate);
+int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb,
+                           int64_t q_sh, const int32_t* block_table, int64_t ld_table, int64_t max_pages,
+                           const int64_t* lengths, int64_t max_length, float scale, int accumulate, void* out,
+                           int64_t o_sb, int64_t o_sh, void* workspace, int64_t workspace_bytes, int32_t* err,
+                           hipStream_t stream);
+
+/* Which slots a sequence over its budget keeps, per key/value head: with n = lengths[b] > budget,
+ * first the slots whose position is above (the largest position) - recent, all of them alike, then by
+ * weight, largest first (a NaN before every number), equal ones by the lower slot; the first `budget`
+ * are kept.  recent <= budget.
+ * The kept slots at or past `budget` (src, ascending) fill the slots below it that are not kept
+ * (dst, ascending): row i of dst and src (B, kv_heads, cap) int32, -1 from counts[b, h] on; cap =
+ * max(0, min(budget, max_length - budget)), max_length (negative: max_pages * page_size) as above.
+ * new_lengths[b] = min(n, budget) (not lengths itself).  The pages need weight and position;
+ * nothing of them is written. */
+int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
+                         int64_t max_pages, const int64_t* lengths, int64_t max_length, int64_t budget,
+                         int64_t recent, int32_t* dst, int32_t* src, int32_t* counts, int64_t* new_lengths,
+                         int32_t* err, hipStream_t stream);
+/* Moves slot src to slot dst for every entry of a plan: key and value rows and, where the pages
+ * have them, scales, weight and position.  Entries from counts[b, h] on are not read. */
+int cortex_kv_evict_apply(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
+                          int64_t max_pages, const int32_t* dst, const int32_t* src, int64_t cap,
+                          const int32_t* counts, int32_t* err, hipStream_t stream);
+
+/* Host page table of the event page cache (no device work; not thread-safe, one caller per
  * table).  Replaces the Python bookkeeping of StreamingKVCache with the same policy
  * (cortex/cache/streaming.py:133-233): a lookup of a present key touches its page
  * (most recently used) and counts a hit, an absent key counts a miss; a write reuses
