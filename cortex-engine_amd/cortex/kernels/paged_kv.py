@@ -142,7 +142,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     es = t.element_size()
     s0, s1, s2 = t.stride()
     if s2 != 1 or t.data_ptr() % 16 or (s0 * es) % 16 or (s1 * es) % 16:
-        return t.contiguous()
+        return t.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps rows that only start off)
     return t
 
 

@@ -1,4 +1,23 @@
 // Attention of one new token per sequence over its paged keys and values.
+//
+//   s_j = scale q . k_j   m = max_j s_j   p_j = exp(s_j - m)   l = sum_j p_j   out = sum_j p_j v_j / l
+//
+// Every key and value row is read once, for all query heads of its key head: a streaming kernel, bound by HBM as long
+// as enough bytes are in flight.  The G query heads of a key head are the columns of the matrix products (16 at a time; 16
+// are multiplied also where there are fewer, which the matrix cores have the time for).
+//
+// A wavefront takes tiles of 32 keys.  Both operands come straight from memory into registers, without LDS:
+//   scores  S^T = K Q^T: lane (r, g) = (l % 16, l / 16) loads its part of key row key_of(st, r) = 8 (r / 4) + 4 st + r % 4
+//           for st 0 and 1; the score registers of group g are then the 8 consecutive keys 8 g .. 8 g + 7;
+//   output  O^T += V^T P^T: P^T of those 8 keys is the B operand as it stands.  For V^T lane (r, g) loads the same 8
+//           keys at E = DHP / 16 consecutive dims r E .. r E + E - 1, so a row is read whole by 16 lanes; the transpose is
+//           one byte permute per register, and product j gives the dims {r E + j}.
+// K's registers are free after the scores and V's after the output: the next tile's loads are issued there.
+//
+// Split over the length: all tiles of all (sequence, key head) units are laid end to end and cut into equal shares, one a
+// workgroup, from the lengths on the device (a replayed graph follows them, ragged batches need no plan, and the grid
+// is one workgroup per slot of the card).  A unit cut by a share leaves its running (m, l, sum p v) in the workspace, at
+// most two a workgroup (the end of a unit and the beginning of another), and a second launch joins them in order.
 #include <hip/hip_runtime.h>
 
 #include "paged_kv.h"
@@ -6,19 +25,33 @@
 namespace cortex {
 namespace {
 
+constexpr int PA_KT = 32;       // keys per tile
+constexpr int PA_WAVES = 4;
+constexpr int PA_THREADS = 64 * PA_WAVES;
+constexpr int PA_ROWS = 16;     // query heads of a unit
+constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
+constexpr int PA_PER_CU = 2;    // workgroups
+constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before the sums are rescaled: p <= 2^8
+
 struct PagedArgs {
   KvPages p;
-  int64_t B;
-  int heads, group;  // query heads, and of them to a key head
+  int B, heads, group;  // query heads, and of them to a key head
+  int row_tiles;        // units a key head: ceil(group / PA_ROWS)
+  int units;            // units a sequence: kv_heads * row_tiles
+  int shares;
   const void* q;
   int64_t q_sb, q_sh;
   const int64_t* lengths;
   int64_t max_length;
   float scale_log2;
-  int accumulate;
   void* out;
   int64_t o_sb, o_sh;
   int32_t* err;
+  // workspace
+  float* part;    // (2 shares, PA_ROWS, DHP + 2): sum p v, then m and l
+  float* score;   // (B, heads, score_ld), for accumulate
+  float* stats;   // (B, heads, 2): m and 1 / l, for accumulate
+  int64_t score_ld;
 };
 
 template <class P>
@@ -30,81 +63,475 @@ struct Query<int8_t> {
   typedef bf16 type;
 };
 
-// One workgroup a (sequence, key head): its query heads one after the other, 256 keys at a time.
-template <class P>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const void* p) {
+  Words<N> r;
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(r.w + i) = reinterpret_cast<const uint4*>(p)[i / 4];
+  } else if constexpr (N == 2) {
+    *reinterpret_cast<uint2*>(r.w) = *reinterpret_cast<const uint2*>(p);
+  } else {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+  return r;
+}
+
+// max / sum over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48), in every lane
+__device__ __forceinline__ float group_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float group_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, int b) {
+  bool ok;
+  return (int)((a.p.length_of(a.lengths, b, a.max_length, &ok) + PA_KT - 1) / PA_KT);
+}
+
+__device__ __forceinline__ int wave_scan_int(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ int wave_sum_int(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Tiles of a share, from all tiles; every wavefront computes it for itself.
+__device__ __forceinline__ int share_of(const PagedArgs& a, int total) {
+  return max(PA_MIN_TILES, (total + a.shares - 1) / a.shares);
+}
+
+template <class P, int DHP, bool PAD, bool W>
+__global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(PagedArgs a) {
   typedef typename Query<P>::type Q;
-  __shared__ float q[128], prob[256], red[4], stats[2][1024];
+  constexpr int ES = sizeof(P);
+  constexpr int CE = 16 / ES;           // elements of a 16-byte chunk
+  constexpr int NK = DHP / (4 * CE);    // chunks of a key row a lane: d = 4 CE c + CE g
+  constexpr int E = DHP / 16;           // dims of a value row a lane: d = E r
+  constexpr int VW = E * ES / 4;
+  constexpr int LD = DHP + 4;
+  __shared__ __attribute__((aligned(16))) float so[PA_WAVES][PA_ROWS][LD];
+  __shared__ float sm[PA_WAVES][PA_ROWS], sl[PA_WAVES][PA_ROWS];
   const KvPages& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int64_t b = blockIdx.x / p.kv_heads;
-  const int h = blockIdx.x - (int)b * p.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, wid = wave_uniform(tid >> 6);
+  const int fr = lane & 15, g = lane >> 4;
+  const int Dh = PAD ? p.head_dim : DHP;
+
+  // this workgroup's share of the tiles
+  int total = 0;
   bool ok = true;
-  const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
-  if (!ok && tid == 0) kv_flag(a.err);
-  const P* k = reinterpret_cast<const P*>(p.k) + h * p.k_head;
-  const P* v = reinterpret_cast<const P*>(p.v) + h * p.v_head;
-  auto score = [&](int64_t j) {
-    const int page = p.page_of(b, j);
-    if (page < 0) {
-      kv_flag(a.err);
-      return -INFINITY;
+  for (int b = lane; b < a.B; b += 64) {
+    total += (int)((p.length_of(a.lengths, b, a.max_length, &ok) + PA_KT - 1) / PA_KT);
+  }
+  if (blockIdx.x == 0 && !ok) kv_flag(a.err);
+  total = wave_sum_int(total) * a.units;
+  const int per = share_of(a, total);
+  int t0 = blockIdx.x * per;
+  const int t1 = min(total, t0 + per);
+  if (t0 >= t1) return;
+  int b = 0, off = t0;  // its first sequence, and the tile of that sequence's units
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int v = b0 + lane < a.B ? tiles_of(a, b0 + lane) * a.units : 0;
+    const int inc = wave_scan_int(v, lane);
+    const uint64_t past = __ballot(inc > off);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      off -= __shfl(inc - v, l, 64);
+      break;
     }
-    const P* row = k + page * p.k_page + p.row_of(j) * p.k_slot;
-    float s = 0.0f;
-    for (int d = 0; d < p.head_dim; ++d) s = fmaf(q[d], to_f32(row[d]), s);
-    if (sizeof(P) == 1) s *= p.k_scale[p.scalar_at(page, h, p.row_of(j))];
-    return s * a.scale_log2;
-  };
-  auto load_q = [&](int g) {
-    __syncthreads();
-    if (tid < p.head_dim) q[tid] = to_f32(reinterpret_cast<const Q*>(a.q)[b * a.q_sb + (h * a.group + g) * a.q_sh + tid]);
-    __syncthreads();
-  };
-  for (int g = 0; g < a.group; ++g) {
-    load_q(g);
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (int64_t j0 = 0; j0 < n; j0 += 256) {
-      const int64_t j = j0 + tid;
-      const float s = j < n ? score(j) : -INFINITY;
-      float t = wave_max(s);
-      if (lane == 0) red[wid] = t;
-      __syncthreads();
-      const float m_new = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-      const float ref = m_new == -INFINITY ? 0.0f : m_new;
-      const float pr = j < n ? exp2f(s - ref) : 0.0f;
-      prob[tid] = pr;
-      t = wave_sum(pr);
-      __syncthreads();
-      if (lane == 0) red[wid] = t;
-      __syncthreads();
-      const float alpha = exp2f(m - ref);
-      l = l * alpha + ((red[0] + red[1]) + (red[2] + red[3]));
-      acc *= alpha;
-      if (tid < p.head_dim)
-        for (int i = 0; i < 256 && j0 + i < n; ++i) {
-          const int page = p.page_of(b, j0 + i);
-          if (page < 0) continue;
-          float x = to_f32(v[page * p.v_page + p.row_of(j0 + i) * p.v_slot + tid]);
-          if (sizeof(P) == 1) x *= p.v_scale[p.scalar_at(page, h, p.row_of(j0 + i))];
-          acc = fmaf(prob[i], x, acc);
+    off -= __shfl(inc, 63, 64);
+  }
+  b = wave_uniform(b);
+  off = wave_uniform(off);
+
+  while (t0 < t1 && b < a.B) {
+    const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
+    const int tiles = (int)((n + PA_KT - 1) / PA_KT);
+    if (off >= tiles * a.units) {  // done, or empty
+      ++b;
+      off = 0;
+      continue;
+    }
+    const int u = off / tiles, ta = off - u * tiles, tb = min(tiles, ta + (t1 - t0));
+    const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * PA_ROWS;
+    const int rows = min(PA_ROWS, a.group - row0);  // query heads of this unit
+    const int head0 = h * a.group + row0;
+
+    // query rows as the B operand of the scores
+    Q q[NK][CE];
+    {
+      const Q* src = reinterpret_cast<const Q*>(a.q) + b * a.q_sb + (head0 + (fr < rows ? fr : 0)) * a.q_sh;
+#pragma unroll
+      for (int c = 0; c < NK; ++c) {
+        const int d = c * 4 * CE + g * CE;
+        const bool in = fr < rows && (!PAD || d < Dh);
+        Words<CE * sizeof(Q) / 4> w = load_words<CE * sizeof(Q) / 4>(src + (!PAD || d < Dh ? d : 0));
+#pragma unroll
+        for (int i = 0; i < (int)(CE * sizeof(Q) / 4); ++i) w.w[i] = in ? w.w[i] : 0u;
+        __builtin_memcpy(q[c], w.w, sizeof(w.w));
+      }
+    }
+
+    const char* kbase = reinterpret_cast<const char*>(p.k) + h * p.k_head * ES;
+    const char* vbase = reinterpret_cast<const char*>(p.v) + h * p.v_head * ES;
+    const int mask = (1 << p.shift) - 1;
+    const int32_t* table = p.table + b * p.ld_table;
+    // the page ids of this lane's 8 keys of a tile: for the key rows (8 (r / 4) ..) and the value rows (8 g ..)
+    auto page_at = [&](int j) { return table[min(j, (int)n - 1) >> p.shift]; };
+    auto kblock = [&](int t) { return t * PA_KT + 8 * (fr >> 2); };
+    auto vblock = [&](int t) { return t * PA_KT + 8 * g; };
+
+    Words<4> kr[2][NK];
+    Words<VW> vr[8];
+    float4 ks[2], vs[2];
+    auto load_k = [&](int t, int page) {
+      const int64_t at = (int64_t)((uint32_t)page < (uint32_t)p.num_pages ? page : 0) * p.k_page;
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const int row = (kblock(t) & mask) + 4 * st + (fr & 3);
+        const char* src = kbase + (at + row * p.k_slot) * ES;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+          const int d = c * 4 * CE + g * CE;
+          kr[st][c] = load_words<4>(src + (!PAD || d < Dh ? d : 0) * ES);
+          if (PAD && d >= Dh) kr[st][c] = Words<4>{{0u, 0u, 0u, 0u}};
         }
-      m = m_new;
-      __syncthreads();
+      }
+    };
+    auto load_v = [&](int t, int page) {
+      const int64_t pg = (uint32_t)page < (uint32_t)p.num_pages ? page : 0;
+      const int row = vblock(t) & mask;
+      const int d = !PAD || fr * E < Dh ? fr * E : 0;
+      const char* src = vbase + (pg * p.v_page + row * p.v_slot + d) * ES;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vr[i] = load_words<VW>(src + i * p.v_slot * ES);
+    };
+    auto load_scales = [&](int t, int page) {
+      if constexpr (ES == 1) {
+        const int64_t i = p.scalar_at((uint32_t)page < (uint32_t)p.num_pages ? page : 0, h, vblock(t) & mask);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          ks[x] = reinterpret_cast<const float4*>(p.k_scale + i)[x];
+          vs[x] = reinterpret_cast<const float4*>(p.v_scale + i)[x];
+        }
+      }
+    };
+
+    float m = -INFINITY, l = 0.0f;  // of query fr; l: the keys of this lane's group only
+    f32x4 o[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+
+    int t = ta + wid;
+    if (t < tb) {
+      int kp = page_at(kblock(t)), vp = page_at(vblock(t));
+      load_k(t, kp);
+      load_v(t, vp);
+      load_scales(t, vp);
+      int kp1 = page_at(kblock(t + PA_WAVES)), vp1 = page_at(vblock(t + PA_WAVES));
+      for (; t < tb; t += PA_WAVES) {
+        const int kp2 = page_at(kblock(t + 2 * PA_WAVES)), vp2 = page_at(vblock(t + 2 * PA_WAVES));
+        const bool more = t + PA_WAVES < tb;
+        // scores of keys 8 g + 4 st + i for query fr
+        f32x4 s[2];
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          s[st] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < NK; ++c) {
+            if constexpr (ES == 2) {
+              bf16x8 qf;
+              __builtin_memcpy(&qf, q[c], 16);
+              s[st] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[st][c]), qf, s[st], 0, 0, 0);
+            } else if constexpr (ES == 4) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[st] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[st][c].w[e]), q[c][e], s[st], 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                bf16x8 qf;
+                __builtin_memcpy(&qf, q[c] + 8 * e, 16);
+                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    widen_i8x8(make_uint2(kr[st][c].w[2 * e], kr[st][c].w[2 * e + 1])), qf, s[st], 0, 0, 0);
+              }
+            }
+          }
+        }
+        const float4 ks0 = ks[0], ks1 = ks[1];
+        if (more) load_k(t + PA_WAVES, kp1);
+        __builtin_amdgcn_sched_barrier(0);
+
+        // how many of this lane's 8 keys there are
+        const bool page_ok = (uint32_t)vp < (uint32_t)p.num_pages;
+        const int left = page_ok ? (int)n - vblock(t) : 0;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * a.scale_log2;
+        if constexpr (ES == 1) {
+          const float sc[8] = {ks0.x, ks0.y, ks0.z, ks0.w, ks1.x, ks1.y, ks1.z, ks1.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= sc[i];
+        }
+        const bool whole = __all(left >= 8);
+        if (!whole) {
+          if (!page_ok && fr == 0 && vblock(t) < (int)n) kv_flag(a.err);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (i >= left) {  // (what these rows hold is not looked at: 0 times it may be NaN)
+              x[i] = -INFINITY;
+              vr[i] = Words<VW>{};
+              if constexpr (ES == 1) reinterpret_cast<float*>(vs)[i] = 0.0f;
+            }
+          }
+        }
+        if constexpr (W) {
+          if (fr < rows) {
+            float* to = a.score + ((int64_t)b * a.heads + head0 + fr) * a.score_ld + vblock(t);
+            reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+          }
+        }
+        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        top = group_max(top);
+        if (__any(top > m + PA_RESCALE)) {  // (m -inf: the first key)
+          const float m_new = fmaxf(m, top);
+          const float alpha = exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
+          l *= alpha;
+#pragma unroll
+          for (int j = 0; j < E; ++j) o[j] *= alpha;
+          m = m_new;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float pr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+
+        // O^T += V^T P^T; product j: dims E (4 g + i) + j of query fr
+        if constexpr (ES == 4) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+              o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i].w[j]), pr[i], o[j], 0, 0, 0);
+        } else {
+          if constexpr (ES == 1) {
+            const float sc[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pr[i] *= sc[i];
+          }
+          bf16x8 pf;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pf[i] = (bf16)pr[i];
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            bf16x8 vf;
+            if constexpr (ES == 2) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[j >> 1], vr[2 * i].w[j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+              __builtin_memcpy(&vf, w, 16);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[i].w[j >> 2] >> (8 * (j & 3)));
+            }
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[j], 0, 0, 0);
+          }
+        }
+        if (more) {
+          load_v(t + PA_WAVES, vp1);
+          load_scales(t + PA_WAVES, vp1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        vp = vp1;
+        kp1 = kp2;
+        vp1 = vp2;
+      }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (tid < p.head_dim)
-      reinterpret_cast<Q*>(a.out)[b * a.o_sb + (h * a.group + g) * a.o_sh + tid] = from_f32<Q>(acc * inv);
-    if (tid == 0) stats[0][g] = m == -INFINITY ? 0.0f : m, stats[1][g] = inv;
+
+    // the wavefronts' sums into one
+    l = group_sum(l);
+    const int active = min(PA_WAVES, tb - ta);
+    if (wid < active && fr < rows) {
+      if (g == 0) sm[wid][fr] = m, sl[wid][fr] = l;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < E; j += 4)
+          *reinterpret_cast<float4*>(&so[wid][fr][E * (4 * g + i) + j]) = make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
+    }
+    __syncthreads();
+    const bool complete = ta == 0 && tb == tiles;
+    float* part = a.part + (2 * (int64_t)blockIdx.x + (ta == 0)) * (PA_ROWS * (DHP + 2));
+    for (int i = tid; i < rows * DHP; i += PA_THREADS) {
+      const int r = i / DHP, d = i - r * DHP;
+      float top = sm[0][r];
+      for (int w = 1; w < active; ++w) top = fmaxf(top, sm[w][r]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, acc = 0.0f;
+      for (int w = 0; w < active; ++w) {
+        const float f = exp2f(sm[w][r] - ref);
+        sum += f * sl[w][r];
+        acc += f * so[w][r][d];
+      }
+      if (complete) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (d < Dh) reinterpret_cast<Q*>(a.out)[b * a.o_sb + (head0 + r) * a.o_sh + d] = from_f32<Q>(acc * inv);
+        if (W && d == 0) {
+          float* st = a.stats + ((int64_t)b * a.heads + head0 + r) * 2;
+          st[0] = ref, st[1] = inv;
+        }
+      } else {
+        part[r * DHP + d] = acc;
+        if (d == 0) part[PA_ROWS * DHP + r] = top, part[PA_ROWS * (DHP + 1) + r] = sum;
+      }
+    }
+    t0 += tb - ta;
+    off += tb - ta;
+    __syncthreads();
   }
-  if (!a.accumulate) return;
-  for (int g = 0; g < a.group; ++g) {
-    load_q(g);
-    for (int64_t j = tid; j < n; j += 256) {
-      const int page = p.page_of(b, j);
-      if (page >= 0) p.weight[p.scalar_at(page, h, p.row_of(j))] += exp2f(score(j) - stats[0][g]) * stats[1][g];
+}
+
+// One workgroup a unit: the parts of a unit that several shares hold, in the order of its keys; 0 for a sequence
+// without keys.
+template <class Q, int DHP, bool W>
+__global__ __launch_bounds__(128) void paged_join_kernel(PagedArgs a) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int b = blockIdx.x / a.units, u = blockIdx.x - b * a.units;
+  const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * PA_ROWS;
+  const int rows = min(PA_ROWS, a.group - row0), head0 = h * a.group + row0;
+  int total = 0, before = 0;
+  for (int i = lane; i < a.B; i += 64) {
+    const int n = tiles_of(a, i);
+    total += n;
+    before += i < b ? n : 0;
+  }
+  total = wave_sum_int(total) * a.units;
+  before = wave_sum_int(before) * a.units;
+  const int tiles = tiles_of(a, b);
+  const int per = share_of(a, total), s = before + u * tiles;
+  const int w0 = tiles ? s / per : 0, w1 = tiles ? (s + tiles - 1) / per : 0;
+  if (tiles && w0 == w1) return;  // written by its one workgroup
+  const float* part = a.part;
+  constexpr int64_t SLOT = PA_ROWS * (DHP + 2);
+  auto slot = [&](int w) { return part + (2 * (int64_t)w + (w == w0)) * SLOT; };
+  for (int i = tid; i < rows * DHP; i += 128) {
+    const int r = i / DHP, d = i - r * DHP;
+    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+    if (tiles) {
+      for (int w = w0; w <= w1; ++w) top = fmaxf(top, slot(w)[PA_ROWS * DHP + r]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      for (int w = w0; w <= w1; ++w) {
+        const float* x = slot(w);
+        const float f = exp2f(x[PA_ROWS * DHP + r] - ref);
+        sum += f * x[PA_ROWS * (DHP + 1) + r];
+        acc += f * x[r * DHP + d];
+      }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (d < a.p.head_dim) reinterpret_cast<Q*>(a.out)[b * a.o_sb + (head0 + r) * a.o_sh + d] = from_f32<Q>(acc * inv);
+    if (W && d == 0) {
+      float* st = a.stats + ((int64_t)b * a.heads + head0 + r) * 2;
+      st[0] = top == -INFINITY ? 0.0f : top, st[1] = inv;
     }
   }
+}
+
+constexpr int PW_KEYS = 256;
+
+// weight_j += sum over the query heads of a key head of p_j, from the scores and the joined m and 1 / l.
+__global__ __launch_bounds__(PW_KEYS) void paged_weight_kernel(PagedArgs a, int chunks) {
+  const int bh = blockIdx.x / chunks, b = bh / a.p.kv_heads, h = bh - b * a.p.kv_heads;
+  bool ok;
+  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
+  const int64_t j = (int64_t)(blockIdx.x - bh * chunks) * PW_KEYS + threadIdx.x;
+  if (j >= n) return;
+  const int page = a.p.page_of(b, j);
+  if (page < 0) return;
+  const float* score = a.score + ((int64_t)b * a.heads + h * a.group) * a.score_ld + j;
+  const float* st = a.stats + ((int64_t)b * a.heads + h * a.group) * 2;
+  float sum = 0.0f;
+  for (int i = 0; i < a.group; ++i) sum += exp2f(score[i * a.score_ld] - st[2 * i]) * st[2 * i + 1];
+  a.p.weight[a.p.scalar_at(page, h, a.p.row_of(j))] += sum;
+}
+
+// How a call is laid out: shares, and the parts of its workspace in bytes.
+struct Layout {
+  int row_tiles, units, shares, dhp;
+  int64_t score_ld, part, score, stats;
+};
+Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t most, int accumulate) {
+  Layout y;
+  const int64_t group = heads / p->kv_heads;
+  y.row_tiles = (int)cdiv(group, PA_ROWS);
+  y.units = (int)(p->kv_heads * y.row_tiles);
+  y.dhp = p->head_dim <= 64 ? 64 : 128;
+  const int64_t tiles = B * y.units * cdiv(most, PA_KT);
+  const int64_t shares = cdiv(tiles, PA_MIN_TILES), slots = (int64_t)cu_count() * PA_PER_CU;
+  y.shares = (int)(shares < 1 ? 1 : shares < slots ? shares : slots);
+  y.score_ld = cdiv(most, PA_KT) * PA_KT;
+  y.part = 2ll * y.shares * PA_ROWS * (y.dhp + 2) * 4;
+  y.score = accumulate ? B * heads * y.score_ld * 4 : 0;
+  y.stats = accumulate ? cdiv(B * heads * 2 * 4, 16) * 16 : 0;
+  return y;
+}
+
+template <class P, int DHP, bool W>
+int launch(const PagedArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.shares), block(PA_THREADS);
+  if (a.p.head_dim == DHP)
+    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, false, W>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, true, W>), grid, block, 0, stream, a);
+  CORTEX_CHECK_LAUNCH("paged_attention_kernel");
+  hipLaunchKernelGGL((paged_join_kernel<typename Query<P>::type, DHP, W>), dim3((unsigned)(a.B * a.units)), dim3(128), 0,
+                     stream, a);
+  CORTEX_CHECK_LAUNCH("paged_join_kernel");
+  if (W && a.max_length > 0) {
+    const int64_t chunks = cdiv(a.max_length, PW_KEYS);
+    hipLaunchKernelGGL(paged_weight_kernel, dim3((unsigned)(chunks * a.B * a.p.kv_heads)), dim3(PW_KEYS), 0, stream, a,
+                       (int)chunks);
+    CORTEX_CHECK_LAUNCH("paged_weight_kernel");
+  }
+  return OK;
+}
+template <class P>
+int launch_type(const PagedArgs& a, int accumulate, hipStream_t stream) {
+  if (a.p.head_dim <= 64) return accumulate ? launch<P, 64, true>(a, stream) : launch<P, 64, false>(a, stream);
+  return accumulate ? launch<P, 128, true>(a, stream) : launch<P, 128, false>(a, stream);
+}
+
+// The length that a call expects at most: max_length, or the table's width where that is negative.
+int64_t expected_length(int64_t max_length, int64_t max_slots) {
+  return max_length < 0 || max_length > max_slots ? max_slots : max_length;
+}
+
+int check_heads(const char* who, const cortex_kv_pages* pages, int64_t B, int64_t heads, int64_t most) {
+  CORTEX_CHECK_ARG(heads >= 1 && pages->kv_heads >= 1 && heads % pages->kv_heads == 0 && heads <= 65536,
+                   "%s: %lld query heads are not a multiple of %lld key heads (up to 65536)", who, (long long)heads,
+                   (long long)pages->kv_heads);
+  CORTEX_CHECK_ARG(B >= 0 && B <= 4096, "%s: %lld sequences (at most 4096)", who, (long long)B);
+  const int64_t units = pages->kv_heads * cdiv(heads / pages->kv_heads, PA_ROWS);
+  CORTEX_CHECK_ARG(most < 0 || B * units <= 0x3fffffffLL / (cdiv(most, PA_KT) + 1),
+                   "%s: %lld sequences of up to %lld keys are too much for one call", who, (long long)B, (long long)most);
+  return OK;
 }
 
 }  // namespace
@@ -112,14 +539,11 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
 
 using namespace cortex;
 
-static int64_t expected_length(int64_t max_length, int64_t max_slots) {
-  return max_length < 0 || max_length > max_slots ? max_slots : max_length;
-}
-
 extern "C" int64_t cortex_paged_attention_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t heads,
                                                           int64_t max_length, int accumulate) {
-  (void)pages, (void)B, (void)heads, (void)max_length, (void)accumulate;
-  return 0;
+  if (!pages || check_heads("cortex_paged_attention_workspace_bytes", pages, B, heads, max_length) || max_length < 0) return 0;
+  const Layout y = layout_of(pages, B, heads, max_length, accumulate);
+  return y.part + y.score + y.stats;
 }
 
 extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q,
@@ -130,35 +554,41 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   const char* who = "cortex_paged_attention";
   PagedArgs a = {};
   if (int rc = kv_check(who, pages, B, block_table, ld_table, max_pages, &a.p)) return rc;
-  CORTEX_CHECK_ARG(heads >= 1 && heads % pages->kv_heads == 0 && heads / pages->kv_heads <= 1024,
-                   "%s: %lld query heads are not a multiple (up to 1024) of %lld key heads", who, (long long)heads,
-                   (long long)pages->kv_heads);
-  CORTEX_CHECK_ARG(B <= 4096, "%s: %lld sequences (at most 4096)", who, (long long)B);
+  a.max_length = expected_length(max_length, a.p.max_slots);
+  if (int rc = check_heads(who, pages, B, heads, a.max_length)) return rc;
   CORTEX_CHECK_ARG(!accumulate || pages->weight, "%s: accumulate needs pages with weight", who);
   if (B == 0) return OK;
   CORTEX_CHECK_ARG(q && out && lengths, "%s: null q, out or lengths", who);
-  a.B = B;
+  const int64_t es = pages->dtype == DT_F32 ? 4 : 2;
+  CORTEX_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_sb * es) % 16 == 0 && (q_sh * es) % 16 == 0,
+                   "%s: query rows must be 16-byte aligned", who);
+  const Layout y = layout_of(pages, B, heads, a.max_length, accumulate);
+  CORTEX_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
+  if (workspace_bytes < y.part + y.score + y.stats) {
+    set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
+              (long long)(y.part + y.score + y.stats));
+    return E_WORKSPACE;
+  }
+  a.B = (int)B;
   a.heads = (int)heads;
   a.group = (int)(heads / pages->kv_heads);
+  a.row_tiles = y.row_tiles;
+  a.units = y.units;
+  a.shares = y.shares;
   a.q = q;
   a.q_sb = q_sb;
   a.q_sh = q_sh;
   a.lengths = lengths;
-  a.max_length = expected_length(max_length, a.p.max_slots);
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.accumulate = accumulate;
   a.out = out;
   a.o_sb = o_sb;
   a.o_sh = o_sh;
   a.err = err;
-  (void)workspace, (void)workspace_bytes;
-  const dim3 grid((unsigned)(B * pages->kv_heads));
-  if (pages->dtype == DT_F32)
-    hipLaunchKernelGGL(paged_attention_kernel<float>, grid, dim3(256), 0, stream, a);
-  else if (pages->dtype == DT_BF16)
-    hipLaunchKernelGGL(paged_attention_kernel<bf16>, grid, dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL(paged_attention_kernel<int8_t>, grid, dim3(256), 0, stream, a);
-  CORTEX_CHECK_LAUNCH("paged_attention_kernel");
-  return OK;
+  a.score_ld = y.score_ld;
+  a.part = reinterpret_cast<float*>(workspace);
+  a.score = a.part + y.part / 4;
+  a.stats = a.score + y.score / 4;
+  if (pages->dtype == DT_F32) return launch_type<float>(a, accumulate, stream);
+  if (pages->dtype == DT_BF16) return launch_type<bf16>(a, accumulate, stream);
+  return launch_type<int8_t>(a, accumulate, stream);
 }

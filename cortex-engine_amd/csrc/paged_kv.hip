@@ -36,7 +36,7 @@ int kv_check(const char* who, const cortex_kv_pages* p, int64_t B, const int32_t
   CORTEX_CHECK_ARG(p->k_slot >= p->head_dim && p->v_slot >= p->head_dim, "%s: rows of a page overlap", who);
   CORTEX_CHECK_ARG(B == 0 || max_pages == 0 || table, "%s: null block table", who);
   CORTEX_CHECK_ARG(B <= 1 || ld_table >= max_pages, "%s: rows of the block table overlap", who);
-  CORTEX_CHECK_ARG(max_pages <= 0x7fffffffLL / ps, "%s: %lld pages of %lld slots are more than 2^31 - 1 slots", who,
+  CORTEX_CHECK_ARG(max_pages <= (1ll << 30) / ps, "%s: %lld pages of %lld slots are more than 2^30 slots", who,
                    (long long)max_pages, (long long)ps);
   *out = KvPages{p->k,       p->v,       p->k_scale, p->v_scale, p->weight,  p->position, p->k_page,
                  p->k_head,  p->k_slot,  p->v_page,  p->v_head,  p->v_slot,  table,       ld_table,

@@ -63,7 +63,7 @@ def test_pages_that_no_operator_takes(call):
     refused(call(tracked(), width=-1), "negative shape")
     refused(call(tracked(), table=None), "block table")
     refused(call(tracked(), ld=2), "overlap")
-    refused(call(tracked(page_size=65536), width=40000, ld=40000), "2^31")
+    refused(call(tracked(page_size=65536), width=20000, ld=20000), "2^30")
 
 
 def test_refused_appends():
@@ -81,6 +81,11 @@ def test_refused_attention():
     refused(attention(pages(), heads=3), "multiple")
     refused(attention(pages(), heads=0), "multiple")
     refused(attention(pages(), B=4097), "at most 4096")
+    refused(attention(pages(), B=4096, heads=1024, width=1 << 20, ld=1 << 20, most=-1), "too much for one call")
+    refused(attention(pages(), ws=None), "workspace")
+    refused(attention(pages(), ws=8), "workspace")
+    refused(attention(pages(), ws_bytes=64), "needed", rc=-4)
+    refused(attention(pages(), q=8), "16-byte")
     refused(attention(pages(), accumulate=1), "weight")
     refused(attention(pages(), q=None), "null q")
     refused(attention(pages(), lengths=None), "null q")
