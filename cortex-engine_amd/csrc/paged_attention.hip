@@ -26,11 +26,13 @@ namespace cortex {
 namespace {
 
 constexpr int PA_KT = 32;       // keys per tile
-constexpr int PA_WAVES = 4;
-constexpr int PA_THREADS = 64 * PA_WAVES;
+constexpr int PA_WAVES = 4;     // wavefronts of a workgroup that takes a share
+constexpr int PA_MORE = 8;      // and of one that has a CU to itself and takes a whole unit
 constexpr int PA_ROWS = 16;     // query heads of a unit
 constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
 constexpr int PA_PER_CU = 2;    // workgroups
+constexpr int PA_MAX_SHARES = 1024;
+constexpr int PA_ONE_TILES = 32;  // tiles of a unit up to which a workgroup takes the whole of it
 constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before the sums are rescaled: p <= 2^8
 
 struct PagedArgs {
@@ -115,8 +117,9 @@ __device__ __forceinline__ int share_of(const PagedArgs& a, int total) {
   return max(PA_MIN_TILES, (total + a.shares - 1) / a.shares);
 }
 
-template <class P, int DHP, bool PAD, bool W>
-__global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(PagedArgs a) {
+// ONE: a workgroup takes a whole unit, so that nothing is left to join (short caches); else a share.
+template <class P, int DHP, bool PAD, bool W, int WAVES, bool ONE>
+__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(PagedArgs a) {
   typedef typename Query<P>::type Q;
   constexpr int ES = sizeof(P);
   constexpr int CE = 16 / ES;           // elements of a 16-byte chunk
@@ -124,50 +127,56 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
   constexpr int E = DHP / 16;           // dims of a value row a lane: d = E r
   constexpr int VW = E * ES / 4;
   constexpr int LD = DHP + 4;
-  __shared__ __attribute__((aligned(16))) float so[PA_WAVES][PA_ROWS][LD];
-  __shared__ float sm[PA_WAVES][PA_ROWS], sl[PA_WAVES][PA_ROWS];
+  constexpr int THREADS = 64 * WAVES;
+  __shared__ __attribute__((aligned(16))) float so[WAVES][PA_ROWS][LD];
+  __shared__ float sm[WAVES][PA_ROWS], sl[WAVES][PA_ROWS];
+  __shared__ float2 stat[PA_ROWS];
   const KvPages& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wid = wave_uniform(tid >> 6);
   const int fr = lane & 15, g = lane >> 4;
   const int Dh = PAD ? p.head_dim : DHP;
 
-  // this workgroup's share of the tiles
-  int total = 0;
+  int b = 0, off = 0, t0 = 0, t1 = 1;  // its first sequence, the tile of that sequence's units, and how many tiles
   bool ok = true;
-  for (int b = lane; b < a.B; b += 64) {
-    total += (int)((p.length_of(a.lengths, b, a.max_length, &ok) + PA_KT - 1) / PA_KT);
-  }
-  if (blockIdx.x == 0 && !ok) kv_flag(a.err);
-  total = wave_sum_int(total) * a.units;
-  const int per = share_of(a, total);
-  int t0 = blockIdx.x * per;
-  const int t1 = min(total, t0 + per);
-  if (t0 >= t1) return;
-  int b = 0, off = t0;  // its first sequence, and the tile of that sequence's units
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int v = b0 + lane < a.B ? tiles_of(a, b0 + lane) * a.units : 0;
-    const int inc = wave_scan_int(v, lane);
-    const uint64_t past = __ballot(inc > off);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      b = b0 + l;
-      off -= __shfl(inc - v, l, 64);
-      break;
+  if constexpr (ONE) {
+    b = blockIdx.x / a.units;
+  } else {
+    int total = 0;
+    for (int i = lane; i < a.B; i += 64) {
+      total += (int)((p.length_of(a.lengths, i, a.max_length, &ok) + PA_KT - 1) / PA_KT);
     }
-    off -= __shfl(inc, 63, 64);
+    if (blockIdx.x == 0 && !ok) kv_flag(a.err);
+    total = wave_sum_int(total) * a.units;
+    const int per = share_of(a, total);
+    off = t0 = blockIdx.x * per;
+    t1 = min(total, t0 + per);
+    if (t0 >= t1) return;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int v = b0 + lane < a.B ? tiles_of(a, b0 + lane) * a.units : 0;
+      const int inc = wave_scan_int(v, lane);
+      const uint64_t past = __ballot(inc > off);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = b0 + l;
+        off -= __shfl(inc - v, l, 64);
+        break;
+      }
+      off -= __shfl(inc, 63, 64);
+    }
+    b = wave_uniform(b);
+    off = wave_uniform(off);
   }
-  b = wave_uniform(b);
-  off = wave_uniform(off);
 
   while (t0 < t1 && b < a.B) {
     const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
     const int tiles = (int)((n + PA_KT - 1) / PA_KT);
-    if (off >= tiles * a.units) {  // done, or empty
+    if (!ONE && off >= tiles * a.units) {  // done, or empty
       ++b;
       off = 0;
       continue;
     }
-    const int u = off / tiles, ta = off - u * tiles, tb = min(tiles, ta + (t1 - t0));
+    const int u = ONE ? blockIdx.x - b * a.units : off / tiles, ta = ONE ? 0 : off - u * tiles;
+    const int tb = ONE ? tiles : min(tiles, ta + (t1 - t0));
     const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * PA_ROWS;
     const int rows = min(PA_ROWS, a.group - row0);  // query heads of this unit
     const int head0 = h * a.group + row0;
@@ -192,7 +201,8 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
     const int mask = (1 << p.shift) - 1;
     const int32_t* table = p.table + b * p.ld_table;
     // the page ids of this lane's 8 keys of a tile: for the key rows (8 (r / 4) ..) and the value rows (8 g ..)
-    auto page_at = [&](int j) { return table[min(j, (int)n - 1) >> p.shift]; };
+    const int last = (int)p.max_slots - 1;  // (not the last key: the lookups need not wait for the length)
+    auto page_at = [&](int j) { return table[min(j, last) >> p.shift]; };
     auto kblock = [&](int t) { return t * PA_KT + 8 * (fr >> 2); };
     auto vblock = [&](int t) { return t * PA_KT + 8 * g; };
 
@@ -238,15 +248,16 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
     for (int j = 0; j < E; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
     int t = ta + wid;
+    int kp = 0, vp = 0;
+    if (last >= 0) kp = page_at(kblock(t)), vp = page_at(vblock(t));  // (a table may have no columns)
     if (t < tb) {
-      int kp = page_at(kblock(t)), vp = page_at(vblock(t));
       load_k(t, kp);
       load_v(t, vp);
       load_scales(t, vp);
-      int kp1 = page_at(kblock(t + PA_WAVES)), vp1 = page_at(vblock(t + PA_WAVES));
-      for (; t < tb; t += PA_WAVES) {
-        const int kp2 = page_at(kblock(t + 2 * PA_WAVES)), vp2 = page_at(vblock(t + 2 * PA_WAVES));
-        const bool more = t + PA_WAVES < tb;
+      int kp1 = page_at(kblock(t + WAVES)), vp1 = page_at(vblock(t + WAVES));
+      for (; t < tb; t += WAVES) {
+        const int kp2 = page_at(kblock(t + 2 * WAVES)), vp2 = page_at(vblock(t + 2 * WAVES));
+        const bool more = t + WAVES < tb;
         // scores of keys 8 g + 4 st + i for query fr
         f32x4 s[2];
 #pragma unroll
@@ -274,7 +285,7 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
           }
         }
         const float4 ks0 = ks[0], ks1 = ks[1];
-        if (more) load_k(t + PA_WAVES, kp1);
+        if (more) load_k(t + WAVES, kp1);
         __builtin_amdgcn_sched_barrier(0);
 
         // how many of this lane's 8 keys there are
@@ -336,9 +347,20 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
 #pragma unroll
             for (int i = 0; i < 8; ++i) pr[i] *= sc[i];
           }
-          bf16x8 pf;
+          // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
+          // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
+          // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
+          bf16x8 hi, lo;
+          uint32_t hw[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) pf[i] = (bf16)pr[i];
+          for (int i = 0; i < 4; ++i)
+            hw[i] = __builtin_amdgcn_perm(__float_as_uint(pr[2 * i + 1]), __float_as_uint(pr[2 * i]), 0x07060302u);
+          __builtin_memcpy(&hi, hw, 16);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float rest = pr[i] - __uint_as_float(__float_as_uint(pr[i]) & 0xffff0000u);
+            lo[i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
+          }
 #pragma unroll
           for (int j = 0; j < E; ++j) {
             bf16x8 vf;
@@ -352,12 +374,13 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
 #pragma unroll
               for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[i].w[j >> 2] >> (8 * (j & 3)));
             }
-            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi, o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo, o[j], 0, 0, 0);
           }
         }
         if (more) {
-          load_v(t + PA_WAVES, vp1);
-          load_scales(t + PA_WAVES, vp1);
+          load_v(t + WAVES, vp1);
+          load_scales(t + WAVES, vp1);
         }
         __builtin_amdgcn_sched_barrier(0);
         vp = vp1;
@@ -368,7 +391,7 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
 
     // the wavefronts' sums into one
     l = group_sum(l);
-    const int active = min(PA_WAVES, tb - ta);
+    const int active = min(WAVES, tb - ta);
     if (wid < active && fr < rows) {
       if (g == 0) sm[wid][fr] = m, sl[wid][fr] = l;
 #pragma unroll
@@ -378,12 +401,12 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
           *reinterpret_cast<float4*>(&so[wid][fr][E * (4 * g + i) + j]) = make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
     }
     __syncthreads();
-    const bool complete = ta == 0 && tb == tiles;
+    const bool complete = ONE || (ta == 0 && tb == tiles);
     float* part = a.part + (2 * (int64_t)blockIdx.x + (ta == 0)) * (PA_ROWS * (DHP + 2));
-    for (int i = tid; i < rows * DHP; i += PA_THREADS) {
+    for (int i = tid; i < rows * DHP; i += THREADS) {
       const int r = i / DHP, d = i - r * DHP;
-      float top = sm[0][r];
-      for (int w = 1; w < active; ++w) top = fmaxf(top, sm[w][r]);
+      float top = -INFINITY;  // (ONE: a sequence without keys has none)
+      for (int w = 0; w < active; ++w) top = fmaxf(top, sm[w][r]);
       const float ref = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f, acc = 0.0f;
       for (int w = 0; w < active; ++w) {
@@ -395,28 +418,53 @@ __global__ __launch_bounds__(PA_THREADS, PA_PER_CU) void paged_attention_kernel(
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (d < Dh) reinterpret_cast<Q*>(a.out)[b * a.o_sb + (head0 + r) * a.o_sh + d] = from_f32<Q>(acc * inv);
         if (W && d == 0) {
-          float* st = a.stats + ((int64_t)b * a.heads + head0 + r) * 2;
-          st[0] = ref, st[1] = inv;
+          if constexpr (ONE)
+            stat[r] = make_float2(ref, inv);
+          else
+            reinterpret_cast<float2*>(a.stats)[(int64_t)b * a.heads + head0 + r] = make_float2(ref, inv);
         }
       } else {
         part[r * DHP + d] = acc;
         if (d == 0) part[PA_ROWS * DHP + r] = top, part[PA_ROWS * (DHP + 1) + r] = sum;
       }
     }
+    __syncthreads();
+    if constexpr (ONE) {
+      if constexpr (W) {  // the weight that its keys received
+        const float* score = a.score + ((int64_t)b * a.heads + head0) * a.score_ld;
+        for (int j = tid; j < (int)n; j += THREADS) {
+          float add = 0.0f;
+          for (int r = 0; r < rows; ++r) add += exp2f(score[r * a.score_ld + j] - stat[r].x) * stat[r].y;
+          const int page = p.page_of(b, j);
+          if (page >= 0) p.weight[p.scalar_at(page, h, p.row_of(j))] += add;
+        }
+      }
+      if (h == 0 && row0 == 0 && tid == 0 && !ok) kv_flag(a.err);
+      return;
+    }
     t0 += tb - ta;
     off += tb - ta;
-    __syncthreads();
   }
 }
 
-// One workgroup a unit: the parts of a unit that several shares hold, in the order of its keys; 0 for a sequence
-// without keys.
+constexpr int PJ_THREADS = 256;
+constexpr int PJ_KEYS = 4 * PJ_THREADS;  // keys a workgroup adds the weight of
+
+// The parts of the units that several shares hold, joined in the order of their keys (0 for a sequence without keys),
+// and with W the weight that every key received, sum over the query heads of a key head of p_j.  `chunks` workgroups a
+// (sequence, key head): number c takes the query heads c, c + chunks, .. and the keys PJ_KEYS c ...  The (m, l) of the
+// parts are small: every workgroup that needs them reads them itself.
 template <class Q, int DHP, bool W>
-__global__ __launch_bounds__(128) void paged_join_kernel(PagedArgs a) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int b = blockIdx.x / a.units, u = blockIdx.x - b * a.units;
-  const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * PA_ROWS;
-  const int rows = min(PA_ROWS, a.group - row0), head0 = h * a.group + row0;
+__global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int chunks) {
+  constexpr int64_t SLOT = PA_ROWS * (DHP + 2);
+  constexpr int GROUPS = PJ_THREADS / DHP;  // parts summed side by side
+  __shared__ float share[PA_MAX_SHARES];      // a part's factor
+  __shared__ float sums[GROUPS][DHP];
+  __shared__ float red[2][PJ_THREADS / 64];
+  __shared__ float2 stat[1024];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int bh = blockIdx.x / chunks, c = blockIdx.x - bh * chunks;
+  const int b = bh / a.p.kv_heads, h = bh - b * a.p.kv_heads;
   int total = 0, before = 0;
   for (int i = lane; i < a.B; i += 64) {
     const int n = tiles_of(a, i);
@@ -426,55 +474,110 @@ __global__ __launch_bounds__(128) void paged_join_kernel(PagedArgs a) {
   total = wave_sum_int(total) * a.units;
   before = wave_sum_int(before) * a.units;
   const int tiles = tiles_of(a, b);
-  const int per = share_of(a, total), s = before + u * tiles;
-  const int w0 = tiles ? s / per : 0, w1 = tiles ? (s + tiles - 1) / per : 0;
-  if (tiles && w0 == w1) return;  // written by its one workgroup
-  const float* part = a.part;
-  constexpr int64_t SLOT = PA_ROWS * (DHP + 2);
-  auto slot = [&](int w) { return part + (2 * (int64_t)w + (w == w0)) * SLOT; };
-  for (int i = tid; i < rows * DHP; i += 128) {
-    const int r = i / DHP, d = i - r * DHP;
-    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-    if (tiles) {
-      for (int w = w0; w <= w1; ++w) top = fmaxf(top, slot(w)[PA_ROWS * DHP + r]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      for (int w = w0; w <= w1; ++w) {
-        const float* x = slot(w);
-        const float f = exp2f(x[PA_ROWS * DHP + r] - ref);
-        sum += f * x[PA_ROWS * (DHP + 1) + r];
-        acc += f * x[r * DHP + d];
-      }
+  const int per = share_of(a, total);
+  // the shares w0 .. w1 that hold the unit of query head i
+  auto unit_of = [&](int i, int* w0, int* w1) {
+    const int s = before + (h * a.row_tiles + i / PA_ROWS) * tiles;
+    *w0 = s / per, *w1 = (s + tiles - 1) / per;
+  };
+  auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * SLOT; };
+  Q* out = reinterpret_cast<Q*>(a.out) + b * a.o_sb + (int64_t)h * a.group * a.o_sh;
+
+  for (int i = c; i < a.group; i += chunks) {
+    if (tiles == 0) {
+      if (tid < a.p.head_dim) out[i * a.o_sh + tid] = from_f32<Q>(0.0f);
+      continue;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (d < a.p.head_dim) reinterpret_cast<Q*>(a.out)[b * a.o_sb + (head0 + r) * a.o_sh + d] = from_f32<Q>(acc * inv);
-    if (W && d == 0) {
-      float* st = a.stats + ((int64_t)b * a.heads + head0 + r) * 2;
-      st[0] = top == -INFINITY ? 0.0f : top, st[1] = inv;
+    int w0, w1;
+    unit_of(i, &w0, &w1);
+    if (w0 == w1) continue;  // written by its one workgroup
+    const int r = i % PA_ROWS, parts = w1 - w0 + 1;
+    float top = -INFINITY;
+    for (int w = tid; w < parts; w += PJ_THREADS) {
+      const float m = slot(w0 + w, w0)[PA_ROWS * DHP + r];
+      share[w] = m;
+      top = fmaxf(top, m);
     }
+    top = wave_max(top);
+    if (lane == 0) red[0][wid] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int w = tid; w < parts; w += PJ_THREADS) {
+      const float f = exp2f(share[w] - ref);
+      share[w] = f;
+      sum += f * slot(w0 + w, w0)[PA_ROWS * (DHP + 1) + r];
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) red[1][wid] = sum;
+    __syncthreads();
+    sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    const int d = tid % DHP, group = tid / DHP;
+    float acc = 0.0f;
+#pragma unroll 8
+    for (int w = group; w < parts; w += GROUPS) acc += share[w] * slot(w0 + w, w0)[r * DHP + d];
+    sums[group][d] = acc;
+    __syncthreads();
+    if (tid < a.p.head_dim) {
+      acc = sums[0][tid];
+#pragma unroll
+      for (int x = 1; x < GROUPS; ++x) acc += sums[x][tid];
+      out[i * a.o_sh + tid] = from_f32<Q>(acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    }
+    __syncthreads();  // before the next head's factors
   }
-}
 
-constexpr int PW_KEYS = 256;
-
-// weight_j += sum over the query heads of a key head of p_j, from the scores and the joined m and 1 / l.
-__global__ __launch_bounds__(PW_KEYS) void paged_weight_kernel(PagedArgs a, int chunks) {
-  const int bh = blockIdx.x / chunks, b = bh / a.p.kv_heads, h = bh - b * a.p.kv_heads;
-  bool ok;
-  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
-  const int64_t j = (int64_t)(blockIdx.x - bh * chunks) * PW_KEYS + threadIdx.x;
-  if (j >= n) return;
-  const int page = a.p.page_of(b, j);
-  if (page < 0) return;
-  const float* score = a.score + ((int64_t)b * a.heads + h * a.group) * a.score_ld + j;
-  const float* st = a.stats + ((int64_t)b * a.heads + h * a.group) * 2;
-  float sum = 0.0f;
-  for (int i = 0; i < a.group; ++i) sum += exp2f(score[i * a.score_ld] - st[2 * i]) * st[2 * i + 1];
-  a.p.weight[a.p.scalar_at(page, h, a.p.row_of(j))] += sum;
+  if constexpr (W) {
+    bool ok;
+    const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok), j = (int64_t)c * PJ_KEYS + 4 * tid;
+    if ((int64_t)c * PJ_KEYS >= n) return;
+    // m and 1 / l of the query heads, a wavefront each
+    for (int i = wid; i < a.group; i += PJ_THREADS / 64) {
+      int w0, w1;
+      unit_of(i, &w0, &w1);
+      if (w0 == w1) {
+        if (lane == 0) stat[i] = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.heads + h * a.group + i];
+        continue;
+      }
+      const int r = i % PA_ROWS;
+      float top = -INFINITY, sum = 0.0f;
+      for (int w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, slot(w, w0)[PA_ROWS * DHP + r]);
+      top = wave_max(top);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      for (int w = w0 + lane; w <= w1; w += 64) {
+        const float* x = slot(w, w0) + PA_ROWS * DHP + r;
+        sum += exp2f(x[0] - ref) * x[PA_ROWS];
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) stat[i] = make_float2(ref, sum == 0.0f ? 0.0f : 1.0f / sum);
+    }
+    __syncthreads();
+    if (j >= n) return;
+    const float* score = a.score + ((int64_t)b * a.heads + h * a.group) * a.score_ld + j;
+    float add[4] = {};
+#pragma unroll 4
+    for (int i = 0; i < a.group; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(score + i * a.score_ld);
+      const float2 s = stat[i];
+      add[0] += exp2f(x.x - s.x) * s.y;
+      add[1] += exp2f(x.y - s.x) * s.y;
+      add[2] += exp2f(x.z - s.x) * s.y;
+      add[3] += exp2f(x.w - s.x) * s.y;
+    }
+    const int page = a.p.page_of(b, j);  // four keys of one page
+    if (page < 0) return;
+    float* weight = a.p.weight + a.p.scalar_at(page, h, a.p.row_of(j));
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (j + x < n) weight[x] += add[x];
+  }
 }
 
 // How a call is laid out: shares, and the parts of its workspace in bytes.
 struct Layout {
   int row_tiles, units, shares, dhp;
+  int waves;  // of a workgroup that takes a whole unit; 0: shares
   int64_t score_ld, part, score, stats;
 };
 Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t most, int accumulate) {
@@ -484,38 +587,51 @@ Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t mos
   y.units = (int)(p->kv_heads * y.row_tiles);
   y.dhp = p->head_dim <= 64 ? 64 : 128;
   const int64_t tiles = B * y.units * cdiv(most, PA_KT);
-  const int64_t shares = cdiv(tiles, PA_MIN_TILES), slots = (int64_t)cu_count() * PA_PER_CU;
+  const int64_t shares = cdiv(tiles, PA_MIN_TILES), cus = cu_count();
+  const int64_t slots = cus * PA_PER_CU < PA_MAX_SHARES ? cus * PA_PER_CU : PA_MAX_SHARES;
   y.shares = (int)(shares < 1 ? 1 : shares < slots ? shares : slots);
   y.score_ld = cdiv(most, PA_KT) * PA_KT;
-  y.part = 2ll * y.shares * PA_ROWS * (y.dhp + 2) * 4;
+  y.waves = 0;
+  if (cdiv(most, PA_KT) <= PA_ONE_TILES && (!accumulate || y.row_tiles == 1))
+    y.waves = B * y.units > cus ? PA_WAVES : PA_MORE;
+  y.part = y.waves ? 0 : 2ll * y.shares * PA_ROWS * (y.dhp + 2) * 4;
   y.score = accumulate ? B * heads * y.score_ld * 4 : 0;
-  y.stats = accumulate ? cdiv(B * heads * 2 * 4, 16) * 16 : 0;
+  y.stats = accumulate && !y.waves ? cdiv(B * heads * 2 * 4, 16) * 16 : 0;
   return y;
 }
 
-template <class P, int DHP, bool W>
-int launch(const PagedArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)a.shares), block(PA_THREADS);
+template <class P, int DHP, bool W, int WAVES, bool ONE>
+void launch_main(const PagedArgs& a, unsigned grid, hipStream_t stream) {
   if (a.p.head_dim == DHP)
-    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, false, W>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, false, W, WAVES, ONE>), dim3(grid), dim3(64 * WAVES), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, true, W>), grid, block, 0, stream, a);
-  CORTEX_CHECK_LAUNCH("paged_attention_kernel");
-  hipLaunchKernelGGL((paged_join_kernel<typename Query<P>::type, DHP, W>), dim3((unsigned)(a.B * a.units)), dim3(128), 0,
-                     stream, a);
-  CORTEX_CHECK_LAUNCH("paged_join_kernel");
-  if (W && a.max_length > 0) {
-    const int64_t chunks = cdiv(a.max_length, PW_KEYS);
-    hipLaunchKernelGGL(paged_weight_kernel, dim3((unsigned)(chunks * a.B * a.p.kv_heads)), dim3(PW_KEYS), 0, stream, a,
-                       (int)chunks);
-    CORTEX_CHECK_LAUNCH("paged_weight_kernel");
+    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, true, W, WAVES, ONE>), dim3(grid), dim3(64 * WAVES), 0, stream, a);
+}
+template <class P, int DHP, bool W>
+int launch(const PagedArgs& a, int waves, hipStream_t stream) {
+  if (waves) {
+    const unsigned units = (unsigned)a.B * (unsigned)a.units;
+    if (waves == PA_WAVES)
+      launch_main<P, DHP, W, PA_WAVES, true>(a, units, stream);
+    else
+      launch_main<P, DHP, W, PA_MORE, true>(a, units, stream);
+    CORTEX_CHECK_LAUNCH("paged_attention_kernel");
+    return OK;
   }
+  launch_main<P, DHP, W, PA_WAVES, false>(a, (unsigned)a.shares, stream);
+  CORTEX_CHECK_LAUNCH("paged_attention_kernel");
+  int64_t chunks = a.group;
+  if (W) chunks = cdiv(a.max_length, PJ_KEYS);
+  if (chunks < 1) chunks = 1;
+  hipLaunchKernelGGL((paged_join_kernel<typename Query<P>::type, DHP, W>), dim3((unsigned)(chunks * a.B * a.p.kv_heads)),
+                     dim3(PJ_THREADS), 0, stream, a, (int)chunks);
+  CORTEX_CHECK_LAUNCH("paged_join_kernel");
   return OK;
 }
 template <class P>
-int launch_type(const PagedArgs& a, int accumulate, hipStream_t stream) {
-  if (a.p.head_dim <= 64) return accumulate ? launch<P, 64, true>(a, stream) : launch<P, 64, false>(a, stream);
-  return accumulate ? launch<P, 128, true>(a, stream) : launch<P, 128, false>(a, stream);
+int launch_type(const PagedArgs& a, int waves, int accumulate, hipStream_t stream) {
+  if (a.p.head_dim <= 64) return accumulate ? launch<P, 64, true>(a, waves, stream) : launch<P, 64, false>(a, waves, stream);
+  return accumulate ? launch<P, 128, true>(a, waves, stream) : launch<P, 128, false>(a, waves, stream);
 }
 
 // The length that a call expects at most: max_length, or the table's width where that is negative.
@@ -524,8 +640,8 @@ int64_t expected_length(int64_t max_length, int64_t max_slots) {
 }
 
 int check_heads(const char* who, const cortex_kv_pages* pages, int64_t B, int64_t heads, int64_t most) {
-  CORTEX_CHECK_ARG(heads >= 1 && pages->kv_heads >= 1 && heads % pages->kv_heads == 0 && heads <= 65536,
-                   "%s: %lld query heads are not a multiple of %lld key heads (up to 65536)", who, (long long)heads,
+  CORTEX_CHECK_ARG(heads >= 1 && pages->kv_heads >= 1 && heads % pages->kv_heads == 0 && heads / pages->kv_heads <= 1024,
+                   "%s: %lld query heads are not a multiple (up to 1024) of %lld key heads", who, (long long)heads,
                    (long long)pages->kv_heads);
   CORTEX_CHECK_ARG(B >= 0 && B <= 4096, "%s: %lld sequences (at most 4096)", who, (long long)B);
   const int64_t units = pages->kv_heads * cdiv(heads / pages->kv_heads, PA_ROWS);
@@ -563,7 +679,8 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   CORTEX_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_sb * es) % 16 == 0 && (q_sh * es) % 16 == 0,
                    "%s: query rows must be 16-byte aligned", who);
   const Layout y = layout_of(pages, B, heads, a.max_length, accumulate);
-  CORTEX_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
+  CORTEX_CHECK_ARG((workspace || y.part + y.score + y.stats == 0) && (uintptr_t)workspace % 16 == 0,
+                   "%s: null or unaligned workspace", who);
   if (workspace_bytes < y.part + y.score + y.stats) {
     set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
               (long long)(y.part + y.score + y.stats));
@@ -588,7 +705,7 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   a.part = reinterpret_cast<float*>(workspace);
   a.score = a.part + y.part / 4;
   a.stats = a.score + y.score / 4;
-  if (pages->dtype == DT_F32) return launch_type<float>(a, accumulate, stream);
-  if (pages->dtype == DT_BF16) return launch_type<bf16>(a, accumulate, stream);
-  return launch_type<int8_t>(a, accumulate, stream);
+  if (pages->dtype == DT_F32) return launch_type<float>(a, y.waves, accumulate, stream);
+  if (pages->dtype == DT_BF16) return launch_type<bf16>(a, y.waves, accumulate, stream);
+  return launch_type<int8_t>(a, y.waves, accumulate, stream);
 }

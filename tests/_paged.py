@@ -83,8 +83,9 @@ def attention64(c: Cache, q: torch.Tensor, scale=None, lens=None):
       * a score is a sum of Dh products in fp32, then a product with the scale and, int8, one with the row's scale:
         |ds| <= (Dh + 4) u * scale * sum_d |q_d k_d|; exp of it is off by a factor within exp(+-|ds|) and its own error;
       * the running sums over n keys and their joins add (n + 64) u each to numerator and denominator;
-      * bf16 results: the probabilities enter the second product rounded to bf16 (half a step, 2^-8 of each), and the
-        result is rounded once more (2^-8 of it); fp32: u."""
+      * bf16 and int8: the probabilities enter the second product as two bf16 values, the upper half of the bits (less than a
+        step, 2^-7, below) and the rest rounded (half a step of it): 2^-15 of each; the result is rounded to bf16
+        (2^-8 of it); fp32: u."""
     n_seq, heads, dim = q.shape
     group = heads // c.kv_heads
     scale = dim ** -0.5 if scale is None else scale
@@ -106,7 +107,7 @@ def attention64(c: Cache, q: torch.Tensor, scale=None, lens=None):
             rel = 2 * ds + 2 * (n + 64) * u
             out[b, h] = p @ vh
             mass = p @ vh.abs()
-            tol[b, h] = 1.01 * (rel * mass + (half * mass if half > u else 0) + half * out[b, h].abs()) + 1e-37
+            tol[b, h] = 1.01 * (rel * mass + (2.0 ** -15 * mass if half > u else 0) + half * out[b, h].abs()) + 1e-37
             w[:, h // group] += p
             wt[:, h // group] += p * (rel + group * u)
         added.append(w)

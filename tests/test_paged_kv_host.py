@@ -23,7 +23,7 @@ def append(p, B=2, T=2, x=nat.BF16, k=P, st=128, sh=64, table=P, ld=3, width=3, 
             None, out, None, None)
 
 
-def attention(p, B=2, heads=4, q=P, table=P, ld=3, width=3, lengths=P, most=48, accumulate=0, out=P, ws=P, ws_bytes=1 << 40):
+def attention(p, B=2, heads=4, q=P, table=P, ld=300, width=300, lengths=P, most=4800, accumulate=0, out=P, ws=P, ws_bytes=1 << 40):
     return ("cortex_paged_attention", p and ctypes.byref(p), B, heads, q, 256, 64, table, ld, width, lengths, most,
             ctypes.c_float(0.125), accumulate, out, 256, 64, ws, ws_bytes, None, None)
 
@@ -62,7 +62,7 @@ def test_pages_that_no_operator_takes(call):
     refused(call(tracked(), B=-1), "negative shape")
     refused(call(tracked(), width=-1), "negative shape")
     refused(call(tracked(), table=None), "block table")
-    refused(call(tracked(), ld=2), "overlap")
+    refused(call(tracked(), ld=2, width=3), "overlap")
     refused(call(tracked(page_size=65536), width=20000, ld=20000), "2^30")
 
 
