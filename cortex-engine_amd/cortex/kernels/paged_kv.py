@@ -35,7 +35,8 @@ class KVPages:
     a row is ``code * scale``), ``weight`` fp32 (softmax weight received so far) and ``position`` int32 (where the
     token stood in its sequence), the last two optional.  The tensors of an object do not change."""
 
-    __slots__ = ("k", "v", *_PER_ROW, "num_pages", "kv_heads", "page_size", "head_dim", "device", "_struct", "ref")
+    __slots__ = ("k", "v", *_PER_ROW, "num_pages", "kv_heads", "page_size", "head_dim", "device", "index", "query_dtype",
+                 "_struct", "ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, *, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None, weight: torch.Tensor | None = None,
@@ -52,6 +53,9 @@ class KVPages:
             raise ValueError("k and v need a contiguous last (head) dim")
         if any(t is not None and t.requires_grad for t in (k, v)):
             raise ValueError("pages hold values without gradients")
+        self.index = k.get_device()
+        # of queries and outputs: the pages' own, bfloat16 for int8 pages
+        self.query_dtype = torch.bfloat16 if k.dtype == torch.int8 else k.dtype
         self.k, self.v, self.k_scale, self.v_scale, self.weight, self.position = k, v, k_scale, v_scale, weight, position
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         for name in _PER_ROW:
@@ -84,11 +88,6 @@ class KVPages:
             more["position"] = torch.zeros(shape, dtype=torch.int32, device=device)
         return cls(k, v, **more)
 
-    @property
-    def query_dtype(self) -> torch.dtype:
-        """The dtype of queries and outputs: the pages' own, bfloat16 for int8 pages."""
-        return torch.bfloat16 if self.k.dtype == torch.int8 else self.k.dtype
-
 
 class EvictPlan(NamedTuple):
     """What ``kv_evict_plan`` found: slot ``src[b, h, i]`` moves to ``dst[b, h, i]`` for ``i < counts[b, h]`` (-1
@@ -100,50 +99,56 @@ class EvictPlan(NamedTuple):
     lengths: torch.Tensor
 
 
+_get_device = torch._C._cuda_getDevice  # what torch.cuda.current_device() asks, without its initialisation check
+
+
 def _i64(t: torch.Tensor, n: int, name: str, what: str) -> None:
-    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not torch.int64 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous int64 tensor of {n} values, got {tuple(t.shape)} {t.dtype}")
 
 
-def _common(what: str, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, err_flag, *more) -> int:
-    """Checks what every operator takes; the number of sequences."""
-    dev = nat.require_gpu(block_table, lengths, err_flag, *more, what=what)
-    if dev != pages.device:
-        raise RuntimeError(f"{what}: tensors on different devices ({dev} vs {pages.device})")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"{what}: block_table must be a (B, max_pages) int32 tensor with contiguous rows")
-    B = block_table.shape[0]
-    _i64(lengths, B, "lengths", what)
-    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() != 1):
+def _common(what: str, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, err_flag,
+            *more) -> tuple[int, int, int]:
+    """Checks what every operator takes; the block table's rows, row stride and columns."""
+    idx = pages.index
+    for t in (block_table, lengths, err_flag, *more):
+        if t is not None and t.get_device() != idx:
+            dev = nat.require_gpu(block_table, lengths, err_flag, *more, what=what)
+            raise RuntimeError(f"{what}: tensors on different devices ({dev} vs {pages.device})")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
+        raise ValueError(f"{what}: block_table must be a (B, max_pages) int32 tensor")
+    B, width = block_table.shape
+    ld, unit = block_table.stride()
+    if width > 1 and unit != 1:
+        raise ValueError(f"{what}: the rows of block_table must be contiguous")
+    if lengths.dtype is not torch.int64 or lengths.shape != (B,) or not lengths.is_contiguous():
+        _i64(lengths, B, "lengths", what)
+    if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
         raise ValueError(f"{what}: err_flag must be one int32")
-    return B
+    return B, ld if B > 1 else width, width
 
 
-def _launch(name: str, device: torch.device, *args) -> None:
-    """``nat.call`` on the current stream of ``device``, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        nat.call(name, *args, nat.stream_of(device))
+def _launch(name: str, pages: KVPages, *args) -> None:
+    """``nat.call`` on the current stream of the pages' device, whichever device is current."""
+    if pages.index == _get_device():
+        nat.call(name, pages.ref, *args, nat.stream_of(pages.device))
     else:
-        with torch.cuda.device(device):
-            nat.call(name, *args, nat.stream_of(device))
+        with torch.cuda.device(pages.device):
+            nat.call(name, pages.ref, *args, nat.stream_of(pages.device))
 
 
-def _ld(block_table: torch.Tensor) -> int:
-    return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
-
-
-def _no_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_grad(what: str) -> None:
+    if torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """(n, heads, head_dim) rows that vector loads take: as given, or a contiguous copy."""
-    es = t.element_size()
+def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, int]:
+    """(n, heads, head_dim) rows that vector loads take, as given or copied, and their strides."""
     s0, s1, s2 = t.stride()
-    if s2 != 1 or t.data_ptr() % 16 or (s0 * es) % 16 or (s1 * es) % 16:
-        return t.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps rows that only start off)
-    return t
+    if s2 != 1 or (t.data_ptr() | s0 * es | s1 * es) & 15:
+        t = t.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps rows that only start off)
+        s0, s1, _ = t.stride()
+    return t, s0, s1
 
 
 def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -157,14 +162,20 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
     ``max(max|x|, 1e-8) / 127``, rounded half to even.  Tracked pages get weight 0 and the token's position:
     ``positions`` (T,) int64, by default its slot number.  ``new_lengths`` may be ``lengths`` itself.  A token without
     a slot or a page is dropped and sets bit 2 of ``err_flag`` (int32, never cleared here)."""
-    B = _common("paged_kv_append", pages, block_table, lengths, err_flag, k, v, offsets, positions, new_lengths)
-    _no_grad("paged_kv_append", k, v)
-    T = k.shape[0]
-    if k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (pages.kv_heads, pages.head_dim) or k.dtype != v.dtype:
+    B, ld, width = _common("paged_kv_append", pages, block_table, lengths, err_flag, k, v, offsets, positions, new_lengths)
+    if k.requires_grad or v.requires_grad:
+        _no_grad("paged_kv_append")
+    shape, dtype = k.shape, k.dtype
+    if shape != v.shape or len(shape) != 3 or shape[1:] != (pages.kv_heads, pages.head_dim) or dtype is not v.dtype:
         raise ValueError(f"k and v must be (T, {pages.kv_heads}, {pages.head_dim}) of one dtype, got {tuple(k.shape)} "
                          f"{k.dtype} and {tuple(v.shape)} {v.dtype}")
-    if k.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"rows of dtype {k.dtype} are not supported (bfloat16 or float32)")
+    if dtype is torch.bfloat16:
+        code, es = nat.BF16, 2
+    elif dtype is torch.float32:
+        code, es = nat.F32, 4
+    else:
+        raise ValueError(f"rows of dtype {dtype} are not supported (bfloat16 or float32)")
+    T = shape[0]
     if offsets is not None:
         _i64(offsets, B + 1, "offsets", "paged_kv_append")
     elif T != B:
@@ -175,11 +186,11 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
         new_lengths = torch.empty_like(lengths)
     else:
         _i64(new_lengths, B, "new_lengths", "paged_kv_append")
-    k, v = _rows(k), _rows(v)
-    (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-    _launch("cortex_kv_append", pages.device, pages.ref, B, T, nat.code(k.dtype), k.data_ptr(), kt, kh, v.data_ptr(),
-            vt, vh, block_table.data_ptr(), _ld(block_table), block_table.shape[1], nat.ptr(offsets),
-            lengths.data_ptr(), nat.ptr(positions), new_lengths.data_ptr(), nat.ptr(err_flag))
+    k, kt, kh = _rows(k, es)
+    v, vt, vh = _rows(v, es)
+    _launch("cortex_kv_append", pages, B, T, code, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, block_table.data_ptr(),
+            ld, width, nat.ptr(offsets), lengths.data_ptr(), nat.ptr(positions), new_lengths.data_ptr(),
+            nat.ptr(err_flag))
     return new_lengths
 
 
@@ -194,31 +205,34 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     of its key head; no two sequences of the call may then share a page.  ``max_length``: a bound of the lengths
     known on the host (default: the table's width), which sizes the launch and the workspace; longer sequences are cut
     to it and set bit 2 of ``err_flag``, as lengths outside the table and page ids outside the pool do (such pages hold no keys)."""
-    B = _common("paged_attention", pages, block_table, lengths, err_flag, q, out)
-    _no_grad("paged_attention", q)
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != pages.head_dim or q.dtype != pages.query_dtype:
-        raise ValueError(f"q must be ({B}, heads, {pages.head_dim}) in {pages.query_dtype}, got {tuple(q.shape)} {q.dtype}")
-    heads = q.shape[1]
+    B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag, q, out)
+    if q.requires_grad:
+        _no_grad("paged_attention")
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or shape[0] != B or shape[2] != pages.head_dim or dtype is not pages.query_dtype:
+        raise ValueError(f"q must be ({B}, heads, {pages.head_dim}) in {pages.query_dtype}, got {tuple(shape)} {dtype}")
+    heads = shape[1]
     if heads < 1 or heads % pages.kv_heads:
         raise ValueError(f"{heads} query heads are not a multiple of {pages.kv_heads} key heads")
     if accumulate and pages.weight is None:
         raise ValueError("accumulate needs pages with weight")
-    if max_length is not None and max_length < 0:
+    if max_length is None:
+        max_length = width * pages.page_size
+    elif max_length < 0:
         raise ValueError(f"max_length must not be negative, got {max_length}")
+    else:
+        max_length = min(max_length, width * pages.page_size)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1 or out.data_ptr() == q.data_ptr():
-        raise ValueError(f"out must be a {tuple(q.shape)} {q.dtype} tensor of its own with a contiguous last dim")
-    if B == 0:
-        return out
-    most = block_table.shape[1] * pages.page_size if max_length is None else max_length
-    q = _rows(q)
-    ws_bytes = nat.load().cortex_paged_attention_workspace_bytes(pages.ref, B, heads, most, int(accumulate))
+        out = torch.empty(shape, dtype=dtype, device=pages.device)
+    elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1 or out.data_ptr() == q.data_ptr():
+        raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor of its own with a contiguous last dim")
+    q, qb, qh = _rows(q, 4 if dtype is torch.float32 else 2)
+    ws_bytes = nat.load().cortex_paged_attention_workspace_bytes(pages.ref, B, heads, max_length, accumulate)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=pages.device) if ws_bytes else None
-    _launch("cortex_paged_attention", pages.device, pages.ref, B, heads, q.data_ptr(), q.stride(0), q.stride(1),
-            block_table.data_ptr(), _ld(block_table), block_table.shape[1], lengths.data_ptr(), most,
-            float(scale) if scale is not None else pages.head_dim ** -0.5, int(accumulate), out.data_ptr(),
-            out.stride(0), out.stride(1), nat.ptr(ws), ws_bytes, nat.ptr(err_flag))
+    ob, oh, _ = out.stride()
+    _launch("cortex_paged_attention", pages, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld, width,
+            lengths.data_ptr(), max_length, pages.head_dim ** -0.5 if scale is None else scale, accumulate,
+            out.data_ptr(), ob, oh, nat.ptr(ws), ws_bytes, nat.ptr(err_flag))
     return out
 
 
@@ -229,26 +243,23 @@ def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tens
     equal weights by the lower slot).  Kept slots at or past the budget are to fill the slots below it that are given up (``EvictPlan``);
     shorter sequences stay as they are.  Reads ``pages.weight`` and ``pages.position`` and writes neither.
     ``max_length`` and ``err_flag`` as for ``paged_attention``."""
-    B = _common("kv_evict_plan", pages, block_table, lengths, err_flag)
+    B, ld, width = _common("kv_evict_plan", pages, block_table, lengths, err_flag)
     if pages.weight is None or pages.position is None:
         raise ValueError("eviction needs pages with weight and position (tracked=True)")
     if budget < 0 or recent < 0 or (max_length is not None and max_length < 0):
         raise ValueError(f"budget, recent and max_length must not be negative, got {budget}, {recent}, {max_length}")
     if recent > budget:
         raise ValueError(f"recent ({recent}) exceeds the budget ({budget})")
-    room = block_table.shape[1] * pages.page_size
+    budget, recent = min(budget, 1 << 40), min(recent, 1 << 40)  # (as far as a C integer goes)
+    room = width * pages.page_size
     most = room if max_length is None else min(max_length, room)
     cap = max(0, min(budget, most - budget))
-    H = pages.kv_heads
-    moves = torch.empty((2, B, H, cap), dtype=torch.int32, device=pages.device)
-    counts = torch.empty((B, H), dtype=torch.int32, device=pages.device)
-    after = torch.empty_like(lengths)
-    plan = EvictPlan(moves[0], moves[1], counts, after)
-    if B == 0:
-        return plan
-    _launch("cortex_kv_evict_plan", pages.device, pages.ref, B, block_table.data_ptr(), _ld(block_table),
-            block_table.shape[1], lengths.data_ptr(), most, int(budget), int(recent), plan.dst.data_ptr(),
-            plan.src.data_ptr(), counts.data_ptr(), after.data_ptr(), nat.ptr(err_flag))
+    moves = torch.empty((2, B, pages.kv_heads, cap), dtype=torch.int32, device=pages.device)
+    counts = torch.empty((B, pages.kv_heads), dtype=torch.int32, device=pages.device)
+    dst, src = moves.unbind(0)
+    plan = EvictPlan(dst, src, counts, torch.empty_like(lengths))
+    _launch("cortex_kv_evict_plan", pages, B, block_table.data_ptr(), ld, width, lengths.data_ptr(), most, budget, recent,
+            dst.data_ptr(), src.data_ptr(), counts.data_ptr(), plan.lengths.data_ptr(), nat.ptr(err_flag))
     return plan
 
 
@@ -256,16 +267,15 @@ def kv_evict_apply(pages: KVPages, block_table: torch.Tensor, plan: EvictPlan, *
                    err_flag: torch.Tensor | None = None) -> None:
     """Moves the rows of a plan in place: keys, values and, where the pages have them, scales, weight and position.
     Slots at or past the budget keep what they held.  Sequences of the call may not share pages."""
-    B = _common("kv_evict_apply", pages, block_table, plan.lengths, err_flag, plan.dst, plan.src, plan.counts)
-    shape = plan.dst.shape
-    if (len(shape) != 3 or shape[:2] != (B, pages.kv_heads) or plan.src.shape != shape or plan.counts.shape != shape[:2]
-            or any(t.dtype != torch.int32 or not t.is_contiguous() for t in plan[:3])):
+    dst, src, counts, after = plan
+    B, ld, width = _common("kv_evict_apply", pages, block_table, after, err_flag, dst, src, counts)
+    shape = dst.shape
+    if (len(shape) != 3 or shape[:2] != (B, pages.kv_heads) or src.shape != shape or counts.shape != shape[:2]
+            or not dst.dtype is src.dtype is counts.dtype is torch.int32
+            or not (dst.is_contiguous() and src.is_contiguous() and counts.is_contiguous())):
         raise ValueError(f"the plan must hold contiguous int32 moves of ({B}, {pages.kv_heads}) heads")
-    if B == 0 or shape[2] == 0:
-        return
-    _launch("cortex_kv_evict_apply", pages.device, pages.ref, B, block_table.data_ptr(), _ld(block_table),
-            block_table.shape[1], plan.dst.data_ptr(), plan.src.data_ptr(), shape[2], plan.counts.data_ptr(),
-            nat.ptr(err_flag))
+    _launch("cortex_kv_evict_apply", pages, B, block_table.data_ptr(), ld, width, dst.data_ptr(), src.data_ptr(),
+            shape[2], counts.data_ptr(), nat.ptr(err_flag))
 
 
 __all__ = ["EvictPlan", "KVPages", "kv_evict_apply", "kv_evict_plan", "paged_attention", "paged_kv_append"]

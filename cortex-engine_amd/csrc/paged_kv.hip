@@ -84,28 +84,50 @@ __device__ __forceinline__ void store8(bf16* p, const float (&f)[8]) {
   *reinterpret_cast<bf16x8*>(p) = a;
 }
 
-// The sequence of token t: the number of offsets[1 ..] that are <= t.
-__device__ int64_t sequence_of(const int64_t* offsets, int64_t B, int64_t t) {
-  int64_t lo = 0, hi = B;  // offsets[lo] <= t < offsets[hi + 1] for ascending offsets
+// The lengths after a ragged append, by thread `at` of `threads`.
+__device__ void lengths_after(const AppendArgs& a, int at, int threads) {
+  if (!a.new_lengths) return;
+  for (int64_t b = at; b < a.B; b += threads) {
+    bool ok = true;
+    const int64_t len = a.p.length_of(a.lengths, b, a.p.max_slots, &ok);
+    const int64_t lo = min(max(a.offsets[b], (int64_t)0), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);
+    a.new_lengths[b] = min(len + (hi - lo), a.p.max_slots);
+  }
+}
+
+// The sequence of token t: how many of offsets[1 .. B] are <= t.  The lanes of a wavefront look at 64 of them a
+// round, so the round trips are one for up to 64 sequences and two for up to 4096.
+__device__ int64_t sequence_of(const int64_t* offsets, int64_t B, int64_t t, int lane) {
+  int64_t lo = 0, hi = B;
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (offsets[mid + 1] <= t)
-      lo = mid + 1;
-    else
-      hi = mid;
+    const int64_t step = (hi - lo + 63) >> 6, i = lo + (lane + 1) * step;
+    const int64_t past = __builtin_popcountll(__ballot(i <= hi && offsets[i <= hi ? i : hi] <= t));
+    lo += past * step;
+    hi = min(hi, lo + step - 1);
   }
   return lo;
 }
 
-// One workgroup a token; LPR lanes a (key or value, head) row.
+// One workgroup a token; `lpr` lanes a (key or value, head) row, eight values each.  The rows are loaded before the
+// place is known that they go to: the lookups (offsets, length, table) are a chain of round trips as long as the load.
 template <class X, class P>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr) {
   const int tid = threadIdx.x;
   const KvPages& p = a.p;
   const int64_t t = blockIdx.x;
+  const int d = (tid % lpr) * 8;
+  const int rows = 2 * p.kv_heads, step = 256 / lpr;
+  float f[8];
+  auto load = [&](int r) {
+    if (r < rows && d < p.head_dim)
+      load8(f, reinterpret_cast<const X*>((r & 1) ? a.v : a.k) + t * ((r & 1) ? a.v_st : a.k_st) +
+                   (r >> 1) * ((r & 1) ? a.v_sh : a.k_sh) + d);
+  };
+  load(tid / lpr);
   int64_t b = t, first = t;
   if (a.offsets) {
-    b = sequence_of(a.offsets, a.B, t);
+    if (blockIdx.x == 0 && a.new_lengths != a.lengths) lengths_after(a, tid, 256);
+    b = sequence_of(a.offsets, a.B, t, tid & 63);
     if (b >= a.B) return;  // behind the last sequence
     first = a.offsets[b];
     if (t < first) return;  // before the first
@@ -118,25 +140,23 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr) {
   // lengths may be new_lengths: with a token a sequence this workgroup is the only one that reads lengths[b]
   if (!a.offsets) {
     __syncthreads();
-    if (tid == 0 && a.new_lengths) a.new_lengths[b] = page < 0 && slot >= p.max_slots ? len : len + 1;
+    if (tid == 0 && a.new_lengths) a.new_lengths[b] = min(len + 1, p.max_slots);
   }
   if (page < 0) return;
   const int row = p.row_of(slot);
-  const int d = (tid % lpr) * 8;
-  const int rows = 2 * p.kv_heads, step = 256 / lpr;
   for (int r0 = 0; r0 < rows; r0 += step) {  // whole groups of lanes: the shuffles below take all of them
     const int r = r0 + tid / lpr;
     const bool in = r < rows && d < p.head_dim;
     const int h = r >> 1;
     const bool is_v = r & 1;
-    float f[8] = {};
-    if (in) load8(f, reinterpret_cast<const X*>(is_v ? a.v : a.k) + t * (is_v ? a.v_st : a.k_st) + h * (is_v ? a.v_sh : a.k_sh) + d);
+    if (r0 > 0) load(r);
     const int64_t at = is_v ? page * p.v_page + h * p.v_head + row * p.v_slot : page * p.k_page + h * p.k_head + row * p.k_slot;
     P* to = reinterpret_cast<P*>(is_v ? p.v : p.k) + at + d;
     if constexpr (sizeof(P) == 1) {
       uint32_t most = 0;  // the largest |x|; an infinity or a NaN is above every number's bits
+      if (in)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
       for (int o = 1; o < lpr; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
       const bool finite = most < 0x7f800000u;
       const float s = finite ? fmaxf(__uint_as_float(most), 1e-8f) / 127.0f : __uint_as_float(0x7fc00000u);
@@ -161,15 +181,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr) {
   }
 }
 
-// The lengths after ragged appends, in a launch of its own: lengths may be new_lengths.
-__global__ void kv_lengths_kernel(AppendArgs a) {
-  const int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (b >= a.B) return;
-  bool ok = true;
-  const int64_t len = a.p.length_of(a.lengths, b, a.p.max_slots, &ok);
-  const int64_t lo = min(max(a.offsets[b], (int64_t)0), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);
-  a.new_lengths[b] = min(len + (hi - lo), a.p.max_slots);
-}
+// Where there are no tokens, or lengths are new_lengths: in a launch of its own, behind the appends that read them.
+__global__ void kv_lengths_kernel(AppendArgs a) { lengths_after(a, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x); }
 
 // ---------------------------------------------------------------------------- eviction
 
@@ -184,19 +197,12 @@ struct PlanArgs {
   int32_t* err;
 };
 
-constexpr int EP_THREADS = 1024;
-constexpr int EP_WAVES = EP_THREADS / 64;
-// Ranks held in LDS (16 or 128 KiB); a sequence with more slots computes them again where they are read.
-constexpr int EP_FEW = 4096, EP_MANY = 32768;
+constexpr int EP_COPIES = 8;  // of the histogram, by lane: fewer lanes of a wavefront meet in one counter
 
-// The rank of a slot as an unsigned number: protected slots first, then NaN, then by weight; a slot without a page
-// below all of them.
-__device__ __forceinline__ uint32_t rank_of(const PlanArgs& a, int64_t b, int h, int64_t j, int64_t above) {
-  const int page = a.p.page_of(b, j);
-  if (page < 0) return 0;
-  const int64_t i = a.p.scalar_at(page, h, a.p.row_of(j));
-  if ((int64_t)a.p.position[i] > above) return 0xffffffffu;
-  const float w = a.p.weight[i];
+// The rank of a slot as an unsigned number: protected slots first, then NaN, then by weight (a slot without a page has 0,
+// below all of them).
+__device__ __forceinline__ uint32_t rank_of(float w, int position, int64_t above) {
+  if ((int64_t)position > above) return 0xffffffffu;
   if (w != w) return 0xfffffffeu;
   const uint32_t u = __float_as_uint(w + 0.0f);  // -0 and 0 are equal
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
@@ -212,6 +218,7 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
 }
 
 // Sum of v over the threads before this one, and over all of them (in *total).
+template <int WAVES>
 __device__ int block_scan(int v, int* part, int tid, int* total) {
   const int lane = tid & 63, wid = tid >> 6;
   const int inc = wave_scan(v, lane);
@@ -219,7 +226,8 @@ __device__ int block_scan(int v, int* part, int tid, int* total) {
   if (lane == 63) part[wid] = inc;
   __syncthreads();
   int before = 0, all = 0;
-  for (int w = 0; w < EP_WAVES; ++w) {
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
     const int s = part[w];
     if (w < wid) before += s;
     all += s;
@@ -228,13 +236,15 @@ __device__ int block_scan(int v, int* part, int tid, int* total) {
   return before + inc - v;
 }
 
-// One workgroup a (sequence, key head): the rank of every slot, the budget-th largest by a radix selection over
-// four bytes, then holes and movers in slot order by prefix sums.
-template <int KEYS>
-__global__ __launch_bounds__(EP_THREADS) void kv_evict_plan_kernel(PlanArgs a) {
-  __shared__ uint32_t keys[KEYS];
-  __shared__ int hist[EP_WAVES][256];
-  __shared__ int part[EP_WAVES];
+// One workgroup a (sequence, key head): the rank of every slot, the budget-th largest by a radix selection of up to
+// four bytes, then holes and movers in slot order by prefix sums.  A thread takes Q runs of eight consecutive slots
+// (one page each, four vector loads) and keeps their ranks in registers; Q 0: as many runs as there are, read again in
+// every pass.
+template <int THREADS, int Q>
+__global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ __attribute__((aligned(16))) int hist[EP_COPIES][256];
+  __shared__ int part[WAVES];
   __shared__ int picked[3];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int H = a.p.kv_heads;
@@ -243,93 +253,146 @@ __global__ __launch_bounds__(EP_THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   int32_t* dst = a.dst + (int64_t)blockIdx.x * a.cap;
   int32_t* src = a.src + (int64_t)blockIdx.x * a.cap;
   bool ok = true;
-  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
+  const int n = (int)a.p.length_of(a.lengths, b, a.max_length, &ok);
   if (!ok && tid == 0) kv_flag(a.err);
-  if (h == 0 && tid == 0) a.new_lengths[b] = min(n, a.budget);
+  if (h == 0 && tid == 0) a.new_lengths[b] = min((int64_t)n, a.budget);
   int moved = 0;
   if (n > a.budget && a.budget > 0) {
+    const int budget = (int)a.budget;
+    const int runs = Q ? Q : (int)cdiv(cdiv(n, 8), THREADS), j0 = tid * runs * 8;
+    bool lost = false;
+    // run i of this thread: eight weights and positions, or false where there are none
+    auto load = [&](int i, float (&w)[8], int (&pos)[8]) {
+      const int j = j0 + 8 * i;
+      if (j >= n) return false;
+      const int page = a.p.page_of(b, j);
+      if (page < 0) {
+        lost = true;
+        return false;
+      }
+      const int64_t at = a.p.scalar_at(page, h, a.p.row_of(j));
+#pragma unroll
+      for (int x = 0; x < 8; x += 4) {
+        *reinterpret_cast<float4*>(w + x) = *reinterpret_cast<const float4*>(a.p.weight + at + x);
+        *reinterpret_cast<int4*>(pos + x) = *reinterpret_cast<const int4*>(a.p.position + at + x);
+      }
+      return true;
+    };
+    float w[Q ? Q : 1][8];
+    int pos[Q ? Q : 1][8];
+    bool there[Q ? Q : 1];
     // the newest position
     int newest = INT32_MIN;
-    bool lost = false;
-    for (int64_t j = tid; j < n; j += EP_THREADS) {
-      const int page = a.p.page_of(b, j);
-      if (page < 0)
-        lost = true;
-      else
-        newest = max(newest, a.p.position[a.p.scalar_at(page, h, a.p.row_of(j))]);
+    auto newer = [&](int i, const int (&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j0 + 8 * i + e < n) newest = max(newest, x[e]);
+    };
+    if constexpr (Q > 0) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) there[i] = load(i, w[i], pos[i]);
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+        if (there[i]) newer(i, pos[i]);
+    } else {
+      for (int i = 0; i < runs; ++i)
+        if (load(i, w[0], pos[0])) newer(i, pos[0]);
     }
     if (lost) kv_flag(a.err);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) newest = max(newest, __shfl_xor(newest, o, 64));
     if (lane == 0) part[wid] = newest;
     __syncthreads();
-    for (int w = 0; w < EP_WAVES; ++w) newest = max(newest, part[w]);
+#pragma unroll
+    for (int x = 0; x < WAVES; ++x) newest = max(newest, part[x]);
     const int64_t above = (int64_t)newest - a.recent;
-    const bool held = n <= KEYS;
-    if (held)
-      for (int64_t j = tid; j < n; j += EP_THREADS) keys[j] = rank_of(a, b, h, j, above);
-    auto key = [&](int64_t j) { return held ? keys[j] : rank_of(a, b, h, j, above); };
-
-    // the budget-th largest rank, a byte a round: `kept` of the slots with the rank found so far are kept
-    uint32_t found = 0;
-    int kept = (int)a.budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      for (int i = tid; i < EP_WAVES * 256; i += EP_THREADS) hist[0][i] = 0;
-      __syncthreads();
-      for (int64_t j = tid; j < n; j += EP_THREADS) {
-        const uint32_t x = key(j);
-        if (shift == 24 || (x >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&hist[wid][(x >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (wid == 0) {  // lane l has the bins 255 - 4 l .. 252 - 4 l, the largest ranks first
-        int c[4], s = 0;
+    uint32_t key[Q ? Q : 1][8];
+    auto rank = [&](int i, bool in, const float (&x)[8], const int (&y)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c[i] = 0;
-          for (int w = 0; w < EP_WAVES; ++w) c[i] += hist[w][255 - 4 * lane - i];
-          s += c[i];
+      for (int e = 0; e < 8; ++e) key[i][e] = in ? rank_of(x[e], y[e], above) : 0u;
+    };
+    if constexpr (Q > 0) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) rank(i, there[i], w[i], pos[i]);
+    }
+    // f(slot, rank) for this thread's slots, ascending
+    auto each = [&](auto f) {
+      if constexpr (Q > 0) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j0 + 8 * i + e < n) f(j0 + 8 * i + e, key[i][e]);
+      } else {
+        for (int i = 0; i < runs && j0 + 8 * i < n; ++i) {
+          rank(0, load(i, w[0], pos[0]), w[0], pos[0]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j0 + 8 * i + e < n) f(j0 + 8 * i + e, key[0][e]);
         }
-        int before = wave_scan(s, lane) - s;
+      }
+    };
+
+    // the budget-th largest rank, a byte a round; of the slots that share the bytes found so far, `kept` are kept.  Where
+    // that is all of them the bytes below do not matter: every slot from `found` up stays
+    uint32_t found = 0;
+    int kept = budget;
+    bool whole = false;
+    for (int shift = 24; shift >= 0 && !whole; shift -= 8) {
+      for (int i = tid; i < EP_COPIES * 256; i += THREADS) hist[0][i] = 0;
+      __syncthreads();
+      each([&](int, uint32_t x) {
+        if (shift == 24 || (x >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&hist[lane % EP_COPIES][(x >> shift) & 255], 1);
+      });
+      __syncthreads();
+      if (wid == 0) {  // lane l has the bins 252 - 4 l .. 255 - 4 l
+        int4 c = {0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < EP_COPIES; ++x) {
+          const int4 y = *reinterpret_cast<const int4*>(&hist[x][252 - 4 * lane]);
+          c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
+        }
+        const int count[4] = {c.w, c.z, c.y, c.x};  // the largest ranks first
+        const int sum = (c.x + c.y) + (c.z + c.w);
+        int before = wave_scan(sum, lane) - sum;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (before < kept && before + c[i] >= kept) {  // (one bin of one lane)
-            picked[0] = 255 - 4 * lane - i;
-            picked[1] = before;
-          }
-          before += c[i];
+          if (before < kept && before + count[i] >= kept)  // (one bin of one lane)
+            picked[0] = 255 - 4 * lane - i, picked[1] = before, picked[2] = count[i];
+          before += count[i];
         }
       }
       __syncthreads();
       found |= (uint32_t)picked[0] << shift;
       kept -= picked[1];
+      whole = kept == picked[2];
     }
 
-    // thread i takes the slots [i R, (i + 1) R), R odd: its LDS reads are free of bank conflicts
-    const int64_t R = cdiv(n, EP_THREADS) | 1;
-    const int64_t j0 = min((int64_t)tid * R, n), j1 = min(j0 + R, n);
-    int ties = 0, all;
-    for (int64_t j = j0; j < j1; ++j) ties += key(j) == found;
-    ties = block_scan(ties, part, tid, &all);  // (now: the ties before this thread's slots)
-    int holes = 0, movers = 0, tie = ties;
-    for (int64_t j = j0; j < j1; ++j) {
-      const uint32_t x = key(j);
-      const bool keep = x > found || (x == found && tie++ < kept);
-      holes += !keep && j < a.budget;
-      movers += keep && j >= a.budget;
+    int tie = 0, all;
+    if (!whole) {  // equal ranks: the lower slots stay
+      int ties = 0;
+      each([&](int, uint32_t x) { ties += x == found; });
+      tie = block_scan<WAVES>(ties, part, tid, &all);
     }
-    int hole = block_scan(holes, part, tid, &all);
-    int mover = block_scan(movers, part, tid, &moved);
-    tie = ties;
-    for (int64_t j = j0; j < j1; ++j) {
-      const uint32_t x = key(j);
-      const bool keep = x > found || (x == found && tie++ < kept);
-      if (!keep && j < a.budget) dst[hole++] = (int32_t)j;
-      if (keep && j >= a.budget) src[mover++] = (int32_t)j;
-    }
+    auto stays = [=](uint32_t x, int& t) { return x > found || (x == found && (whole || t++ < kept)); };
+    int holes = 0, movers = 0, t = tie;
+    each([&](int j, uint32_t x) {
+      const bool stay = stays(x, t);
+      holes += !stay && j < budget;
+      movers += stay && j >= budget;
+    });
+    int hole = block_scan<WAVES>(holes, part, tid, &all);
+    int mover = block_scan<WAVES>(movers, part, tid, &moved);
+    t = tie;
+    each([&](int j, uint32_t x) {
+      const bool stay = stays(x, t), low = j < budget;
+      if (stay != low) (low ? dst : src)[low ? hole : mover] = j;
+      hole += !stay && low;
+      mover += stay && !low;
+    });
   }
   if (tid == 0) a.counts[blockIdx.x] = moved;
-  for (int64_t i = moved + tid; i < a.cap; i += EP_THREADS) dst[i] = src[i] = -1;
+  for (int64_t i = moved + tid; i < a.cap; i += THREADS) dst[i] = src[i] = -1;
 }
 
 struct ApplyArgs {
@@ -353,30 +416,57 @@ __global__ __launch_bounds__(256) void kv_evict_apply_kernel(ApplyArgs a, int es
   const int h = bh - (int)b * a.p.kv_heads;
   const int groups = 256 / a.lanes, group = tid / a.lanes, c = (tid % a.lanes) * 16;
   const int64_t n = min((int64_t)a.counts[bh], a.cap);
+  const int64_t i0 = (int64_t)chunk * EA_ROWS * groups + group;
+  if (i0 >= n) return;
+  // all lookups, then all loads, then the stores
+  int64_t to[EA_ROWS], from[EA_ROWS];
+  bool ok[EA_ROWS];
 #pragma unroll
   for (int r = 0; r < EA_ROWS; ++r) {
-    const int64_t i = ((int64_t)chunk * EA_ROWS + r) * groups + group;
-    if (i >= n) return;
-    const int64_t to = a.dst[(int64_t)bh * a.cap + i], from = a.src[(int64_t)bh * a.cap + i];
-    const int tp = a.p.page_of(b, to), fp = a.p.page_of(b, from);
-    if (tp < 0 || fp < 0) {
-      if (c == 0) kv_flag(a.err);
-      continue;
+    const int64_t i = min(i0 + r * groups, n - 1);
+    to[r] = a.dst[(int64_t)bh * a.cap + i], from[r] = a.src[(int64_t)bh * a.cap + i];
+  }
+  int tp[EA_ROWS], fp[EA_ROWS];
+#pragma unroll
+  for (int r = 0; r < EA_ROWS; ++r) tp[r] = a.p.page_of(b, to[r]), fp[r] = a.p.page_of(b, from[r]);
+  bool bad = false;
+#pragma unroll
+  for (int r = 0; r < EA_ROWS; ++r) {
+    const bool in = i0 + r * groups < n;
+    ok[r] = in && tp[r] >= 0 && fp[r] >= 0;
+    bad = bad || (in && !ok[r]);
+  }
+  if (bad && c == 0) kv_flag(a.err);
+  // (what does not move is loaded too, from wherever a row is, and not stored)
+  const bool row_part = c < a.row_bytes;
+  char* k = reinterpret_cast<char*>(a.p.k) + h * a.p.k_head * es + (row_part ? c : 0);
+  char* v = reinterpret_cast<char*>(a.p.v) + h * a.p.v_head * es + (row_part ? c : 0);
+  i32x4 x[EA_ROWS], y[EA_ROWS];
+  float weight[EA_ROWS], ks[EA_ROWS], vs[EA_ROWS];
+  int position[EA_ROWS];
+#pragma unroll
+  for (int r = 0; r < EA_ROWS; ++r) {
+    const int64_t page = ok[r] ? fp[r] : 0, row = a.p.row_of(from[r]);
+    x[r] = *reinterpret_cast<const i32x4*>(k + (page * a.p.k_page + row * a.p.k_slot) * es);
+    y[r] = *reinterpret_cast<const i32x4*>(v + (page * a.p.v_page + row * a.p.v_slot) * es);
+    const int64_t f = a.p.scalar_at((int)page, h, (int)row);  // (every lane of a row: one address)
+    weight[r] = a.p.weight ? a.p.weight[f] : 0.0f;
+    position[r] = a.p.position ? a.p.position[f] : 0;
+    ks[r] = a.p.k_scale ? a.p.k_scale[f] : 0.0f;
+    vs[r] = a.p.k_scale ? a.p.v_scale[f] : 0.0f;
+  }
+#pragma unroll
+  for (int r = 0; r < EA_ROWS; ++r) {
+    const int64_t row = a.p.row_of(to[r]);
+    if (ok[r] && row_part) {
+      *reinterpret_cast<i32x4*>(k + (tp[r] * a.p.k_page + row * a.p.k_slot) * es) = x[r];
+      *reinterpret_cast<i32x4*>(v + (tp[r] * a.p.v_page + row * a.p.v_slot) * es) = y[r];
     }
-    const int tr = a.p.row_of(to), fr = a.p.row_of(from);
-    if (c < a.row_bytes) {
-      char* k = reinterpret_cast<char*>(a.p.k) + h * a.p.k_head * es + c;
-      char* v = reinterpret_cast<char*>(a.p.v) + h * a.p.v_head * es + c;
-      const uint4 x = *reinterpret_cast<const uint4*>(k + (fp * a.p.k_page + fr * a.p.k_slot) * es);
-      const uint4 y = *reinterpret_cast<const uint4*>(v + (fp * a.p.v_page + fr * a.p.v_slot) * es);
-      *reinterpret_cast<uint4*>(k + (tp * a.p.k_page + tr * a.p.k_slot) * es) = x;
-      *reinterpret_cast<uint4*>(v + (tp * a.p.v_page + tr * a.p.v_slot) * es) = y;
-    }
-    if (c == 0) {
-      const int64_t t = a.p.scalar_at(tp, h, tr), f = a.p.scalar_at(fp, h, fr);
-      if (a.p.k_scale) a.p.k_scale[t] = a.p.k_scale[f], a.p.v_scale[t] = a.p.v_scale[f];
-      if (a.p.weight) a.p.weight[t] = a.p.weight[f];
-      if (a.p.position) a.p.position[t] = a.p.position[f];
+    if (ok[r] && c == 0) {
+      const int64_t t = a.p.scalar_at(tp[r], h, (int)row);
+      if (a.p.weight) a.p.weight[t] = weight[r];
+      if (a.p.position) a.p.position[t] = position[r];
+      if (a.p.k_scale) a.p.k_scale[t] = ks[r], a.p.v_scale[t] = vs[r];
     }
   }
 }
@@ -400,7 +490,7 @@ int launch_append(const AppendArgs& a, int dtype, hipStream_t stream) {
       hipLaunchKernelGGL((kv_append_kernel<X, int8_t>), grid, block, 0, stream, a, lpr);
     CORTEX_CHECK_LAUNCH("kv_append_kernel");
   }
-  if (a.offsets && a.new_lengths) {
+  if (a.offsets && a.new_lengths && (a.T == 0 || a.new_lengths == a.lengths)) {
     hipLaunchKernelGGL(kv_lengths_kernel, dim3((unsigned)cdiv(a.B, 256)), block, 0, stream, a);
     CORTEX_CHECK_LAUNCH("kv_lengths_kernel");
   }
@@ -476,10 +566,17 @@ extern "C" int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, con
   a.new_lengths = new_lengths;
   a.err = err;
   const dim3 grid((unsigned)(B * pages->kv_heads));
-  if (a.max_length <= EP_FEW)
-    hipLaunchKernelGGL(kv_evict_plan_kernel<EP_FEW>, grid, dim3(EP_THREADS), 0, stream, a);
+  // the runs of eight slots that the longest sequence has for each thread
+  if (a.max_length <= 8 * 256)
+    hipLaunchKernelGGL((kv_evict_plan_kernel<256, 1>), grid, dim3(256), 0, stream, a);
+  else if (a.max_length <= 8 * 1024)
+    hipLaunchKernelGGL((kv_evict_plan_kernel<1024, 1>), grid, dim3(1024), 0, stream, a);
+  else if (a.max_length <= 2 * 8 * 1024)
+    hipLaunchKernelGGL((kv_evict_plan_kernel<1024, 2>), grid, dim3(1024), 0, stream, a);
+  else if (a.max_length <= 4 * 8 * 1024)
+    hipLaunchKernelGGL((kv_evict_plan_kernel<1024, 4>), grid, dim3(1024), 0, stream, a);
   else
-    hipLaunchKernelGGL(kv_evict_plan_kernel<EP_MANY>, grid, dim3(EP_THREADS), 0, stream, a);
+    hipLaunchKernelGGL((kv_evict_plan_kernel<1024, 0>), grid, dim3(1024), 0, stream, a);
   CORTEX_CHECK_LAUNCH("kv_evict_plan_kernel");
   return OK;
 }
