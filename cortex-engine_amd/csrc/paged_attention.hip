@@ -25,14 +25,17 @@
 namespace cortex {
 namespace {
 
-constexpr int PA_KT = 32;       // keys per tile
+constexpr int PA_KT = 32;       // keys of one matrix product
+// Keys a wavefront takes at a time, so that its loads in flight are 16 KiB: two products' worth where a row is 128
+// bytes or fewer, one where it is more.
+__host__ __device__ constexpr int tile_products(int dhp, int es) { return dhp * es <= 128 ? 2 : 1; }
 constexpr int PA_WAVES = 4;     // wavefronts of a workgroup that takes a share
 constexpr int PA_MORE = 8;      // and of one that has a CU to itself and takes a whole unit
 constexpr int PA_ROWS = 16;     // query heads of a unit
 constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
 constexpr int PA_PER_CU = 2;    // workgroups
 constexpr int PA_MAX_SHARES = 1024;
-constexpr int PA_ONE_TILES = 32;  // tiles of a unit up to which a workgroup takes the whole of it
+constexpr int PA_ONE_KEYS = 1024;  // length up to which a workgroup takes a whole unit
 constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before the sums are rescaled: p <= 2^8
 
 struct PagedArgs {
@@ -41,6 +44,7 @@ struct PagedArgs {
   int row_tiles;        // units a key head: ceil(group / PA_ROWS)
   int units;            // units a sequence: kv_heads * row_tiles
   int shares;
+  int kt;               // keys per tile
   const void* q;
   int64_t q_sb, q_sh;
   const int64_t* lengths;
@@ -93,9 +97,8 @@ __device__ __forceinline__ float group_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-__device__ __forceinline__ int tiles_of(const PagedArgs& a, int b) {
-  bool ok;
-  return (int)((a.p.length_of(a.lengths, b, a.max_length, &ok) + PA_KT - 1) / PA_KT);
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, int b, bool* ok) {
+  return (int)((a.p.length_of(a.lengths, b, a.max_length, ok) + a.kt - 1) / a.kt);
 }
 
 __device__ __forceinline__ int wave_scan_int(int v, int lane) {  // inclusive
@@ -127,6 +130,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
   constexpr int E = DHP / 16;           // dims of a value row a lane: d = E r
   constexpr int VW = E * ES / 4;
   constexpr int LD = DHP + 4;
+  constexpr int NT = tile_products(DHP, ES), KT = NT * PA_KT;
   constexpr int THREADS = 64 * WAVES;
   __shared__ __attribute__((aligned(16))) float so[WAVES][PA_ROWS][LD];
   __shared__ float sm[WAVES][PA_ROWS], sl[WAVES][PA_ROWS];
@@ -143,7 +147,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
   } else {
     int total = 0;
     for (int i = lane; i < a.B; i += 64) {
-      total += (int)((p.length_of(a.lengths, i, a.max_length, &ok) + PA_KT - 1) / PA_KT);
+      total += tiles_of(a, i, &ok);
     }
     if (blockIdx.x == 0 && !ok) kv_flag(a.err);
     total = wave_sum_int(total) * a.units;
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
     t1 = min(total, t0 + per);
     if (t0 >= t1) return;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int v = b0 + lane < a.B ? tiles_of(a, b0 + lane) * a.units : 0;
+      const int v = b0 + lane < a.B ? tiles_of(a, b0 + lane, &ok) * a.units : 0;
       const int inc = wave_scan_int(v, lane);
       const uint64_t past = __ballot(inc > off);
       if (past) {
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
 
   while (t0 < t1 && b < a.B) {
     const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
-    const int tiles = (int)((n + PA_KT - 1) / PA_KT);
+    const int tiles = (int)((n + KT - 1) / KT);
     if (!ONE && off >= tiles * a.units) {  // done, or empty
       ++b;
       off = 0;
@@ -203,41 +207,59 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
     // the page ids of this lane's 8 keys of a tile: for the key rows (8 (r / 4) ..) and the value rows (8 g ..)
     const int last = (int)p.max_slots - 1;  // (not the last key: the lookups need not wait for the length)
     auto page_at = [&](int j) { return table[min(j, last) >> p.shift]; };
-    auto kblock = [&](int t) { return t * PA_KT + 8 * (fr >> 2); };
-    auto vblock = [&](int t) { return t * PA_KT + 8 * g; };
+    auto kblock = [&](int t, int u) { return t * KT + u * PA_KT + 8 * (fr >> 2); };
+    auto vblock = [&](int t, int u) { return t * KT + u * PA_KT + 8 * g; };
+    auto in_pool = [&](int page) { return (int64_t)((uint32_t)page < (uint32_t)p.num_pages ? page : 0); };
 
-    Words<4> kr[2][NK];
-    Words<VW> vr[8];
-    float4 ks[2], vs[2];
-    auto load_k = [&](int t, int page) {
-      const int64_t at = (int64_t)((uint32_t)page < (uint32_t)p.num_pages ? page : 0) * p.k_page;
+    struct Ids {
+      int k[NT], v[NT];
+    };
+    auto ids_of = [&](int t) {
+      Ids x;
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const int row = (kblock(t) & mask) + 4 * st + (fr & 3);
-        const char* src = kbase + (at + row * p.k_slot) * ES;
+      for (int u = 0; u < NT; ++u) x.k[u] = page_at(kblock(t, u)), x.v[u] = page_at(vblock(t, u));
+      return x;
+    };
+    Words<4> kr[NT][2][NK];
+    Words<VW> vr[NT][8];
+    f32x4 ks[NT][2], vs[NT][2];
+    auto load_k = [&](int t, const Ids& ids) {
 #pragma unroll
-        for (int c = 0; c < NK; ++c) {
-          const int d = c * 4 * CE + g * CE;
-          kr[st][c] = load_words<4>(src + (!PAD || d < Dh ? d : 0) * ES);
-          if (PAD && d >= Dh) kr[st][c] = Words<4>{{0u, 0u, 0u, 0u}};
+      for (int u = 0; u < NT; ++u) {
+        const int64_t at = in_pool(ids.k[u]) * p.k_page;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const int row = (kblock(t, u) & mask) + 4 * st + (fr & 3);
+          const char* src = kbase + (at + row * p.k_slot) * ES;
+#pragma unroll
+          for (int c = 0; c < NK; ++c) {
+            const int d = c * 4 * CE + g * CE;
+            kr[u][st][c] = load_words<4>(src + (!PAD || d < Dh ? d : 0) * ES);
+          }
         }
       }
     };
-    auto load_v = [&](int t, int page) {
-      const int64_t pg = (uint32_t)page < (uint32_t)p.num_pages ? page : 0;
-      const int row = vblock(t) & mask;
-      const int d = !PAD || fr * E < Dh ? fr * E : 0;
-      const char* src = vbase + (pg * p.v_page + row * p.v_slot + d) * ES;
+    auto load_v = [&](int t, const Ids& ids) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) vr[i] = load_words<VW>(src + i * p.v_slot * ES);
+      for (int u = 0; u < NT; ++u) {
+        const int64_t page = in_pool(ids.v[u]);
+        const int row = vblock(t, u) & mask;
+        const int d = !PAD || fr * E < Dh ? fr * E : 0;
+        const char* src = vbase + (page * p.v_page + row * p.v_slot + d) * ES;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vr[u][i] = load_words<VW>(src + i * p.v_slot * ES);
+      }
     };
-    auto load_scales = [&](int t, int page) {
+    auto load_scales = [&](int t, const Ids& ids) {
       if constexpr (ES == 1) {
-        const int64_t i = p.scalar_at((uint32_t)page < (uint32_t)p.num_pages ? page : 0, h, vblock(t) & mask);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          ks[x] = reinterpret_cast<const float4*>(p.k_scale + i)[x];
-          vs[x] = reinterpret_cast<const float4*>(p.v_scale + i)[x];
+        for (int u = 0; u < NT; ++u) {
+          const int64_t i = p.scalar_at((int)in_pool(ids.v[u]), h, vblock(t, u) & mask);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            ks[u][x] = reinterpret_cast<const f32x4*>(p.k_scale + i)[x];
+            vs[u][x] = reinterpret_cast<const f32x4*>(p.v_scale + i)[x];
+          }
         }
       }
     };
@@ -248,77 +270,88 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
     for (int j = 0; j < E; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
     int t = ta + wid;
-    int kp = 0, vp = 0;
-    if (last >= 0) kp = page_at(kblock(t)), vp = page_at(vblock(t));  // (a table may have no columns)
+    Ids id = {};
+    if (last >= 0) id = ids_of(t);  // (a table may have no columns)
     if (t < tb) {
-      load_k(t, kp);
-      load_v(t, vp);
-      load_scales(t, vp);
-      int kp1 = page_at(kblock(t + WAVES)), vp1 = page_at(vblock(t + WAVES));
+      load_k(t, id);
+      load_scales(t, id);
+      load_v(t, id);
+      Ids id1 = ids_of(t + WAVES);
       for (; t < tb; t += WAVES) {
-        const int kp2 = page_at(kblock(t + 2 * WAVES)), vp2 = page_at(vblock(t + 2 * WAVES));
+        const Ids id2 = ids_of(t + 2 * WAVES);
         const bool more = t + WAVES < tb;
-        // scores of keys 8 g + 4 st + i for query fr
-        f32x4 s[2];
+        // scores of keys 8 g + 4 st + i (of product u) for query fr
+        f32x4 x[NT][2];
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          s[st] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-          for (int c = 0; c < NK; ++c) {
-            if constexpr (ES == 2) {
-              bf16x8 qf;
-              __builtin_memcpy(&qf, q[c], 16);
-              s[st] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[st][c]), qf, s[st], 0, 0, 0);
-            } else if constexpr (ES == 4) {
+          for (int st = 0; st < 2; ++st) {
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s[st] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[st][c].w[e]), q[c][e], s[st], 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
+            for (int c = 0; c < NK; ++c) {
+              Words<4> kk = kr[u][st][c];
+              if (PAD && c * 4 * CE + g * CE >= Dh) kk = Words<4>{{0u, 0u, 0u, 0u}};  // (the query is 0 there, the key maybe not finite)
+              if constexpr (ES == 2) {
                 bf16x8 qf;
-                __builtin_memcpy(&qf, q[c] + 8 * e, 16);
-                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    widen_i8x8(make_uint2(kr[st][c].w[2 * e], kr[st][c].w[2 * e + 1])), qf, s[st], 0, 0, 0);
+                __builtin_memcpy(&qf, q[c], 16);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), qf, s, 0, 0, 0);
+              } else if constexpr (ES == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk.w[e]), q[c][e], s, 0, 0, 0);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  bf16x8 qf;
+                  __builtin_memcpy(&qf, q[c] + 8 * e, 16);
+                  s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_i8x8(make_uint2(kk.w[2 * e], kk.w[2 * e + 1])), qf, s,
+                                                              0, 0, 0);
+                }
               }
             }
+            x[u][st] = s * a.scale_log2;
+            if constexpr (ES == 1) x[u][st] *= ks[u][st];
           }
-        }
-        const float4 ks0 = ks[0], ks1 = ks[1];
-        if (more) load_k(t + WAVES, kp1);
+        if (more) load_k(t + WAVES, id1);
         __builtin_amdgcn_sched_barrier(0);
 
-        // how many of this lane's 8 keys there are
-        const bool page_ok = (uint32_t)vp < (uint32_t)p.num_pages;
-        const int left = page_ok ? (int)n - vblock(t) : 0;
-        float x[8];
+        // where not all of this lane's 8 keys (of each product) are there
+        bool whole = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * a.scale_log2;
-        if constexpr (ES == 1) {
-          const float sc[8] = {ks0.x, ks0.y, ks0.z, ks0.w, ks1.x, ks1.y, ks1.z, ks1.w};
+        for (int u = 0; u < NT; ++u)
+          whole = whole && (uint32_t)id.v[u] < (uint32_t)p.num_pages && (int)n - vblock(t, u) >= 8;
+        if (!__all(whole)) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= sc[i];
-        }
-        const bool whole = __all(left >= 8);
-        if (!whole) {
-          if (!page_ok && fr == 0 && vblock(t) < (int)n) kv_flag(a.err);
+          for (int u = 0; u < NT; ++u) {
+            const bool page_ok = (uint32_t)id.v[u] < (uint32_t)p.num_pages;
+            const int left = page_ok ? (int)n - vblock(t, u) : 0;
+            if (!page_ok && fr == 0 && vblock(t, u) < (int)n) kv_flag(a.err);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (i >= left) {  // (what these rows hold is not looked at: 0 times it may be NaN)
-              x[i] = -INFINITY;
-              vr[i] = Words<VW>{};
-              if constexpr (ES == 1) reinterpret_cast<float*>(vs)[i] = 0.0f;
+            for (int i = 0; i < 8; ++i) {
+              if (i >= left) {  // (what these rows hold is not looked at: 0 times it may be NaN)
+                x[u][i >> 2][i & 3] = -INFINITY;
+                vr[u][i] = Words<VW>{};
+                if constexpr (ES == 1) vs[u][i >> 2][i & 3] = 0.0f;
+              }
             }
           }
         }
         if constexpr (W) {
           if (fr < rows) {
-            float* to = a.score + ((int64_t)b * a.heads + head0 + fr) * a.score_ld + vblock(t);
-            reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+              float* to = a.score + ((int64_t)b * a.heads + head0 + fr) * a.score_ld + vblock(t, u);
+              reinterpret_cast<f32x4*>(to)[0] = x[u][0];
+              reinterpret_cast<f32x4*>(to)[1] = x[u][1];
+            }
           }
         }
-        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int st = 0; st < 2; ++st)
+            top = fmaxf(top, fmaxf(fmaxf(x[u][st][0], x[u][st][1]), fmaxf(x[u][st][2], x[u][st][3])));
         top = group_max(top);
         if (__any(top > m + PA_RESCALE)) {  // (m -inf: the first key)
           const float m_new = fmaxf(m, top);
@@ -329,63 +362,65 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
           m = m_new;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        float pr[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(x[i] - ref);
-        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+        for (int u = 0; u < NT; ++u) {
+          float pr[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(x[u][i >> 2][i & 3] - ref);
+          l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
 
-        // O^T += V^T P^T; product j: dims E (4 g + i) + j of query fr
-        if constexpr (ES == 4) {
+          // O^T += V^T P^T; product j: dims E (4 g + i) + j of query fr
+          if constexpr (ES == 4) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-              o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i].w[j]), pr[i], o[j], 0, 0, 0);
-        } else {
-          if constexpr (ES == 1) {
-            const float sc[8] = {vs[0].x, vs[0].y, vs[0].z, vs[0].w, vs[1].x, vs[1].y, vs[1].z, vs[1].w};
+              for (int j = 0; j < E; ++j)
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[u][i].w[j]), pr[i], o[j], 0, 0, 0);
+          } else {
+            if constexpr (ES == 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) pr[i] *= sc[i];
-          }
-          // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
-          // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
-          // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
-          bf16x8 hi, lo;
-          uint32_t hw[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            hw[i] = __builtin_amdgcn_perm(__float_as_uint(pr[2 * i + 1]), __float_as_uint(pr[2 * i]), 0x07060302u);
-          __builtin_memcpy(&hi, hw, 16);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float rest = pr[i] - __uint_as_float(__float_as_uint(pr[i]) & 0xffff0000u);
-            lo[i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
-          }
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            bf16x8 vf;
-            if constexpr (ES == 2) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[j >> 1], vr[2 * i].w[j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
-              __builtin_memcpy(&vf, w, 16);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[i].w[j >> 2] >> (8 * (j & 3)));
+              for (int i = 0; i < 8; ++i) pr[i] *= vs[u][i >> 2][i & 3];
             }
-            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi, o[j], 0, 0, 0);
-            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo, o[j], 0, 0, 0);
+            // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
+            // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
+            // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
+            bf16x8 hi, lo;
+            uint32_t hw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              hw[i] = __builtin_amdgcn_perm(__float_as_uint(pr[2 * i + 1]), __float_as_uint(pr[2 * i]), 0x07060302u);
+            __builtin_memcpy(&hi, hw, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float rest = pr[i] - __uint_as_float(__float_as_uint(pr[i]) & 0xffff0000u);
+              lo[i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              bf16x8 vf;
+              if constexpr (ES == 2) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  w[i] = __builtin_amdgcn_perm(vr[u][2 * i + 1].w[j >> 1], vr[u][2 * i].w[j >> 1],
+                                               (j & 1) ? 0x07060302u : 0x05040100u);
+                __builtin_memcpy(&vf, w, 16);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[u][i].w[j >> 2] >> (8 * (j & 3)));
+              }
+              o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi, o[j], 0, 0, 0);
+              o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo, o[j], 0, 0, 0);
+            }
           }
         }
         if (more) {
-          load_v(t + WAVES, vp1);
-          load_scales(t + WAVES, vp1);
+          load_scales(t + WAVES, id1);
+          load_v(t + WAVES, id1);
         }
         __builtin_amdgcn_sched_barrier(0);
-        vp = vp1;
-        kp1 = kp2;
-        vp1 = vp2;
+        id = id1;
+        id1 = id2;
       }
     }
 
@@ -449,31 +484,37 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
 
 constexpr int PJ_THREADS = 256;
 constexpr int PJ_KEYS = 4 * PJ_THREADS;  // keys a workgroup adds the weight of
+constexpr int PJ_AHEAD = 8;              // loads issued before the factors that they are multiplied by are known
 
 // The parts of the units that several shares hold, joined in the order of their keys (0 for a sequence without keys),
-// and with W the weight that every key received, sum over the query heads of a key head of p_j.  `chunks` workgroups a
-// (sequence, key head): number c takes the query heads c, c + chunks, .. and the keys PJ_KEYS c ...  The (m, l) of the
-// parts are small: every workgroup that needs them reads them itself.
+// and with W the weight that every key received, sum over the query heads of a key head of p_j.  Of a (sequence, key
+// head) the first `chunks` workgroups take PJ_KEYS keys' weights each, the others a query head each.  The (m, l) of
+// the parts are small: every workgroup that needs them reads them itself.  A chain of round trips (lengths, parts, and
+// with W the scores): what does not depend on the one before is loaded beside it.
 template <class Q, int DHP, bool W>
 __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int chunks) {
   constexpr int64_t SLOT = PA_ROWS * (DHP + 2);
   constexpr int GROUPS = PJ_THREADS / DHP;  // parts summed side by side
-  __shared__ float share[PA_MAX_SHARES];      // a part's factor
+  __shared__ float share[PA_MAX_SHARES];    // a part's factor
   __shared__ float sums[GROUPS][DHP];
   __shared__ float red[2][PJ_THREADS / 64];
-  __shared__ float2 stat[1024];
+  __shared__ float2 stat[W ? 1024 : 1];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int bh = blockIdx.x / chunks, c = blockIdx.x - bh * chunks;
+  const int per_head = chunks + a.group;
+  const int bh = blockIdx.x / per_head, c = blockIdx.x - bh * per_head;
   const int b = bh / a.p.kv_heads, h = bh - b * a.p.kv_heads;
+  bool ok;
+  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
+  if (W && c < chunks && (int64_t)c * PJ_KEYS >= n) return;
   int total = 0, before = 0;
   for (int i = lane; i < a.B; i += 64) {
-    const int n = tiles_of(a, i);
-    total += n;
-    before += i < b ? n : 0;
+    const int x = tiles_of(a, i, &ok);
+    total += x;
+    before += i < b ? x : 0;
   }
   total = wave_sum_int(total) * a.units;
   before = wave_sum_int(before) * a.units;
-  const int tiles = tiles_of(a, b);
+  const int tiles = (int)((n + a.kt - 1) / a.kt);
   const int per = share_of(a, total);
   // the shares w0 .. w1 that hold the unit of query head i
   auto unit_of = [&](int i, int* w0, int* w1) {
@@ -481,22 +522,31 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
     *w0 = s / per, *w1 = (s + tiles - 1) / per;
   };
   auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * SLOT; };
-  Q* out = reinterpret_cast<Q*>(a.out) + b * a.o_sb + (int64_t)h * a.group * a.o_sh;
 
-  for (int i = c; i < a.group; i += chunks) {
+  if (!W || c >= chunks) {
+    const int i = c - chunks, r = i % PA_ROWS;
+    Q* out = reinterpret_cast<Q*>(a.out) + b * a.o_sb + (int64_t)(h * a.group + i) * a.o_sh;
     if (tiles == 0) {
-      if (tid < a.p.head_dim) out[i * a.o_sh + tid] = from_f32<Q>(0.0f);
-      continue;
+      if (tid < a.p.head_dim) out[tid] = from_f32<Q>(0.0f);
+      return;
     }
     int w0, w1;
     unit_of(i, &w0, &w1);
-    if (w0 == w1) continue;  // written by its one workgroup
-    const int r = i % PA_ROWS, parts = w1 - w0 + 1;
-    float top = -INFINITY;
+    if (w0 == w1) return;  // written by its one workgroup
+    const int parts = w1 - w0 + 1;
+    const int d = tid % DHP, group = tid / DHP;
+    float ahead[PJ_AHEAD];
+#pragma unroll
+    for (int x = 0; x < PJ_AHEAD; ++x) {
+      const int w = group + x * GROUPS;
+      ahead[x] = w < parts ? slot(w0 + w, w0)[r * DHP + d] : 0.0f;
+    }
+    float top = -INFINITY, l0 = 0.0f;
     for (int w = tid; w < parts; w += PJ_THREADS) {
-      const float m = slot(w0 + w, w0)[PA_ROWS * DHP + r];
-      share[w] = m;
-      top = fmaxf(top, m);
+      const float* x = slot(w0 + w, w0) + PA_ROWS * DHP + r;
+      share[w] = x[0];
+      top = fmaxf(top, x[0]);
+      if (w == tid) l0 = x[PA_ROWS];
     }
     top = wave_max(top);
     if (lane == 0) red[0][wid] = top;
@@ -507,31 +557,39 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
     for (int w = tid; w < parts; w += PJ_THREADS) {
       const float f = exp2f(share[w] - ref);
       share[w] = f;
-      sum += f * slot(w0 + w, w0)[PA_ROWS * (DHP + 1) + r];
+      sum += f * (w == tid ? l0 : slot(w0 + w, w0)[PA_ROWS * (DHP + 1) + r]);
     }
     sum = wave_sum(sum);
     if (lane == 0) red[1][wid] = sum;
     __syncthreads();
     sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const int d = tid % DHP, group = tid / DHP;
     float acc = 0.0f;
+#pragma unroll
+    for (int x = 0; x < PJ_AHEAD; ++x)
+      if (group + x * GROUPS < parts) acc += share[group + x * GROUPS] * ahead[x];
 #pragma unroll 8
-    for (int w = group; w < parts; w += GROUPS) acc += share[w] * slot(w0 + w, w0)[r * DHP + d];
+    for (int w = group + PJ_AHEAD * GROUPS; w < parts; w += GROUPS) acc += share[w] * slot(w0 + w, w0)[r * DHP + d];
     sums[group][d] = acc;
     __syncthreads();
     if (tid < a.p.head_dim) {
       acc = sums[0][tid];
 #pragma unroll
       for (int x = 1; x < GROUPS; ++x) acc += sums[x][tid];
-      out[i * a.o_sh + tid] = from_f32<Q>(acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
+      out[tid] = from_f32<Q>(acc * (sum == 0.0f ? 0.0f : 1.0f / sum));
     }
-    __syncthreads();  // before the next head's factors
+    return;
   }
 
   if constexpr (W) {
-    bool ok;
-    const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok), j = (int64_t)c * PJ_KEYS + 4 * tid;
-    if ((int64_t)c * PJ_KEYS >= n) return;
+    const int64_t j = (int64_t)c * PJ_KEYS + 4 * tid, at = j < n ? j : 0;
+    const float* score = a.score + ((int64_t)b * a.heads + h * a.group) * a.score_ld + at;
+    f32x4 ahead[PJ_AHEAD];
+#pragma unroll
+    for (int i = 0; i < PJ_AHEAD; ++i)
+      ahead[i] = *reinterpret_cast<const f32x4*>(score + (i < a.group ? i : 0) * a.score_ld);
+    const int page = a.p.page_of(b, at);  // (four keys of one page)
+    f32x4* weight = reinterpret_cast<f32x4*>(a.p.weight + a.p.scalar_at(page < 0 ? 0 : page, h, a.p.row_of(at)));
+    const f32x4 old = *weight;
     // m and 1 / l of the query heads, a wavefront each
     for (int i = wid; i < a.group; i += PJ_THREADS / 64) {
       int w0, w1;
@@ -553,30 +611,28 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
       if (lane == 0) stat[i] = make_float2(ref, sum == 0.0f ? 0.0f : 1.0f / sum);
     }
     __syncthreads();
-    if (j >= n) return;
-    const float* score = a.score + ((int64_t)b * a.heads + h * a.group) * a.score_ld + j;
-    float add[4] = {};
-#pragma unroll 4
-    for (int i = 0; i < a.group; ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(score + i * a.score_ld);
-      const float2 s = stat[i];
-      add[0] += exp2f(x.x - s.x) * s.y;
-      add[1] += exp2f(x.y - s.x) * s.y;
-      add[2] += exp2f(x.z - s.x) * s.y;
-      add[3] += exp2f(x.w - s.x) * s.y;
-    }
-    const int page = a.p.page_of(b, j);  // four keys of one page
-    if (page < 0) return;
-    float* weight = a.p.weight + a.p.scalar_at(page, h, a.p.row_of(j));
+    f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto head = [&](const f32x4& x, const float2 s) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (j + x < n) weight[x] += add[x];
+      for (int e = 0; e < 4; ++e) add[e] += exp2f(x[e] - s.x) * s.y;
+    };
+#pragma unroll
+    for (int i = 0; i < PJ_AHEAD; ++i)
+      if (i < a.group) head(ahead[i], stat[i]);
+#pragma unroll 4
+    for (int i = PJ_AHEAD; i < a.group; ++i) head(*reinterpret_cast<const f32x4*>(score + i * a.score_ld), stat[i]);
+    if (j >= n || page < 0) return;
+    if (j + 4 <= n) {
+      *weight = old + add;
+    } else {
+      for (int e = 0; j + e < n; ++e) reinterpret_cast<float*>(weight)[e] = old[e] + add[e];
+    }
   }
 }
 
 // How a call is laid out: shares, and the parts of its workspace in bytes.
 struct Layout {
-  int row_tiles, units, shares, dhp;
+  int row_tiles, units, shares, dhp, kt;
   int waves;  // of a workgroup that takes a whole unit; 0: shares
   int64_t score_ld, part, score, stats;
 };
@@ -586,13 +642,14 @@ Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t mos
   y.row_tiles = (int)cdiv(group, PA_ROWS);
   y.units = (int)(p->kv_heads * y.row_tiles);
   y.dhp = p->head_dim <= 64 ? 64 : 128;
-  const int64_t tiles = B * y.units * cdiv(most, PA_KT);
+  y.kt = PA_KT * tile_products(y.dhp, p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1);
+  const int64_t tiles = B * y.units * cdiv(most, y.kt);
   const int64_t shares = cdiv(tiles, PA_MIN_TILES), cus = cu_count();
   const int64_t slots = cus * PA_PER_CU < PA_MAX_SHARES ? cus * PA_PER_CU : PA_MAX_SHARES;
   y.shares = (int)(shares < 1 ? 1 : shares < slots ? shares : slots);
-  y.score_ld = cdiv(most, PA_KT) * PA_KT;
+  y.score_ld = cdiv(most, y.kt) * y.kt;
   y.waves = 0;
-  if (cdiv(most, PA_KT) <= PA_ONE_TILES && (!accumulate || y.row_tiles == 1))
+  if (most <= PA_ONE_KEYS && (!accumulate || y.row_tiles == 1))
     y.waves = B * y.units > cus ? PA_WAVES : PA_MORE;
   y.part = y.waves ? 0 : 2ll * y.shares * PA_ROWS * (y.dhp + 2) * 4;
   y.score = accumulate ? B * heads * y.score_ld * 4 : 0;
@@ -620,11 +677,9 @@ int launch(const PagedArgs& a, int waves, hipStream_t stream) {
   }
   launch_main<P, DHP, W, PA_WAVES, false>(a, (unsigned)a.shares, stream);
   CORTEX_CHECK_LAUNCH("paged_attention_kernel");
-  int64_t chunks = a.group;
-  if (W) chunks = cdiv(a.max_length, PJ_KEYS);
-  if (chunks < 1) chunks = 1;
-  hipLaunchKernelGGL((paged_join_kernel<typename Query<P>::type, DHP, W>), dim3((unsigned)(chunks * a.B * a.p.kv_heads)),
-                     dim3(PJ_THREADS), 0, stream, a, (int)chunks);
+  const int64_t chunks = W ? cdiv(a.max_length, PJ_KEYS) : 0;
+  hipLaunchKernelGGL((paged_join_kernel<typename Query<P>::type, DHP, W>),
+                     dim3((unsigned)((chunks + a.group) * a.B * a.p.kv_heads)), dim3(PJ_THREADS), 0, stream, a, (int)chunks);
   CORTEX_CHECK_LAUNCH("paged_join_kernel");
   return OK;
 }
@@ -692,6 +747,7 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   a.row_tiles = y.row_tiles;
   a.units = y.units;
   a.shares = y.shares;
+  a.kt = y.kt;
   a.q = q;
   a.q_sb = q_sb;
   a.q_sh = q_sh;

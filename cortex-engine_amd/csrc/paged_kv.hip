@@ -63,16 +63,24 @@ struct AppendArgs {
   int32_t* err;
 };
 
-// Eight values of a row a lane.
-__device__ __forceinline__ void load8(float (&f)[8], const float* p) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-}
-__device__ __forceinline__ void load8(float (&f)[8], const bf16* p) {
-  const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+// Eight values of a row as they are loaded, and as numbers.
+template <class X>
+struct Eight {
+  i32x4 w[sizeof(X) / 2];
+  __device__ __forceinline__ void load(const X* p) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = (float)a[j];
-}
+    for (int i = 0; i < (int)sizeof(X) / 2; ++i) w[i] = reinterpret_cast<const i32x4*>(p)[i];
+  }
+  __device__ __forceinline__ void numbers(float (&f)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (sizeof(X) == 4)
+        f[j] = __int_as_float(w[j >> 2][j & 3]);
+      else
+        f[j] = __int_as_float((j & 1) ? (w[0][j >> 1] & 0xffff0000) : (w[0][j >> 1] << 16));
+    }
+  }
+};
 __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -95,88 +103,108 @@ __device__ void lengths_after(const AppendArgs& a, int at, int threads) {
   }
 }
 
-// The sequence of token t: how many of offsets[1 .. B] are <= t.  The lanes of a wavefront look at 64 of them a
-// round, so the round trips are one for up to 64 sequences and two for up to 4096.
-__device__ int64_t sequence_of(const int64_t* offsets, int64_t B, int64_t t, int lane) {
+// The sequence of token t: how many of offsets[1 .. B] are <= t.
+__device__ int64_t sequence_of(const int64_t* offsets, int64_t B, int64_t t) {
   int64_t lo = 0, hi = B;
   while (lo < hi) {
-    const int64_t step = (hi - lo + 63) >> 6, i = lo + (lane + 1) * step;
-    const int64_t past = __builtin_popcountll(__ballot(i <= hi && offsets[i <= hi ? i : hi] <= t));
-    lo += past * step;
-    hi = min(hi, lo + step - 1);
+    const int64_t mid = (lo + hi) >> 1;
+    if (offsets[mid + 1] <= t)
+      lo = mid + 1;
+    else
+      hi = mid;
   }
   return lo;
 }
 
-// One workgroup a token; `lpr` lanes a (key or value, head) row, eight values each.  The rows are loaded before the
-// place is known that they go to: the lookups (offsets, length, table) are a chain of round trips as long as the load.
+constexpr int AP_TOKENS = 64;  // tokens of a workgroup, at most
+constexpr int AP_AHEAD = 4;    // values in flight, in eights a thread
+
+// A workgroup takes `tokens` tokens, a thread eight values of a (token, key or value, head) row; `lpr` lanes a row.  The
+// first threads look up where the tokens go while the others load the rows.  Bound by HBM for many tokens (16,800 of 8
+// heads x 128, bf16: MEASURE), by the chain of lookups for few.
 template <class X, class P>
-__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr) {
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr, int tokens) {
+  __shared__ int at_page[AP_TOKENS], at_row[AP_TOKENS], at_slot[AP_TOKENS];
   const int tid = threadIdx.x;
   const KvPages& p = a.p;
-  const int64_t t = blockIdx.x;
-  const int d = (tid % lpr) * 8;
-  const int rows = 2 * p.kv_heads, step = 256 / lpr;
-  float f[8];
-  auto load = [&](int r) {
-    if (r < rows && d < p.head_dim)
-      load8(f, reinterpret_cast<const X*>((r & 1) ? a.v : a.k) + t * ((r & 1) ? a.v_st : a.k_st) +
-                   (r >> 1) * ((r & 1) ? a.v_sh : a.k_sh) + d);
-  };
-  load(tid / lpr);
-  int64_t b = t, first = t;
-  if (a.offsets) {
-    if (blockIdx.x == 0 && a.new_lengths != a.lengths) lengths_after(a, tid, 256);
-    b = sequence_of(a.offsets, a.B, t, tid & 63);
-    if (b >= a.B) return;  // behind the last sequence
-    first = a.offsets[b];
-    if (t < first) return;  // before the first
+  const int64_t t0 = (int64_t)blockIdx.x * tokens;
+  const int count = (int)min((int64_t)tokens, a.T - t0);
+  if (a.offsets && blockIdx.x == 0 && a.new_lengths != a.lengths) lengths_after(a, tid, 256);
+  if (tid < count) {
+    const int64_t t = t0 + tid;
+    int64_t b = t, first = t;
+    bool mine = true;
+    if (a.offsets) {
+      b = sequence_of(a.offsets, a.B, t);
+      mine = b < a.B && (first = a.offsets[b]) <= t;  // not behind the last sequence, nor before the first
+    }
+    int page = -1;
+    if (mine) {
+      bool ok = true;
+      const int64_t len = p.length_of(a.lengths, b, p.max_slots, &ok), slot = len + (t - first);
+      page = p.page_of(b, slot);
+      if (!ok || page < 0) kv_flag(a.err);
+      at_row[tid] = p.row_of(slot);
+      at_slot[tid] = (int)slot;
+      // (may be lengths[b], which this thread alone reads: a token a sequence)
+      if (!a.offsets && a.new_lengths) a.new_lengths[b] = min(len + 1, p.max_slots);
+    }
+    at_page[tid] = page;
   }
-  bool ok = true;
-  const int64_t len = p.length_of(a.lengths, b, p.max_slots, &ok);
-  const int64_t slot = len + (t - first);
-  const int page = p.page_of(b, slot);
-  if (tid == 0 && (!ok || page < 0)) kv_flag(a.err);
-  // lengths may be new_lengths: with a token a sequence this workgroup is the only one that reads lengths[b]
-  if (!a.offsets) {
-    __syncthreads();
-    if (tid == 0 && a.new_lengths) a.new_lengths[b] = min(len + 1, p.max_slots);
-  }
-  if (page < 0) return;
-  const int row = p.row_of(slot);
-  for (int r0 = 0; r0 < rows; r0 += step) {  // whole groups of lanes: the shuffles below take all of them
-    const int r = r0 + tid / lpr;
-    const bool in = r < rows && d < p.head_dim;
-    const int h = r >> 1;
-    const bool is_v = r & 1;
-    if (r0 > 0) load(r);
-    const int64_t at = is_v ? page * p.v_page + h * p.v_head + row * p.v_slot : page * p.k_page + h * p.k_head + row * p.k_slot;
-    P* to = reinterpret_cast<P*>(is_v ? p.v : p.k) + at + d;
-    if constexpr (sizeof(P) == 1) {
-      uint32_t most = 0;  // the largest |x|; an infinity or a NaN is above every number's bits
-      if (in)
+  const int rows = 2 * p.kv_heads, per = rows * lpr, items = count * per;
+  const int d = (tid & (lpr - 1)) * 8;  // (256 is a multiple of lpr)
+  bool looked = false;
+  for (int i0 = 0; i0 < items; i0 += 256 * AP_AHEAD) {
+    Eight<X> x[AP_AHEAD];
+#pragma unroll
+    for (int s = 0; s < AP_AHEAD; ++s) {
+      const int i = i0 + 256 * s + tid;
+      if (i < items && d < p.head_dim) {
+        const int k = i / per, r = (i - k * per) / lpr, h = r >> 1;
+        x[s].load((r & 1) ? reinterpret_cast<const X*>(a.v) + (t0 + k) * a.v_st + h * a.v_sh + d
+                          : reinterpret_cast<const X*>(a.k) + (t0 + k) * a.k_st + h * a.k_sh + d);
+      } else {
+        x[s] = Eight<X>{};
+      }
+    }
+    if (!looked) __syncthreads();  // the lookups
+    looked = true;
+#pragma unroll
+    for (int s = 0; s < AP_AHEAD; ++s) {
+      const int i = i0 + 256 * s + tid;
+      if (i0 + 256 * s >= items) break;
+      const int k = min(i / per, count - 1), r = (i - k * per) / lpr, h = r >> 1;
+      const int page = at_page[k], row = at_row[k];
+      const bool in = i < items && d < p.head_dim && page >= 0, is_v = r & 1;
+      float f[8];
+      x[s].numbers(f);
+      const int64_t to = (is_v ? page * p.v_page + h * p.v_head + row * p.v_slot
+                               : page * p.k_page + h * p.k_head + row * p.k_slot) + d;
+      if constexpr (sizeof(P) == 1) {
+        uint32_t most = 0;  // the largest |x|; an infinity or a NaN is above every number's bits
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
-      for (int o = 1; o < lpr; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-      const bool finite = most < 0x7f800000u;
-      const float s = finite ? fmaxf(__uint_as_float(most), 1e-8f) / 127.0f : __uint_as_float(0x7fc00000u);
-      if (in) {
+        for (int o = 1; o < lpr; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+        const bool finite = most < 0x7f800000u;
+        const float s8 = finite ? fmaxf(__uint_as_float(most), 1e-8f) / 127.0f : __uint_as_float(0x7fc00000u);
         union {
           int8_t c[8];
           uint2 u;
         } q;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q.c[j] = finite ? (int8_t)(int)fminf(fmaxf(rintf(f[j] / s), -127.0f), 127.0f) : 0;
-        *reinterpret_cast<uint2*>(to) = q.u;
-        if (d == 0) (is_v ? p.v_scale : p.k_scale)[p.scalar_at(page, h, row)] = s;
+        for (int j = 0; j < 8; ++j) q.c[j] = finite ? (int8_t)(int)fminf(fmaxf(rintf(f[j] / s8), -127.0f), 127.0f) : 0;
+        if (in) {
+          *reinterpret_cast<uint2*>(reinterpret_cast<P*>(is_v ? p.v : p.k) + to) = q.u;
+          if (d == 0) (is_v ? p.v_scale : p.k_scale)[p.scalar_at(page, h, row)] = s8;
+        }
+      } else if (in) {
+        store8(reinterpret_cast<P*>(is_v ? p.v : p.k) + to, f);
       }
-    } else if (in) {
-      store8(to, f);
-    }
-    if (in && d == 0 && !is_v) {
-      const int64_t i = p.scalar_at(page, h, row);
-      if (p.weight) p.weight[i] = 0.0f;
-      if (p.position) p.position[i] = (int32_t)(a.positions ? a.positions[t] : slot);
+      if (in && d == 0 && !is_v) {
+        const int64_t e = p.scalar_at(page, h, row);
+        if (p.weight) p.weight[e] = 0.0f;
+        if (p.position) p.position[e] = a.positions ? (int32_t)a.positions[t0 + k] : at_slot[k];
+      }
     }
   }
 }
@@ -480,14 +508,18 @@ int pow2_lanes(int64_t n) {
 template <class X>
 int launch_append(const AppendArgs& a, int dtype, hipStream_t stream) {
   const int lpr = pow2_lanes(a.p.head_dim / 8);
-  const dim3 grid((unsigned)a.T), block(256);
+  // as many tokens a workgroup as its threads have loads in flight for, while every CU gets eight workgroups
+  int64_t tokens = 256 * AP_AHEAD / (2ll * a.p.kv_heads * lpr), spread = a.T / (8 * cu_count());
+  tokens = tokens < spread ? tokens : spread;
+  tokens = tokens < 1 ? 1 : tokens > AP_TOKENS ? AP_TOKENS : tokens;
+  const dim3 grid((unsigned)cdiv(a.T, tokens)), block(256);
   if (a.T > 0) {
     if (dtype == DT_F32)
-      hipLaunchKernelGGL((kv_append_kernel<X, float>), grid, block, 0, stream, a, lpr);
+      hipLaunchKernelGGL((kv_append_kernel<X, float>), grid, block, 0, stream, a, lpr, (int)tokens);
     else if (dtype == DT_BF16)
-      hipLaunchKernelGGL((kv_append_kernel<X, bf16>), grid, block, 0, stream, a, lpr);
+      hipLaunchKernelGGL((kv_append_kernel<X, bf16>), grid, block, 0, stream, a, lpr, (int)tokens);
     else
-      hipLaunchKernelGGL((kv_append_kernel<X, int8_t>), grid, block, 0, stream, a, lpr);
+      hipLaunchKernelGGL((kv_append_kernel<X, int8_t>), grid, block, 0, stream, a, lpr, (int)tokens);
     CORTEX_CHECK_LAUNCH("kv_append_kernel");
   }
   if (a.offsets && a.new_lengths && (a.T == 0 || a.new_lengths == a.lengths)) {
