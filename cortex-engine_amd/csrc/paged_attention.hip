@@ -26,15 +26,17 @@ namespace cortex {
 namespace {
 
 constexpr int PA_KT = 32;       // keys of one matrix product
-// Keys a wavefront takes at a time, so that its loads in flight are 16 KiB: two products' worth where a row is 128
-// bytes or fewer, one where it is more.
-__host__ __device__ constexpr int tile_products(int dhp, int es) { return dhp * es <= 128 ? 2 : 1; }
 constexpr int PA_WAVES = 4;     // wavefronts of a workgroup that takes a share
 constexpr int PA_MORE = 8;      // and of one that has a CU to itself and takes a whole unit
 constexpr int PA_ROWS = 16;     // query heads of a unit
 constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
-constexpr int PA_PER_CU = 2;    // workgroups
+// Workgroups that a CU holds at once, by the registers of a tile: 128 dims 160 to 246, 64 dims in fp32 146, in fewer
+// bits 117.  (64 sequences of 500 .. 3000 keys x 64 dims, bf16: 2 a CU 55.5 us, 4 54.2; 128 dims as 3: 105 -> 110)
+__host__ __device__ constexpr int per_cu(int dhp, int es) { return dhp == 128 ? 2 : es == 4 ? 3 : 4; }
 constexpr int PA_MAX_SHARES = 1024;
+// What it costs to begin a unit (fill and drain the loads, sum up), in tiles: without it the shares of short sequences
+// are the last to end (32 sequences of 150 .. 8003 keys 118 us, 2: 107.1, 4: 107.2, 8: 105.2; one of 8192 16.8, 18.1, 18.6, 18.3)
+constexpr int PA_BEGIN = 4;
 constexpr int PA_ONE_KEYS = 1024;  // length up to which a workgroup takes a whole unit
 constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before the sums are rescaled: p <= 2^8
 
@@ -44,7 +46,6 @@ struct PagedArgs {
   int row_tiles;        // units a key head: ceil(group / PA_ROWS)
   int units;            // units a sequence: kv_heads * row_tiles
   int shares;
-  int kt;               // keys per tile
   const void* q;
   int64_t q_sb, q_sh;
   const int64_t* lengths;
@@ -98,8 +99,11 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 __device__ __forceinline__ int tiles_of(const PagedArgs& a, int b, bool* ok) {
-  return (int)((a.p.length_of(a.lengths, b, a.max_length, ok) + a.kt - 1) / a.kt);
+  return (int)((a.p.length_of(a.lengths, b, a.max_length, ok) + PA_KT - 1) / PA_KT);
 }
+
+// What a unit counts for when the shares are cut: its tiles, and what it costs to begin one.
+__device__ __forceinline__ int work_of(int tiles) { return tiles ? tiles + PA_BEGIN : 0; }
 
 __device__ __forceinline__ int wave_scan_int(int v, int lane) {  // inclusive
 #pragma unroll
@@ -122,7 +126,7 @@ __device__ __forceinline__ int share_of(const PagedArgs& a, int total) {
 
 // ONE: a workgroup takes a whole unit, so that nothing is left to join (short caches); else a share.
 template <class P, int DHP, bool PAD, bool W, int WAVES, bool ONE>
-__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(P)) : 2) void paged_attention_kernel(PagedArgs a) {
   typedef typename Query<P>::type Q;
   constexpr int ES = sizeof(P);
   constexpr int CE = 16 / ES;           // elements of a 16-byte chunk
@@ -130,7 +134,6 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
   constexpr int E = DHP / 16;           // dims of a value row a lane: d = E r
   constexpr int VW = E * ES / 4;
   constexpr int LD = DHP + 4;
-  constexpr int NT = tile_products(DHP, ES), KT = NT * PA_KT;
   constexpr int THREADS = 64 * WAVES;
   __shared__ __attribute__((aligned(16))) float so[WAVES][PA_ROWS][LD];
   __shared__ float sm[WAVES][PA_ROWS], sl[WAVES][PA_ROWS];
@@ -147,16 +150,16 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
   } else {
     int total = 0;
     for (int i = lane; i < a.B; i += 64) {
-      total += tiles_of(a, i, &ok);
+      total += work_of(tiles_of(a, i, &ok));
     }
     if (blockIdx.x == 0 && !ok) kv_flag(a.err);
-    total = wave_sum_int(total) * a.units;
+    total = wave_uniform(wave_sum_int(total)) * a.units;
     const int per = share_of(a, total);
     off = t0 = blockIdx.x * per;
     t1 = min(total, t0 + per);
     if (t0 >= t1) return;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int v = b0 + lane < a.B ? tiles_of(a, b0 + lane, &ok) * a.units : 0;
+      const int v = b0 + lane < a.B ? work_of(tiles_of(a, b0 + lane, &ok)) * a.units : 0;
       const int inc = wave_scan_int(v, lane);
       const uint64_t past = __ballot(inc > off);
       if (past) {
@@ -173,14 +176,18 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
 
   while (t0 < t1 && b < a.B) {
     const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
-    const int tiles = (int)((n + KT - 1) / KT);
-    if (!ONE && off >= tiles * a.units) {  // done, or empty
+    const int tiles = (int)((n + PA_KT - 1) / PA_KT), work = work_of(tiles);
+    if (!ONE && off >= work * a.units) {  // done, or empty
       ++b;
       off = 0;
       continue;
     }
-    const int u = ONE ? blockIdx.x - b * a.units : off / tiles, ta = ONE ? 0 : off - u * tiles;
-    const int tb = ONE ? tiles : min(tiles, ta + (t1 - t0));
+    const int u = ONE ? blockIdx.x - b * a.units : off / work, from = off - u * work;
+    const int step = ONE ? 0 : min(work - from, t1 - t0);
+    const int ta = ONE ? 0 : max(0, from - PA_BEGIN), tb = ONE ? tiles : max(0, from + step - PA_BEGIN);
+    t0 += step;
+    off += step;
+    if (!ONE && ta == tb) continue;
     const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * PA_ROWS;
     const int rows = min(PA_ROWS, a.group - row0);  // query heads of this unit
     const int head0 = h * a.group + row0;
@@ -207,59 +214,45 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
     // the page ids of this lane's 8 keys of a tile: for the key rows (8 (r / 4) ..) and the value rows (8 g ..)
     const int last = (int)p.max_slots - 1;  // (not the last key: the lookups need not wait for the length)
     auto page_at = [&](int j) { return table[min(j, last) >> p.shift]; };
-    auto kblock = [&](int t, int u) { return t * KT + u * PA_KT + 8 * (fr >> 2); };
-    auto vblock = [&](int t, int u) { return t * KT + u * PA_KT + 8 * g; };
+    auto kblock = [&](int t) { return t * PA_KT + 8 * (fr >> 2); };
+    auto vblock = [&](int t) { return t * PA_KT + 8 * g; };
     auto in_pool = [&](int page) { return (int64_t)((uint32_t)page < (uint32_t)p.num_pages ? page : 0); };
 
     struct Ids {
-      int k[NT], v[NT];
+      int k, v;
     };
-    auto ids_of = [&](int t) {
-      Ids x;
-#pragma unroll
-      for (int u = 0; u < NT; ++u) x.k[u] = page_at(kblock(t, u)), x.v[u] = page_at(vblock(t, u));
-      return x;
-    };
-    Words<4> kr[NT][2][NK];
-    Words<VW> vr[NT][8];
-    f32x4 ks[NT][2], vs[NT][2];
+    auto ids_of = [&](int t) { return Ids{page_at(kblock(t)), page_at(vblock(t))}; };
+    Words<4> kr[2][NK];
+    Words<VW> vr[8];
+    f32x4 ks[2], vs[2];
     auto load_k = [&](int t, const Ids& ids) {
+      const int64_t at = in_pool(ids.k) * p.k_page;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        const int64_t at = in_pool(ids.k[u]) * p.k_page;
+      for (int st = 0; st < 2; ++st) {
+        const int row = (kblock(t) & mask) + 4 * st + (fr & 3);
+        const char* src = kbase + (at + row * p.k_slot) * ES;
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const int row = (kblock(t, u) & mask) + 4 * st + (fr & 3);
-          const char* src = kbase + (at + row * p.k_slot) * ES;
-#pragma unroll
-          for (int c = 0; c < NK; ++c) {
-            const int d = c * 4 * CE + g * CE;
-            kr[u][st][c] = load_words<4>(src + (!PAD || d < Dh ? d : 0) * ES);
-          }
+        for (int c = 0; c < NK; ++c) {
+          const int d = c * 4 * CE + g * CE;
+          kr[st][c] = load_words<4>(src + (!PAD || d < Dh ? d : 0) * ES);
         }
       }
     };
     auto load_v = [&](int t, const Ids& ids) {
+      const int64_t page = in_pool(ids.v);
+      const int row = vblock(t) & mask;
+      const int d = !PAD || fr * E < Dh ? fr * E : 0;
+      const char* src = vbase + (page * p.v_page + row * p.v_slot + d) * ES;
 #pragma unroll
-      for (int u = 0; u < NT; ++u) {
-        const int64_t page = in_pool(ids.v[u]);
-        const int row = vblock(t, u) & mask;
-        const int d = !PAD || fr * E < Dh ? fr * E : 0;
-        const char* src = vbase + (page * p.v_page + row * p.v_slot + d) * ES;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vr[u][i] = load_words<VW>(src + i * p.v_slot * ES);
-      }
+      for (int i = 0; i < 8; ++i) vr[i] = load_words<VW>(src + i * p.v_slot * ES);
     };
     auto load_scales = [&](int t, const Ids& ids) {
       if constexpr (ES == 1) {
+        const int64_t i = p.scalar_at((int)in_pool(ids.v), h, vblock(t) & mask);
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          const int64_t i = p.scalar_at((int)in_pool(ids.v[u]), h, vblock(t, u) & mask);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            ks[u][x] = reinterpret_cast<const f32x4*>(p.k_scale + i)[x];
-            vs[u][x] = reinterpret_cast<const f32x4*>(p.v_scale + i)[x];
-          }
+        for (int x = 0; x < 2; ++x) {
+          ks[x] = reinterpret_cast<const f32x4*>(p.k_scale + i)[x];
+          vs[x] = reinterpret_cast<const f32x4*>(p.v_scale + i)[x];
         }
       }
     };
@@ -280,78 +273,64 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
       for (; t < tb; t += WAVES) {
         const Ids id2 = ids_of(t + 2 * WAVES);
         const bool more = t + WAVES < tb;
-        // scores of keys 8 g + 4 st + i (of product u) for query fr
-        f32x4 x[NT][2];
+        // scores of keys 8 g + 4 st + i for query fr
+        f32x4 x[2];
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
+        for (int st = 0; st < 2; ++st) {
+          f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int c = 0; c < NK; ++c) {
+            Words<4> kk = kr[st][c];
+            if (PAD && c * 4 * CE + g * CE >= Dh) kk = Words<4>{{0u, 0u, 0u, 0u}};  // (the query is 0 there, the key maybe not finite)
+            if constexpr (ES == 2) {
+              bf16x8 qf;
+              __builtin_memcpy(&qf, q[c], 16);
+              s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), qf, s, 0, 0, 0);
+            } else if constexpr (ES == 4) {
 #pragma unroll
-            for (int c = 0; c < NK; ++c) {
-              Words<4> kk = kr[u][st][c];
-              if (PAD && c * 4 * CE + g * CE >= Dh) kk = Words<4>{{0u, 0u, 0u, 0u}};  // (the query is 0 there, the key maybe not finite)
-              if constexpr (ES == 2) {
+              for (int e = 0; e < 4; ++e)
+                s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk.w[e]), q[c][e], s, 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
                 bf16x8 qf;
-                __builtin_memcpy(&qf, q[c], 16);
-                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), qf, s, 0, 0, 0);
-              } else if constexpr (ES == 4) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk.w[e]), q[c][e], s, 0, 0, 0);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  bf16x8 qf;
-                  __builtin_memcpy(&qf, q[c] + 8 * e, 16);
-                  s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_i8x8(make_uint2(kk.w[2 * e], kk.w[2 * e + 1])), qf, s,
-                                                              0, 0, 0);
-                }
+                __builtin_memcpy(&qf, q[c] + 8 * e, 16);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_i8x8(make_uint2(kk.w[2 * e], kk.w[2 * e + 1])), qf, s,
+                                                            0, 0, 0);
               }
             }
-            x[u][st] = s * a.scale_log2;
-            if constexpr (ES == 1) x[u][st] *= ks[u][st];
           }
+          x[st] = s * a.scale_log2;
+          if constexpr (ES == 1) x[st] *= ks[st];
+        }
         if (more) load_k(t + WAVES, id1);
         __builtin_amdgcn_sched_barrier(0);
 
-        // where not all of this lane's 8 keys (of each product) are there
-        bool whole = true;
+        // where not all of this lane's 8 keys are there
+        const bool page_ok = (uint32_t)id.v < (uint32_t)p.num_pages;
+        const int left = page_ok ? (int)n - vblock(t) : 0;
+        if (!__all(left >= 8)) {
+          if (!page_ok && fr == 0 && vblock(t) < (int)n) kv_flag(a.err);
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-          whole = whole && (uint32_t)id.v[u] < (uint32_t)p.num_pages && (int)n - vblock(t, u) >= 8;
-        if (!__all(whole)) {
-#pragma unroll
-          for (int u = 0; u < NT; ++u) {
-            const bool page_ok = (uint32_t)id.v[u] < (uint32_t)p.num_pages;
-            const int left = page_ok ? (int)n - vblock(t, u) : 0;
-            if (!page_ok && fr == 0 && vblock(t, u) < (int)n) kv_flag(a.err);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i >= left) {  // (what these rows hold is not looked at: 0 times it may be NaN)
-                x[u][i >> 2][i & 3] = -INFINITY;
-                vr[u][i] = Words<VW>{};
-                if constexpr (ES == 1) vs[u][i >> 2][i & 3] = 0.0f;
-              }
+          for (int i = 0; i < 8; ++i) {
+            if (i >= left) {  // (what these rows hold is not looked at: 0 times it may be NaN)
+              x[i >> 2][i & 3] = -INFINITY;
+              vr[i] = Words<VW>{};
+              if constexpr (ES == 1) vs[i >> 2][i & 3] = 0.0f;
             }
           }
         }
         if constexpr (W) {
           if (fr < rows) {
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-              float* to = a.score + ((int64_t)b * a.heads + head0 + fr) * a.score_ld + vblock(t, u);
-              reinterpret_cast<f32x4*>(to)[0] = x[u][0];
-              reinterpret_cast<f32x4*>(to)[1] = x[u][1];
-            }
+            float* to = a.score + ((int64_t)b * a.heads + head0 + fr) * a.score_ld + vblock(t);
+            reinterpret_cast<f32x4*>(to)[0] = x[0];
+            reinterpret_cast<f32x4*>(to)[1] = x[1];
           }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-          for (int st = 0; st < 2; ++st)
-            top = fmaxf(top, fmaxf(fmaxf(x[u][st][0], x[u][st][1]), fmaxf(x[u][st][2], x[u][st][3])));
+        for (int st = 0; st < 2; ++st)
+          top = fmaxf(top, fmaxf(fmaxf(x[st][0], x[st][1]), fmaxf(x[st][2], x[st][3])));
         top = group_max(top);
         if (__any(top > m + PA_RESCALE)) {  // (m -inf: the first key)
           const float m_new = fmaxf(m, top);
@@ -362,56 +341,53 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
           m = m_new;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
+        float pr[8];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          float pr[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(x[u][i >> 2][i & 3] - ref);
-          l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+        for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] - ref);
+        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
 
-          // O^T += V^T P^T; product j: dims E (4 g + i) + j of query fr
-          if constexpr (ES == 4) {
+        // O^T += V^T P^T; product j: dims E (4 g + i) + j of query fr
+        if constexpr (ES == 4) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 8; ++i)
 #pragma unroll
-              for (int j = 0; j < E; ++j)
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[u][i].w[j]), pr[i], o[j], 0, 0, 0);
-          } else {
-            if constexpr (ES == 1) {
+            for (int j = 0; j < E; ++j)
+              o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i].w[j]), pr[i], o[j], 0, 0, 0);
+        } else {
+          if constexpr (ES == 1) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) pr[i] *= vs[u][i >> 2][i & 3];
+            for (int i = 0; i < 8; ++i) pr[i] *= vs[i >> 2][i & 3];
+          }
+          // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
+          // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
+          // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
+          bf16x8 hi, lo;
+          uint32_t hw[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            hw[i] = __builtin_amdgcn_perm(__float_as_uint(pr[2 * i + 1]), __float_as_uint(pr[2 * i]), 0x07060302u);
+          __builtin_memcpy(&hi, hw, 16);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float rest = pr[i] - __uint_as_float(__float_as_uint(pr[i]) & 0xffff0000u);
+            lo[i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
+          }
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            bf16x8 vf;
+            if constexpr (ES == 2) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = __builtin_amdgcn_perm(vr[2 * i + 1].w[j >> 1], vr[2 * i].w[j >> 1],
+                                             (j & 1) ? 0x07060302u : 0x05040100u);
+              __builtin_memcpy(&vf, w, 16);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[i].w[j >> 2] >> (8 * (j & 3)));
             }
-            // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
-            // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
-            // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
-            bf16x8 hi, lo;
-            uint32_t hw[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              hw[i] = __builtin_amdgcn_perm(__float_as_uint(pr[2 * i + 1]), __float_as_uint(pr[2 * i]), 0x07060302u);
-            __builtin_memcpy(&hi, hw, 16);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float rest = pr[i] - __uint_as_float(__float_as_uint(pr[i]) & 0xffff0000u);
-              lo[i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
-            }
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-              bf16x8 vf;
-              if constexpr (ES == 2) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  w[i] = __builtin_amdgcn_perm(vr[u][2 * i + 1].w[j >> 1], vr[u][2 * i].w[j >> 1],
-                                               (j & 1) ? 0x07060302u : 0x05040100u);
-                __builtin_memcpy(&vf, w, 16);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[u][i].w[j >> 2] >> (8 * (j & 3)));
-              }
-              o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi, o[j], 0, 0, 0);
-              o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo, o[j], 0, 0, 0);
-            }
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi, o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo, o[j], 0, 0, 0);
           }
         }
         if (more) {
@@ -477,8 +453,6 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void paged_attention_kernel(
       if (h == 0 && row0 == 0 && tid == 0 && !ok) kv_flag(a.err);
       return;
     }
-    t0 += tb - ta;
-    off += tb - ta;
   }
 }
 
@@ -508,18 +482,18 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
   if (W && c < chunks && (int64_t)c * PJ_KEYS >= n) return;
   int total = 0, before = 0;
   for (int i = lane; i < a.B; i += 64) {
-    const int x = tiles_of(a, i, &ok);
+    const int x = work_of(tiles_of(a, i, &ok));
     total += x;
     before += i < b ? x : 0;
   }
-  total = wave_sum_int(total) * a.units;
-  before = wave_sum_int(before) * a.units;
-  const int tiles = (int)((n + a.kt - 1) / a.kt);
+  total = wave_uniform(wave_sum_int(total)) * a.units;
+  before = wave_uniform(wave_sum_int(before)) * a.units;
+  const int tiles = (int)((n + PA_KT - 1) / PA_KT);
   const int per = share_of(a, total);
   // the shares w0 .. w1 that hold the unit of query head i
   auto unit_of = [&](int i, int* w0, int* w1) {
-    const int s = before + (h * a.row_tiles + i / PA_ROWS) * tiles;
-    *w0 = s / per, *w1 = (s + tiles - 1) / per;
+    const int s = before + (h * a.row_tiles + i / PA_ROWS) * (tiles + PA_BEGIN);
+    *w0 = (s + PA_BEGIN) / per, *w1 = (s + PA_BEGIN + tiles - 1) / per;
   };
   auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * SLOT; };
 
@@ -632,7 +606,7 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
 
 // How a call is laid out: shares, and the parts of its workspace in bytes.
 struct Layout {
-  int row_tiles, units, shares, dhp, kt;
+  int row_tiles, units, shares, dhp;
   int waves;  // of a workgroup that takes a whole unit; 0: shares
   int64_t score_ld, part, score, stats;
 };
@@ -642,12 +616,11 @@ Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t mos
   y.row_tiles = (int)cdiv(group, PA_ROWS);
   y.units = (int)(p->kv_heads * y.row_tiles);
   y.dhp = p->head_dim <= 64 ? 64 : 128;
-  y.kt = PA_KT * tile_products(y.dhp, p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1);
-  const int64_t tiles = B * y.units * cdiv(most, y.kt);
-  const int64_t shares = cdiv(tiles, PA_MIN_TILES), cus = cu_count();
-  const int64_t slots = cus * PA_PER_CU < PA_MAX_SHARES ? cus * PA_PER_CU : PA_MAX_SHARES;
+  const int64_t tiles = B * y.units * cdiv(most, PA_KT);
+  const int64_t shares = cdiv(tiles, PA_MIN_TILES), cus = cu_count(), pcu = per_cu(y.dhp, p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1);
+  const int64_t slots = cus * pcu < PA_MAX_SHARES ? cus * pcu : PA_MAX_SHARES;
   y.shares = (int)(shares < 1 ? 1 : shares < slots ? shares : slots);
-  y.score_ld = cdiv(most, y.kt) * y.kt;
+  y.score_ld = cdiv(most, PA_KT) * PA_KT;
   y.waves = 0;
   if (most <= PA_ONE_KEYS && (!accumulate || y.row_tiles == 1))
     y.waves = B * y.units > cus ? PA_WAVES : PA_MORE;
@@ -700,7 +673,7 @@ int check_heads(const char* who, const cortex_kv_pages* pages, int64_t B, int64_
                    (long long)pages->kv_heads);
   CORTEX_CHECK_ARG(B >= 0 && B <= 4096, "%s: %lld sequences (at most 4096)", who, (long long)B);
   const int64_t units = pages->kv_heads * cdiv(heads / pages->kv_heads, PA_ROWS);
-  CORTEX_CHECK_ARG(most < 0 || B * units <= 0x3fffffffLL / (cdiv(most, PA_KT) + 1),
+  CORTEX_CHECK_ARG(most < 0 || B * units <= 0x3fffffffLL / (cdiv(most, PA_KT) + PA_BEGIN),
                    "%s: %lld sequences of up to %lld keys are too much for one call", who, (long long)B, (long long)most);
   return OK;
 }
@@ -747,7 +720,6 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   a.row_tiles = y.row_tiles;
   a.units = y.units;
   a.shares = y.shares;
-  a.kt = y.kt;
   a.q = q;
   a.q_sb = q_sb;
   a.q_sh = q_sh;

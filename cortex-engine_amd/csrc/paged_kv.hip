@@ -274,6 +274,7 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   __shared__ __attribute__((aligned(16))) int hist[EP_COPIES][256];
   __shared__ int part[WAVES];
   __shared__ int picked[3];
+  __shared__ uint16_t list[Q ? 8 * Q * THREADS : 1];  // holes, then movers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int H = a.p.kv_heads;
   const int64_t b = blockIdx.x / H;
@@ -409,15 +410,30 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
       holes += !stay && j < budget;
       movers += stay && j >= budget;
     });
-    int hole = block_scan<WAVES>(holes, part, tid, &all);
-    int mover = block_scan<WAVES>(movers, part, tid, &moved);
+    int hole, mover;
+    if constexpr (Q > 0) {  // both at once: at most half of 32768 slots each
+      const int both = block_scan<WAVES>(holes << 16 | movers, part, tid, &all);
+      hole = both >> 16, mover = both & 0xffff, moved = all & 0xffff;
+    } else {
+      hole = block_scan<WAVES>(holes, part, tid, &all);
+      mover = block_scan<WAVES>(movers, part, tid, &moved);
+    }
     t = tie;
     each([&](int j, uint32_t x) {
       const bool stay = stays(x, t), low = j < budget;
-      if (stay != low) (low ? dst : src)[low ? hole : mover] = j;
+      if (stay != low) {
+        if constexpr (Q > 0)
+          list[low ? hole : moved + mover] = (uint16_t)j;
+        else
+          (low ? dst : src)[low ? hole : mover] = j;
+      }
       hole += !stay && low;
       mover += stay && !low;
     });
+    if constexpr (Q > 0) {  // in whole lines
+      __syncthreads();
+      for (int i = tid; i < moved; i += THREADS) dst[i] = list[i], src[i] = list[moved + i];
+    }
   }
   if (tid == 0) a.counts[blockIdx.x] = moved;
   for (int64_t i = moved + tid; i < a.cap; i += THREADS) dst[i] = src[i] = -1;
