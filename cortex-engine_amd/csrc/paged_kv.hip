@@ -81,15 +81,17 @@ struct Eight {
     }
   }
 };
+// (non-temporal: rows are written once, and read much later than most of what is in the caches.  16,800 tokens of 8 heads
+// x 128 in bf16: 33.7 us with plain stores, 26.4 with these)
 __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4*>(p));
+  __builtin_nontemporal_store(f32x4{f[4], f[5], f[6], f[7]}, reinterpret_cast<f32x4*>(p) + 1);
 }
 __device__ __forceinline__ void store8(bf16* p, const float (&f)[8]) {
   bf16x8 a;
 #pragma unroll
   for (int j = 0; j < 8; ++j) a[j] = (bf16)f[j];
-  *reinterpret_cast<bf16x8*>(p) = a;
+  __builtin_nontemporal_store(__builtin_bit_cast(i32x4, a), reinterpret_cast<i32x4*>(p));
 }
 
 // The lengths after a ragged append, by thread `at` of `threads`.
@@ -121,7 +123,7 @@ constexpr int AP_AHEAD = 4;    // values in flight, in eights a thread
 
 // A workgroup takes `tokens` tokens, a thread eight values of a (token, key or value, head) row; `lpr` lanes a row.  The
 // first threads look up where the tokens go while the others load the rows.  Bound by HBM for many tokens (16,800 of 8
-// heads x 128, bf16: MEASURE), by the chain of lookups for few.
+// heads x 128, bf16, 139 MB: 26.4 us, 5.3 TB/s), by the chain of lookups for few.
 template <class X, class P>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr, int tokens) {
   __shared__ int at_page[AP_TOKENS], at_row[AP_TOKENS], at_slot[AP_TOKENS];
@@ -271,7 +273,7 @@ __device__ int block_scan(int v, int* part, int tid, int* total) {
 template <int THREADS, int Q>
 __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   constexpr int WAVES = THREADS / 64;
-  __shared__ __attribute__((aligned(16))) int hist[EP_COPIES][256];
+  __shared__ __attribute__((aligned(16))) int hist[2][EP_COPIES][256];  // of this round, and cleared for the next
   __shared__ int part[WAVES];
   __shared__ int picked[3];
   __shared__ uint16_t list[Q ? 8 * Q * THREADS : 1];  // holes, then movers
@@ -367,18 +369,19 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
     uint32_t found = 0;
     int kept = budget;
     bool whole = false;
+    for (int i = tid; i < EP_COPIES * 256; i += THREADS) hist[0][0][i] = 0;
+    __syncthreads();
     for (int shift = 24; shift >= 0 && !whole; shift -= 8) {
-      for (int i = tid; i < EP_COPIES * 256; i += THREADS) hist[0][i] = 0;
-      __syncthreads();
+      int(*now)[256] = hist[(shift >> 3) & 1 ^ 1], *next = hist[(shift >> 3) & 1][0];
       each([&](int, uint32_t x) {
-        if (shift == 24 || (x >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&hist[lane % EP_COPIES][(x >> shift) & 255], 1);
+        if (shift == 24 || (x >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&now[lane % EP_COPIES][((x >> shift) & 255)], 1);
       });
       __syncthreads();
       if (wid == 0) {  // lane l has the bins 252 - 4 l .. 255 - 4 l
         int4 c = {0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < EP_COPIES; ++x) {
-          const int4 y = *reinterpret_cast<const int4*>(&hist[x][252 - 4 * lane]);
+          const int4 y = *reinterpret_cast<const int4*>(&now[x][252 - 4 * lane]);
           c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
         }
         const int count[4] = {c.w, c.z, c.y, c.x};  // the largest ranks first
@@ -390,6 +393,8 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
             picked[0] = 255 - 4 * lane - i, picked[1] = before, picked[2] = count[i];
           before += count[i];
         }
+      } else {
+        for (int i = tid - 64; i < EP_COPIES * 256; i += THREADS - 64) next[i] = 0;
       }
       __syncthreads();
       found |= (uint32_t)picked[0] << shift;
@@ -439,6 +444,8 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   for (int64_t i = moved + tid; i < a.cap; i += THREADS) dst[i] = src[i] = -1;
 }
 
+constexpr int EA_PER_CU = 16;
+
 struct ApplyArgs {
   KvPages p;
   const int32_t* dst;
@@ -451,66 +458,43 @@ struct ApplyArgs {
   int row_bytes;
 };
 
-constexpr int EA_ROWS = 4;  // rows of a group of lanes
-
+// `lanes` lanes a row, 16 bytes of the key and of the value each; a group of lanes takes a row at a time, with the next
+// row's place looked up beside it.  Bound by HBM: rows of 256 bytes read and written at random (32 sequences of 2000 ..
+// 9001 slots down to 2048, 8 heads x 128 in bf16, 305 MB: 70 us, 4.4 TB/s; four rows a group at once 83 us, plain stores 72; a
+// workgroup for every 16 rows that there may be 71, 15 of them for the launch).
 __global__ __launch_bounds__(256) void kv_evict_apply_kernel(ApplyArgs a, int es) {
   const int tid = threadIdx.x;
   const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;
   const int64_t b = bh / a.p.kv_heads;
   const int h = bh - (int)b * a.p.kv_heads;
-  const int groups = 256 / a.lanes, group = tid / a.lanes, c = (tid % a.lanes) * 16;
+  const int groups = 256 / a.lanes, c = (tid % a.lanes) * 16;
+  const int64_t step = (int64_t)a.chunks * groups, row0 = (int64_t)bh * a.cap;
+  int64_t i = (int64_t)chunk * groups + tid / a.lanes;
+  if (i >= a.cap) return;
+  int to = a.dst[row0 + i], from = a.src[row0 + i];  // (beside the count of moves)
   const int64_t n = min((int64_t)a.counts[bh], a.cap);
-  const int64_t i0 = (int64_t)chunk * EA_ROWS * groups + group;
-  if (i0 >= n) return;
-  // all lookups, then all loads, then the stores
-  int64_t to[EA_ROWS], from[EA_ROWS];
-  bool ok[EA_ROWS];
-#pragma unroll
-  for (int r = 0; r < EA_ROWS; ++r) {
-    const int64_t i = min(i0 + r * groups, n - 1);
-    to[r] = a.dst[(int64_t)bh * a.cap + i], from[r] = a.src[(int64_t)bh * a.cap + i];
-  }
-  int tp[EA_ROWS], fp[EA_ROWS];
-#pragma unroll
-  for (int r = 0; r < EA_ROWS; ++r) tp[r] = a.p.page_of(b, to[r]), fp[r] = a.p.page_of(b, from[r]);
-  bool bad = false;
-#pragma unroll
-  for (int r = 0; r < EA_ROWS; ++r) {
-    const bool in = i0 + r * groups < n;
-    ok[r] = in && tp[r] >= 0 && fp[r] >= 0;
-    bad = bad || (in && !ok[r]);
-  }
-  if (bad && c == 0) kv_flag(a.err);
-  // (what does not move is loaded too, from wherever a row is, and not stored)
-  const bool row_part = c < a.row_bytes;
-  char* k = reinterpret_cast<char*>(a.p.k) + h * a.p.k_head * es + (row_part ? c : 0);
-  char* v = reinterpret_cast<char*>(a.p.v) + h * a.p.v_head * es + (row_part ? c : 0);
-  i32x4 x[EA_ROWS], y[EA_ROWS];
-  float weight[EA_ROWS], ks[EA_ROWS], vs[EA_ROWS];
-  int position[EA_ROWS];
-#pragma unroll
-  for (int r = 0; r < EA_ROWS; ++r) {
-    const int64_t page = ok[r] ? fp[r] : 0, row = a.p.row_of(from[r]);
-    x[r] = *reinterpret_cast<const i32x4*>(k + (page * a.p.k_page + row * a.p.k_slot) * es);
-    y[r] = *reinterpret_cast<const i32x4*>(v + (page * a.p.v_page + row * a.p.v_slot) * es);
-    const int64_t f = a.p.scalar_at((int)page, h, (int)row);  // (every lane of a row: one address)
-    weight[r] = a.p.weight ? a.p.weight[f] : 0.0f;
-    position[r] = a.p.position ? a.p.position[f] : 0;
-    ks[r] = a.p.k_scale ? a.p.k_scale[f] : 0.0f;
-    vs[r] = a.p.k_scale ? a.p.v_scale[f] : 0.0f;
-  }
-#pragma unroll
-  for (int r = 0; r < EA_ROWS; ++r) {
-    const int64_t row = a.p.row_of(to[r]);
-    if (ok[r] && row_part) {
-      *reinterpret_cast<i32x4*>(k + (tp[r] * a.p.k_page + row * a.p.k_slot) * es) = x[r];
-      *reinterpret_cast<i32x4*>(v + (tp[r] * a.p.v_page + row * a.p.v_slot) * es) = y[r];
+  while (i < n) {
+    const int tp = a.p.page_of(b, to), fp = a.p.page_of(b, from);
+    const int64_t tr = a.p.row_of(to), fr = a.p.row_of(from);
+    i += step;
+    if (i < n) to = a.dst[row0 + i], from = a.src[row0 + i];
+    if (tp < 0 || fp < 0) {
+      if (c == 0) kv_flag(a.err);
+      continue;
     }
-    if (ok[r] && c == 0) {
-      const int64_t t = a.p.scalar_at(tp[r], h, (int)row);
-      if (a.p.weight) a.p.weight[t] = weight[r];
-      if (a.p.position) a.p.position[t] = position[r];
-      if (a.p.k_scale) a.p.k_scale[t] = ks[r], a.p.v_scale[t] = vs[r];
+    if (c < a.row_bytes) {
+      char* k = reinterpret_cast<char*>(a.p.k) + h * a.p.k_head * es + c;
+      char* v = reinterpret_cast<char*>(a.p.v) + h * a.p.v_head * es + c;
+      const i32x4 x = *reinterpret_cast<const i32x4*>(k + (fp * a.p.k_page + fr * a.p.k_slot) * es);
+      const i32x4 y = *reinterpret_cast<const i32x4*>(v + (fp * a.p.v_page + fr * a.p.v_slot) * es);
+      __builtin_nontemporal_store(x, reinterpret_cast<i32x4*>(k + (tp * a.p.k_page + tr * a.p.k_slot) * es));
+      __builtin_nontemporal_store(y, reinterpret_cast<i32x4*>(v + (tp * a.p.v_page + tr * a.p.v_slot) * es));
+    }
+    if (c == 0) {
+      const int64_t t = a.p.scalar_at(tp, h, (int)tr), f = a.p.scalar_at(fp, h, (int)fr);
+      if (a.p.weight) a.p.weight[t] = a.p.weight[f];
+      if (a.p.position) a.p.position[t] = a.p.position[f];
+      if (a.p.k_scale) a.p.k_scale[t] = a.p.k_scale[f], a.p.v_scale[t] = a.p.v_scale[f];
     }
   }
 }
@@ -646,7 +630,9 @@ extern "C" int cortex_kv_evict_apply(const cortex_kv_pages* pages, int64_t B, co
   a.err = err;
   a.row_bytes = (int)pages->head_dim * es;
   a.lanes = pow2_lanes(a.row_bytes / 16);
-  const int64_t chunks = cdiv(cap, (256 / a.lanes) * EA_ROWS);
+  // up to EA_PER_CU workgroups a CU for all heads together
+  int64_t chunks = cdiv((int64_t)cu_count() * EA_PER_CU, B * pages->kv_heads);
+  if (chunks > cdiv(cap, 256 / a.lanes)) chunks = cdiv(cap, 256 / a.lanes);
   CORTEX_CHECK_ARG(chunks * B * pages->kv_heads <= 0x7fffffffLL, "%s: too many rows", who);
   a.chunks = (int)chunks;
   hipLaunchKernelGGL(kv_evict_apply_kernel, dim3((unsigned)(chunks * B * pages->kv_heads)), dim3(256), 0, stream, a, es);
