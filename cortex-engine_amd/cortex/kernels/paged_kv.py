@@ -107,25 +107,35 @@ def _i64(t: torch.Tensor, n: int, name: str, what: str) -> None:
         raise ValueError(f"{what}: {name} must be a contiguous int64 tensor of {n} values, got {tuple(t.shape)} {t.dtype}")
 
 
-def _common(what: str, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, err_flag,
-            *more) -> tuple[int, int, int]:
+def _common(what: str, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
+            err_flag) -> tuple[int, int, int]:
     """Checks what every operator takes; the block table's rows, row stride and columns."""
     idx = pages.index
-    for t in (block_table, lengths, err_flag, *more):
-        if t is not None and t.get_device() != idx:
-            dev = nat.require_gpu(block_table, lengths, err_flag, *more, what=what)
-            raise RuntimeError(f"{what}: tensors on different devices ({dev} vs {pages.device})")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
+    if (block_table.get_device() != idx or lengths.get_device() != idx
+            or (err_flag is not None and err_flag.get_device() != idx)):
+        _elsewhere(what, pages, block_table, lengths, err_flag)
+    shape = block_table.shape
+    if len(shape) != 2 or block_table.dtype is not torch.int32:
         raise ValueError(f"{what}: block_table must be a (B, max_pages) int32 tensor")
-    B, width = block_table.shape
-    ld, unit = block_table.stride()
-    if width > 1 and unit != 1:
-        raise ValueError(f"{what}: the rows of block_table must be contiguous")
+    B, width = shape
+    if block_table.is_contiguous():
+        ld = width
+    else:
+        ld, unit = block_table.stride()
+        if width > 1 and unit != 1:
+            raise ValueError(f"{what}: the rows of block_table must be contiguous")
+        if B < 2:
+            ld = width
     if lengths.dtype is not torch.int64 or lengths.shape != (B,) or not lengths.is_contiguous():
         _i64(lengths, B, "lengths", what)
     if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
         raise ValueError(f"{what}: err_flag must be one int32")
-    return B, ld if B > 1 else width, width
+    return B, ld, width
+
+
+def _elsewhere(what: str, pages: KVPages, *tensors) -> None:
+    dev = nat.require_gpu(*tensors, what=what)
+    raise RuntimeError(f"{what}: tensors on different devices ({dev} vs {pages.device})")
 
 
 def _launch(name: str, pages: KVPages, *args) -> None:
@@ -162,7 +172,12 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
     ``max(max|x|, 1e-8) / 127``, rounded half to even.  Tracked pages get weight 0 and the token's position:
     ``positions`` (T,) int64, by default its slot number.  ``new_lengths`` may be ``lengths`` itself.  A token without
     a slot or a page is dropped and sets bit 2 of ``err_flag`` (int32, never cleared here)."""
-    B, ld, width = _common("paged_kv_append", pages, block_table, lengths, err_flag, k, v, offsets, positions, new_lengths)
+    B, ld, width = _common("paged_kv_append", pages, block_table, lengths, err_flag)
+    idx = pages.index
+    if (k.get_device() != idx or v.get_device() != idx or (offsets is not None and offsets.get_device() != idx)
+            or (positions is not None and positions.get_device() != idx)
+            or (new_lengths is not None and new_lengths.get_device() != idx)):
+        _elsewhere("paged_kv_append", pages, k, v, offsets, positions, new_lengths)
     if k.requires_grad or v.requires_grad:
         _no_grad("paged_kv_append")
     shape, dtype = k.shape, k.dtype
@@ -205,7 +220,9 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     of its key head; no two sequences of the call may then share a page.  ``max_length``: a bound of the lengths
     known on the host (default: the table's width), which sizes the launch and the workspace; longer sequences are cut
     to it and set bit 2 of ``err_flag``, as lengths outside the table and page ids outside the pool do (such pages hold no keys)."""
-    B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag, q, out)
+    B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag)
+    if q.get_device() != pages.index or (out is not None and out.get_device() != pages.index):
+        _elsewhere("paged_attention", pages, q, out)
     if q.requires_grad:
         _no_grad("paged_attention")
     shape, dtype = q.shape, q.dtype
@@ -223,7 +240,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     else:
         max_length = min(max_length, width * pages.page_size)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=pages.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1 or out.data_ptr() == q.data_ptr():
         raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor of its own with a contiguous last dim")
     q, qb, qh = _rows(q, 4 if dtype is torch.float32 else 2)
@@ -254,13 +271,13 @@ def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tens
     room = width * pages.page_size
     most = room if max_length is None else min(max_length, room)
     cap = max(0, min(budget, most - budget))
-    moves = torch.empty((2, B, pages.kv_heads, cap), dtype=torch.int32, device=pages.device)
-    counts = torch.empty((B, pages.kv_heads), dtype=torch.int32, device=pages.device)
-    dst, src = moves.unbind(0)
-    plan = EvictPlan(dst, src, counts, torch.empty_like(lengths))
+    dst = block_table.new_empty((B, pages.kv_heads, cap))
+    src = torch.empty_like(dst)
+    counts = block_table.new_empty((B, pages.kv_heads))
+    after = torch.empty_like(lengths)
     _launch("cortex_kv_evict_plan", pages, B, block_table.data_ptr(), ld, width, lengths.data_ptr(), most, budget, recent,
-            dst.data_ptr(), src.data_ptr(), counts.data_ptr(), plan.lengths.data_ptr(), nat.ptr(err_flag))
-    return plan
+            dst.data_ptr(), src.data_ptr(), counts.data_ptr(), after.data_ptr(), nat.ptr(err_flag))
+    return EvictPlan(dst, src, counts, after)
 
 
 def kv_evict_apply(pages: KVPages, block_table: torch.Tensor, plan: EvictPlan, *,
@@ -268,7 +285,9 @@ def kv_evict_apply(pages: KVPages, block_table: torch.Tensor, plan: EvictPlan, *
     """Moves the rows of a plan in place: keys, values and, where the pages have them, scales, weight and position.
     Slots at or past the budget keep what they held.  Sequences of the call may not share pages."""
     dst, src, counts, after = plan
-    B, ld, width = _common("kv_evict_apply", pages, block_table, after, err_flag, dst, src, counts)
+    B, ld, width = _common("kv_evict_apply", pages, block_table, after, err_flag)
+    if dst.get_device() != pages.index or src.get_device() != pages.index or counts.get_device() != pages.index:
+        _elsewhere("kv_evict_apply", pages, dst, src, counts)
     shape = dst.shape
     if (len(shape) != 3 or shape[:2] != (B, pages.kv_heads) or src.shape != shape or counts.shape != shape[:2]
             or not dst.dtype is src.dtype is counts.dtype is torch.int32
