@@ -34,9 +34,10 @@ constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
 // bits 117.  (64 sequences of 500 .. 3000 keys x 64 dims, bf16: 2 a CU 55.5 us, 4 54.2; 128 dims as 3: 105 -> 110)
 __host__ __device__ constexpr int per_cu(int dhp, int es) { return dhp == 128 ? 2 : es == 4 ? 3 : 4; }
 constexpr int PA_MAX_SHARES = 1024;
-// What it costs to begin a unit (fill and drain the loads, sum up), in tiles: without it the shares of short sequences
-// are the last to end (32 sequences of 150 .. 8003 keys 118 us, 2: 107.1, 4: 107.2, 8: 105.2; one of 8192 16.8, 18.1, 18.6, 18.3)
-constexpr int PA_BEGIN = 4;
+// What it costs to begin a unit (fill and drain the loads, sum up), in tiles, where a share may have PA_LONG tiles and
+// where it has fewer: without it the shares with many short sequences are the last to end (32 sequences of 150 .. 8003
+// keys: 0 118 us, 2 107, 4 107, 8 104.6; 8 of 101 .. 2049 in fp32: 0 22.2, 2 20.6, 4 20.1, 8 21.7; one of 8192: 0 16.8, 2 18)
+constexpr int PA_LONG = 16, PA_BEGIN_LONG = 8, PA_BEGIN_SHORT = 2;
 constexpr int PA_ONE_KEYS = 1024;  // length up to which a workgroup takes a whole unit
 constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before the sums are rescaled: p <= 2^8
 
@@ -46,6 +47,7 @@ struct PagedArgs {
   int row_tiles;        // units a key head: ceil(group / PA_ROWS)
   int units;            // units a sequence: kv_heads * row_tiles
   int shares;
+  int begin;            // tiles that beginning a unit counts for
   const void* q;
   int64_t q_sb, q_sh;
   const int64_t* lengths;
@@ -103,7 +105,7 @@ __device__ __forceinline__ int tiles_of(const PagedArgs& a, int b, bool* ok) {
 }
 
 // What a unit counts for when the shares are cut: its tiles, and what it costs to begin one.
-__device__ __forceinline__ int work_of(int tiles) { return tiles ? tiles + PA_BEGIN : 0; }
+__device__ __forceinline__ int work_of(const PagedArgs& a, int tiles) { return tiles ? tiles + a.begin : 0; }
 
 __device__ __forceinline__ int wave_scan_int(int v, int lane) {  // inclusive
 #pragma unroll
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
   } else {
     int total = 0;
     for (int i = lane; i < a.B; i += 64) {
-      total += work_of(tiles_of(a, i, &ok));
+      total += work_of(a, tiles_of(a, i, &ok));
     }
     if (blockIdx.x == 0 && !ok) kv_flag(a.err);
     total = wave_uniform(wave_sum_int(total)) * a.units;
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
     t1 = min(total, t0 + per);
     if (t0 >= t1) return;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int v = b0 + lane < a.B ? work_of(tiles_of(a, b0 + lane, &ok)) * a.units : 0;
+      const int v = b0 + lane < a.B ? work_of(a, tiles_of(a, b0 + lane, &ok)) * a.units : 0;
       const int inc = wave_scan_int(v, lane);
       const uint64_t past = __ballot(inc > off);
       if (past) {
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
 
   while (t0 < t1 && b < a.B) {
     const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
-    const int tiles = (int)((n + PA_KT - 1) / PA_KT), work = work_of(tiles);
+    const int tiles = (int)((n + PA_KT - 1) / PA_KT), work = work_of(a, tiles);
     if (!ONE && off >= work * a.units) {  // done, or empty
       ++b;
       off = 0;
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
     }
     const int u = ONE ? blockIdx.x - b * a.units : off / work, from = off - u * work;
     const int step = ONE ? 0 : min(work - from, t1 - t0);
-    const int ta = ONE ? 0 : max(0, from - PA_BEGIN), tb = ONE ? tiles : max(0, from + step - PA_BEGIN);
+    const int ta = ONE ? 0 : max(0, from - a.begin), tb = ONE ? tiles : max(0, from + step - a.begin);
     t0 += step;
     off += step;
     if (!ONE && ta == tb) continue;
@@ -304,7 +306,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
           if constexpr (ES == 1) x[st] *= ks[st];
         }
         if (more) load_k(t + WAVES, id1);
-        __builtin_amdgcn_sched_barrier(0);
 
         // where not all of this lane's 8 keys are there
         const bool page_ok = (uint32_t)id.v < (uint32_t)p.num_pages;
@@ -394,7 +395,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
           load_scales(t + WAVES, id1);
           load_v(t + WAVES, id1);
         }
-        __builtin_amdgcn_sched_barrier(0);
         id = id1;
         id1 = id2;
       }
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
   if (W && c < chunks && (int64_t)c * PJ_KEYS >= n) return;
   int total = 0, before = 0;
   for (int i = lane; i < a.B; i += 64) {
-    const int x = work_of(tiles_of(a, i, &ok));
+    const int x = work_of(a, tiles_of(a, i, &ok));
     total += x;
     before += i < b ? x : 0;
   }
@@ -492,8 +492,8 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
   const int per = share_of(a, total);
   // the shares w0 .. w1 that hold the unit of query head i
   auto unit_of = [&](int i, int* w0, int* w1) {
-    const int s = before + (h * a.row_tiles + i / PA_ROWS) * (tiles + PA_BEGIN);
-    *w0 = (s + PA_BEGIN) / per, *w1 = (s + PA_BEGIN + tiles - 1) / per;
+    const int s = before + (h * a.row_tiles + i / PA_ROWS) * (tiles + a.begin);
+    *w0 = (s + a.begin) / per, *w1 = (s + a.begin + tiles - 1) / per;
   };
   auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * SLOT; };
 
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
 
 // How a call is laid out: shares, and the parts of its workspace in bytes.
 struct Layout {
-  int row_tiles, units, shares, dhp;
+  int row_tiles, units, shares, begin, dhp;
   int waves;  // of a workgroup that takes a whole unit; 0: shares
   int64_t score_ld, part, score, stats;
 };
@@ -620,6 +620,7 @@ Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t mos
   const int64_t shares = cdiv(tiles, PA_MIN_TILES), cus = cu_count(), pcu = per_cu(y.dhp, p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1);
   const int64_t slots = cus * pcu < PA_MAX_SHARES ? cus * pcu : PA_MAX_SHARES;
   y.shares = (int)(shares < 1 ? 1 : shares < slots ? shares : slots);
+  y.begin = tiles / y.shares >= PA_LONG ? PA_BEGIN_LONG : PA_BEGIN_SHORT;
   y.score_ld = cdiv(most, PA_KT) * PA_KT;
   y.waves = 0;
   if (most <= PA_ONE_KEYS && (!accumulate || y.row_tiles == 1))
@@ -673,7 +674,7 @@ int check_heads(const char* who, const cortex_kv_pages* pages, int64_t B, int64_
                    (long long)pages->kv_heads);
   CORTEX_CHECK_ARG(B >= 0 && B <= 4096, "%s: %lld sequences (at most 4096)", who, (long long)B);
   const int64_t units = pages->kv_heads * cdiv(heads / pages->kv_heads, PA_ROWS);
-  CORTEX_CHECK_ARG(most < 0 || B * units <= 0x3fffffffLL / (cdiv(most, PA_KT) + PA_BEGIN),
+  CORTEX_CHECK_ARG(most < 0 || B * units <= 0x3fffffffLL / (cdiv(most, PA_KT) + PA_BEGIN_LONG),
                    "%s: %lld sequences of up to %lld keys are too much for one call", who, (long long)B, (long long)most);
   return OK;
 }
@@ -720,6 +721,7 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   a.row_tiles = y.row_tiles;
   a.units = y.units;
   a.shares = y.shares;
+  a.begin = y.begin;
   a.q = q;
   a.q_sb = q_sb;
   a.q_sh = q_sh;
