@@ -38,7 +38,11 @@ constexpr int PA_MAX_SHARES = 1024;
 // where it has fewer: without it the shares with many short sequences are the last to end (32 sequences of 150 .. 8003
 // keys: 0 118 us, 2 107, 4 107, 8 104.6; 8 of 101 .. 2049 in fp32: 0 22.2, 2 20.6, 4 20.1, 8 21.7; one of 8192: 0 16.8, 2 18)
 constexpr int PA_LONG = 16, PA_BEGIN_LONG = 8, PA_BEGIN_SHORT = 2;
-constexpr int PA_ONE_KEYS = 1024;  // length up to which a workgroup takes a whole unit
+// Length up to which a workgroup takes a whole unit, and where there are units for every CU (us, shares against whole units:
+// 600 keys, 8 units of 64 dims 14.2 / 10.0; 1000, 64 units of 128 17.3 / 14.6; 2048, 8 units of 128 13.9 / 22.5; 1000 ..
+// 2000, 256 units of 64 26.7 / 21.1, 512 of 128 85.8 / 76.8, 128 of 128 27.6 / 28.6; 500 .. 4000, 512 of 128 119 / 121; fp32
+// 200 .. 2000, 384 of 64 53.2 / 55.9)
+constexpr int PA_ONE_KEYS = 1024, PA_ONE_KEYS_FULL = 2048;
 constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before the sums are rescaled: p <= 2^8
 
 struct PagedArgs {
@@ -623,7 +627,8 @@ Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t mos
   y.begin = tiles / y.shares >= PA_LONG ? PA_BEGIN_LONG : PA_BEGIN_SHORT;
   y.score_ld = cdiv(most, PA_KT) * PA_KT;
   y.waves = 0;
-  if (most <= PA_ONE_KEYS && (!accumulate || y.row_tiles == 1))
+  const bool full = B * y.units >= cus && p->dtype != DT_F32;
+  if (most <= (full ? PA_ONE_KEYS_FULL : PA_ONE_KEYS) && (!accumulate || y.row_tiles == 1))
     y.waves = B * y.units > cus ? PA_WAVES : PA_MORE;
   y.part = y.waves ? 0 : 2ll * y.shares * PA_ROWS * (y.dhp + 2) * 4;
   y.score = accumulate ? B * heads * y.score_ld * 4 : 0;
