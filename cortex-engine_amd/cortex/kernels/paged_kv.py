@@ -161,6 +161,26 @@ def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, int]:
     return t, s0, s1
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two (n, heads, head_dim) tensors may share memory (parts of one buffer that lie in each other's gaps, such as
+    the columns of a joint projection, do not)."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    es = a.element_size()
+
+    def span(t):  # bytes from the first to past the last value of the tensor, and of a row of it
+        row = ((t.shape[1] - 1) * t.stride(1) + t.shape[2]) * es
+        return (t.shape[0] - 1) * t.stride(0) * es + row, row
+
+    (na, ra), (nb, rb) = span(a), span(b)
+    if a0 + na <= b0 or b0 + nb <= a0:
+        return False
+    pitch = a.stride(0) * es
+    if a.stride(0) != b.stride(0) or not 0 < max(ra, rb) <= pitch:
+        return True
+    d = (b0 - a0) % pitch
+    return d < ra or d + rb > pitch
+
+
 def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
                     lengths: torch.Tensor, *, offsets: torch.Tensor | None = None,
                     positions: torch.Tensor | None = None, new_lengths: torch.Tensor | None = None,
@@ -170,7 +190,7 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
     ``k``, ``v`` (T, kv_heads, head_dim) bf16 or fp32: token b of sequence b, or with ``offsets`` (B + 1,) int64 the
     tokens ``[offsets[b], offsets[b + 1])`` of sequence b (no two tokens may share a slot).  Int8 pages take each row at scale
     ``max(max|x|, 1e-8) / 127``, rounded half to even.  Tracked pages get weight 0 and the token's position:
-    ``positions`` (T,) int64, by default its slot number.  ``new_lengths`` may be ``lengths`` itself.  A token without
+    ``positions`` (T,) int64 (kept in 32 bits), by default its slot number.  ``new_lengths`` may be ``lengths`` itself.  A token without
     a slot or a page is dropped and sets bit 2 of ``err_flag`` (int32, never cleared here)."""
     B, ld, width = _common("paged_kv_append", pages, block_table, lengths, err_flag)
     idx = pages.index
@@ -217,7 +237,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     ``h // (heads // kv_heads)``), ``scale`` ``head_dim ** -0.5`` by default.  A sequence of length 0 gives 0.
 
     ``accumulate`` adds to ``pages.weight`` the softmax weight that each key received, summed over the query heads
-    of its key head; no two sequences of the call may then share a page.  ``max_length``: a bound of the lengths
+    of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q``.  ``max_length``: a bound of the lengths
     known on the host (default: the table's width), which sizes the launch and the workspace; longer sequences are cut
     to it and set bit 2 of ``err_flag``, as lengths outside the table and page ids outside the pool do (such pages hold no keys)."""
     B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag)
@@ -241,8 +261,10 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         max_length = min(max_length, width * pages.page_size)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1 or out.data_ptr() == q.data_ptr():
-        raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor of its own with a contiguous last dim")
+    elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor with a contiguous last dim")
+    elif _overlap(out, q):
+        raise ValueError("out may not overlap q")
     q, qb, qh = _rows(q, 4 if dtype is torch.float32 else 2)
     ws_bytes = nat.load().cortex_paged_attention_workspace_bytes(pages.ref, B, heads, max_length, accumulate)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=pages.device) if ws_bytes else None

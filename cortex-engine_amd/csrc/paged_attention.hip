@@ -497,7 +497,8 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
   // the shares w0 .. w1 that hold the unit of query head i
   auto unit_of = [&](int i, int* w0, int* w1) {
     const int s = before + (h * a.row_tiles + i / PA_ROWS) * (tiles + a.begin);
-    *w0 = (s + a.begin) / per, *w1 = (s + a.begin + tiles - 1) / per;
+    *w0 = min((s + a.begin) / per, a.shares - 1);
+    *w1 = min((s + a.begin + tiles - 1) / per, a.shares - 1);  // (in the workspace, whatever becomes of the lengths meanwhile)
   };
   auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * SLOT; };
 

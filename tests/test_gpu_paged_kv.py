@@ -569,6 +569,62 @@ def test_captured_steps(dtype):
         assert torch.equal(x.float().nan_to_num(9.0), y.float().nan_to_num(9.0)), n
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_two_graphs_at_once(dtype):
+    """Two graphs over the same pages (long enough for a join), replayed at once on two streams: each has its workspace."""
+    c = Cache([5000, 1300, 0, 40], 2, 64, 16, DTYPES[dtype], seed=51)
+    qs = [c.query(8).to(DEV), c.query(8).to(DEV)]
+    want = [attend(c, q) for q in qs]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, outs = [], []
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(attend(c, q))
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for i in range(10):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, graph in zip(side, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = attend(c, qs[i % 2])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[i % 2])
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), i
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pages_past_four_gib(dtype):
+    """The same rows in pages at the end of a pool of more than 4 GiB and in a small one: the same bits."""
+    from cortex.kernels.paged_kv import KVPages, kv_evict_apply, kv_evict_plan, paged_attention, paged_kv_append
+
+    dt = DTYPES[dtype]
+    es = torch.empty(0, dtype=dt).element_size()
+    big = (9 << 29) // (2 * 64 * 128 * es)  # pages of 4.5 GiB
+    g = torch.Generator().manual_seed(61)
+    k, v = (torch.randn(900, 2, 128, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    q = torch.randn(3, 8, 128, generator=g).to(torch.float32 if dtype == "fp32" else torch.bfloat16).to(DEV)
+    off = torch.tensor([0, 500, 500, 900], device=DEV)
+    got = []
+    for num in (30, big):
+        pages = KVPages.allocate(num, 2, 64, 128, dt, tracked=True)
+        table = (num - 1 - torch.randperm(30, generator=torch.Generator().manual_seed(1))).reshape(3, 10).int().to(DEV)
+        n = paged_kv_append(pages, k, v, table, torch.zeros(3, dtype=torch.int64, device=DEV), offsets=off)
+        out = [n, paged_attention(q, pages, table, n, accumulate=True)]
+        plan = kv_evict_plan(pages, table, n, 200, 50)
+        kv_evict_apply(pages, table, plan)
+        out += [*plan, paged_attention(q, pages, table, plan.lengths), pages.weight[table.long()], pages.position[table.long()],
+                pages.k[table.long()]]
+        got.append([t.cpu() for t in out])
+        del pages
+        torch.cuda.empty_cache()
+    assert int(got[0][4].min()) == 0 and int(got[0][4].max()) > 0  # (an empty sequence and ones that were cut)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_empty_batches_and_caches():
     from cortex.kernels.paged_kv import KVPages, kv_evict_apply, kv_evict_plan, paged_attention, paged_kv_append
 
@@ -622,6 +678,16 @@ def test_refusals():
                {"err_flag": lengths}]:
         with pytest.raises(ValueError):
             paged_attention(*good, **kw)
+    buf = pool(2, 12, 64)  # queries and outputs in one buffer
+    for ok, out in [(True, buf[:, 4:8]), (True, buf[:, 8:]), (False, buf[:, 2:6]), (False, buf[:, :4])]:
+        if ok:
+            paged_attention(buf[:, :4], *good[1:], out=out)
+        else:
+            with pytest.raises(ValueError, match="overlap"):
+                paged_attention(buf[:, :4], *good[1:], out=out)
+    flat = pool(3, 4, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        paged_attention(flat[:2], *good[1:], out=flat[1:])
     with pytest.raises(RuntimeError):
         paged_attention(q.cpu(), *good[1:])
     with pytest.raises(RuntimeError, match="backward"):
