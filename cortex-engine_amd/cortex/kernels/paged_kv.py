@@ -138,25 +138,20 @@ def _elsewhere(what: str, pages: KVPages, *tensors) -> None:
     raise RuntimeError(f"{what}: tensors on different devices ({dev} vs {pages.device})")
 
 
-def _launch(name: str, pages: KVPages, *args) -> None:
-    """``nat.call`` on the current stream of the pages' device, whichever device is current."""
-    if pages.index == _get_device():
-        nat.call(name, pages.ref, *args, nat.stream_of(pages.device))
-    else:
-        with torch.cuda.device(pages.device):
-            nat.call(name, pages.ref, *args, nat.stream_of(pages.device))
-
-
 def _no_grad(what: str) -> None:
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
-def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, int]:
+def _rows(t: torch.Tensor, pages: KVPages, es: int) -> tuple[torch.Tensor, int, int]:
     """(n, heads, head_dim) rows that vector loads take, as given or copied, and their strides."""
+    if t.is_contiguous():
+        if t.data_ptr() & 15:
+            t = t.clone()
+        return t, t.shape[1] * pages.head_dim, pages.head_dim
     s0, s1, s2 = t.stride()
     if s2 != 1 or (t.data_ptr() | s0 * es | s1 * es) & 15:
-        t = t.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps rows that only start off)
+        t = t.clone(memory_format=torch.contiguous_format)
         s0, s1, _ = t.stride()
     return t, s0, s1
 
@@ -188,12 +183,17 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
     """Writes the rows of new tokens behind the ``lengths`` of their sequences and returns the new lengths (B,).
 
     ``k``, ``v`` (T, kv_heads, head_dim) bf16 or fp32: token b of sequence b, or with ``offsets`` (B + 1,) int64 the
-    tokens ``[offsets[b], offsets[b + 1])`` of sequence b (no two tokens may share a slot).  Int8 pages take each row at scale
-    ``max(max|x|, 1e-8) / 127``, rounded half to even.  Tracked pages get weight 0 and the token's position:
-    ``positions`` (T,) int64 (kept in 32 bits), by default its slot number.  ``new_lengths`` may be ``lengths`` itself.  A token without
-    a slot or a page is dropped and sets bit 2 of ``err_flag`` (int32, never cleared here)."""
-    B, ld, width = _common("paged_kv_append", pages, block_table, lengths, err_flag)
+    tokens ``[offsets[b], offsets[b + 1])`` of sequence b (no two tokens may share a slot).  Int8 pages take each row at
+    scale ``max(max|x|, 1e-8) / 127``, rounded half to even; a row with an infinity or a NaN becomes NaN.  Tracked
+    pages get weight 0 and the token's position: ``positions`` (T,) int64 (kept in 32 bits), by default its slot number.
+    ``new_lengths`` may be ``lengths`` itself.  A token without a slot or a page is dropped and sets bit 2 of
+    ``err_flag`` (int32, never cleared here)."""
     idx = pages.index
+    if idx != _get_device():
+        with torch.cuda.device(idx):
+            return paged_kv_append(pages, k, v, block_table, lengths, offsets=offsets, positions=positions,
+                                   new_lengths=new_lengths, err_flag=err_flag)
+    B, ld, width = _common("paged_kv_append", pages, block_table, lengths, err_flag)
     if (k.get_device() != idx or v.get_device() != idx or (offsets is not None and offsets.get_device() != idx)
             or (positions is not None and positions.get_device() != idx)
             or (new_lengths is not None and new_lengths.get_device() != idx)):
@@ -221,11 +221,11 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
         new_lengths = torch.empty_like(lengths)
     else:
         _i64(new_lengths, B, "new_lengths", "paged_kv_append")
-    k, kt, kh = _rows(k, es)
-    v, vt, vh = _rows(v, es)
-    _launch("cortex_kv_append", pages, B, T, code, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, block_table.data_ptr(),
-            ld, width, nat.ptr(offsets), lengths.data_ptr(), nat.ptr(positions), new_lengths.data_ptr(),
-            nat.ptr(err_flag))
+    k, kt, kh = _rows(k, pages, es)
+    v, vt, vh = _rows(v, pages, es)
+    nat.call("cortex_kv_append", pages.ref, B, T, code, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+             block_table.data_ptr(), ld, width, nat.ptr(offsets), lengths.data_ptr(), nat.ptr(positions),
+             new_lengths.data_ptr(), nat.ptr(err_flag), nat.stream_of(pages.device))
     return new_lengths
 
 
@@ -237,9 +237,14 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     ``h // (heads // kv_heads)``), ``scale`` ``head_dim ** -0.5`` by default.  A sequence of length 0 gives 0.
 
     ``accumulate`` adds to ``pages.weight`` the softmax weight that each key received, summed over the query heads
-    of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q``.  ``max_length``: a bound of the lengths
-    known on the host (default: the table's width), which sizes the launch and the workspace; longer sequences are cut
-    to it and set bit 2 of ``err_flag``, as lengths outside the table and page ids outside the pool do (such pages hold no keys)."""
+    of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q``.
+    ``max_length``: a bound of the lengths known on the host (default: the table's width), which sizes the launch and
+    the workspace; longer sequences are cut to it and set bit 2 of ``err_flag``, as lengths outside the table and page
+    ids outside the pool do (such pages hold no keys)."""
+    if pages.index != _get_device():
+        with torch.cuda.device(pages.index):
+            return paged_attention(q, pages, block_table, lengths, scale=scale, accumulate=accumulate,
+                                   max_length=max_length, out=out, err_flag=err_flag)
     B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag)
     if q.get_device() != pages.index or (out is not None and out.get_device() != pages.index):
         _elsewhere("paged_attention", pages, q, out)
@@ -265,13 +270,13 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor with a contiguous last dim")
     elif _overlap(out, q):
         raise ValueError("out may not overlap q")
-    q, qb, qh = _rows(q, 4 if dtype is torch.float32 else 2)
+    q, qb, qh = _rows(q, pages, 4 if dtype is torch.float32 else 2)
     ws_bytes = nat.load().cortex_paged_attention_workspace_bytes(pages.ref, B, heads, max_length, accumulate)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=pages.device) if ws_bytes else None
     ob, oh, _ = out.stride()
-    _launch("cortex_paged_attention", pages, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld, width,
-            lengths.data_ptr(), max_length, pages.head_dim ** -0.5 if scale is None else scale, accumulate,
-            out.data_ptr(), ob, oh, nat.ptr(ws), ws_bytes, nat.ptr(err_flag))
+    nat.call("cortex_paged_attention", pages.ref, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld, width,
+             lengths.data_ptr(), max_length, pages.head_dim ** -0.5 if scale is None else scale, accumulate,
+             out.data_ptr(), ob, oh, nat.ptr(ws), ws_bytes, nat.ptr(err_flag), nat.stream_of(pages.device))
     return out
 
 
@@ -282,6 +287,9 @@ def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tens
     equal weights by the lower slot).  Kept slots at or past the budget are to fill the slots below it that are given up (``EvictPlan``);
     shorter sequences stay as they are.  Reads ``pages.weight`` and ``pages.position`` and writes neither.
     ``max_length`` and ``err_flag`` as for ``paged_attention``."""
+    if pages.index != _get_device():
+        with torch.cuda.device(pages.index):
+            return kv_evict_plan(pages, block_table, lengths, budget, recent, max_length=max_length, err_flag=err_flag)
     B, ld, width = _common("kv_evict_plan", pages, block_table, lengths, err_flag)
     if pages.weight is None or pages.position is None:
         raise ValueError("eviction needs pages with weight and position (tracked=True)")
@@ -297,8 +305,9 @@ def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tens
     src = torch.empty_like(dst)
     counts = block_table.new_empty((B, pages.kv_heads))
     after = torch.empty_like(lengths)
-    _launch("cortex_kv_evict_plan", pages, B, block_table.data_ptr(), ld, width, lengths.data_ptr(), most, budget, recent,
-            dst.data_ptr(), src.data_ptr(), counts.data_ptr(), after.data_ptr(), nat.ptr(err_flag))
+    nat.call("cortex_kv_evict_plan", pages.ref, B, block_table.data_ptr(), ld, width, lengths.data_ptr(), most, budget,
+             recent, dst.data_ptr(), src.data_ptr(), counts.data_ptr(), after.data_ptr(), nat.ptr(err_flag),
+             nat.stream_of(pages.device))
     return EvictPlan(dst, src, counts, after)
 
 
@@ -306,6 +315,9 @@ def kv_evict_apply(pages: KVPages, block_table: torch.Tensor, plan: EvictPlan, *
                    err_flag: torch.Tensor | None = None) -> None:
     """Moves the rows of a plan in place: keys, values and, where the pages have them, scales, weight and position.
     Slots at or past the budget keep what they held.  Sequences of the call may not share pages."""
+    if pages.index != _get_device():
+        with torch.cuda.device(pages.index):
+            return kv_evict_apply(pages, block_table, plan, err_flag=err_flag)
     dst, src, counts, after = plan
     B, ld, width = _common("kv_evict_apply", pages, block_table, after, err_flag)
     if dst.get_device() != pages.index or src.get_device() != pages.index or counts.get_device() != pages.index:
@@ -315,8 +327,8 @@ def kv_evict_apply(pages: KVPages, block_table: torch.Tensor, plan: EvictPlan, *
             or not dst.dtype is src.dtype is counts.dtype is torch.int32
             or not (dst.is_contiguous() and src.is_contiguous() and counts.is_contiguous())):
         raise ValueError(f"the plan must hold contiguous int32 moves of ({B}, {pages.kv_heads}) heads")
-    _launch("cortex_kv_evict_apply", pages, B, block_table.data_ptr(), ld, width, dst.data_ptr(), src.data_ptr(),
-            shape[2], counts.data_ptr(), nat.ptr(err_flag))
+    nat.call("cortex_kv_evict_apply", pages.ref, B, block_table.data_ptr(), ld, width, dst.data_ptr(), src.data_ptr(),
+             shape[2], counts.data_ptr(), nat.ptr(err_flag), nat.stream_of(pages.device))
 
 
 __all__ = ["EvictPlan", "KVPages", "kv_evict_apply", "kv_evict_plan", "paged_attention", "paged_kv_append"]
