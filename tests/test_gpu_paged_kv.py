@@ -53,7 +53,8 @@ def test_attention_lengths_around_pages_and_tiles(dtype, page):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("lens", [[20011], [9000, 3, 0, 4097], [5000] * 9 + [1, 0], [0], [0, 0, 0], [2100] * 70],
+@pytest.mark.parametrize("lens", [[20011], [9000, 3, 0, 4097], [5000] * 9 + [1, 0], [0], [0, 0, 0], [2100] * 70,
+                                  [1900, 5, 0, 1025] * 40, [2048, 700, 64, 33] * 32],
                          ids=lambda v: f"{len(v)}x{max(v)}")
 def test_attention_long_and_ragged(dtype, lens):
     c = Cache(lens, 2, 64, 32, DTYPES[dtype], seed=len(lens))
@@ -123,7 +124,7 @@ def test_attention_infinities(dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim,lens", [(8, 2, 64, [5, 0, 130, 64]), (32, 8, 128, [1000, 2500, 31]),
-                                                     (20, 1, 96, [300, 33]), (4, 4, 32, [7000])])
+                                                     (20, 1, 96, [300, 33]), (4, 4, 32, [7000]), (8, 2, 64, [1500, 3, 0, 40] * 33)])
 def test_accumulated_weights(dtype, heads, kv_heads, dim, lens):
     c = Cache(lens, kv_heads, dim, 16, DTYPES[dtype], seed=11, tracked=True)
     q = c.query(heads)
