@@ -28,11 +28,11 @@ namespace {
 constexpr int PA_KT = 32;       // keys of one matrix product
 constexpr int PA_WAVES = 4;     // wavefronts of a workgroup that takes a share
 constexpr int PA_MORE = 8;      // and of one that has a CU to itself and takes a whole unit
-constexpr int PA_ROWS = 16;     // query heads of a unit
+constexpr int PA_ROWS = 16;     // query heads of one matrix product
 constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
 // Workgroups that a CU holds at once, by the registers of a tile: 128 dims 160 to 246, 64 dims in fp32 146, in fewer
 // bits 117.  (64 sequences of 500 .. 3000 keys x 64 dims, bf16: 2 a CU 55.5 us, 4 54.2; 128 dims as 3: 105 -> 110)
-__host__ __device__ constexpr int per_cu(int dhp, int es) { return dhp == 128 ? 2 : es == 4 ? 3 : 4; }
+__host__ __device__ constexpr int per_cu(int dhp, int es, int rt) { return dhp == 128 ? 2 : es == 4 || rt == 2 ? 3 : 4; }
 constexpr int PA_MAX_SHARES = 1024;
 // What it costs to begin a unit (fill and drain the loads, sum up), in tiles, where a share may have PA_LONG tiles and
 // where it has fewer: without it the shares with many short sequences are the last to end (32 sequences of 150 .. 8003
@@ -48,7 +48,8 @@ constexpr float PA_RESCALE = 8.0f;  // how far (log2) a maximum may rise before 
 struct PagedArgs {
   KvPages p;
   int B, heads, group;  // query heads, and of them to a key head
-  int row_tiles;        // units a key head: ceil(group / PA_ROWS)
+  int rows;             // query heads of a unit: 16, or 32
+  int row_tiles;        // units a key head: ceil(group / rows)
   int units;            // units a sequence: kv_heads * row_tiles
   int shares;
   int begin;            // tiles that beginning a unit counts for
@@ -61,7 +62,7 @@ struct PagedArgs {
   int64_t o_sb, o_sh;
   int32_t* err;
   // workspace
-  float* part;    // (2 shares, PA_ROWS, DHP + 2): sum p v, then m and l
+  float* part;    // (2 shares, rows, DHP + 2): sum p v, then m and l
   float* score;   // (B, heads, score_ld), for accumulate
   float* stats;   // (B, heads, 2): m and 1 / l, for accumulate
   int64_t score_ld;
@@ -130,9 +131,11 @@ __device__ __forceinline__ int share_of(const PagedArgs& a, int total) {
   return max(PA_MIN_TILES, (total + a.shares - 1) / a.shares);
 }
 
-// ONE: a workgroup takes a whole unit, so that nothing is left to join (short caches); else a share.
-template <class P, int DHP, bool PAD, bool W, int WAVES, bool ONE>
-__global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(P)) : 2) void paged_attention_kernel(PagedArgs a) {
+// ONE: a workgroup takes a whole unit, so that nothing is left to join (short caches); else a share.  RT: products of 16
+// query heads that share the rows loaded.
+template <class P, int DHP, bool PAD, bool W, int WAVES, bool ONE, int RT>
+__global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(P), RT) : 2)
+void paged_attention_kernel(PagedArgs a) {
   typedef typename Query<P>::type Q;
   constexpr int ES = sizeof(P);
   constexpr int CE = 16 / ES;           // elements of a 16-byte chunk
@@ -140,10 +143,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
   constexpr int E = DHP / 16;           // dims of a value row a lane: d = E r
   constexpr int VW = E * ES / 4;
   constexpr int LD = DHP + 4;
-  constexpr int THREADS = 64 * WAVES;
-  __shared__ __attribute__((aligned(16))) float so[WAVES][PA_ROWS][LD];
-  __shared__ float sm[WAVES][PA_ROWS], sl[WAVES][PA_ROWS];
-  __shared__ float2 stat[PA_ROWS];
+  constexpr int THREADS = 64 * WAVES, ROWS = PA_ROWS * RT;
+  __shared__ __attribute__((aligned(16))) float so[WAVES][ROWS][LD];
+  __shared__ float sm[WAVES][ROWS], sl[WAVES][ROWS];
+  __shared__ float2 stat[ROWS];
   const KvPages& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wid = wave_uniform(tid >> 6);
   const int fr = lane & 15, g = lane >> 4;
@@ -194,22 +197,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
     t0 += step;
     off += step;
     if (!ONE && ta == tb) continue;
-    const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * PA_ROWS;
-    const int rows = min(PA_ROWS, a.group - row0);  // query heads of this unit
+    const int h = u / a.row_tiles, row0 = (u - h * a.row_tiles) * ROWS;
+    const int rows = min(ROWS, a.group - row0);  // query heads of this unit
     const int head0 = h * a.group + row0;
 
     // query rows as the B operand of the scores
-    Q q[NK][CE];
-    {
-      const Q* src = reinterpret_cast<const Q*>(a.q) + b * a.q_sb + (head0 + (fr < rows ? fr : 0)) * a.q_sh;
+    Q q[RT][NK][CE];
+#pragma unroll
+    for (int y = 0; y < RT; ++y) {
+      const int row = 16 * y + fr;
+      const Q* src = reinterpret_cast<const Q*>(a.q) + b * a.q_sb + (head0 + (row < rows ? row : 0)) * a.q_sh;
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
         const int d = c * 4 * CE + g * CE;
-        const bool in = fr < rows && (!PAD || d < Dh);
+        const bool in = row < rows && (!PAD || d < Dh);
         Words<CE * sizeof(Q) / 4> w = load_words<CE * sizeof(Q) / 4>(src + (!PAD || d < Dh ? d : 0));
 #pragma unroll
         for (int i = 0; i < (int)(CE * sizeof(Q) / 4); ++i) w.w[i] = in ? w.w[i] : 0u;
-        __builtin_memcpy(q[c], w.w, sizeof(w.w));
+        __builtin_memcpy(q[y][c], w.w, sizeof(w.w));
       }
     }
 
@@ -263,10 +268,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
       }
     };
 
-    float m = -INFINITY, l = 0.0f;  // of query fr; l: the keys of this lane's group only
-    f32x4 o[E];
+    float m[RT], l[RT];  // of query 16 y + fr; l: the keys of this lane's group only
+    f32x4 o[RT][E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int y = 0; y < RT; ++y) {
+      m[y] = -INFINITY, l[y] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[y][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     int t = ta + wid;
     Ids id = {};
@@ -279,35 +288,44 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
       for (; t < tb; t += WAVES) {
         const Ids id2 = ids_of(t + 2 * WAVES);
         const bool more = t + WAVES < tb;
-        // scores of keys 8 g + 4 st + i for query fr
-        f32x4 x[2];
+        // scores of keys 8 g + 4 st + i for query 16 y + fr
+        f32x4 x[RT][2];
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+          f32x4 s[RT];
+#pragma unroll
+          for (int y = 0; y < RT; ++y) s[y] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int c = 0; c < NK; ++c) {
             Words<4> kk = kr[st][c];
-            if (PAD && c * 4 * CE + g * CE >= Dh) kk = Words<4>{{0u, 0u, 0u, 0u}};  // (the query is 0 there, the key maybe not finite)
-            if constexpr (ES == 2) {
-              bf16x8 qf;
-              __builtin_memcpy(&qf, q[c], 16);
-              s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), qf, s, 0, 0, 0);
-            } else if constexpr (ES == 4) {
+            // (the query is 0 there, the key maybe not finite)
+            if (PAD && c * 4 * CE + g * CE >= Dh) kk = Words<4>{{0u, 0u, 0u, 0u}};
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk.w[e]), q[c][e], s, 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
+            for (int y = 0; y < RT; ++y) {
+              if constexpr (ES == 2) {
                 bf16x8 qf;
-                __builtin_memcpy(&qf, q[c] + 8 * e, 16);
-                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_i8x8(make_uint2(kk.w[2 * e], kk.w[2 * e + 1])), qf, s,
-                                                            0, 0, 0);
+                __builtin_memcpy(&qf, q[y][c], 16);
+                s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kk), qf, s[y], 0, 0, 0);
+              } else if constexpr (ES == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  s[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk.w[e]), q[y][c][e], s[y], 0, 0, 0);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  bf16x8 qf;
+                  __builtin_memcpy(&qf, q[y][c] + 8 * e, 16);
+                  s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_i8x8(make_uint2(kk.w[2 * e], kk.w[2 * e + 1])), qf,
+                                                                 s[y], 0, 0, 0);
+                }
               }
             }
           }
-          x[st] = s * a.scale_log2;
-          if constexpr (ES == 1) x[st] *= ks[st];
+#pragma unroll
+          for (int y = 0; y < RT; ++y) {
+            x[y][st] = s[y] * a.scale_log2;
+            if constexpr (ES == 1) x[y][st] *= ks[st];
+          }
         }
         if (more) load_k(t + WAVES, id1);
 
@@ -319,64 +337,75 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (i >= left) {  // (what these rows hold is not looked at: 0 times it may be NaN)
-              x[i >> 2][i & 3] = -INFINITY;
+#pragma unroll
+              for (int y = 0; y < RT; ++y) x[y][i >> 2][i & 3] = -INFINITY;
               vr[i] = Words<VW>{};
               if constexpr (ES == 1) vs[i >> 2][i & 3] = 0.0f;
             }
           }
         }
         if constexpr (W) {
-          if (fr < rows) {
-            float* to = a.score + ((int64_t)b * a.heads + head0 + fr) * a.score_ld + vblock(t);
-            reinterpret_cast<f32x4*>(to)[0] = x[0];
-            reinterpret_cast<f32x4*>(to)[1] = x[1];
+#pragma unroll
+          for (int y = 0; y < RT; ++y)
+            if (16 * y + fr < rows) {
+              float* to = a.score + ((int64_t)b * a.heads + head0 + 16 * y + fr) * a.score_ld + vblock(t);
+              reinterpret_cast<f32x4*>(to)[0] = x[y][0];
+              reinterpret_cast<f32x4*>(to)[1] = x[y][1];
+            }
+        }
+        float pr[RT][8];
+        bf16x8 hi[RT], lo[RT];
+#pragma unroll
+        for (int y = 0; y < RT; ++y) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int st = 0; st < 2; ++st)
+            top = fmaxf(top, fmaxf(fmaxf(x[y][st][0], x[y][st][1]), fmaxf(x[y][st][2], x[y][st][3])));
+          top = group_max(top);
+          if (__any(top > m[y] + PA_RESCALE)) {  // (m -inf: the first key)
+            const float m_new = fmaxf(m[y], top);
+            const float alpha = exp2f(m[y] - (m_new == -INFINITY ? 0.0f : m_new));
+            l[y] *= alpha;
+#pragma unroll
+            for (int j = 0; j < E; ++j) o[y][j] *= alpha;
+            m[y] = m_new;
+          }
+          const float ref = m[y] == -INFINITY ? 0.0f : m[y];
+          float(&p8)[8] = pr[y];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p8[i] = __builtin_amdgcn_exp2f(x[y][i >> 2][i & 3] - ref);
+          l[y] += ((p8[0] + p8[1]) + (p8[2] + p8[3])) + ((p8[4] + p8[5]) + (p8[6] + p8[7]));
+          if constexpr (ES != 4) {
+            if constexpr (ES == 1) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) p8[i] *= vs[i >> 2][i & 3];
+            }
+            // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
+            // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
+            // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
+            uint32_t hw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              hw[i] = __builtin_amdgcn_perm(__float_as_uint(p8[2 * i + 1]), __float_as_uint(p8[2 * i]), 0x07060302u);
+            __builtin_memcpy(&hi[y], hw, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float rest = p8[i] - __uint_as_float(__float_as_uint(p8[i]) & 0xffff0000u);
+              lo[y][i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
+            }
           }
         }
-        float top = -INFINITY;
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-          top = fmaxf(top, fmaxf(fmaxf(x[st][0], x[st][1]), fmaxf(x[st][2], x[st][3])));
-        top = group_max(top);
-        if (__any(top > m + PA_RESCALE)) {  // (m -inf: the first key)
-          const float m_new = fmaxf(m, top);
-          const float alpha = exp2f(m - (m_new == -INFINITY ? 0.0f : m_new));
-          l *= alpha;
-#pragma unroll
-          for (int j = 0; j < E; ++j) o[j] *= alpha;
-          m = m_new;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float pr[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(x[i >> 2][i & 3] - ref);
-        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
 
-        // O^T += V^T P^T; product j: dims E (4 g + i) + j of query fr
+        // O^T += V^T P^T; product j: dims E (4 g + i) + j of query 16 y + fr
         if constexpr (ES == 4) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int j = 0; j < E; ++j)
-              o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i].w[j]), pr[i], o[j], 0, 0, 0);
+#pragma unroll
+              for (int y = 0; y < RT; ++y)
+                o[y][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i].w[j]), pr[y][i], o[y][j], 0, 0, 0);
         } else {
-          if constexpr (ES == 1) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pr[i] *= vs[i >> 2][i & 3];
-          }
-          // p as two bf16 values: its upper half and what is left.  One product with p rounded to bf16 puts the result
-          // 1.4 times as far from 64 bits (2.3e-3 against 1.7e-3, the rounding of the result) and saves nothing.  With
-          // bf16 rows the rest is kept above 0: 0 times an infinite value would be NaN
-          bf16x8 hi, lo;
-          uint32_t hw[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            hw[i] = __builtin_amdgcn_perm(__float_as_uint(pr[2 * i + 1]), __float_as_uint(pr[2 * i]), 0x07060302u);
-          __builtin_memcpy(&hi, hw, 16);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float rest = pr[i] - __uint_as_float(__float_as_uint(pr[i]) & 0xffff0000u);
-            lo[i] = (bf16)(ES == 2 ? fmaxf(rest, 1.17549435e-38f) : rest);
-          }
 #pragma unroll
           for (int j = 0; j < E; ++j) {
             bf16x8 vf;
@@ -391,8 +420,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
 #pragma unroll
               for (int i = 0; i < 8; ++i) vf[i] = (bf16)(float)(int)(int8_t)(vr[i].w[j >> 2] >> (8 * (j & 3)));
             }
-            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi, o[j], 0, 0, 0);
-            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo, o[j], 0, 0, 0);
+#pragma unroll
+            for (int y = 0; y < RT; ++y) {
+              o[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi[y], o[y][j], 0, 0, 0);
+              o[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[y], o[y][j], 0, 0, 0);
+            }
           }
         }
         if (more) {
@@ -405,19 +437,24 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
     }
 
     // the wavefronts' sums into one
-    l = group_sum(l);
     const int active = min(WAVES, tb - ta);
-    if (wid < active && fr < rows) {
-      if (g == 0) sm[wid][fr] = m, sl[wid][fr] = l;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int y = 0; y < RT; ++y) {
+      const int row = 16 * y + fr;
+      const float sum = group_sum(l[y]);
+      if (wid < active && row < rows) {
+        if (g == 0) sm[wid][row] = m[y], sl[wid][row] = sum;
 #pragma unroll
-        for (int j = 0; j < E; j += 4)
-          *reinterpret_cast<float4*>(&so[wid][fr][E * (4 * g + i) + j]) = make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < E; j += 4)
+            *reinterpret_cast<f32x4*>(&so[wid][row][E * (4 * g + i) + j]) =
+                f32x4{o[y][j][i], o[y][j + 1][i], o[y][j + 2][i], o[y][j + 3][i]};
+      }
     }
     __syncthreads();
     const bool complete = ONE || (ta == 0 && tb == tiles);
-    float* part = a.part + (2 * (int64_t)blockIdx.x + (ta == 0)) * (PA_ROWS * (DHP + 2));
+    float* part = a.part + (2 * (int64_t)blockIdx.x + (ta == 0)) * (ROWS * (DHP + 2));
     for (int i = tid; i < rows * DHP; i += THREADS) {
       const int r = i / DHP, d = i - r * DHP;
       float top = -INFINITY;  // (ONE: a sequence without keys has none)
@@ -440,7 +477,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == PA_WAVES ? per_cu(DHP, sizeof(
         }
       } else {
         part[r * DHP + d] = acc;
-        if (d == 0) part[PA_ROWS * DHP + r] = top, part[PA_ROWS * (DHP + 1) + r] = sum;
+        if (d == 0) part[ROWS * DHP + r] = top, part[ROWS * (DHP + 1) + r] = sum;
       }
     }
     __syncthreads();
@@ -471,7 +508,7 @@ constexpr int PJ_AHEAD = 8;              // loads issued before the factors that
 // with W the scores): what does not depend on the one before is loaded beside it.
 template <class Q, int DHP, bool W>
 __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int chunks) {
-  constexpr int64_t SLOT = PA_ROWS * (DHP + 2);
+  const int64_t stride = a.rows * (DHP + 2);
   constexpr int GROUPS = PJ_THREADS / DHP;  // parts summed side by side
   __shared__ float share[PA_MAX_SHARES];    // a part's factor
   __shared__ float sums[GROUPS][DHP];
@@ -496,14 +533,14 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
   const int per = share_of(a, total);
   // the shares w0 .. w1 that hold the unit of query head i
   auto unit_of = [&](int i, int* w0, int* w1) {
-    const int s = before + (h * a.row_tiles + i / PA_ROWS) * (tiles + a.begin);
+    const int s = before + (h * a.row_tiles + i / a.rows) * (tiles + a.begin);
     *w0 = min((s + a.begin) / per, a.shares - 1);
     *w1 = min((s + a.begin + tiles - 1) / per, a.shares - 1);  // (in the workspace, whatever becomes of the lengths meanwhile)
   };
-  auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * SLOT; };
+  auto slot = [&](int w, int w0) { return a.part + (2 * (int64_t)w + (w == w0)) * stride; };
 
   if (!W || c >= chunks) {
-    const int i = c - chunks, r = i % PA_ROWS;
+    const int i = c - chunks, r = i % a.rows;
     Q* out = reinterpret_cast<Q*>(a.out) + b * a.o_sb + (int64_t)(h * a.group + i) * a.o_sh;
     if (tiles == 0) {
       if (tid < a.p.head_dim) out[tid] = from_f32<Q>(0.0f);
@@ -522,10 +559,10 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
     }
     float top = -INFINITY, l0 = 0.0f;
     for (int w = tid; w < parts; w += PJ_THREADS) {
-      const float* x = slot(w0 + w, w0) + PA_ROWS * DHP + r;
+      const float* x = slot(w0 + w, w0) + a.rows * DHP + r;
       share[w] = x[0];
       top = fmaxf(top, x[0]);
-      if (w == tid) l0 = x[PA_ROWS];
+      if (w == tid) l0 = x[a.rows];
     }
     top = wave_max(top);
     if (lane == 0) red[0][wid] = top;
@@ -536,7 +573,7 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
     for (int w = tid; w < parts; w += PJ_THREADS) {
       const float f = exp2f(share[w] - ref);
       share[w] = f;
-      sum += f * (w == tid ? l0 : slot(w0 + w, w0)[PA_ROWS * (DHP + 1) + r]);
+      sum += f * (w == tid ? l0 : slot(w0 + w, w0)[a.rows * (DHP + 1) + r]);
     }
     sum = wave_sum(sum);
     if (lane == 0) red[1][wid] = sum;
@@ -577,14 +614,14 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
         if (lane == 0) stat[i] = reinterpret_cast<const float2*>(a.stats)[(int64_t)b * a.heads + h * a.group + i];
         continue;
       }
-      const int r = i % PA_ROWS;
+      const int r = i % a.rows;
       float top = -INFINITY, sum = 0.0f;
-      for (int w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, slot(w, w0)[PA_ROWS * DHP + r]);
+      for (int w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, slot(w, w0)[a.rows * DHP + r]);
       top = wave_max(top);
       const float ref = top == -INFINITY ? 0.0f : top;
       for (int w = w0 + lane; w <= w1; w += 64) {
-        const float* x = slot(w, w0) + PA_ROWS * DHP + r;
-        sum += exp2f(x[0] - ref) * x[PA_ROWS];
+        const float* x = slot(w, w0) + a.rows * DHP + r;
+        sum += exp2f(x[0] - ref) * x[a.rows];
       }
       sum = wave_sum(sum);
       if (lane == 0) stat[i] = make_float2(ref, sum == 0.0f ? 0.0f : 1.0f / sum);
@@ -611,51 +648,65 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
 
 // How a call is laid out: shares, and the parts of its workspace in bytes.
 struct Layout {
-  int row_tiles, units, shares, begin, dhp;
+  int rows, row_tiles, units, shares, begin, dhp;
   int waves;  // of a workgroup that takes a whole unit; 0: shares
   int64_t score_ld, part, score, stats;
 };
 Layout layout_of(const cortex_kv_pages* p, int64_t B, int64_t heads, int64_t most, int accumulate) {
   Layout y;
-  const int64_t group = heads / p->kv_heads;
-  y.row_tiles = (int)cdiv(group, PA_ROWS);
-  y.units = (int)(p->kv_heads * y.row_tiles);
+  const int64_t group = heads / p->kv_heads, cus = cu_count();
+  const int es = p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1;
   y.dhp = p->head_dim <= 64 ? 64 : 128;
-  const int64_t tiles = B * y.units * cdiv(most, PA_KT);
-  const int64_t shares = cdiv(tiles, PA_MIN_TILES), cus = cu_count(), pcu = per_cu(y.dhp, p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1);
+  // whole units take 16 query heads (what more there are read short caches again), shares up to 32 at once where their
+  // registers hold them (32 sequences of 8000 .. 16000 keys, one key head of 128: 32 heads 73.5 -> 64.7 us, 64 130 -> 90)
+  y.rows = PA_ROWS;
+  y.row_tiles = (int)cdiv(group, y.rows);
+  const bool full = B * p->kv_heads * y.row_tiles >= cus && es < 4;
+  y.waves = 0;
+  if (most <= (full ? PA_ONE_KEYS_FULL : PA_ONE_KEYS) && (!accumulate || y.row_tiles == 1))
+    y.waves = B * p->kv_heads * y.row_tiles > cus ? PA_WAVES : PA_MORE;
+  else if (group > PA_ROWS && es < 4)
+    y.row_tiles = (int)cdiv(group, y.rows = 2 * PA_ROWS);
+  y.units = (int)(p->kv_heads * y.row_tiles);
+  const int64_t tiles = B * y.units * cdiv(most, PA_KT), shares = cdiv(tiles, PA_MIN_TILES);
+  const int64_t pcu = per_cu(y.dhp, es, y.rows / PA_ROWS);
   const int64_t slots = cus * pcu < PA_MAX_SHARES ? cus * pcu : PA_MAX_SHARES;
   y.shares = (int)(shares < 1 ? 1 : shares < slots ? shares : slots);
   y.begin = tiles / y.shares >= PA_LONG ? PA_BEGIN_LONG : PA_BEGIN_SHORT;
   y.score_ld = cdiv(most, PA_KT) * PA_KT;
-  y.waves = 0;
-  const bool full = B * y.units >= cus && p->dtype != DT_F32;
-  if (most <= (full ? PA_ONE_KEYS_FULL : PA_ONE_KEYS) && (!accumulate || y.row_tiles == 1))
-    y.waves = B * y.units > cus ? PA_WAVES : PA_MORE;
-  y.part = y.waves ? 0 : 2ll * y.shares * PA_ROWS * (y.dhp + 2) * 4;
+  y.part = y.waves ? 0 : 2ll * y.shares * y.rows * (y.dhp + 2) * 4;
   y.score = accumulate ? B * heads * y.score_ld * 4 : 0;
   y.stats = accumulate && !y.waves ? cdiv(B * heads * 2 * 4, 16) * 16 : 0;
   return y;
 }
 
-template <class P, int DHP, bool W, int WAVES, bool ONE>
+template <class P, int DHP, bool W, int WAVES, bool ONE, int RT>
 void launch_main(const PagedArgs& a, unsigned grid, hipStream_t stream) {
+  const dim3 block(64 * WAVES);
   if (a.p.head_dim == DHP)
-    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, false, W, WAVES, ONE>), dim3(grid), dim3(64 * WAVES), 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, false, W, WAVES, ONE, RT>), dim3(grid), block, 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, true, W, WAVES, ONE>), dim3(grid), dim3(64 * WAVES), 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<P, DHP, true, W, WAVES, ONE, RT>), dim3(grid), block, 0, stream, a);
 }
 template <class P, int DHP, bool W>
 int launch(const PagedArgs& a, int waves, hipStream_t stream) {
   if (waves) {
     const unsigned units = (unsigned)a.B * (unsigned)a.units;
     if (waves == PA_WAVES)
-      launch_main<P, DHP, W, PA_WAVES, true>(a, units, stream);
+      launch_main<P, DHP, W, PA_WAVES, true, 1>(a, units, stream);
     else
-      launch_main<P, DHP, W, PA_MORE, true>(a, units, stream);
+      launch_main<P, DHP, W, PA_MORE, true, 1>(a, units, stream);
     CORTEX_CHECK_LAUNCH("paged_attention_kernel");
     return OK;
   }
-  launch_main<P, DHP, W, PA_WAVES, false>(a, (unsigned)a.shares, stream);
+  if constexpr (sizeof(P) < 4) {
+    if (a.rows > PA_ROWS)
+      launch_main<P, DHP, W, PA_WAVES, false, 2>(a, (unsigned)a.shares, stream);
+    else
+      launch_main<P, DHP, W, PA_WAVES, false, 1>(a, (unsigned)a.shares, stream);
+  } else {
+    launch_main<P, DHP, W, PA_WAVES, false, 1>(a, (unsigned)a.shares, stream);
+  }
   CORTEX_CHECK_LAUNCH("paged_attention_kernel");
   const int64_t chunks = W ? cdiv(a.max_length, PJ_KEYS) : 0;
   hipLaunchKernelGGL((paged_join_kernel<typename Query<P>::type, DHP, W>),
@@ -724,6 +775,7 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   a.B = (int)B;
   a.heads = (int)heads;
   a.group = (int)(heads / pages->kv_heads);
+  a.rows = y.rows;
   a.row_tiles = y.row_tiles;
   a.units = y.units;
   a.shares = y.shares;

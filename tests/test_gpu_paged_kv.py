@@ -64,6 +64,23 @@ def test_attention_long_and_ragged(dtype, lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(17, 1, 64), (32, 1, 128), (66, 2, 96), (80, 2, 48), (34, 2, 128)])
+def test_attention_many_heads_on_long_keys(dtype, heads, kv_heads, dim):
+    """More query heads to a key head than one product has, on keys that are split: with the weights and without."""
+    lens = [3000, 1, 0, 1100, 65]
+    c = Cache(lens, kv_heads, dim, 16, DTYPES[dtype], seed=heads, tracked=True)
+    q = c.query(heads)
+    want, added, tol, wtol = attention64(c, q)
+    check(attend(c, q), want, tol, "out")
+    check(attend(c, q, accumulate=True), want, tol, "out with weights")
+    after = c.pages.weight.cpu()
+    for b, n in enumerate(lens):
+        at = c.at(b, torch.arange(n))
+        total = c.weight[at].double() + added[b]
+        check(after[at], total, wtol[b] + 2.0 ** -24 * total, f"weight {b}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", ["row", "gap"])
 def test_attention_strided_pages_queries_and_outputs(dtype, layout):
     c = Cache([300, 41, 0, 130], 3, 64, 16, DTYPES[dtype], seed=5, layout=layout)
