@@ -18,6 +18,9 @@
 // workgroup, from the lengths on the device (a replayed graph follows them, ragged batches need no plan, and the grid
 // is one workgroup per slot of the card).  A unit cut by a share leaves its running (m, l, sum p v) in the workspace, at
 // most two a workgroup (the end of a unit and the beginning of another), and a second launch joins them in order.
+//
+// Measured (bf16, 32 query heads on 8 key heads of 128): one sequence of 131,072 keys, 537 MB, 95 us, 5.6 TB/s; 32 of 150
+// .. 8003 keys, 535 MB, 99 us.  Int8, 135 MB, 32 us: the widening on the VALU beside HBM.
 #include <hip/hip_runtime.h>
 
 #include "paged_kv.h"
@@ -505,7 +508,8 @@ constexpr int PJ_AHEAD = 8;              // loads issued before the factors that
 // and with W the weight that every key received, sum over the query heads of a key head of p_j.  Of a (sequence, key
 // head) the first `chunks` workgroups take PJ_KEYS keys' weights each, the others a query head each.  The (m, l) of
 // the parts are small: every workgroup that needs them reads them itself.  A chain of round trips (lengths, parts, and
-// with W the scores): what does not depend on the one before is loaded beside it.
+// with W the scores): what does not depend on the one before is loaded beside it.  4 to 6 us, 7 with the weights of 16
+// sequences of 2048 .. 4160 keys.
 template <class Q, int DHP, bool W>
 __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int chunks) {
   const int64_t stride = a.rows * (DHP + 2);

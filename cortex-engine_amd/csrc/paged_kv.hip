@@ -267,7 +267,9 @@ __device__ int block_scan(int v, int* part, int tid, int* total) {
 }
 
 // One workgroup a (sequence, key head): the rank of every slot, the budget-th largest by a radix selection of up to
-// four bytes, then holes and movers in slot order by prefix sums.  A thread takes Q runs of eight consecutive slots
+// four bytes, then holes and movers in slot order by prefix sums.  Bound by the chain of rounds between barriers, not by
+// bytes (256 heads of 2000 .. 9001 slots, 11 MB: 22 .. 24 us; 12 up to the ranks and the lists, 9 the selection, 3 the end;
+// 512 threads 29, 256 49).  A thread takes Q runs of eight consecutive slots
 // (one page each, four vector loads) and keeps their ranks in registers; Q 0: as many runs as there are, read again in
 // every pass.
 template <int THREADS, int Q>
@@ -460,8 +462,8 @@ struct ApplyArgs {
 
 // `lanes` lanes a row, 16 bytes of the key and of the value each; a group of lanes takes a row at a time, with the next
 // row's place looked up beside it.  Bound by HBM: rows of 256 bytes read and written at random (32 sequences of 2000 ..
-// 9001 slots down to 2048, 8 heads x 128 in bf16, 305 MB: 70 us, 4.4 TB/s; four rows a group at once 83 us, plain stores 72; a
-// workgroup for every 16 rows that there may be 71, 15 of them for the launch).
+// 9001 slots down to 2048, 8 heads x 128 in bf16, 305 MB: 70 us, 4.4 TB/s; four rows a group at once 83 us, one 72
+// with plain and with non-temporal stores, in a workgroup for every 16 rows that there may be: 15 us without a move).
 __global__ __launch_bounds__(256) void kv_evict_apply_kernel(ApplyArgs a, int es) {
   const int tid = threadIdx.x;
   const int bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;

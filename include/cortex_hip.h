@@ -550,8 +550,9 @@ int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t n_tokens, 
  * A sequence without keys gives 0.  accumulate != 0: weight of slot j += sum over the query heads
  * of its key head of p (no two sequences of the call may then share a page).  Lengths up to
  * max_length (negative: max_pages * page_size) are expected; a longer one is cut to it, as a
- * malformed length.  out may not overlap q.  B up to 4096.  workspace: cortex_paged_attention_workspace_bytes(...) bytes (0: none is
- * needed), 16-byte aligned, written before it is read. */
+ * malformed length.  out may not overlap q.  B up to 4096.  workspace:
+ * cortex_paged_attention_workspace_bytes bytes for the call's own max_length, given as the length that it
+ * stands for, not negative (0: none is needed); 16-byte aligned, written before it is read. */
 int64_t cortex_paged_attention_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t heads,
                                                int64_t max_length, int accumulate);
 int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb,
