@@ -118,6 +118,22 @@ def test_attention_scale_and_peaked_scores(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,dim", [(40, 64), (300, 128), (5000, 64)])
+def test_attention_large_values_without_weight(dtype, n, dim):
+    """Keys whose weight is below exp(-200) add nothing, whatever finite values they have."""
+    c = Cache([n], 1, dim, 16, DTYPES[dtype], seed=n)
+    q = c.query(1)
+    for j, value in [(3, 3e38), (17, -3e38), (n - 1, 1e38), (n // 2, -2e37)]:
+        at = c.table[0][j // 16].long(), 0, j % 16
+        c.k[at] = (-60 * q[0, 0].float()).to(c.k.dtype)
+        c.v[at] = value
+        for pool, own in ((c.gk, c.k), (c.gv, c.v)):
+            pool[at] = own[at].to(DEV)
+    want, _, tol, _ = attention64(c, q)
+    check(attend(c, q), want, tol, "out")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_attention_infinities(dtype):
     """Values of +-inf and NaN reach the heads and dims that they belong to and no others; a key whose score is
     -inf has no weight; a sequence with only such keys gives 0, as rows without allowed keys do elsewhere."""
