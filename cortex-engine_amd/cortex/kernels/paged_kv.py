@@ -51,7 +51,7 @@ class KVPages:
             raise ValueError("int8 pages need k_scale and v_scale, float pages take none")
         if k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("k and v need a contiguous last (head) dim")
-        if any(t is not None and t.requires_grad for t in (k, v)):
+        if any(t is not None and t.requires_grad for t in (k, v, k_scale, v_scale, weight)):
             raise ValueError("pages hold values without gradients")
         self.index = k.get_device()
         # of queries and outputs: the pages' own, bfloat16 for int8 pages
@@ -70,6 +70,8 @@ class KVPages:
         es = k.element_size()
         if any(x % 16 for t in (k, v) for x in (t.data_ptr(), *(s * es for s in t.stride()[:3]))):
             raise ValueError("page rows must be 16-byte aligned")
+        if any(t is not None and t.data_ptr() % 16 for t in (k_scale, v_scale, weight, position)):
+            raise ValueError("k_scale, v_scale, weight and position must be 16-byte aligned")
         self._struct = nat.KvPagesStruct(*k.shape, nat.code(k.dtype), *k.stride()[:3], *v.stride()[:3], nat.ptr(k),
                                          nat.ptr(v), *(nat.ptr(getattr(self, n)) for n in _PER_ROW))
         self.ref = ctypes.addressof(self._struct)
@@ -156,6 +158,15 @@ def _rows(t: torch.Tensor, pages: KVPages, es: int) -> tuple[torch.Tensor, int, 
     return t, s0, s1
 
 
+def _own_overlap(t: torch.Tensor) -> bool:
+    """Whether rows of a (n, heads, head_dim) tensor may share memory."""
+    n, m, d = t.shape
+    s, r = t.stride(0), t.stride(1)
+    if r > s and n > 1:  # (heads outside)
+        n, m, s, r = m, n, r, s
+    return (m > 1 and r < d) or (n > 1 and s < (m - 1) * r + d)
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two (n, heads, head_dim) tensors may share memory (parts of one buffer that lie in each other's gaps, such as
     the columns of a joint projection, do not)."""
@@ -183,10 +194,10 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
     """Writes the rows of new tokens behind the ``lengths`` of their sequences and returns the new lengths (B,).
 
     ``k``, ``v`` (T, kv_heads, head_dim) bf16 or fp32: token b of sequence b, or with ``offsets`` (B + 1,) int64 the
-    tokens ``[offsets[b], offsets[b + 1])`` of sequence b (no two tokens may share a slot).  Int8 pages take each row at
+    tokens ``[offsets[b], offsets[b + 1])`` of sequence b (no two tokens may share a slot).   Int8 pages take each row at
     scale ``max(max|x|, 1e-8) / 127``, rounded half to even; a row with an infinity or a NaN becomes NaN.  Tracked
     pages get weight 0 and the token's position: ``positions`` (T,) int64 (kept in 32 bits), by default its slot number.
-    ``new_lengths`` may be ``lengths`` itself.  A token without a slot or a page is dropped and sets bit 2 of
+    ``new_lengths`` may be ``lengths`` itself and overlaps no other input.  A token without a slot or a page is dropped and sets bit 2 of
     ``err_flag`` (int32, never cleared here)."""
     idx = pages.index
     if idx != _get_device():
@@ -237,7 +248,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     ``h // (heads // kv_heads)``), ``scale`` ``head_dim ** -0.5`` by default.  A sequence of length 0 gives 0.
 
     ``accumulate`` adds to ``pages.weight`` the softmax weight that each key received, summed over the query heads
-    of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q``.
+    of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q`` or itself.
     ``max_length``: a bound of the lengths known on the host (default: the table's width), which sizes the launch and
     the workspace; longer sequences are cut to it and set bit 2 of ``err_flag``, as lengths outside the table and page
     ids outside the pool do (such pages hold no keys)."""
@@ -248,7 +259,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag)
     if q.get_device() != pages.index or (out is not None and out.get_device() != pages.index):
         _elsewhere("paged_attention", pages, q, out)
-    if q.requires_grad:
+    if q.requires_grad or (out is not None and out.requires_grad):
         _no_grad("paged_attention")
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or shape[0] != B or shape[2] != pages.head_dim or dtype is not pages.query_dtype:
@@ -268,6 +279,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1:
         raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor with a contiguous last dim")
+    elif _own_overlap(out):
+        raise ValueError("out may not overlap itself (an expanded tensor)")
     elif _overlap(out, q):
         raise ValueError("out may not overlap q")
     q, qb, qh = _rows(q, pages, 4 if dtype is torch.float32 else 2)

@@ -739,6 +739,10 @@ int check_heads(const char* who, const cortex_kv_pages* pages, int64_t B, int64_
   const int64_t units = pages->kv_heads * cdiv(heads / pages->kv_heads, PA_ROWS);
   CORTEX_CHECK_ARG(most < 0 || B * units <= 0x3fffffffLL / (cdiv(most, PA_KT) + PA_BEGIN_LONG),
                    "%s: %lld sequences of up to %lld keys are too much for one call", who, (long long)B, (long long)most);
+  // (a launch has fewer than 2^32 threads: whole units of up to 512, a joining workgroup of 256 a query head and 1024 keys)
+  CORTEX_CHECK_ARG(B * units <= 0xffffffffLL / 512 &&
+                       (most < 0 || B * pages->kv_heads <= 0xffffffffLL / PJ_THREADS / (cdiv(most, PJ_KEYS) + heads / pages->kv_heads)),
+                   "%s: %lld sequences of %lld heads are too much for one call", who, (long long)B, (long long)heads);
   return OK;
 }
 

@@ -33,6 +33,8 @@ int kv_check(const char* who, const cortex_kv_pages* p, int64_t B, const int32_t
   for (int64_t s : {p->k_page, p->k_head, p->k_slot, p->v_page, p->v_head, p->v_slot})
     vec = vec && s >= 0 && (s * es) % 16 == 0;
   CORTEX_CHECK_ARG(vec, "%s: page rows must be 16-byte aligned, with strides >= 0", who);
+  CORTEX_CHECK_ARG(((uintptr_t)p->k_scale | (uintptr_t)p->v_scale | (uintptr_t)p->weight | (uintptr_t)p->position) % 16 == 0,
+                   "%s: scales, weight and position must be 16-byte aligned", who);
   CORTEX_CHECK_ARG(p->k_slot >= p->head_dim && p->v_slot >= p->head_dim, "%s: rows of a page overlap", who);
   CORTEX_CHECK_ARG(B == 0 || max_pages == 0 || table, "%s: null block table", who);
   CORTEX_CHECK_ARG(B <= 1 || ld_table >= max_pages, "%s: rows of the block table overlap", who);
@@ -507,6 +509,12 @@ int pow2_lanes(int64_t n) {
   return l;
 }
 
+// Whether n values of 64 bits at a share memory with m at b.
+bool meet(const int64_t* a, int64_t n, const int64_t* b, int64_t m) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && x < y + 8 * (uintptr_t)m && y < x + 8 * (uintptr_t)n;
+}
+
 template <class X>
 int launch_append(const AppendArgs& a, int dtype, hipStream_t stream) {
   const int lpr = pow2_lanes(a.p.head_dim / 8);
@@ -514,6 +522,8 @@ int launch_append(const AppendArgs& a, int dtype, hipStream_t stream) {
   int64_t tokens = 256 * AP_AHEAD / (2ll * a.p.kv_heads * lpr), spread = a.T / (8 * cu_count());
   tokens = tokens < spread ? tokens : spread;
   tokens = tokens < 1 ? 1 : tokens > AP_TOKENS ? AP_TOKENS : tokens;
+  CORTEX_CHECK_ARG(cdiv(a.T, tokens) <= 0xffffffffLL / 256, "cortex_kv_append: %lld tokens are too many for one call",
+                   (long long)a.T);  // (a launch has fewer than 2^32 threads)
   const dim3 grid((unsigned)cdiv(a.T, tokens)), block(256);
   if (a.T > 0) {
     if (dtype == DT_F32)
@@ -550,6 +560,9 @@ extern "C" int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t
   CORTEX_CHECK_ARG(x_dtype == DT_F32 || x_dtype == DT_BF16, "%s: rows of dtype %d (f32 or bf16)", who, x_dtype);
   if (B == 0) return OK;
   CORTEX_CHECK_ARG(lengths, "%s: null lengths", who);
+  CORTEX_CHECK_ARG((new_lengths == lengths || !meet(new_lengths, B, lengths, B)) && !meet(new_lengths, B, offsets, B + 1) &&
+                       !meet(new_lengths, B, positions, n_tokens),
+                   "%s: new_lengths overlaps an input (it may only be lengths itself)", who);
   if (n_tokens > 0) {
     CORTEX_CHECK_ARG(k && v, "%s: null k or v", who);
     const int64_t es = x_dtype == DT_F32 ? 4 : 2;
@@ -591,8 +604,9 @@ extern "C" int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, con
   a.recent = recent;
   a.cap = a.max_length > budget ? (a.max_length - budget < budget ? a.max_length - budget : budget) : 0;
   CORTEX_CHECK_ARG(lengths && counts && new_lengths && ((dst && src) || a.cap == 0), "%s: null pointer", who);
-  CORTEX_CHECK_ARG(new_lengths != lengths, "%s: new_lengths may not be lengths", who);
-  CORTEX_CHECK_ARG(B * pages->kv_heads <= 0x7fffffffLL, "%s: too many heads", who);
+  // (a launch has fewer than 2^32 threads)
+  CORTEX_CHECK_ARG(B <= 0xffffffffLL / 1024 / pages->kv_heads, "%s: too many heads", who);
+  CORTEX_CHECK_ARG(!meet(new_lengths, B, lengths, B), "%s: new_lengths may not be lengths, nor overlap them", who);
   a.lengths = lengths;
   a.dst = dst;
   a.src = src;
@@ -624,6 +638,7 @@ extern "C" int cortex_kv_evict_apply(const cortex_kv_pages* pages, int64_t B, co
   CORTEX_CHECK_ARG(cap >= 0, "%s: negative cap", who);
   if (B == 0 || cap == 0) return OK;
   CORTEX_CHECK_ARG(dst && src && counts, "%s: null pointer", who);
+  CORTEX_CHECK_ARG(B <= 0xffffffffLL / 256 / pages->kv_heads, "%s: too many heads", who);
   const int es = pages->dtype == DT_F32 ? 4 : pages->dtype == DT_BF16 ? 2 : 1;
   a.dst = dst;
   a.src = src;
@@ -635,7 +650,6 @@ extern "C" int cortex_kv_evict_apply(const cortex_kv_pages* pages, int64_t B, co
   // up to EA_PER_CU workgroups a CU for all heads together
   int64_t chunks = cdiv((int64_t)cu_count() * EA_PER_CU, B * pages->kv_heads);
   if (chunks > cdiv(cap, 256 / a.lanes)) chunks = cdiv(cap, 256 / a.lanes);
-  CORTEX_CHECK_ARG(chunks * B * pages->kv_heads <= 0x7fffffffLL, "%s: too many rows", who);
   a.chunks = (int)chunks;
   hipLaunchKernelGGL(kv_evict_apply_kernel, dim3((unsigned)(chunks * B * pages->kv_heads)), dim3(256), 0, stream, a, es);
   CORTEX_CHECK_LAUNCH("kv_evict_apply_kernel");

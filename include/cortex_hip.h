@@ -512,7 +512,7 @@ int cortex_linear_residual_ln_splitk(int64_t M, int64_t N, int64_t K, const void
  * strides; d contiguous), v likewise.  dtype 0 f32, 1 bf16, or 3 int8 with a scale per row
  * (k_scale, v_scale; the row is code * scale).  weight (the softmax weight that a key received
  * so far) and position (where in its sequence the token stood) are optional.  The four per-row
- * arrays are contiguous (num_pages, kv_heads, page_size).
+ * arrays are contiguous (num_pages, kv_heads, page_size) and 16-byte aligned.
  * page_size a power of two from 8 to 65536; head_dim a multiple of 16 up to 128; rows 16-byte
  * aligned.  A page id outside [0, num_pages), a length outside [0, max_pages * page_size] or a
  * slot without a page never reads or writes out of bounds: its rows are taken as absent and bit
@@ -536,7 +536,8 @@ typedef struct cortex_kv_pages {
  * pages s = max(max|x|, 1e-8) / 127 and clamp(rint(x / s), -127, 127), as cortex_quantize_int8
  * does (a row with an infinity or a NaN gets a scale that makes all of it NaN).  The slot's
  * weight becomes 0 and its position positions[t] (the slot number when NULL), where the pages have
- * these.  new_lengths[b] (may be lengths itself) = lengths[b] + the tokens of b that have a slot. */
+ * these.  new_lengths[b] = lengths[b] + the tokens of b that have a slot; it may be lengths itself and
+ * overlaps no other input. */
 int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t n_tokens, int x_dtype, const void* k,
                      int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                      const int32_t* block_table, int64_t ld_table, int64_t max_pages, const int64_t* offsets,
@@ -550,7 +551,7 @@ int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t n_tokens, 
  * A sequence without keys gives 0.  accumulate != 0: weight of slot j += sum over the query heads
  * of its key head of p (no two sequences of the call may then share a page).  Lengths up to
  * max_length (negative: max_pages * page_size) are expected; a longer one is cut to it, as a
- * malformed length.  out may not overlap q.  B up to 4096.  workspace:
+ * malformed length.  out may not overlap q or itself.  B up to 4096.  workspace:
  * cortex_paged_attention_workspace_bytes bytes for the call's own max_length, given as the length that it
  * stands for, not negative (0: none is needed); 16-byte aligned, written before it is read. */
 int64_t cortex_paged_attention_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t heads,
@@ -568,7 +569,7 @@ int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t head
  * The kept slots at or past `budget` (src, ascending) fill the slots below it that are not kept
  * (dst, ascending): row i of dst and src (B, kv_heads, cap) int32, -1 from counts[b, h] on; cap =
  * max(0, min(budget, max_length - budget)), max_length (negative: max_pages * page_size) as above.
- * new_lengths[b] = min(n, budget) (not lengths itself).  The pages need weight and position;
+ * new_lengths[b] = min(n, budget) (no part of lengths).  At most (2^32 - 1) / 1024 heads in all.  The pages need weight and position;
  * nothing of them is written. */
 int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
                          int64_t max_pages, const int64_t* lengths, int64_t max_length, int64_t budget,

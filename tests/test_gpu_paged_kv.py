@@ -678,6 +678,34 @@ def test_empty_batches_and_caches():
 # ------------------------------------------------------------------------------- refusals
 
 
+def test_refused_tensors():
+    from cortex.kernels.paged_kv import KVPages, paged_attention, paged_kv_append
+
+    c = Cache([40, 9], 2, 64, 16, torch.bfloat16, tracked=True)
+    q = c.query(4).to(DEV)
+    for out in (torch.empty(1, 4, 64, device=DEV, dtype=q.dtype).expand(2, 4, 64),
+                torch.empty(2, 1, 64, device=DEV, dtype=q.dtype).expand(2, 4, 64),
+                torch.empty(512, device=DEV, dtype=q.dtype).as_strided((2, 4, 64), (192, 64, 1)),
+                torch.empty(512, device=DEV, dtype=q.dtype).as_strided((2, 4, 64), (64, 32, 1))):
+        with pytest.raises(ValueError, match="overlap itself"):
+            paged_attention(q, c.pages, c.block_table, c.lengths, out=out)
+    heads_first = torch.empty(4, 2, 64, device=DEV, dtype=q.dtype).transpose(0, 1)
+    want = paged_attention(q, c.pages, c.block_table, c.lengths)
+    assert torch.equal(paged_attention(q, c.pages, c.block_table, c.lengths, out=heads_first), want)
+    with pytest.raises(RuntimeError, match="backward"):
+        paged_attention(q, c.pages, c.block_table, c.lengths, out=torch.empty_like(q, requires_grad=True))
+    off = torch.zeros(c.weight.numel() + 1, device=DEV)[1:].view(c.weight.shape)
+    with pytest.raises(ValueError, match="16-byte"):
+        KVPages(c.gk, c.gv, weight=off)
+    with pytest.raises(ValueError, match="gradients"):
+        KVPages(c.gk, c.gv, weight=c.weight.to(DEV).requires_grad_())
+    buf = torch.tensor([20, 5, 7], device=DEV)
+    rows = torch.zeros(2, 2, 64, device=DEV, dtype=q.dtype)
+    with pytest.raises(Exception, match="overlaps"):
+        paged_kv_append(c.pages, rows, rows, c.block_table, buf[:2], new_lengths=buf[1:])
+    assert buf.tolist() == [20, 5, 7]
+
+
 def test_refusals():
     from cortex.kernels.paged_kv import EvictPlan, KVPages, kv_evict_apply, kv_evict_plan, paged_attention, paged_kv_append
 

@@ -5,8 +5,12 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
 from cortex import _native as nat
+
+# the pointers are made up: where there is a GPU, a call that should have been refused and was not would follow them
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers: only where nothing can be launched")
 
 P = 16  # a pointer that no check may follow
 
@@ -75,6 +79,34 @@ def test_refused_appends():
     refused(append(pages(), k=8), "16-byte")
     refused(append(pages(), st=132), "16-byte")
     assert append(pages(), B=0, T=0) and getattr(nat.load(), "cortex_kv_append")(*append(pages(), B=0, T=0)[1:]) == 0
+
+
+def test_per_row_arrays_off_their_alignment():
+    for name in ("weight", "position"):
+        for call in (append, attention, plan, apply):
+            refused(call(pages(**{"weight": P, "position": P, name: 4})), "16-byte")
+    for name in ("k_scale", "v_scale"):
+        refused(attention(pages(dtype=nat.I8, **{"k_scale": P, "v_scale": P, name: 24})), "16-byte")
+
+
+def test_new_lengths_that_overlap_an_input():
+    n = 1 << 20
+    for out in (n + 8, n - 8):
+        refused(append(pages(), lengths=n, out=out), "overlaps")
+        refused(plan(tracked(), lengths=n, after=out), "may not be lengths")
+    for out in (n, n + 16, n - 8):  # offsets are one more than the sequences
+        refused(append(pages(), lengths=2 * n, offsets=n, out=out), "overlaps")
+    call = list(append(pages(), lengths=2 * n, out=n + 8))
+    call[-4] = n  # positions
+    refused(tuple(call), "overlaps")
+
+
+def test_launches_of_too_many_threads():
+    refused(plan(tracked(kv_heads=65535), B=65), "too many heads")
+    refused(apply(pages(kv_heads=65535), B=257), "too many heads")
+    refused(attention(pages(kv_heads=65535), B=129, heads=65535, most=32), "too much for one call")
+    refused(attention(pages(kv_heads=1024, head_dim=64), B=16, heads=1 << 20, most=16, width=1, ld=1), "too much")
+    refused(append(pages(kv_heads=65535), B=1 << 24, T=1 << 24), "too many for one call")
 
 
 def test_refused_attention():
