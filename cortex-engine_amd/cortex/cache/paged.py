@@ -34,7 +34,7 @@ class KVBatch(NamedTuple):
     """Sessions of a step as the operators take them (device tensors): ``block_table`` (B, pages) int32, the slots in use
     before the step's tokens (``before``) and with them (``lengths``), ``offsets`` (B + 1,) of the tokens (None: one a
     session), their ``positions``, and on the host ``tokens`` and ``max_length``.  It holds until one of its sessions is
-    cut or dropped; ``append`` and ``attend`` refuse it from then on."""
+    cut or dropped; ``append`` and ``attend`` refuse it from then on.  ``filled``: the layers that have its tokens' rows."""
 
     sessions: tuple[str, ...]
     block_table: torch.Tensor
@@ -48,10 +48,11 @@ class KVBatch(NamedTuple):
     versions: tuple[int, ...]
     epoch: int
     stream: torch.cuda.Stream  # that its tensors were made on
+    filled: set[int]
 
 
 class _Session:
-    __slots__ = ("pages", "used", "length", "seen", "version")
+    __slots__ = ("pages", "used", "length", "seen", "version", "pending")
 
     def __init__(self) -> None:
         self.pages = np.empty(8, dtype=np.int32)
@@ -59,6 +60,7 @@ class _Session:
         self.length = 0  # slots in use
         self.seen = 0  # tokens ever appended: the position of the next
         self.version = 0  # counts what makes batches of this session out of date
+        self.pending: list[set[int]] = []  # ``filled`` of the batches whose rows some layer may lack
 
 
 class PagedKVCache:
@@ -129,7 +131,7 @@ class PagedKVCache:
                 self.evict_session(name)
         before = np.empty(len(names), dtype=np.int64)
         positions = np.empty(int(new.sum()), dtype=np.int64)
-        at = 0
+        at, filled = 0, set()
         for i, (name, c) in enumerate(zip(names, new.tolist())):
             s = held[i]
             if s is None:
@@ -145,7 +147,9 @@ class PagedKVCache:
             at += c
             s.length += c
             s.seen += c
-        return self._batch(names, held, before, new, positions)
+            if c:
+                s.pending = [f for f in s.pending if len(f) < len(self.layers)] + [filled]
+        return self._batch(names, held, before, new, positions, filled)
 
     def batch(self, session_ids) -> KVBatch:
         """The sessions as they stand, without new tokens (KeyError: an unknown one)."""
@@ -162,19 +166,23 @@ class PagedKVCache:
         self._enter(batch)
         paged_kv_append(self.layers[layer], k, v, batch.block_table, batch.before, offsets=batch.offsets,
                         positions=batch.positions)
+        batch.filled.add(layer % len(self.layers))
 
     def attend(self, batch: KVBatch, q: torch.Tensor, layer: int = 0, *, scale: float | None = None,
                accumulate: bool | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """``paged_attention`` of one query (B, heads, head_dim) a session over its slots, the batch's new tokens among
-        them.  ``accumulate``: by default where the pages are tracked."""
+        them: ``layer`` must have their rows by then (``append``).  ``accumulate``: by default where the pages are
+        tracked."""
+        if batch.tokens and layer % len(self.layers) not in batch.filled:
+            raise RuntimeError(f"the batch's new tokens have no rows in layer {layer}: append them first")
         self._enter(batch)
         return paged_attention(q, self.layers[layer], batch.block_table, batch.lengths, scale=scale, out=out,
                                accumulate=self.tracked if accumulate is None else accumulate, max_length=batch.max_length)
 
     def evict(self, session_ids, budget: int, recent: int) -> int:
         """Cuts sessions of more than ``budget`` slots down to it in every layer, each key head keeping its ``recent``
-        newest slots and then those with the most weight (``kv_evict_plan``); returns the pages freed.  Batches made
-        before no longer hold for these sessions."""
+        newest slots and then those with the most weight (``kv_evict_plan``); returns the pages freed.  Every layer
+        must have the rows of the sessions' tokens.  Batches made before no longer hold for these sessions."""
         if not self.tracked:
             raise ValueError("eviction by weight needs tracked=True")
         if budget < 1 or not 0 <= recent <= budget:
@@ -186,6 +194,9 @@ class PagedKVCache:
         names = [n for n in names if self._sessions[n].length > budget]
         if not names:
             return 0
+        for n in names:
+            if any(len(f) < len(self.layers) for f in self._sessions[n].pending):
+                raise RuntimeError(f"session {n!r} has slots without rows in some layer: append them first")
         b = self.batch(names)
         for pages in self.layers:
             plan = kv_evict_plan(pages, b.block_table, b.lengths, budget, recent, max_length=b.max_length)
@@ -233,7 +244,7 @@ class PagedKVCache:
             batch.lengths.record_stream(stream)  # (all of a batch is one allocation)
         self._stream = stream
 
-    def _batch(self, names, held, before, new, positions) -> KVBatch:
+    def _batch(self, names, held, before, new, positions, filled) -> KVBatch:
         B, T = len(names), positions.shape[0]
         width = max((s.used for s in held), default=0)
         ragged = not (new == 1).all()
@@ -257,5 +268,5 @@ class PagedKVCache:
         parts = dev.split([c.shape[0] for c in cols])
         return KVBatch(names, parts[4].view(torch.int32)[:table.size].view(B, width), parts[0], parts[1],
                        parts[3] if ragged else None, parts[2], T, int(lengths.max()) if B else 0, tuple(held),
-                       tuple(s.version for s in held), self._epoch, self._stream)
+                       tuple(s.version for s in held), self._epoch, self._stream, filled)
 

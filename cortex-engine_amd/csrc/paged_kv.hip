@@ -271,9 +271,8 @@ __device__ int block_scan(int v, int* part, int tid, int* total) {
 // One workgroup a (sequence, key head): the rank of every slot, the budget-th largest by a radix selection of up to
 // four bytes, then holes and movers in slot order by prefix sums.  Bound by the chain of rounds between barriers, not by
 // bytes (256 heads of 2000 .. 9001 slots, 11 MB: 22 .. 24 us; 12 up to the ranks and the lists, 9 the selection, 3 the end;
-// 512 threads 29, 256 49).  A thread takes Q runs of eight consecutive slots
-// (one page each, four vector loads) and keeps their ranks in registers; Q 0: as many runs as there are, read again in
-// every pass.
+// 512 threads 29, 256 49).  A thread takes Q runs of eight consecutive slots (one page each, four vector loads) and keeps
+// their ranks in registers; Q 0: as many runs as there are, read again in every pass.
 template <int THREADS, int Q>
 __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   constexpr int WAVES = THREADS / 64;

@@ -150,6 +150,36 @@ def test_cut_sessions_refuse_older_batches():
     assert cache.evict(["a", "b"], 24, 4) == 0
 
 
+def test_slots_without_rows_are_not_read():
+    """Slots of new tokens hold what the pages' last owner left there until the rows are appended."""
+    from cortex.cache import PagedKVCache
+
+    cache = PagedKVCache(8, 1, 16, page_size=8, layers=2, tracked=True)
+    rows = torch.randn(20, 1, 16, device=DEV).bfloat16()
+    q = torch.randn(1, 2, 16, device=DEV).bfloat16()
+    first = cache.extend(["a"], [20])
+    cache.append(first, rows, rows, 0)
+    cache.attend(first, q, 0)
+    for layer in (1, -1):
+        with pytest.raises(RuntimeError, match="layer"):
+            cache.attend(first, q, layer)
+    second = cache.extend(["a"])
+    for layer in (0, -1):
+        cache.append(second, rows[:1], rows[:1], layer)
+    with pytest.raises(RuntimeError, match="without rows"):
+        cache.evict(["a"], 8, 2)  # layer 1 lacks the rows of the first batch
+    assert cache.length("a") == 21 and cache.pages_used == 3
+    assert cache.evict(["a"], 21, 2) == 0  # nothing to cut
+    cache.append(first, rows, rows, 1)
+    cache.attend(second, q, 1)
+    assert cache.evict(["a"], 8, 2) == 2
+    cache.attend(cache.batch(["a"]), q, 1)
+    third = cache.extend(["a"])
+    for layer in (0, 1):
+        cache.append(third, rows[:1], rows[:1], layer)
+    assert cache.evict(["a"], 8, 2) == 1
+
+
 def test_streams_follow_each_other():
     """Appends on one stream and attention on another, without a synchronisation by the caller."""
     from cortex.cache import PagedKVCache
