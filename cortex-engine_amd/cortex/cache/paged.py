@@ -16,7 +16,8 @@ As in the reference's paged cache (cortex/cache/streaming.py:203-233) pages come
 empty, from what was used least recently: here whole sessions, since a sequence with a gap is of no use.
 
 Not thread-safe: like the other caches it is meant for the single inference executor thread.  The operators run on
-torch's current stream; a call on another stream than the one before first waits, on the device, for that one.
+torch's current stream; a call on another stream than the one before (the first: than the one that the cache was made
+on) first waits, on the device, for that one.
 """
 
 from __future__ import annotations
@@ -79,7 +80,7 @@ class PagedKVCache:
         self._sessions: OrderedDict[str, _Session] = OrderedDict()  # least recently used first
         self._stage = torch.empty(1 << 12, dtype=torch.int64).pin_memory()
         self._staged = torch.cuda.Event()
-        self._stream: torch.cuda.Stream | None = None  # of the last call
+        self._stream = torch.cuda.current_stream(self.device)  # of the last call: here, of the pools' zero fills
         self._epoch = 0  # counts the changes of any session's version
 
     @property
@@ -232,7 +233,7 @@ class PagedKVCache:
                 if s.version != version:
                     raise RuntimeError(f"the batch is out of date: session {name!r} was cut or dropped since")
         stream = torch.cuda.current_stream(self.device)
-        if self._stream is not None and self._stream != stream:
+        if self._stream != stream:
             done = torch.cuda.Event()
             done.record(self._stream)
             stream.wait_event(done)

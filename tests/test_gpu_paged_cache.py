@@ -207,6 +207,37 @@ def test_streams_follow_each_other():
     assert torch.equal(play([one, one]), play([torch.cuda.Stream(), torch.cuda.Stream()]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8])
+def test_first_rows_on_another_stream_outlast_the_fill(dtype):
+    """The pools' zero fills wait behind other work of their stream while the first rows come on another one."""
+    from cortex.cache import PagedKVCache
+
+    rows = torch.randn(40, 2, 64, device=DEV).bfloat16()
+    busy = torch.empty(1 << 30, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(40):  # 4 GiB each
+        busy.fill_(i)
+    cache = PagedKVCache(64, 2, 64, page_size=8, dtype=dtype, layers=2, tracked=True)
+    with torch.cuda.stream(side):
+        batch = cache.extend(["a"], [40])
+        for layer in range(2):
+            cache.append(batch, rows, rows, layer)
+    torch.cuda.synchronize()
+    slots = torch.arange(40)
+    at = batch.block_table[0].cpu()[slots // 8].long(), slice(None), slots % 8
+    for p in cache.layers:
+        want = rows.cpu().double()
+        for pool, scale in ((p.k, p.k_scale), (p.v, p.v_scale)):
+            got = pool.cpu()[at].double()
+            if dtype == torch.int8:
+                c, s = codes(want.float())
+                assert torch.equal(got, c.double()) and torch.equal(scale.cpu()[at], s)
+            else:
+                assert torch.equal(got, want)
+        assert p.position.cpu()[at].tolist() == [[i, i] for i in range(40)]
+
+
 def test_refusals():
     from cortex.cache import PagedKVCache
 

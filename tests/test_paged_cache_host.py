@@ -1,0 +1,110 @@
+"""What PagedKVCache does on the host, on the CPU: streams, events and operators are stand-ins that write down what they
+were asked for."""
+
+from __future__ import annotations
+
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from cortex.cache import PagedKVCache, paged
+
+
+class Stream:
+    def __init__(self, log, name):
+        self.log, self.name = log, name
+
+    def wait_event(self, event):
+        self.log.append(("wait", self.name, event.on))
+
+    def __repr__(self):
+        return self.name
+
+
+class Host:
+    """The stand-ins: ``log`` has what was asked, in order; ``on(name)`` makes a stream the current one."""
+
+    def __init__(self, patch):
+        self.log = log = []
+        self.streams: dict[str, Stream] = {}
+        self.current = self.stream("first")
+        host = self
+
+        class Event:
+            on = None
+
+            def record(self, stream):
+                self.on = stream.name
+
+            def synchronize(self):
+                pass
+
+        def allocate(num_pages, kv_heads, page_size, head_dim, dtype, device, *, tracked=False):
+            shape = (num_pages, kv_heads, page_size)
+            made = {n: torch.zeros(*shape, head_dim) for n in ("k", "v")}
+            for n, there in [("k_scale", False), ("v_scale", False), ("weight", tracked), ("position", tracked)]:
+                made[n] = torch.zeros(shape) if there else None
+            return SimpleNamespace(**made, device=torch.device("cpu"), page_size=page_size, kv_heads=kv_heads)
+
+        def plan(pages, table, lengths, budget, recent, **kw):
+            log.append(("plan", pages))
+            return SimpleNamespace(of=pages)
+
+        patch.setattr(torch.cuda, "Event", Event)
+        patch.setattr(torch.cuda, "current_stream", lambda device=None: host.current)
+        patch.setattr(torch.Tensor, "pin_memory", lambda t: t, raising=False)
+        patch.setattr(torch.Tensor, "record_stream", lambda t, s: log.append(("record", s.name, t)), raising=False)
+        patch.setattr(paged.KVPages, "allocate", allocate)
+        patch.setattr(paged, "paged_kv_append", lambda pages, *a, **kw: log.append(("append", pages)))
+        patch.setattr(paged, "paged_attention", lambda q, pages, table, lengths, **kw: log.append(("attend", pages)))
+        patch.setattr(paged, "kv_evict_plan", plan)
+        patch.setattr(paged, "kv_evict_apply", lambda pages, table, plan: log.append(("apply", pages)))
+
+    def stream(self, name):
+        return self.streams.setdefault(name, Stream(self.log, name))
+
+    @contextlib.contextmanager
+    def on(self, name):
+        before, self.current = self.current, self.stream(name)
+        yield
+        self.current = before
+
+    def of(self, what):
+        return [e[1:] for e in self.log if e[0] == what]
+
+
+@pytest.fixture
+def host(monkeypatch):
+    return Host(monkeypatch)
+
+
+def rows(n):
+    return torch.zeros(n, 1, 16)
+
+
+def test_the_first_call_on_another_stream_waits_for_the_fill(host):
+    """The pools are zeroed on the stream that is current where the cache is made: a first call on another one waits for
+    that, and the pools are recorded for it."""
+    with host.on("made"):
+        cache = PagedKVCache(8, 1, 16, page_size=8, layers=2, tracked=True)
+    with host.on("side"):
+        batch = cache.extend(["a"], [3])
+        assert host.of("wait") == [("side", "made")]
+        cache.append(batch, rows(3), rows(3), 1)
+    assert host.of("wait") == [("side", "made")]
+    held = [t for name, t in host.of("record") if name == "side"]
+    for p in cache.layers:
+        assert all(any(t is x for x in held) for t in (p.k, p.v, p.weight, p.position))
+    with host.on("made"):
+        cache.attend(cache.extend(["b"], [0]), rows(1))
+    assert host.of("wait") == [("side", "made"), ("made", "side")]
+
+
+def test_calls_on_the_stream_of_the_fill_wait_for_nothing(host):
+    cache = PagedKVCache(8, 1, 16, page_size=8)
+    batch = cache.extend(["a"], [3])
+    cache.append(batch, rows(3), rows(3))
+    cache.attend(batch, rows(1))
+    assert not host.of("wait") and not host.of("record")
