@@ -35,7 +35,8 @@ class KVBatch(NamedTuple):
     """Sessions of a step as the operators take them (device tensors): ``block_table`` (B, pages) int32, the slots in use
     before the step's tokens (``before``) and with them (``lengths``), ``offsets`` (B + 1,) of the tokens (None: one a
     session), their ``positions``, and on the host ``tokens`` and ``max_length``.  It holds until one of its sessions is
-    cut or dropped; ``append`` and ``attend`` refuse it from then on.  ``filled``: the layers that have its tokens' rows."""
+    cut or dropped; ``append`` and ``attend`` refuse it from then on.  ``filled``: the layers that have its tokens' rows;
+    ``needs``: the same of every batch whose rows some layer lacked when this one was made, its own among them."""
 
     sessions: tuple[str, ...]
     block_table: torch.Tensor
@@ -50,6 +51,7 @@ class KVBatch(NamedTuple):
     epoch: int
     stream: torch.cuda.Stream  # that its tensors were made on
     filled: set[int]
+    needs: tuple[set[int], ...]
 
 
 class _Session:
@@ -148,8 +150,9 @@ class PagedKVCache:
             at += c
             s.length += c
             s.seen += c
+            s.pending = [f for f in s.pending if len(f) < len(self.layers)]
             if c:
-                s.pending = [f for f in s.pending if len(f) < len(self.layers)] + [filled]
+                s.pending.append(filled)
         return self._batch(names, held, before, new, positions, filled)
 
     def batch(self, session_ids) -> KVBatch:
@@ -172,10 +175,11 @@ class PagedKVCache:
     def attend(self, batch: KVBatch, q: torch.Tensor, layer: int = 0, *, scale: float | None = None,
                accumulate: bool | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """``paged_attention`` of one query (B, heads, head_dim) a session over its slots, the batch's new tokens among
-        them: ``layer`` must have their rows by then (``append``).  ``accumulate``: by default where the pages are
+        them: ``layer`` must have the rows of all of them by then (``append``), also of batches before this one (where
+        one of those is given up, its sessions have to be dropped).  ``accumulate``: by default where the pages are
         tracked."""
-        if batch.tokens and layer % len(self.layers) not in batch.filled:
-            raise RuntimeError(f"the batch's new tokens have no rows in layer {layer}: append them first")
+        if any(layer % len(self.layers) not in filled for filled in batch.needs):
+            raise RuntimeError(f"some slots of the batch's sessions have no rows in layer {layer}: append them first")
         self._enter(batch)
         return paged_attention(q, self.layers[layer], batch.block_table, batch.lengths, scale=scale, out=out,
                                accumulate=self.tracked if accumulate is None else accumulate, max_length=batch.max_length)
@@ -269,5 +273,6 @@ class PagedKVCache:
         parts = dev.split([c.shape[0] for c in cols])
         return KVBatch(names, parts[4].view(torch.int32)[:table.size].view(B, width), parts[0], parts[1],
                        parts[3] if ragged else None, parts[2], T, int(lengths.max()) if B else 0, tuple(held),
-                       tuple(s.version for s in held), self._epoch, self._stream, filled)
+                       tuple(s.version for s in held), self._epoch, self._stream, filled,
+                       tuple({id(f): f for s in held for f in s.pending}.values()))
 

@@ -28,7 +28,19 @@ def _has_gpu() -> bool:
         return False
 
 
+# Tests that expect what the operators' documentation rules out, kept as they are: each has to fail in the way given, and
+# the test named beside it holds what is right.
+_OVERTAKEN = {
+    "test_gpu_paged_cache.py::test_pages_come_from_the_least_recently_used_session": (
+        RuntimeError, "attends to 24 slots that no append has filled: test_pages_come_from_the_oldest_session"),
+}
+
+
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        if item.nodeid.split("/")[-1] in _OVERTAKEN:
+            raises, reason = _OVERTAKEN[item.nodeid.split("/")[-1]]
+            item.add_marker(pytest.mark.xfail(raises=raises, reason=reason, strict=True))
     if _has_gpu():
         return
     skip = pytest.mark.skip(reason="no ROCm GPU visible")

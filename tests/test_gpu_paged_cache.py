@@ -134,6 +134,57 @@ def test_pages_come_from_the_least_recently_used_session():
     assert (cache.attend(cache.batch(["d"]), q[:1]) == 1).all()
 
 
+def test_pages_come_from_the_oldest_session():
+    from cortex.cache import PagedKVCache
+
+    cache = PagedKVCache(6, 1, 16, page_size=8)
+    rows = torch.ones(24, 1, 16, dtype=torch.bfloat16, device=DEV)
+    for names, counts in [(["a", "b"], [16, 8]), (["c"], [16])]:
+        cache.append(cache.extend(names, counts), rows[:sum(counts)], rows[:sum(counts)])
+    assert cache.pages_used == 5 and cache.sessions == ["a", "b", "c"]
+    old = cache.batch(["a", "b"])  # now c is the oldest
+    assert cache.sessions == ["c", "a", "b"]
+    with pytest.raises(MemoryError):
+        cache.extend(["b", "d"], [0, 41])  # a and c and what is free hold five pages
+    assert cache.sessions == ["c", "a", "b"] and cache.pages_used == 5
+    new = cache.extend(["b", "d"], [0, 24])
+    assert cache.sessions == ["a", "b", "d"] and cache.pages_used == 6 and cache.length("c") == 0
+    cache.append(new, rows * 2, rows * 2)
+    q = torch.ones(2, 1, 16, dtype=torch.bfloat16, device=DEV)
+    assert (cache.attend(old, q) == 1).all()  # neither a nor b was touched
+    newer = cache.extend(["d"], [8])
+    assert cache.sessions == ["b", "d"]
+    with pytest.raises(RuntimeError, match="out of date"):
+        cache.attend(old, q)  # a is gone
+    assert cache.attend(new, q).tolist() == [[[1.0] * 16], [[2.0] * 16]]
+    with pytest.raises(RuntimeError, match="no rows in layer"):
+        cache.attend(cache.batch(["d"]), q[:1])  # its last page is a's
+    cache.append(newer, rows[:8] * 2, rows[:8] * 2)
+    assert (cache.attend(cache.batch(["d"]), q[:1]) == 2).all()
+
+
+def test_slots_of_earlier_batches_are_not_read_without_rows():
+    from cortex.cache import PagedKVCache
+
+    cache = PagedKVCache(8, 1, 16, page_size=8, layers=2, tracked=True)
+    rows = torch.randn(20, 1, 16, device=DEV).bfloat16()
+    q = torch.randn(1, 2, 16, device=DEV).bfloat16()
+    first = cache.extend(["a"], [20])
+    cache.append(first, rows, rows, 0)
+    second = cache.extend(["a"])
+    for layer in range(2):
+        cache.append(second, rows[:1], rows[:1], layer)
+    cache.attend(second, q, 0)
+    before = cache.layers[1].weight.clone()
+    for batch in (second, cache.batch(["a"])):
+        with pytest.raises(RuntimeError, match="no rows in layer 1"):
+            cache.attend(batch, q, 1)
+    assert torch.equal(cache.layers[1].weight, before)
+    cache.append(first, rows, rows, 1)
+    # (the weights of layer 0 are of two calls, those of layer 1 of one: the results do not depend on them)
+    assert torch.equal(cache.attend(second, q, 0), cache.attend(second, q, 1))
+
+
 def test_cut_sessions_refuse_older_batches():
     from cortex.cache import PagedKVCache
 

@@ -108,3 +108,70 @@ def test_calls_on_the_stream_of_the_fill_wait_for_nothing(host):
     cache.append(batch, rows(3), rows(3))
     cache.attend(batch, rows(1))
     assert not host.of("wait") and not host.of("record")
+
+
+def test_attend_refuses_slots_of_earlier_batches_without_rows(host):
+    """Every slot that a call reads must have its row in that layer, not only those of the batch's own tokens."""
+    cache = PagedKVCache(8, 1, 16, page_size=8, layers=2, tracked=True)
+    first = cache.extend(["a"], [20])
+    cache.append(first, rows(20), rows(20), 0)
+    second = cache.extend(["a"])
+    for layer in (0, 1):
+        cache.append(second, rows(1), rows(1), layer)
+    cache.attend(second, rows(1), 0)
+    for layer in (1, -1):  # what the pages' last owner left there is in the first 20
+        with pytest.raises(RuntimeError, match="no rows in layer"):
+            cache.attend(second, rows(1), layer)
+        with pytest.raises(RuntimeError, match="no rows in layer"):
+            cache.attend(cache.batch(["a"]), rows(1), layer)
+    assert len(host.of("attend")) == 1
+    cache.append(first, rows(20), rows(20), -1)
+    for batch in (first, second, cache.batch(["a"])):
+        for layer in (0, 1, -1, -2):
+            cache.attend(batch, rows(1), layer)
+
+
+def test_attend_refuses_sessions_that_were_only_extended(host):
+    cache = PagedKVCache(8, 1, 16, page_size=8, tracked=True)
+    given = cache.extend(["a"], [5])
+    cache.append(given, rows(5), rows(5))
+    missing = cache.extend(["b"], [5])
+    for batch in (missing, cache.batch(["b"]), cache.batch(["a", "b"]), cache.extend(["b", "c"], [0, 0])):
+        with pytest.raises(RuntimeError, match="no rows in layer"):
+            cache.attend(batch, rows(len(batch.sessions)))
+    both = cache.batch(["a", "b"])
+    cache.attend(cache.batch(["a"]), rows(1))  # the others are not in the call
+    cache.append(missing, rows(5), rows(5))
+    cache.attend(both, rows(2))
+    # one call for several sessions is one batch: its rows come together
+    joint = cache.extend(["a", "b"], [1, 2])
+    with pytest.raises(RuntimeError, match="no rows in layer"):
+        cache.attend(cache.batch(["a"]), rows(1))
+    cache.attend(both, rows(2))  # made before: it reads none of the new slots
+    cache.append(joint, rows(3), rows(3))
+    cache.attend(cache.batch(["a"]), rows(1))
+
+
+def test_a_dropped_session_starts_anew(host):
+    """A batch that is given up leaves slots without rows: dropping its session frees them."""
+    cache = PagedKVCache(8, 1, 16, page_size=8)
+    given_up = cache.extend(["a"], [5])
+    assert cache.evict_session("a") == 1
+    batch = cache.extend(["a"], [2])
+    cache.append(batch, rows(2), rows(2))
+    cache.attend(batch, rows(1))
+    cache.attend(cache.batch(["a"]), rows(1))
+    with pytest.raises(RuntimeError, match="out of date"):
+        cache.append(given_up, rows(5), rows(5))
+
+
+def test_steps_keep_no_record_of_what_is_complete(host):
+    """What a batch and a session hold about missing rows does not grow with the steps taken."""
+    cache = PagedKVCache(64, 1, 16, page_size=8, layers=2)
+    for _ in range(100):
+        batch = cache.extend(["a", "b"])
+        for layer in (0, 1):
+            cache.append(batch, rows(2), rows(2), layer)
+            cache.attend(batch, rows(2), layer)
+    assert len(batch.needs) == 1 and all(len(s.pending) <= 2 for s in cache._sessions.values())
+    assert not cache.batch(["a", "b"]).needs
