@@ -117,11 +117,12 @@ class PagedKVCache:
             new = np.asarray(counts, dtype=np.int64).reshape(-1)
             if new.shape[0] != len(names) or (new < 0).any():
                 raise ValueError(f"counts must be {len(names)} numbers >= 0")
-        held = [self._sessions.get(n) for n in names]
-        need = [-(-((s.length if s else 0) + int(c)) // self.page_size) - (s.used if s else 0) for s, c in zip(held, new)]
-        missing = sum(n for n in need if n > 0) - len(self._free)
+        held = [self._sessions.get(n) or _Session() for n in names]
+        need = [max(0, -(-(s.length + int(c)) // self.page_size) - s.used) for s, c in zip(held, new)]
+        total = sum(need)
+        missing, victims = total - len(self._free), []
         if missing > 0:
-            keep, victims = set(names), []
+            keep = set(names)
             for name, s in self._sessions.items():
                 if missing <= 0:
                     break
@@ -129,31 +130,55 @@ class PagedKVCache:
                     victims.append(name)
                     missing -= s.used
             if missing > 0:
-                raise MemoryError(f"{missing} pages short of {sum(n for n in need if n > 0)} (of {self.num_pages} in all)")
-            for name in victims:
-                self.evict_session(name)
-        before = np.empty(len(names), dtype=np.int64)
+                raise MemoryError(f"{missing} pages short of {total} (of {self.num_pages} in all)")
+        # the end of the free list as it is once the victims are gone, the last one first
+        taken = [p for name in victims for p in self._sessions[name].pages[:self._sessions[name].used].tolist()][::-1]
+        taken = taken[:total] + self._free[len(self._free) - max(0, total - len(taken)):][::-1]
+        B, width = len(names), max((s.used + n for s, n in zip(held, need)), default=0)
+        table = np.full((B, width), -1, dtype=np.int32)
+        before = np.empty(B, dtype=np.int64)
         positions = np.empty(int(new.sum()), dtype=np.int64)
-        at, filled = 0, set()
-        for i, (name, c) in enumerate(zip(names, new.tolist())):
-            s = held[i]
-            if s is None:
-                s = self._sessions[name] = held[i] = _Session()
-            self._sessions.move_to_end(name)
-            for _ in range(need[i]):
-                if s.used == s.pages.shape[0]:
-                    s.pages = np.concatenate([s.pages, np.empty_like(s.pages)])
-                s.pages[s.used] = self._free.pop()
-                s.used += 1
+        at = row = 0
+        for i, (s, n, c) in enumerate(zip(held, need, new.tolist())):
+            table[i, :s.used] = s.pages[:s.used]
+            if n:
+                table[i, s.used:s.used + n] = taken[at:at + n]
+                at += n
             before[i] = s.length
-            positions[at:at + c] = np.arange(s.seen, s.seen + c)
-            at += c
+            if c == 1:
+                positions[row] = s.seen
+            else:
+                positions[row:row + c] = np.arange(s.seen, s.seen + c)
+            row += c
+        ragged = not (new == 1).all()
+        offsets = np.concatenate([[0], np.cumsum(new)]) if ragged else np.empty(0, dtype=np.int64)
+        flat = np.zeros(-(-table.size // 2) * 2, dtype=np.int32)
+        flat[:table.size] = table.reshape(-1)
+        parts = self._upload([before, before + new, positions, offsets.astype(np.int64, copy=False), flat.view(np.int64)])
+
+        # nothing that may fail comes after this
+        for name in victims:
+            self.evict_session(name)
+        del self._free[len(self._free) - total:]
+        filled: set[int] = set()
+        for name, s, n, c, pages in zip(names, held, need, new.tolist(), table):
+            self._sessions[name] = s
+            self._sessions.move_to_end(name)
+            if n:
+                if s.used + n > s.pages.shape[0]:
+                    s.pages = np.concatenate([s.pages[:s.used], np.empty(s.used + 2 * n, dtype=np.int32)])
+                s.pages[s.used:s.used + n] = pages[s.used:s.used + n]
+                s.used += n
             s.length += c
             s.seen += c
-            s.pending = [f for f in s.pending if len(f) < len(self.layers)]
+            if s.pending:
+                s.pending = [f for f in s.pending if len(f) < len(self.layers)]
             if c:
                 s.pending.append(filled)
-        return self._batch(names, held, before, new, positions, filled)
+        return KVBatch(names, parts[4].view(torch.int32)[:table.size].view(B, width), parts[0], parts[1],
+                       parts[3] if ragged else None, parts[2], positions.shape[0],
+                       int((before + new).max()) if B else 0, tuple(held), tuple(s.version for s in held), self._epoch,
+                       self._stream, filled, tuple({id(f): f for s in held for f in s.pending}.values()))
 
     def batch(self, session_ids) -> KVBatch:
         """The sessions as they stand, without new tokens (KeyError: an unknown one)."""
@@ -249,18 +274,8 @@ class PagedKVCache:
             batch.lengths.record_stream(stream)  # (all of a batch is one allocation)
         self._stream = stream
 
-    def _batch(self, names, held, before, new, positions, filled) -> KVBatch:
-        B, T = len(names), positions.shape[0]
-        width = max((s.used for s in held), default=0)
-        ragged = not (new == 1).all()
-        table = np.full((B, width), -1, dtype=np.int32)
-        for i, s in enumerate(held):
-            table[i, :s.used] = s.pages[:s.used]
-        lengths = before + new
-        offsets = np.concatenate([[0], np.cumsum(new)]) if ragged else np.empty(0, dtype=np.int64)
-        flat = np.zeros(-(-table.size // 2) * 2, dtype=np.int32)
-        flat[:table.size] = table.reshape(-1)
-        cols = [before, lengths, positions, offsets.astype(np.int64, copy=False), flat.view(np.int64)]
+    def _upload(self, cols: list[np.ndarray]) -> list[torch.Tensor]:
+        """int64 arrays on the device, parts of one allocation and one pinned copy."""
         need = sum(c.shape[0] for c in cols)
         self._enter()
         self._staged.synchronize()  # the copy before has left the pinned buffer
@@ -270,9 +285,4 @@ class PagedKVCache:
         dev = torch.empty(need, dtype=torch.int64, device=self.device)
         dev.copy_(self._stage[:need], non_blocking=True)
         self._staged.record(torch.cuda.current_stream(self.device))
-        parts = dev.split([c.shape[0] for c in cols])
-        return KVBatch(names, parts[4].view(torch.int32)[:table.size].view(B, width), parts[0], parts[1],
-                       parts[3] if ragged else None, parts[2], T, int(lengths.max()) if B else 0, tuple(held),
-                       tuple(s.version for s in held), self._epoch, self._stream, filled,
-                       tuple({id(f): f for s in held for f in s.pending}.values()))
-
+        return dev.split([c.shape[0] for c in cols])

@@ -175,3 +175,45 @@ def test_steps_keep_no_record_of_what_is_complete(host):
             cache.attend(batch, rows(2), layer)
     assert len(batch.needs) == 1 and all(len(s.pending) <= 2 for s in cache._sessions.values())
     assert not cache.batch(["a", "b"]).needs
+
+
+def state(cache):
+    return {"free": list(cache._free), "order": cache.sessions, "epoch": cache._epoch,
+            "sessions": {n: (s.pages[:s.used].tolist(), s.length, s.seen, s.version, [set(f) for f in s.pending])
+                         for n, s in cache._sessions.items()}}
+
+
+@pytest.mark.parametrize("fails", ["memory of the device", "pinned memory", "copy"])
+def test_an_extend_that_fails_changes_nothing(host, monkeypatch, fails):
+    """Neither the sessions of the call nor those that would have given way."""
+    cache = PagedKVCache(700, 1, 16, page_size=8)
+    for name, count in [("a", 8 * 600), ("b", 8 * 90), ("c", 9)]:
+        batch = cache.extend([name], [count])
+        cache.append(batch, rows(count), rows(count))
+    pending = cache.extend(["c"])
+    before = state(cache)
+
+    def out_of_memory(*args, **kw):
+        raise torch.OutOfMemoryError("out of memory")
+
+    with monkeypatch.context() as m:
+        if fails == "pinned memory":
+            m.setattr(torch.Tensor, "pin_memory", out_of_memory, raising=False)
+            cache._stage = cache._stage[:1]
+        elif fails == "copy":
+            m.setattr(torch.Tensor, "copy_", out_of_memory)
+        else:
+            empty = torch.empty
+
+            def no_device(*args, **kw):
+                return out_of_memory() if "device" in kw else empty(*args, **kw)
+
+            m.setattr(torch, "empty", no_device)
+        for names, counts in [(["c"], [4000]), (["d", "b"], [4095, 1]), (["d"], [0]), (["c", "d"], [1, 8 * 650])]:
+            with pytest.raises(torch.OutOfMemoryError):
+                cache.extend(names, counts)
+            assert state(cache) == before
+    cache.append(pending, rows(1), rows(1))
+    batch = cache.extend(["d", "c"], [4000, 1])
+    assert cache.sessions == ["b", "d", "c"] and cache.length("c") == 11 and batch.positions[-1] == 10
+    assert sorted(cache._free + [p for s in cache._sessions.values() for p in s.pages[:s.used].tolist()]) == list(range(700))
