@@ -197,8 +197,9 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
     tokens ``[offsets[b], offsets[b + 1])`` of sequence b (no two tokens may share a slot).   Int8 pages take each row at
     scale ``max(max|x|, 1e-8) / 127``, rounded half to even; a row with an infinity or a NaN becomes NaN.  Tracked
     pages get weight 0 and the token's position: ``positions`` (T,) int64 (kept in 32 bits), by default its slot number.
-    ``new_lengths`` may be ``lengths`` itself and overlaps no other input.  A token without a slot or a page is dropped and sets bit 2 of
-    ``err_flag`` (int32, never cleared here)."""
+    ``new_lengths`` may be ``lengths`` itself and overlaps no other input.  A token without a slot or a page, or of a sequence
+    whose length is negative or past the table, is dropped and sets bit 2 of ``err_flag`` (int32, never cleared here); a
+    negative length stays negative."""
     idx = pages.index
     if idx != _get_device():
         with torch.cuda.device(idx):

@@ -96,14 +96,17 @@ __device__ __forceinline__ void store8(bf16* p, const float (&f)[8]) {
   __builtin_nontemporal_store(__builtin_bit_cast(i32x4, a), reinterpret_cast<i32x4*>(p));
 }
 
+// The length after n more tokens.  A negative one stays as it is: as 0 the next call would write over the first rows.
+__device__ __forceinline__ int64_t length_after(const KvPages& p, int64_t len, int64_t n) {
+  return len < 0 ? len : min(min(len, p.max_slots) + n, p.max_slots);
+}
+
 // The lengths after a ragged append, by thread `at` of `threads`.
 __device__ void lengths_after(const AppendArgs& a, int at, int threads) {
   if (!a.new_lengths) return;
   for (int64_t b = at; b < a.B; b += threads) {
-    bool ok = true;
-    const int64_t len = a.p.length_of(a.lengths, b, a.p.max_slots, &ok);
     const int64_t lo = min(max(a.offsets[b], (int64_t)0), a.T), hi = min(max(a.offsets[b + 1], lo), a.T);
-    a.new_lengths[b] = min(len + (hi - lo), a.p.max_slots);
+    a.new_lengths[b] = length_after(a.p, a.lengths[b], hi - lo);
   }
 }
 
@@ -144,14 +147,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr, i
     }
     int page = -1;
     if (mine) {
-      bool ok = true;
-      const int64_t len = p.length_of(a.lengths, b, p.max_slots, &ok), slot = len + (t - first);
-      page = p.page_of(b, slot);
-      if (!ok || page < 0) kv_flag(a.err);
+      const int64_t len = a.lengths[b], slot = min(len, p.max_slots) + (t - first);
+      if (len >= 0 && len <= p.max_slots) page = p.page_of(b, slot);  // (a malformed length has no slots)
+      if (page < 0) kv_flag(a.err);
       at_row[tid] = p.row_of(slot);
       at_slot[tid] = (int)slot;
       // (may be lengths[b], which this thread alone reads: a token a sequence)
-      if (!a.offsets && a.new_lengths) a.new_lengths[b] = min(len + 1, p.max_slots);
+      if (!a.offsets && a.new_lengths) a.new_lengths[b] = length_after(p, len, 1);
     }
     at_page[tid] = page;
   }
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   bool ok = true;
   const int n = (int)a.p.length_of(a.lengths, b, a.max_length, &ok);
   if (!ok && tid == 0) kv_flag(a.err);
-  if (h == 0 && tid == 0) a.new_lengths[b] = min((int64_t)n, a.budget);
+  if (h == 0 && tid == 0) a.new_lengths[b] = a.lengths[b] < 0 ? a.lengths[b] : min((int64_t)n, a.budget);
   int moved = 0;
   if (n > a.budget && a.budget > 0) {
     const int budget = (int)a.budget;

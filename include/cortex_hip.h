@@ -537,7 +537,8 @@ typedef struct cortex_kv_pages {
  * does (a row with an infinity or a NaN gets a scale that makes all of it NaN).  The slot's
  * weight becomes 0 and its position positions[t] (the slot number when NULL), where the pages have
  * these.  new_lengths[b] = lengths[b] + the tokens of b that have a slot; it may be lengths itself and
- * overlaps no other input. */
+ * overlaps no other input.  The tokens of a sequence with a malformed length have none and are dropped; a
+ * negative length stays as it is, one past the table becomes max_pages * page_size. */
 int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t n_tokens, int x_dtype, const void* k,
                      int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                      const int32_t* block_table, int64_t ld_table, int64_t max_pages, const int64_t* offsets,
@@ -569,7 +570,7 @@ int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t head
  * The kept slots at or past `budget` (src, ascending) fill the slots below it that are not kept
  * (dst, ascending): row i of dst and src (B, kv_heads, cap) int32, -1 from counts[b, h] on; cap =
  * max(0, min(budget, max_length - budget)), max_length (negative: max_pages * page_size) as above.
- * new_lengths[b] = min(n, budget) (no part of lengths).  At most (2^32 - 1) / 1024 heads in all.  The pages need weight and position;
+ * new_lengths[b] = min(n, budget) (no part of lengths), a negative length as it is.  At most (2^32 - 1) / 1024 heads in all.  The pages need weight and position;
  * nothing of them is written. */
 int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
                          int64_t max_pages, const int64_t* lengths, int64_t max_length, int64_t budget,

@@ -33,6 +33,8 @@ def _has_gpu() -> bool:
 _OVERTAKEN = {
     "test_gpu_paged_cache.py::test_pages_come_from_the_least_recently_used_session": (
         RuntimeError, "attends to 24 slots that no append has filled: test_pages_come_from_the_oldest_session"),
+    "test_gpu_paged_kv.py::test_append_without_room_or_page": (
+        AssertionError, "a negative length has the token written over the first row: test_append_without_room_page_or_length"),
 }
 
 

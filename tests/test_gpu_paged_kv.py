@@ -359,6 +359,64 @@ def test_append_without_room_or_page():
     assert torch.equal(c.gk[c.table[0, 1].long(), :, 7], many[11])
 
 
+def test_append_without_room_page_or_length():
+    from cortex.kernels.paged_kv import paged_kv_append
+
+    c = Cache([16, 15, 3, 5, 4], 2, 32, 8, torch.bfloat16, seed=4, tracked=True)
+    k = torch.randn(5, 2, 32, generator=c.g).to(torch.bfloat16)
+    c.block_table[2, 0] = c.num
+    c.lengths[3] = -1
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    before = c.gk.clone()
+    got = paged_kv_append(c.pages, k.to(DEV), k.to(DEV), c.block_table, c.lengths, err_flag=flag)
+    assert got.tolist() == [16, 16, 4, -1, 5] and int(flag) == 4
+    changed = (c.gk.nan_to_num(9.0) != before.nan_to_num(9.0)).any(-1).any(1).nonzero().tolist()
+    assert sorted(changed) == sorted([[int(c.table[1, 1]), 7], [int(c.table[4, 0]), 4]])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts", [None, [3, 2, 0, 4, 1, 40]])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_append_to_malformed_lengths(dtype, counts, in_place):
+    """Step after step the rows of other sequences arrive and those of a malformed length touch nothing; no step makes a
+    negative length a valid one."""
+    from cortex.kernels.paged_kv import kv_evict_plan, paged_attention, paged_kv_append
+
+    lens = [9, 5, 7, 6, 4, 3]
+    c = Cache(lens, 2, 32, 8, DTYPES[dtype], seed=12, room=87, tracked=True)
+    most = c.width * 8
+    bad = {0: -1, 2: -(1 << 62), 3: most + 1, 5: (1 << 63) - 2}
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([bad.get(b, n) for b, n in enumerate(lens)], device=DEV)
+    pools = _append_plain(c, torch.zeros(0, 2, 32), torch.zeros(0, 2, 32), [0] * 7, None, DTYPES[dtype])
+    per = counts or [1] * 6
+    off = [sum(per[:i]) for i in range(7)]
+    want = list(lens)
+    for _ in range(2):
+        k, v = (torch.randn(off[-1], 2, 32, generator=c.g).to(torch.bfloat16) for _ in range(2))
+        lengths = paged_kv_append(c.pages, k.to(DEV), v.to(DEV), c.block_table, lengths, err_flag=flag,
+                                  offsets=None if counts is None else torch.tensor(off, device=DEV),
+                                  new_lengths=lengths if in_place else None)
+        for b in (1, 4):
+            slots = torch.arange(want[b], want[b] + per[b])
+            at = c.at(b, slots)
+            for name, x in (("k", k), ("v", v)):
+                x = x[off[b]:off[b + 1]]
+                if dtype == "int8":
+                    pools[name][at], pools[name + "_scale"][at] = codes(x.float())
+                else:
+                    pools[name][at] = x.to(DTYPES[dtype])
+            pools["weight"][at] = 0.0
+            pools["position"][at] = slots[:, None].int()
+            want[b] += per[b]
+        assert lengths.tolist() == [-1, want[1], -(1 << 62), most, want[4], most] and int(flag) == 4
+        _same(c, pools)
+    for n in (0, 1):
+        assert kv_evict_plan(c.pages, c.block_table, lengths, 2, n).lengths.tolist() == [-1, 2, -(1 << 62), 2, 2, 2]
+    out = paged_attention(c.query(4).to(DEV), c.pages, c.block_table, lengths)
+    assert (out[[0, 2]] == 0).all()
+
+
 # ------------------------------------------------------------------------------- eviction
 
 
