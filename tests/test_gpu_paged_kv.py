@@ -310,6 +310,30 @@ def test_append_ragged(dtype, counts):
 
 
 @pytest.mark.parametrize("x", ["bf16", "fp32"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,kv_heads,dim", [(4099, 2, 64), (6151, 3, 48), (16801, 8, 128), (133001, 1, 16), (70001, 1, 32)])
+def test_append_several_tokens_a_workgroup(x, dtype, tokens, kv_heads, dim):
+    """Enough tokens that a workgroup takes several of them (2, 3, 4, 64 and 34 on 256 CUs), the last one fewer, and sequences
+    begin and end inside its share."""
+    from cortex.kernels.paged_kv import paged_kv_append
+
+    g = torch.Generator().manual_seed(tokens)
+    cuts = torch.randint(0, tokens + 1, (40,), generator=g).sort().values.tolist()
+    off = [0, 0, *cuts, tokens, tokens]  # (empty sequences at both ends)
+    counts = [b - a for a, b in zip(off, off[1:])]
+    lens = [(5 * i) % 23 for i in range(len(counts))]
+    c = Cache(lens, kv_heads, dim, 32, DTYPES[dtype], seed=tokens, room=max(counts), tracked=True)
+    k, v = (torch.randn(tokens + 2, kv_heads, dim, generator=g).to(DTYPES[x]) for _ in range(2))
+    pos = torch.randint(0, 10 ** 6, (tokens + 2,), generator=g)
+    pools = _append_plain(c, k, v, off, pos, DTYPES[dtype])
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = paged_kv_append(c.pages, k.to(DEV), v.to(DEV), c.block_table, c.lengths, offsets=torch.tensor(off, device=DEV),
+                          positions=pos.to(DEV), err_flag=flag)
+    assert got.tolist() == [n + m for n, m in zip(lens, counts)] and int(flag) == 0
+    _same(c, pools)
+
+
+@pytest.mark.parametrize("x", ["bf16", "fp32"])
 def test_append_int8_rows_without_a_scale(x):
     """Ties round half to even; an infinity or a NaN makes all of its row NaN, and no other row."""
     from cortex.kernels.paged_kv import paged_kv_append
@@ -493,6 +517,43 @@ def test_evict_long(lens, budget):
         assert plan.dst[b, 0, :len(dst)].tolist() == dst and plan.src[b, 0, :len(src)].tolist() == src
         assert int(plan.counts[b, 0]) == len(dst) and (plan.dst[b, 0, len(dst):] == -1).all()
     assert moves
+
+
+@pytest.mark.parametrize("values", ["random", "ties", "swapped"])
+@pytest.mark.parametrize("most", [2048, 2049, 8192, 8193, 16384, 16385, 32768, 32769])
+def test_evict_around_the_forms_of_the_plan(values, most):
+    """The longest sequence that a form of the plan takes (one, two and four runs of slots a thread, or any number), and one
+    more; with every kept slot in the upper half all of the lower half is filled from there."""
+    lens, budget = [most, most - 1, most // 2 + 1, most - 9, 3], most // 2
+    c = Cache(lens, 2, 16, 64, torch.bfloat16, seed=most, tracked=True)
+    for b, n in enumerate(lens):
+        at = c.at(b, torch.arange(n))
+        if values == "ties":
+            c.weight[at] = torch.randint(0, 3, (n, 2), generator=c.g).float()
+        elif values == "swapped":
+            c.weight[at] = torch.where(torch.arange(n) < n // 2, 0.0, 1.0)[:, None] + torch.rand(n, 2, generator=c.g) / 2
+        c.position[at] = torch.stack([torch.randperm(n, generator=c.g) for _ in range(2)], 1).int()
+    c.pages.weight.copy_(c.weight)
+    recent = 0 if values == "swapped" else 33
+    c.pages.position.copy_(c.position)
+    pools = {n: getattr(c.pages, n).cpu() for n in ("k", "v", "weight", "position")}
+    plan = _evict(c, budget, recent, max_length=most)
+    cap = min(budget, most - budget)
+    assert plan.dst.shape == plan.src.shape == (len(lens), 2, cap)
+    assert plan.lengths.tolist() == [min(n, budget) for n in lens]
+    for b, n in enumerate(lens):
+        at = c.at(b, torch.arange(n))
+        for h in range(2):
+            dst, src = evict64(c.weight[at][:, h], c.position[at][:, h], n, budget, recent)
+            if values == "swapped" and n == most and most % 2 == 0:
+                assert len(dst) == most // 2
+            assert int(plan.counts[b, h]) == len(dst) == len(src)
+            assert plan.dst[b, h].tolist() == dst + [-1] * (cap - len(dst))
+            assert plan.src[b, h].tolist() == src + [-1] * (cap - len(src))
+            d, s = torch.tensor(dst, dtype=torch.int64), torch.tensor(src, dtype=torch.int64)
+            for t in pools.values():
+                t[c.table[b, d // 64].long(), h, d % 64] = t[c.table[b, s // 64].long(), h, s % 64]
+    _same(c, pools)
 
 
 @pytest.mark.parametrize("values", ["ties", "one", "special", "tiny"])
