@@ -13,7 +13,7 @@ current stream, never synchronising:
 
 ``cortex.cache.PagedKVCache`` keeps pages, tables and lengths for named sessions.  No reference counterpart:
 its StreamingKVCache (cortex/cache/streaming.py:79-236) pages embedding rows and attends to none of them.
-Inference only: inputs that require a gradient are refused.
+Inference only: inputs that require a gradient or carry a forward-mode tangent are refused.
 """
 
 from __future__ import annotations
@@ -22,6 +22,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from cortex import _native as nat
 
@@ -53,6 +54,8 @@ class KVPages:
             raise ValueError("k and v need a contiguous last (head) dim")
         if any(t is not None and t.requires_grad for t in (k, v, k_scale, v_scale, weight)):
             raise ValueError("pages hold values without gradients")
+        if forward_ad._current_level >= 0:
+            _no_tangent("KVPages", k, v, k_scale, v_scale, weight)
         self.index = k.get_device()
         # of queries and outputs: the pages' own, bfloat16 for int8 pages
         self.query_dtype = torch.bfloat16 if k.dtype == torch.int8 else k.dtype
@@ -145,6 +148,12 @@ def _no_grad(what: str) -> None:
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
+def _no_tangent(what: str, *tensors: torch.Tensor | None) -> None:
+    """Within a level of forward-mode differentiation (the callers ask for that, which is cheaper)."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
+
+
 def _rows(t: torch.Tensor, pages: KVPages, es: int) -> tuple[torch.Tensor, int, int]:
     """(n, heads, head_dim) rows that vector loads take, as given or copied, and their strides."""
     if t.is_contiguous():
@@ -212,6 +221,8 @@ def paged_kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_tabl
         _elsewhere("paged_kv_append", pages, k, v, offsets, positions, new_lengths)
     if k.requires_grad or v.requires_grad:
         _no_grad("paged_kv_append")
+    if forward_ad._current_level >= 0:
+        _no_tangent("paged_kv_append", k, v)
     shape, dtype = k.shape, k.dtype
     if shape != v.shape or len(shape) != 3 or shape[1:] != (pages.kv_heads, pages.head_dim) or dtype is not v.dtype:
         raise ValueError(f"k and v must be (T, {pages.kv_heads}, {pages.head_dim}) of one dtype, got {tuple(k.shape)} "
@@ -262,6 +273,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         _elsewhere("paged_attention", pages, q, out)
     if q.requires_grad or (out is not None and out.requires_grad):
         _no_grad("paged_attention")
+    if forward_ad._current_level >= 0:
+        _no_tangent("paged_attention", q, out)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or shape[0] != B or shape[2] != pages.head_dim or dtype is not pages.query_dtype:
         raise ValueError(f"q must be ({B}, heads, {pages.head_dim}) in {pages.query_dtype}, got {tuple(shape)} {dtype}")

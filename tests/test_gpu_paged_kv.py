@@ -825,6 +825,38 @@ def test_refused_tensors():
     assert buf.tolist() == [20, 5, 7]
 
 
+def test_refused_tangents():
+    """The tangent of a forward-mode dual tensor would be lost."""
+    from torch.autograd import forward_ad
+
+    from cortex.kernels.paged_kv import KVPages, paged_attention, paged_kv_append
+
+    c = Cache([40, 9], 2, 64, 16, torch.bfloat16, room=1, tracked=True)
+    q, rows = c.query(4).to(DEV), torch.ones(2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    want = paged_attention(q, c.pages, c.block_table, c.lengths)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t.clone(), torch.ones_like(t))
+
+        before = c.gk.clone()
+        for k, v in [(dual(rows), rows), (rows, dual(rows))]:
+            with pytest.raises(RuntimeError, match="tangent"):
+                paged_kv_append(c.pages, k, v, c.block_table, c.lengths)
+        assert torch.equal(c.gk.nan_to_num(9.0), before.nan_to_num(9.0))
+        for bad in [dual(q), dual(q)[:], dual(q).transpose(0, 1).contiguous().transpose(0, 1)]:
+            for grad in (True, False):
+                with pytest.raises(RuntimeError, match="tangent"), torch.set_grad_enabled(grad):
+                    paged_attention(bad, c.pages, c.block_table, c.lengths)
+        with pytest.raises(RuntimeError, match="tangent"):
+            paged_attention(q, c.pages, c.block_table, c.lengths, out=dual(q))
+        with pytest.raises(RuntimeError, match="tangent"):
+            KVPages(c.gk, dual(c.gv))
+        assert torch.equal(paged_attention(forward_ad.unpack_dual(dual(q)).primal, c.pages, c.block_table, c.lengths), want)
+        paged_kv_append(c.pages, rows, rows, c.block_table, c.lengths)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: paged_attention(x, c.pages, c.block_table, c.lengths), (q,), (torch.ones_like(q),))
+
+
 def test_refusals():
     from cortex.kernels.paged_kv import EvictPlan, KVPages, kv_evict_apply, kv_evict_plan, paged_attention, paged_kv_append
 
