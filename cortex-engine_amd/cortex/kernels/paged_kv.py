@@ -31,7 +31,7 @@ _PER_ROW = ("k_scale", "v_scale", "weight", "position")
 
 class KVPages:
     """Pools of pages: ``k`` and ``v`` (num_pages, kv_heads, page_size, head_dim) in bf16, fp32 or int8 (any
-    strides, head_dim contiguous, rows 16-byte aligned; ``page_size`` a power of two from 8, ``head_dim`` a multiple of
+    strides, head_dim contiguous, rows 16-byte aligned, for append and eviction none that share memory; ``page_size`` a power of two from 8, ``head_dim`` a multiple of
     16 up to 128) and contiguous (num_pages, kv_heads, page_size) arrays: ``k_scale``, ``v_scale`` fp32 (int8 pages:
     a row is ``code * scale``), ``weight`` fp32 (softmax weight received so far) and ``position`` int32 (where the
     token stood in its sequence), the last two optional.  The tensors of an object do not change."""

@@ -51,4 +51,9 @@ __device__ __forceinline__ void kv_flag(int32_t* err) {
 int kv_check(const char* who, const cortex_kv_pages* pages, int64_t B, const int32_t* table, int64_t ld_table,
              int64_t max_pages, KvPages* out);
 
+// Whether rows of k and v that an operator writes share memory, among themselves or with each other (an expanded pool, the
+// same one for both).  Views of whole pools never do: ordered by stride, every dimension steps over all of those before.
+// Pools of other strides than each other's are only looked at for themselves.
+bool kv_rows_meet(const cortex_kv_pages* pages);
+
 }  // namespace cortex

@@ -7,6 +7,8 @@
 // (below it) are disjoint: every row moves independently of the others.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "paged_kv.h"
 
 namespace cortex {
@@ -45,6 +47,31 @@ int kv_check(const char* who, const cortex_kv_pages* p, int64_t B, const int32_t
                  (int32_t)p->num_pages, (int32_t)p->kv_heads, (int32_t)p->head_dim,
                  __builtin_ctzll((unsigned long long)ps), max_pages * ps};
   return OK;
+}
+
+bool kv_rows_meet(const cortex_kv_pages* p) {
+  struct Dim {
+    int64_t stride, size;
+  };
+  auto steps_over = [&](Dim a, Dim b, Dim c, Dim d) {  // all rows of the dimensions, one behind the other
+    Dim dims[] = {a, b, c, d};
+    std::sort(dims, dims + 4, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+    __int128 extent = p->head_dim;
+    for (const Dim& x : dims) {
+      if (x.size < 2) continue;
+      if (x.stride < extent) return false;
+      extent += (__int128)x.stride * (x.size - 1);
+    }
+    return true;
+  };
+  const int64_t es = p->dtype == DT_F32 ? 4 : p->dtype == DT_BF16 ? 2 : 1;
+  const Dim kd[] = {{p->k_page, p->num_pages}, {p->k_head, p->kv_heads}, {p->k_slot, p->page_size}};
+  const Dim vd[] = {{p->v_page, p->num_pages}, {p->v_head, p->kv_heads}, {p->v_slot, p->page_size}};
+  const uintptr_t k = (uintptr_t)p->k, v = (uintptr_t)p->v;
+  Dim apart = {0, 1};  // v as a second part of k
+  if (p->k_page == p->v_page && p->k_head == p->v_head && p->k_slot == p->v_slot)
+    apart = {(int64_t)((k < v ? v - k : k - v) / es), 2};
+  return k == v || !steps_over(kd[0], kd[1], kd[2], apart) || !steps_over(vd[0], vd[1], vd[2], apart);
 }
 
 namespace {
@@ -517,7 +544,8 @@ bool meet(const int64_t* a, int64_t n, const int64_t* b, int64_t m) {
 }
 
 template <class X>
-int launch_append(const AppendArgs& a, int dtype, hipStream_t stream) {
+int launch_append(const AppendArgs& a, const cortex_kv_pages* pages, hipStream_t stream) {
+  const int dtype = (int)pages->dtype;
   const int lpr = pow2_lanes(a.p.head_dim / 8);
   // as many tokens a workgroup as its threads have loads in flight for, while every CU gets eight workgroups
   int64_t tokens = 256 * AP_AHEAD / (2ll * a.p.kv_heads * lpr), spread = a.T / (8 * cu_count());
@@ -527,6 +555,7 @@ int launch_append(const AppendArgs& a, int dtype, hipStream_t stream) {
                    (long long)a.T);  // (a launch has fewer than 2^32 threads)
   const dim3 grid((unsigned)cdiv(a.T, tokens)), block(256);
   if (a.T > 0) {
+    CORTEX_CHECK_ARG(!kv_rows_meet(pages), "cortex_kv_append: rows of k and v share memory");
     if (dtype == DT_F32)
       hipLaunchKernelGGL((kv_append_kernel<X, float>), grid, block, 0, stream, a, lpr, (int)tokens);
     else if (dtype == DT_BF16)
@@ -584,8 +613,7 @@ extern "C" int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t
   a.positions = positions;
   a.new_lengths = new_lengths;
   a.err = err;
-  return x_dtype == DT_F32 ? launch_append<float>(a, (int)pages->dtype, stream)
-                           : launch_append<bf16>(a, (int)pages->dtype, stream);
+  return x_dtype == DT_F32 ? launch_append<float>(a, pages, stream) : launch_append<bf16>(a, pages, stream);
 }
 
 extern "C" int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table,
@@ -640,6 +668,7 @@ extern "C" int cortex_kv_evict_apply(const cortex_kv_pages* pages, int64_t B, co
   if (B == 0 || cap == 0) return OK;
   CORTEX_CHECK_ARG(dst && src && counts, "%s: null pointer", who);
   CORTEX_CHECK_ARG(B <= 0xffffffffLL / 256 / pages->kv_heads, "%s: too many heads", who);
+  CORTEX_CHECK_ARG(!kv_rows_meet(pages), "%s: rows of k and v share memory", who);
   const int es = pages->dtype == DT_F32 ? 4 : pages->dtype == DT_BF16 ? 2 : 1;
   a.dst = dst;
   a.src = src;

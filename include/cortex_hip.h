@@ -514,7 +514,8 @@ int cortex_linear_residual_ln_splitk(int64_t M, int64_t N, int64_t K, const void
  * so far) and position (where in its sequence the token stood) are optional.  The four per-row
  * arrays are contiguous (num_pages, kv_heads, page_size) and 16-byte aligned.
  * page_size a power of two from 8 to 65536; head_dim a multiple of 16 up to 128; rows 16-byte
- * aligned.  A page id outside [0, num_pages), a length outside [0, max_pages * page_size] or a
+ * aligned; where an operator writes rows, no two of them share memory (an expanded pool, or one
+ * pool as k and v, is for reading).  A page id outside [0, num_pages), a length outside [0, max_pages * page_size] or a
  * slot without a page never reads or writes out of bounds: its rows are taken as absent and bit
  * 2 (value 4) is OR-ed into *err (when given). */
 typedef struct cortex_kv_pages {

@@ -825,6 +825,73 @@ def test_refused_tensors():
     assert buf.tolist() == [20, 5, 7]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["planes", "columns", "halves", "every other", "heads", "rows outside"])
+def test_keys_and_values_in_one_buffer(dtype, layout):
+    """Views of one allocation are written like pools of their own."""
+    from cortex.kernels.paged_kv import KVPages, kv_evict_apply, kv_evict_plan, paged_kv_append
+
+    def z(*shape):
+        return torch.zeros(*shape, dtype=DTYPES[dtype], device=DEV)
+
+    n, H, S, D = 6, 2, 8, 32
+    if layout == "planes":
+        both = z(n, 2, H, S, D)
+        k, v = both[:, 1], both[:, 0]
+    elif layout == "columns":
+        both = z(n, H, S, 2 * D)
+        k, v = both[..., :D], both[..., D:]
+    elif layout == "halves":
+        both = z(2 * n, H, S, D)
+        k, v = both[:n], both[n:]
+    elif layout == "every other":
+        both = z(2 * n, H, S, D)
+        k, v = both[1::2], both[::2]
+    elif layout == "heads":
+        both = z(n, S, 2 * H, D)
+        k, v = both[:, :, :H].transpose(1, 2), both[:, :, H:].transpose(1, 2)
+    else:
+        both = z(2, S, n, H, D)
+        k, v = (both[i].permute(1, 2, 0, 3) for i in (0, 1))
+    scales = {"k_scale": torch.zeros(n, H, S, device=DEV), "v_scale": torch.zeros(n, H, S, device=DEV)} if dtype == "int8" else {}
+    tracked = [{"weight": torch.zeros(n, H, S, device=DEV), "position": torch.zeros(n, H, S, dtype=torch.int32, device=DEV)}
+               for _ in range(2)]
+    one = KVPages(k, v, **scales, **tracked[0])
+    two = KVPages(z(n, H, S, D), z(n, H, S, D), **{a: t.clone() for a, t in scales.items()}, **tracked[1])
+    g = torch.Generator(DEV).manual_seed(1)
+    rows = [torch.randn(37, H, D, generator=g, device=DEV).bfloat16() for _ in range(2)]
+    table = torch.tensor([[3, 0, 5], [1, 4, 2]], dtype=torch.int32, device=DEV)
+    for p in (one, two):
+        lengths = paged_kv_append(p, *rows, table, torch.zeros(2, dtype=torch.int64, device=DEV),
+                                  offsets=torch.tensor([0, 20, 37], device=DEV))
+        kv_evict_apply(p, table, kv_evict_plan(p, table, lengths, 9, 4))
+    for a in ("k", "v", "k_scale", "v_scale", "position"):
+        if getattr(one, a) is not None:
+            assert torch.equal(getattr(one, a), getattr(two, a)), a
+    assert not torch.equal(one.k, one.v)
+
+
+def test_pools_whose_rows_share_memory():
+    """They are read like others, and not written."""
+    from cortex.kernels.paged_kv import KVPages, kv_evict_apply, kv_evict_plan, paged_attention, paged_kv_append
+
+    c = Cache([40, 9], 1, 64, 16, torch.bfloat16, tracked=True)
+    q = c.query(4)
+    want, _, tol, _ = attention64(c, q)
+    more = {n: getattr(c.pages, n).expand(-1, 2, -1).contiguous() for n in ("weight", "position")}
+    wide = KVPages(c.gk.expand(-1, 2, -1, -1), c.gv.expand(-1, 2, -1, -1), **more)
+    check(paged_attention(q.to(DEV), wide, c.block_table, c.lengths), want, tol, "expanded")
+    tied = KVPages(c.gk, c.gk, weight=c.pages.weight, position=c.pages.position)
+    before = c.gk.clone()
+    for pages, heads in ((wide, 2), (tied, 1)):
+        rows = torch.ones(2, heads, 64, dtype=torch.bfloat16, device=DEV)
+        with pytest.raises(Exception, match="share memory"):
+            paged_kv_append(pages, rows, rows, c.block_table, c.lengths)
+        with pytest.raises(Exception, match="share memory"):
+            kv_evict_apply(pages, c.block_table, kv_evict_plan(pages, c.block_table, c.lengths, 8, 2))
+    assert torch.equal(c.gk.nan_to_num(9.0), before.nan_to_num(9.0))
+
+
 def test_refused_tangents():
     """The tangent of a forward-mode dual tensor would be lost."""
     from torch.autograd import forward_ad

@@ -134,3 +134,14 @@ def test_refused_evictions():
     refused(apply(pages(), counts=None), "null pointer")
     lib = nat.load()
     assert lib.cortex_kv_evict_plan(*plan(tracked(), B=0)[1:]) == 0 and lib.cortex_kv_evict_apply(*apply(pages(), cap=0)[1:]) == 0
+
+
+def test_pools_whose_rows_share_memory_are_not_written():
+    n = 1 << 20
+    for kw in [{"k_head": 0}, {"v_head": 0}, {"k_page": 0}, {"k_page": 1024}, {"v_page": 2032}, {"k_head": 512}, {"k_slot": 80}]:
+        for call in (append, apply):
+            refused(call(pages(v=n, **kw)), "share memory")
+    for shift in (0, 32, 64, 1024, 2048, 4096, 8192 - 64):  # k and v in one buffer, `shift` elements apart
+        for call in (append, apply):
+            refused(call(pages(k=n, v=n + 2 * shift)), "share memory")
+            refused(call(pages(k=n + 2 * shift, v=n)), "share memory")
