@@ -228,8 +228,10 @@ class PagedKVCache:
             if any(len(f) < len(self.layers) for f in self._sessions[n].pending):
                 raise RuntimeError(f"session {n!r} has slots without rows in some layer: append them first")
         b = self.batch(names)
-        for pages in self.layers:
-            plan = kv_evict_plan(pages, b.block_table, b.lengths, budget, recent, max_length=b.max_length)
+        # all plans, which need memory, before the first row moves: a session is cut in every layer or in none
+        plans = [kv_evict_plan(pages, b.block_table, b.lengths, budget, recent, max_length=b.max_length)
+                 for pages in self.layers]
+        for pages, plan in zip(self.layers, plans):
             kv_evict_apply(pages, b.block_table, plan)
         freed = 0
         for n in names:

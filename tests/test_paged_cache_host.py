@@ -177,9 +177,9 @@ def test_steps_keep_no_record_of_what_is_complete(host):
     assert not cache.batch(["a", "b"]).needs
 
 
-def state(cache):
+def state(cache):  # (of the records of missing rows those that miss some)
     return {"free": list(cache._free), "order": cache.sessions, "epoch": cache._epoch,
-            "sessions": {n: (s.pages[:s.used].tolist(), s.length, s.seen, s.version, [set(f) for f in s.pending])
+            "sessions": {n: (s.pages[:s.used].tolist(), s.length, s.seen, s.version, [set(f) for f in s.pending if len(f) < len(cache.layers)])
                          for n, s in cache._sessions.items()}}
 
 
@@ -217,3 +217,26 @@ def test_an_extend_that_fails_changes_nothing(host, monkeypatch, fails):
     batch = cache.extend(["d", "c"], [4000, 1])
     assert cache.sessions == ["b", "d", "c"] and cache.length("c") == 11 and batch.positions[-1] == 10
     assert sorted(cache._free + [p for s in cache._sessions.values() for p in s.pages[:s.used].tolist()]) == list(range(700))
+
+
+def test_an_eviction_that_fails_moves_nothing(host, monkeypatch):
+    """The plans of all layers are made before the first row of any layer moves."""
+    cache = PagedKVCache(8, 1, 16, page_size=8, layers=3, tracked=True)
+    batch = cache.extend(["a"], [20])
+    for layer in range(3):
+        cache.append(batch, rows(20), rows(20), layer)
+    before = state(cache)
+    plan = paged.kv_evict_plan
+    with monkeypatch.context() as m:
+        def out_of_memory(pages, *args, **kw):
+            if pages is cache.layers[2]:
+                raise torch.OutOfMemoryError("out of memory")
+            return plan(pages, *args, **kw)
+
+        m.setattr(paged, "kv_evict_plan", out_of_memory)
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.evict(["a"], 8, 2)
+    assert not host.of("apply") and state(cache) == before
+    cache.attend(batch, rows(1))  # still holds
+    assert cache.evict(["a"], 8, 2) == 2
+    assert host.of("apply") == [(p,) for p in cache.layers]
