@@ -17,7 +17,9 @@ empty, from what was used least recently: here whole sessions, since a sequence 
 
 Not thread-safe: like the other caches it is meant for the single inference executor thread.  The operators run on
 torch's current stream; a call on another stream than the one before (the first: than the one that the cache was made
-on) first waits, on the device, for that one.
+on) first waits, on the device, for that one.  A graph cannot follow its steps, each of which has a table of its own: in a
+capture ``extend`` is refused, and so is a call on another stream than the one before (``cortex.kernels.paged_kv`` on tables
+that the program keeps can be captured).
 """
 
 from __future__ import annotations
@@ -265,6 +267,7 @@ class PagedKVCache:
                     raise RuntimeError(f"the batch is out of date: session {name!r} was cut or dropped since")
         stream = torch.cuda.current_stream(self.device)
         if self._stream != stream:
+            self._not_captured()
             done = torch.cuda.Event()
             done.record(self._stream)
             stream.wait_event(done)
@@ -276,9 +279,15 @@ class PagedKVCache:
             batch.lengths.record_stream(stream)  # (all of a batch is one allocation)
         self._stream = stream
 
+    def _not_captured(self) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the steps of a PagedKVCache are not captured: a graph takes the operators of "
+                               "cortex.kernels.paged_kv on tables and lengths that its program keeps")
+
     def _upload(self, cols: list[np.ndarray]) -> list[torch.Tensor]:
         """int64 arrays on the device, parts of one allocation and one pinned copy."""
         need = sum(c.shape[0] for c in cols)
+        self._not_captured()
         self._enter()
         self._staged.synchronize()  # the copy before has left the pinned buffer
         if self._stage.numel() < need:

@@ -54,6 +54,7 @@ class Host:
 
         patch.setattr(torch.cuda, "Event", Event)
         patch.setattr(torch.cuda, "current_stream", lambda device=None: host.current)
+        patch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
         patch.setattr(torch.Tensor, "pin_memory", lambda t: t, raising=False)
         patch.setattr(torch.Tensor, "record_stream", lambda t, s: log.append(("record", s.name, t)), raising=False)
         patch.setattr(paged.KVPages, "allocate", allocate)
@@ -240,3 +241,19 @@ def test_an_eviction_that_fails_moves_nothing(host, monkeypatch):
     cache.attend(batch, rows(1))  # still holds
     assert cache.evict(["a"], 8, 2) == 2
     assert host.of("apply") == [(p,) for p in cache.layers]
+
+
+def test_steps_are_not_captured(host, monkeypatch):
+    """A graph would replay the copy of a buffer that has moved on, or wait for work outside of it."""
+    cache = PagedKVCache(8, 1, 16, page_size=8)
+    batch = cache.extend(["a"], [5])
+    cache.append(batch, rows(5), rows(5))
+    before = state(cache)
+    with monkeypatch.context() as m, host.on("captured"):
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: host.current.name == "captured")
+        for call in (lambda: cache.extend(["a"]), lambda: cache.batch(["a"]), lambda: cache.attend(batch, rows(1)),
+                     lambda: cache.append(batch, rows(5), rows(5))):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    assert state(cache) == before and not host.of("wait") and not host.of("record")
+    cache.attend(batch, rows(1))
