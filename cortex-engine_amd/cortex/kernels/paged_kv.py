@@ -31,10 +31,10 @@ _PER_ROW = ("k_scale", "v_scale", "weight", "position")
 
 class KVPages:
     """Pools of pages: ``k`` and ``v`` (num_pages, kv_heads, page_size, head_dim) in bf16, fp32 or int8 (any
-    strides, head_dim contiguous, rows 16-byte aligned, for append and eviction none that share memory; ``page_size`` a power of two from 8, ``head_dim`` a multiple of
-    16 up to 128) and contiguous (num_pages, kv_heads, page_size) arrays: ``k_scale``, ``v_scale`` fp32 (int8 pages:
-    a row is ``code * scale``), ``weight`` fp32 (softmax weight received so far) and ``position`` int32 (where the
-    token stood in its sequence), the last two optional.  The tensors of an object do not change."""
+    strides, head_dim contiguous, rows 16-byte aligned, none that share memory where append or eviction write them;
+    ``page_size`` a power of two from 8, ``head_dim`` a multiple of 16 up to 128) and contiguous (num_pages, kv_heads,
+    page_size) arrays: ``k_scale``, ``v_scale`` fp32 (int8 pages: a row is ``code * scale``), ``weight`` fp32 (softmax weight
+    received so far) and ``position`` int32 (where the token stood in its sequence), the last two optional.  The tensors of an object do not change."""
 
     __slots__ = ("k", "v", *_PER_ROW, "num_pages", "kv_heads", "page_size", "head_dim", "device", "index", "query_dtype",
                  "_struct", "ref")
@@ -263,7 +263,9 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q`` or itself.
     ``max_length``: a bound of the lengths known on the host (default: the table's width), which sizes the launch and
     the workspace; longer sequences are cut to it and set bit 2 of ``err_flag``, as lengths outside the table and page
-    ids outside the pool do (such pages hold no keys)."""
+    ids outside the pool do (such pages hold no keys).  With ``accumulate`` the workspace holds ``B * heads * max_length`` fp32
+    scores beside the parts, whatever the lengths are: give the bound where tables are wide.  Up to 4096 sequences and 1024
+    query heads a key head.  Values are summed in fp32 before they are divided: ``lengths[b] * max|v|`` is to stay below 2^120."""
     if pages.index != _get_device():
         with torch.cuda.device(pages.index):
             return paged_attention(q, pages, block_table, lengths, scale=scale, accumulate=accumulate,
@@ -312,7 +314,8 @@ def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tens
     """Which slots each key head keeps where a sequence holds more than ``budget``: those of the last ``recent``
     positions first (``recent <= budget``), then the ones with the largest ``pages.weight`` (a NaN before every number,
     equal weights by the lower slot).  Kept slots at or past the budget are to fill the slots below it that are given up (``EvictPlan``);
-    shorter sequences stay as they are.  Reads ``pages.weight`` and ``pages.position`` and writes neither.
+    shorter sequences stay as they are.  Slots that no query has attended to with ``accumulate`` have weight 0, all of a new
+    prompt among them: of those the newest stay, then the first ones.  Reads ``pages.weight`` and ``pages.position`` and writes neither.
     ``max_length`` and ``err_flag`` as for ``paged_attention``."""
     if pages.index != _get_device():
         with torch.cuda.device(pages.index):

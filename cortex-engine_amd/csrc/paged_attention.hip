@@ -19,8 +19,11 @@
 // is one workgroup per slot of the card).  A unit cut by a share leaves its running (m, l, sum p v) in the workspace, at
 // most two a workgroup (the end of a unit and the beginning of another), and a second launch joins them in order.
 //
-// Measured (bf16, 32 query heads on 8 key heads of 128): one sequence of 131,072 keys, 537 MB, 95 us, 5.6 TB/s; 32 of 150
-// .. 8003 keys, 535 MB, 99 us.  Int8, 135 MB, 32 us: the widening on the VALU beside HBM.
+// Measured (bf16, 32 query heads on 8 key heads of 128): one sequence of 131,072 keys, 537 MB, 95 us, 5.7 TB/s; 32 of 150
+// .. 8003 keys, 535 MB, 99 us.  Int8, 135 MB, 32 us, 4.2 TB/s: the VALU, widening among others, is busy 58 % of the time (8.4 of
+// 28.9 M wavefront cycles, two wavefronts a SIMD), 45 % of a wavefront's is waiting, and two workgroups a CU have half the bytes
+// of bf16 in flight.  fp32, 12 heads of 64, 885 MB, 159 us, 5.6 TB/s.  With the weights, 16 of 2048 .. 4160 keys: 47 us, 42
+// without storing the scores.
 #include <hip/hip_runtime.h>
 
 #include "paged_kv.h"
@@ -33,8 +36,10 @@ constexpr int PA_WAVES = 4;     // wavefronts of a workgroup that takes a share
 constexpr int PA_MORE = 8;      // and of one that has a CU to itself and takes a whole unit
 constexpr int PA_ROWS = 16;     // query heads of one matrix product
 constexpr int PA_MIN_TILES = PA_WAVES;  // tiles of a share
-// Workgroups that a CU holds at once, by the registers of a tile: 128 dims 160 to 246, 64 dims in fp32 146, in fewer
-// bits 117.  (64 sequences of 500 .. 3000 keys x 64 dims, bf16: 2 a CU 55.5 us, 4 54.2; 128 dims as 3: 105 -> 110)
+// Workgroups that a CU holds at once, by the registers of a form that takes shares: 128 dims 168 (int8) to 249, fp32 242 to
+// 256 and where head_dim < 128 spills 5, 13 with the weights (not measured apart); 64 dims in fp32 146 to 159, in fewer bits 115
+// to 119 and for two products 157 to 163.  (64 sequences of 500 .. 3000 keys x 64 dims, bf16: 2 a CU 55.5 us, 4 54.2; bf16, 128
+// dims as 3: 105 -> 110.  Int8 of 128 dims would go in three times; not tried)
 __host__ __device__ constexpr int per_cu(int dhp, int es, int rt) { return dhp == 128 ? 2 : es == 4 || rt == 2 ? 3 : 4; }
 constexpr int PA_MAX_SHARES = 1024;
 // What it costs to begin a unit (fill and drain the loads, sum up), in tiles, where a share may have PA_LONG tiles and

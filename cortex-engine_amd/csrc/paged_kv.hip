@@ -155,7 +155,8 @@ constexpr int AP_AHEAD = 4;    // values in flight, in eights a thread
 
 // A workgroup takes `tokens` tokens, a thread eight values of a (token, key or value, head) row; `lpr` lanes a row.  The
 // first threads look up where the tokens go while the others load the rows.  Bound by HBM for many tokens (16,800 of 8
-// heads x 128, bf16, 139 MB: 26.4 us, 5.3 TB/s), by the chain of lookups for few.
+// heads x 128, bf16, 139 MB: 26.4 us, 5.3 TB/s), by the chain of lookups for few.  Int8 pages (105 MB) take 53.9 us, 2.0 TB/s:
+// eight divisions a thread, the row's maximum over its lanes and stores of eight bytes; which of them bounds it was not measured.
 template <class X, class P>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int lpr, int tokens) {
   __shared__ int at_page[AP_TOKENS], at_row[AP_TOKENS], at_slot[AP_TOKENS];
@@ -301,7 +302,7 @@ __device__ int block_scan(int v, int* part, int tid, int* total) {
 // four bytes, then holes and movers in slot order by prefix sums.  Bound by the chain of rounds between barriers, not by
 // bytes (256 heads of 2000 .. 9001 slots, 11 MB: 22 .. 24 us; 12 up to the ranks and the lists, 9 the selection, 3 the end;
 // 512 threads 29, 256 49).  A thread takes Q runs of eight consecutive slots (one page each, four vector loads) and keeps
-// their ranks in registers; Q 0: as many runs as there are, read again in every pass.
+// their ranks in registers (Q 4 spills 6 of 128); Q 0: as many runs as there are, read again in every pass.
 template <int THREADS, int Q>
 __global__ __launch_bounds__(THREADS) void kv_evict_plan_kernel(PlanArgs a) {
   constexpr int WAVES = THREADS / 64;
@@ -492,7 +493,7 @@ struct ApplyArgs {
 
 // `lanes` lanes a row, 16 bytes of the key and of the value each; a group of lanes takes a row at a time, with the next
 // row's place looked up beside it.  Bound by HBM: rows of 256 bytes read and written at random (32 sequences of 2000 ..
-// 9001 slots down to 2048, 8 heads x 128 in bf16, 305 MB: 70 us, 4.4 TB/s; four rows a group at once 83 us, one 72
+// 9001 slots down to 2048, 8 heads x 128 in bf16, 305 MB: 68.5 us, 4.5 TB/s; four rows a group at once 83 us, one 72
 // with plain and with non-temporal stores, in a workgroup for every 16 rows that there may be: 15 us without a move).
 __global__ __launch_bounds__(256) void kv_evict_apply_kernel(ApplyArgs a, int es) {
   const int tid = threadIdx.x;

@@ -555,7 +555,9 @@ int cortex_kv_append(const cortex_kv_pages* pages, int64_t B, int64_t n_tokens, 
  * max_length (negative: max_pages * page_size) are expected; a longer one is cut to it, as a
  * malformed length.  out may not overlap q or itself.  B up to 4096.  workspace:
  * cortex_paged_attention_workspace_bytes bytes for the call's own max_length, given as the length that it
- * stands for, not negative (0: none is needed); 16-byte aligned, written before it is read. */
+ * stands for, not negative (0: none is needed); 16-byte aligned, written before it is read.  With accumulate it
+ * has B * heads * max_length scores in fp32, whatever the lengths are.  Values are summed in fp32 before they
+ * are divided: lengths[b] * max|v| is to stay below 2^120. */
 int64_t cortex_paged_attention_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t heads,
                                                int64_t max_length, int accumulate);
 int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb,
