@@ -34,7 +34,8 @@ class KVPages:
     strides, head_dim contiguous, rows 16-byte aligned, none that share memory where append or eviction write them;
     ``page_size`` a power of two from 8, ``head_dim`` a multiple of 16 up to 128) and contiguous (num_pages, kv_heads,
     page_size) arrays: ``k_scale``, ``v_scale`` fp32 (int8 pages: a row is ``code * scale``), ``weight`` fp32 (softmax weight
-    received so far) and ``position`` int32 (where the token stood in its sequence), the last two optional.  The tensors of an object do not change."""
+    received so far) and ``position`` int32 (where the token stood in its sequence), the last two optional.  The tensors of
+    an object do not change."""
 
     __slots__ = ("k", "v", *_PER_ROW, "num_pages", "kv_heads", "page_size", "head_dim", "device", "index", "query_dtype",
                  "_struct", "ref")
@@ -313,10 +314,10 @@ def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tens
                   max_length: int | None = None, err_flag: torch.Tensor | None = None) -> EvictPlan:
     """Which slots each key head keeps where a sequence holds more than ``budget``: those of the last ``recent``
     positions first (``recent <= budget``), then the ones with the largest ``pages.weight`` (a NaN before every number,
-    equal weights by the lower slot).  Kept slots at or past the budget are to fill the slots below it that are given up (``EvictPlan``);
-    shorter sequences stay as they are.  Slots that no query has attended to with ``accumulate`` have weight 0, all of a new
-    prompt among them: of those the newest stay, then the first ones.  Reads ``pages.weight`` and ``pages.position`` and writes neither.
-    ``max_length`` and ``err_flag`` as for ``paged_attention``."""
+    equal weights by the lower slot).  Kept slots at or past the budget are to fill the slots below it that are given up
+    (``EvictPlan``); shorter sequences stay as they are.  Slots that no query has attended to with ``accumulate`` have weight
+    0, all of a new prompt among them: of those the newest stay, then the first ones.  Reads ``pages.weight`` and
+    ``pages.position`` and writes neither; a negative length stays negative in ``EvictPlan.lengths``.  ``max_length`` and ``err_flag`` as for ``paged_attention``."""
     if pages.index != _get_device():
         with torch.cuda.device(pages.index):
             return kv_evict_plan(pages, block_table, lengths, budget, recent, max_length=max_length, err_flag=err_flag)
