@@ -148,6 +148,18 @@ _SIGNATURES = {
     "cortex_paged_attention": (
         _int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _f32, _int, _ptr, _i64, _i64, _ptr, _i64,
                _ptr, _ptr]),
+    "cortex_paged_attention_tables": (
+        _int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _f32, _int, _ptr, _i64, _i64, _ptr,
+               _i64, _ptr, _ptr]),
+    "cortex_kv_copy_pages": (_int, [_ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr]),
+    "cortex_kv_block_bounds": (_int, [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr]),
+    "cortex_kv_select_workspace_bytes": (_i64, [_ptr, _i64, _i64, _i64]),
+    "cortex_kv_select": (
+        _int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64,
+               _ptr, _ptr]),
+    "cortex_qk_norm_rope": (
+        _int, [_i64, _i64, _i64, _i64, _int, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr,
+               _int, _int, _f32, _ptr, _ptr, _int, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr]),
     "cortex_kv_evict_plan": (
         _int, [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "cortex_kv_evict_apply": (_int, [_ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _ptr, _ptr]),
@@ -170,7 +182,7 @@ class KvPagesStruct(ctypes.Structure):
 
     _fields_ = [(n, _i64) for n in ("num_pages", "kv_heads", "page_size", "head_dim", "dtype", "k_page", "k_head",
                                     "k_slot", "v_page", "v_head", "v_slot")] + \
-               [(n, _ptr) for n in ("k", "v", "k_scale", "v_scale", "weight", "position")]
+               [(n, _ptr) for n in ("k", "v", "k_scale", "v_scale", "weight", "position", "bounds")]
 
 
 _lib: ctypes.CDLL | None = None

@@ -1,4 +1,5 @@
-"""Paged K/V cache on gfx950: append, attention of one new token, eviction by accumulated weight.
+"""Paged K/V cache on gfx950: append, attention of one new token (to all pages or to selected ones), eviction by accumulated
+weight, copies of pages.
 
 The keys and values of a sequence live in pages of a shared pool: slot ``j`` of sequence ``b`` is row
 ``j % page_size`` of page ``block_table[b, j // page_size]``.  ``KVPages`` holds the pools; the operators take
@@ -10,6 +11,13 @@ current stream, never synchronising:
     out = paged_attention(q, pages, block_table, lengths, accumulate=True)  # (B, heads, head_dim)
     plan = kv_evict_plan(pages, block_table, lengths, budget=4096, recent=512)
     kv_evict_apply(pages, block_table, plan)                                # then plan.lengths slots are in use
+
+With ``bounded=True`` the pools also hold the bounds of each page's keys, and a query can be shown the pages alone that its
+largest scores may be in:
+
+    kv_block_bounds(pages, block_table, lengths, since=before, max_new=1)   # after an append
+    few = paged_block_select(q, pages, block_table, lengths, count=64)      # a table for each key head
+    out = paged_attention(q, pages, few.table, few.lengths)
 
 ``cortex.cache.PagedKVCache`` keeps pages, tables and lengths for named sessions.  No reference counterpart:
 its StreamingKVCache (cortex/cache/streaming.py:79-236) pages embedding rows and attends to none of them.
@@ -34,16 +42,17 @@ class KVPages:
     strides, head_dim contiguous, rows 16-byte aligned, none that share memory where append or eviction write them;
     ``page_size`` a power of two from 8, ``head_dim`` a multiple of 16 up to 128) and contiguous (num_pages, kv_heads,
     page_size) arrays: ``k_scale``, ``v_scale`` fp32 (int8 pages: a row is ``code * scale``), ``weight`` fp32 (softmax weight
-    received so far) and ``position`` int32 (where the token stood in its sequence), the last two optional.  The tensors of
-    an object do not change."""
+    received so far) and ``position`` int32 (where the token stood in its sequence), the last two optional.  ``bounds``
+    (num_pages, kv_heads, 2, head_dim), optional, in the dtype of ``k`` (fp32 for int8 pages): the largest and the smallest
+    value of a page's keys in every dim, as ``kv_block_bounds`` last left them.  The tensors of an object do not change."""
 
-    __slots__ = ("k", "v", *_PER_ROW, "num_pages", "kv_heads", "page_size", "head_dim", "device", "index", "query_dtype",
+    __slots__ = ("k", "v", *_PER_ROW, "bounds", "num_pages", "kv_heads", "page_size", "head_dim", "device", "index", "query_dtype",
                  "_struct", "ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, *, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None, weight: torch.Tensor | None = None,
-                 position: torch.Tensor | None = None) -> None:
-        self.device = nat.require_gpu(k, v, k_scale, v_scale, weight, position, what="KVPages")
+                 position: torch.Tensor | None = None, bounds: torch.Tensor | None = None) -> None:
+        self.device = nat.require_gpu(k, v, k_scale, v_scale, weight, position, bounds, what="KVPages")
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError(f"k and v must be (num_pages, kv_heads, page_size, head_dim) of one dtype, got "
                              f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
@@ -53,20 +62,25 @@ class KVPages:
             raise ValueError("int8 pages need k_scale and v_scale, float pages take none")
         if k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("k and v need a contiguous last (head) dim")
-        if any(t is not None and t.requires_grad for t in (k, v, k_scale, v_scale, weight)):
+        if any(t is not None and t.requires_grad for t in (k, v, k_scale, v_scale, weight, bounds)):
             raise ValueError("pages hold values without gradients")
         if forward_ad._current_level >= 0:
-            _no_tangent("KVPages", k, v, k_scale, v_scale, weight)
+            _no_tangent("KVPages", k, v, k_scale, v_scale, weight, bounds)
         self.index = k.get_device()
         # of queries and outputs: the pages' own, bfloat16 for int8 pages
         self.query_dtype = torch.bfloat16 if k.dtype == torch.int8 else k.dtype
         self.k, self.v, self.k_scale, self.v_scale, self.weight, self.position = k, v, k_scale, v_scale, weight, position
+        self.bounds = bounds
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         for name in _PER_ROW:
             t = getattr(self, name)
             want = torch.int32 if name == "position" else torch.float32
             if t is not None and (t.shape != k.shape[:3] or t.dtype != want or not t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous {want} tensor of shape {tuple(k.shape[:3])}")
+        want = torch.float32 if k.dtype == torch.int8 else k.dtype
+        if bounds is not None and (bounds.shape != (*k.shape[:2], 2, k.shape[3]) or bounds.dtype != want
+                                   or not bounds.is_contiguous()):
+            raise ValueError(f"bounds must be a contiguous {want} tensor of shape {(*k.shape[:2], 2, k.shape[3])}")
         if self.page_size < 8 or self.page_size > 65536 or self.page_size & (self.page_size - 1):
             raise ValueError(f"page_size must be a power of two from 8 to 65536, got {self.page_size}")
         if self.head_dim % 16 or not 16 <= self.head_dim <= 128:
@@ -74,16 +88,17 @@ class KVPages:
         es = k.element_size()
         if any(x % 16 for t in (k, v) for x in (t.data_ptr(), *(s * es for s in t.stride()[:3]))):
             raise ValueError("page rows must be 16-byte aligned")
-        if any(t is not None and t.data_ptr() % 16 for t in (k_scale, v_scale, weight, position)):
-            raise ValueError("k_scale, v_scale, weight and position must be 16-byte aligned")
+        if any(t is not None and t.data_ptr() % 16 for t in (k_scale, v_scale, weight, position, bounds)):
+            raise ValueError("k_scale, v_scale, weight, position and bounds must be 16-byte aligned")
         self._struct = nat.KvPagesStruct(*k.shape, nat.code(k.dtype), *k.stride()[:3], *v.stride()[:3], nat.ptr(k),
-                                         nat.ptr(v), *(nat.ptr(getattr(self, n)) for n in _PER_ROW))
+                                         nat.ptr(v), *(nat.ptr(getattr(self, n)) for n in _PER_ROW), nat.ptr(bounds))
         self.ref = ctypes.addressof(self._struct)
 
     @classmethod
     def allocate(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
-                 device: str | torch.device = "cuda", *, tracked: bool = False) -> KVPages:
-        """Zeroed pools; ``tracked`` adds ``weight`` and ``position`` (eviction needs them)."""
+                 device: str | torch.device = "cuda", *, tracked: bool = False, bounded: bool = False) -> KVPages:
+        """Zeroed pools; ``tracked`` adds ``weight`` and ``position`` (eviction needs them), ``bounded`` the ``bounds`` that
+        a selection of pages reads."""
         shape = (num_pages, kv_heads, page_size)
         k, v = (torch.zeros(*shape, head_dim, dtype=dtype, device=device) for _ in range(2))
         more = {}
@@ -92,6 +107,9 @@ class KVPages:
         if tracked:
             more["weight"] = torch.zeros(shape, device=device)
             more["position"] = torch.zeros(shape, dtype=torch.int32, device=device)
+        if bounded:
+            more["bounds"] = torch.zeros(num_pages, kv_heads, 2, head_dim, device=device,
+                                         dtype=torch.float32 if dtype == torch.int8 else dtype)
         return cls(k, v, **more)
 
 
@@ -114,18 +132,25 @@ def _i64(t: torch.Tensor, n: int, name: str, what: str) -> None:
 
 
 def _common(what: str, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
-            err_flag) -> tuple[int, int, int]:
-    """Checks what every operator takes; the block table's rows, row stride and columns."""
+            err_flag, by_head: bool = False) -> tuple[int, int, int]:
+    """Checks what every operator takes; the block table's rows, row stride and columns.  ``by_head``: a table that is
+    (B, kv_heads, max_pages)."""
     idx = pages.index
     if (block_table.get_device() != idx or lengths.get_device() != idx
             or (err_flag is not None and err_flag.get_device() != idx)):
         _elsewhere(what, pages, block_table, lengths, err_flag)
     shape = block_table.shape
-    if len(shape) != 2 or block_table.dtype is not torch.int32:
+    if by_head:
+        if shape[1] != pages.kv_heads or block_table.dtype is not torch.int32 or not block_table.is_contiguous():
+            raise ValueError(f"{what}: a block_table by key heads must be a contiguous (B, {pages.kv_heads}, max_pages) "
+                             "int32 tensor")
+        block_table = block_table.view(shape[0], shape[1] * shape[2])
+        shape = shape[0], shape[2]
+    elif len(shape) != 2 or block_table.dtype is not torch.int32:
         raise ValueError(f"{what}: block_table must be a (B, max_pages) int32 tensor")
     B, width = shape
     if block_table.is_contiguous():
-        ld = width
+        ld = width * pages.kv_heads if by_head else width
     else:
         ld, unit = block_table.stride()
         if width > 1 and unit != 1:
@@ -259,6 +284,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     """``softmax_{j < lengths[b]}(scale * q . k_j) v_j`` of one query a sequence: ``q`` (B, heads, head_dim) in
     ``pages.query_dtype`` with ``heads`` a multiple of the key heads (query head h reads key head
     ``h // (heads // kv_heads)``), ``scale`` ``head_dim ** -0.5`` by default.  A sequence of length 0 gives 0.
+    ``block_table``: also a contiguous (B, kv_heads, max_pages), a row of pages for each key head (``paged_block_select``).
 
     ``accumulate`` adds to ``pages.weight`` the softmax weight that each key received, summed over the query heads
     of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q`` or itself.
@@ -271,7 +297,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         with torch.cuda.device(pages.index):
             return paged_attention(q, pages, block_table, lengths, scale=scale, accumulate=accumulate,
                                    max_length=max_length, out=out, err_flag=err_flag)
-    B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag)
+    by_head = block_table.dim() == 3
+    B, ld, width = _common("paged_attention", pages, block_table, lengths, err_flag, by_head)
     if q.get_device() != pages.index or (out is not None and out.get_device() != pages.index):
         _elsewhere("paged_attention", pages, q, out)
     if q.requires_grad or (out is not None and out.requires_grad):
@@ -304,10 +331,139 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     ws_bytes = nat.load().cortex_paged_attention_workspace_bytes(pages.ref, B, heads, max_length, accumulate)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=pages.device) if ws_bytes else None
     ob, oh, _ = out.stride()
-    nat.call("cortex_paged_attention", pages.ref, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld, width,
-             lengths.data_ptr(), max_length, pages.head_dim ** -0.5 if scale is None else scale, accumulate,
-             out.data_ptr(), ob, oh, nat.ptr(ws), ws_bytes, nat.ptr(err_flag), nat.stream_of(pages.device))
+    scale = pages.head_dim ** -0.5 if scale is None else scale
+    if by_head:
+        nat.call("cortex_paged_attention_tables", pages.ref, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld,
+                 width, width, lengths.data_ptr(), max_length, scale, accumulate, out.data_ptr(), ob, oh, nat.ptr(ws),
+                 ws_bytes, nat.ptr(err_flag), nat.stream_of(pages.device))
+    else:
+        nat.call("cortex_paged_attention", pages.ref, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld, width,
+                 lengths.data_ptr(), max_length, scale, accumulate, out.data_ptr(), ob, oh, nat.ptr(ws), ws_bytes,
+                 nat.ptr(err_flag), nat.stream_of(pages.device))
     return out
+
+
+class BlockSelection(NamedTuple):
+    """What ``paged_block_select`` found, as ``paged_attention`` takes it: ``table`` (B, kv_heads, n) int32, the pages of
+    each key head in the order of their blocks (-1 behind), and ``lengths`` (B,) int64, the slots in use in them."""
+
+    table: torch.Tensor
+    lengths: torch.Tensor
+
+
+def _max_length(max_length: int | None, room: int) -> int:
+    if max_length is None:
+        return room
+    if max_length < 0:
+        raise ValueError(f"max_length must not be negative, got {max_length}")
+    return min(max_length, room)
+
+
+def kv_block_bounds(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, *,
+                    since: torch.Tensor | None = None, max_new: int | None = None, max_length: int | None = None,
+                    err_flag: torch.Tensor | None = None) -> None:
+    """Writes ``pages.bounds`` of the pages that hold a slot of ``[since[b], lengths[b])`` (``since`` (B,) int64, by default
+    0: all pages in use), each from all of its keys below ``lengths[b]``; NaN in the dims where a key has one.
+
+    Append, eviction and everything else that writes keys leaves the bounds as they were: call this behind it, after an
+    append with the lengths before it as ``since``.  ``max_new``: a bound of ``lengths - since`` known on the host, which
+    sizes the launch.  ``max_length`` and ``err_flag`` as for ``paged_attention``."""
+    if pages.index != _get_device():
+        with torch.cuda.device(pages.index):
+            return kv_block_bounds(pages, block_table, lengths, since=since, max_new=max_new, max_length=max_length,
+                                   err_flag=err_flag)
+    B, ld, width = _common("kv_block_bounds", pages, block_table, lengths, err_flag)
+    if pages.bounds is None:
+        raise ValueError("kv_block_bounds needs pages with bounds (bounded=True)")
+    if since is not None:
+        if since.get_device() != pages.index:
+            _elsewhere("kv_block_bounds", pages, since)
+        _i64(since, B, "since", "kv_block_bounds")
+    if max_new is not None and max_new < 0:
+        raise ValueError(f"max_new must not be negative, got {max_new}")
+    nat.call("cortex_kv_block_bounds", pages.ref, B, block_table.data_ptr(), ld, width, lengths.data_ptr(),
+             _max_length(max_length, width * pages.page_size), nat.ptr(since),
+             -1 if max_new is None else min(max_new, 1 << 40), nat.ptr(err_flag), nat.stream_of(pages.device))
+
+
+def paged_block_select(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, count: int, *,
+                       first: int = 1, recent: int = 1, max_length: int | None = None,
+                       err_flag: torch.Tensor | None = None) -> BlockSelection:
+    """Up to ``count`` pages of each sequence and key head that ``q`` (B, heads, head_dim) may find its largest scores in,
+    as a table that ``paged_attention`` takes.
+
+    A page's score is the largest ``sum_d max(q_d max_d, q_d min_d)`` (``pages.bounds``) over the query heads of the key
+    head, which no ``q . k`` of the page exceeds; it is summed in 64 bits and rounded to 32.  The ``first`` and the last
+    ``recent`` (>= 1) pages of a sequence are always kept (``first + recent <= count``), then those with the largest scores:
+    a NaN before every number, a page id outside the pool last, equal scores by the lower page of the sequence.  Sequences
+    of up to ``count`` pages keep all of them.  (Scores stand for ``scale > 0`` in the attention.)  ``max_length`` and
+    ``err_flag`` as for ``paged_attention``."""
+    if pages.index != _get_device():
+        with torch.cuda.device(pages.index):
+            return paged_block_select(q, pages, block_table, lengths, count, first=first, recent=recent,
+                                      max_length=max_length, err_flag=err_flag)
+    B, ld, width = _common("paged_block_select", pages, block_table, lengths, err_flag)
+    if q.get_device() != pages.index:
+        _elsewhere("paged_block_select", pages, q)
+    if q.requires_grad:
+        _no_grad("paged_block_select")
+    if forward_ad._current_level >= 0:
+        _no_tangent("paged_block_select", q)
+    if pages.bounds is None:
+        raise ValueError("paged_block_select needs pages with bounds (bounded=True)")
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or shape[0] != B or shape[2] != pages.head_dim or dtype is not pages.query_dtype:
+        raise ValueError(f"q must be ({B}, heads, {pages.head_dim}) in {pages.query_dtype}, got {tuple(shape)} {dtype}")
+    heads = shape[1]
+    if heads < 1 or heads % pages.kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {pages.kv_heads} key heads")
+    if first < 0 or recent < 1 or first + recent > count:
+        raise ValueError(f"count ({count}) has to hold the first {first} and the last {recent} (one at least) pages")
+    most = _max_length(max_length, width * pages.page_size)
+    blocks = -(-most // pages.page_size)
+    table = block_table.new_empty((B, pages.kv_heads, min(count, blocks)))
+    kept = torch.empty_like(lengths)
+    q, qb, qh = _rows(q, pages, 4 if dtype is torch.float32 else 2)
+    count, first, recent = min(count, 1 << 40), min(first, 1 << 30), min(recent, 1 << 30)  # (as far as a C integer goes)
+    ws_bytes = nat.load().cortex_kv_select_workspace_bytes(pages.ref, B, most, count)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=pages.device) if ws_bytes else None
+    nat.call("cortex_kv_select", pages.ref, B, heads, q.data_ptr(), qb, qh, block_table.data_ptr(), ld, width,
+             lengths.data_ptr(), most, count, first, recent, table.data_ptr(), kept.data_ptr(), nat.ptr(ws), ws_bytes,
+             nat.ptr(err_flag), nat.stream_of(pages.device))
+    return BlockSelection(table, kept)
+
+
+def kv_copy_pages(pages: KVPages, src: torch.Tensor, dst: torch.Tensor, *, into: KVPages | None = None,
+                  err_flag: torch.Tensor | None = None) -> None:
+    """Copies page ``src[i]`` to page ``dst[i]`` (int32, of one length) of the same pools, or of ``into``: keys, values and
+    what else the pools have.  ``into`` has pages of the same shape and kind, and shares no memory with ``pages``.
+
+    No page may be in ``dst`` twice, nor, within one pool, in ``dst`` and elsewhere in ``src``: the copies run side by
+    side, so what such a page then holds is not defined.  A pair with an id outside its pool is skipped and sets bit 2 of
+    ``err_flag``."""
+    if pages.index != _get_device():
+        with torch.cuda.device(pages.index):
+            return kv_copy_pages(pages, src, dst, into=into, err_flag=err_flag)
+    to = pages if into is None else into
+    idx = pages.index
+    if (src.get_device() != idx or dst.get_device() != idx or to.index != idx
+            or (err_flag is not None and err_flag.get_device() != idx)):
+        _elsewhere("kv_copy_pages", pages, src, dst, to.k, err_flag)
+    if (src.dtype is not torch.int32 or dst.dtype is not torch.int32 or src.dim() != 1 or dst.shape != src.shape
+            or not src.is_contiguous() or not dst.is_contiguous()):
+        raise ValueError(f"src and dst must be contiguous int32 tensors of one length, got {tuple(src.shape)} {src.dtype} and "
+                         f"{tuple(dst.shape)} {dst.dtype}")
+    if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
+        raise ValueError("kv_copy_pages: err_flag must be one int32")
+    if into is not None:
+        if to.k.shape[1:] != pages.k.shape[1:] or to.k.dtype is not pages.k.dtype:
+            raise ValueError(f"into must have pages of (kv_heads, page_size, head_dim) {tuple(pages.k.shape[1:])} "
+                             f"{pages.k.dtype}, got {tuple(to.k.shape[1:])} {to.k.dtype}")
+        for name in ("weight", "position", "bounds"):
+            if (getattr(to, name) is None) != (getattr(pages, name) is None):
+                raise ValueError(f"{name} must be in both pools or in neither")
+    nat.call("cortex_kv_copy_pages", pages.ref, to.ref, src.shape[0], src.data_ptr(), dst.data_ptr(), nat.ptr(err_flag),
+             nat.stream_of(pages.device))
 
 
 def kv_evict_plan(pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, budget: int, recent: int, *,
@@ -362,4 +518,5 @@ def kv_evict_apply(pages: KVPages, block_table: torch.Tensor, plan: EvictPlan, *
              shape[2], counts.data_ptr(), nat.ptr(err_flag), nat.stream_of(pages.device))
 
 
-__all__ = ["EvictPlan", "KVPages", "kv_evict_apply", "kv_evict_plan", "paged_attention", "paged_kv_append"]
+__all__ = ["BlockSelection", "EvictPlan", "KVPages", "kv_block_bounds", "kv_copy_pages", "kv_evict_apply", "kv_evict_plan",
+           "paged_attention", "paged_block_select", "paged_kv_append"]

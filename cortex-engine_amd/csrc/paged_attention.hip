@@ -61,6 +61,7 @@ struct PagedArgs {
   int units;            // units a sequence: kv_heads * row_tiles
   int shares;
   int begin;            // tiles that beginning a unit counts for
+  int64_t table_sh;     // from a key head's row of the block table to the next one's: 0, one row for all of them
   const void* q;
   int64_t q_sb, q_sh;
   const int64_t* lengths;
@@ -229,7 +230,7 @@ void paged_attention_kernel(PagedArgs a) {
     const char* kbase = reinterpret_cast<const char*>(p.k) + h * p.k_head * ES;
     const char* vbase = reinterpret_cast<const char*>(p.v) + h * p.v_head * ES;
     const int mask = (1 << p.shift) - 1;
-    const int32_t* table = p.table + b * p.ld_table;
+    const int32_t* table = p.table + b * p.ld_table + h * a.table_sh;
     // the page ids of this lane's 8 keys of a tile: for the key rows (8 (r / 4) ..) and the value rows (8 g ..)
     const int last = (int)p.max_slots - 1;  // (not the last key: the lookups need not wait for the length)
     auto page_at = [&](int j) { return table[min(j, last) >> p.shift]; };
@@ -497,7 +498,7 @@ void paged_attention_kernel(PagedArgs a) {
         for (int j = tid; j < (int)n; j += THREADS) {
           float add = 0.0f;
           for (int r = 0; r < rows; ++r) add += exp2f(score[r * a.score_ld + j] - stat[r].x) * stat[r].y;
-          const int page = p.page_of(b, j);
+          const int page = p.page_of(b, j, h * a.table_sh);
           if (page >= 0) p.weight[p.scalar_at(page, h, p.row_of(j))] += add;
         }
       }
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(PJ_THREADS) void paged_join_kernel(PagedArgs a, int
 #pragma unroll
     for (int i = 0; i < PJ_AHEAD; ++i)
       ahead[i] = *reinterpret_cast<const f32x4*>(score + (i < a.group ? i : 0) * a.score_ld);
-    const int page = a.p.page_of(b, at);  // (four keys of one page)
+    const int page = a.p.page_of(b, at, h * a.table_sh);  // (four keys of one page)
     f32x4* weight = reinterpret_cast<f32x4*>(a.p.weight + a.p.scalar_at(page < 0 ? 0 : page, h, a.p.row_of(at)));
     const f32x4 old = *weight;
     // m and 1 / l of the query heads, a wavefront each
@@ -763,12 +764,13 @@ extern "C" int64_t cortex_paged_attention_workspace_bytes(const cortex_kv_pages*
   return y.part + y.score + y.stats;
 }
 
-extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q,
-                                      int64_t q_sb, int64_t q_sh, const int32_t* block_table, int64_t ld_table,
-                                      int64_t max_pages, const int64_t* lengths, int64_t max_length, float scale,
-                                      int accumulate, void* out, int64_t o_sb, int64_t o_sh, void* workspace,
-                                      int64_t workspace_bytes, int32_t* err, hipStream_t stream) {
-  const char* who = "cortex_paged_attention";
+namespace cortex {
+namespace {
+
+int paged_attention(const char* who, const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb,
+                    int64_t q_sh, const int32_t* block_table, int64_t ld_table, int64_t table_sh, int64_t max_pages,
+                    const int64_t* lengths, int64_t max_length, float scale, int accumulate, void* out, int64_t o_sb,
+                    int64_t o_sh, void* workspace, int64_t workspace_bytes, int32_t* err, hipStream_t stream) {
   PagedArgs a = {};
   if (int rc = kv_check(who, pages, B, block_table, ld_table, max_pages, &a.p)) return rc;
   a.max_length = expected_length(max_length, a.p.max_slots);
@@ -795,6 +797,7 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   a.units = y.units;
   a.shares = y.shares;
   a.begin = y.begin;
+  a.table_sh = table_sh;
   a.q = q;
   a.q_sb = q_sb;
   a.q_sh = q_sh;
@@ -811,4 +814,29 @@ extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, i
   if (pages->dtype == DT_F32) return launch_type<float>(a, y.waves, accumulate, stream);
   if (pages->dtype == DT_BF16) return launch_type<bf16>(a, y.waves, accumulate, stream);
   return launch_type<int8_t>(a, y.waves, accumulate, stream);
+}
+
+}  // namespace
+}  // namespace cortex
+
+extern "C" int cortex_paged_attention(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q,
+                                      int64_t q_sb, int64_t q_sh, const int32_t* block_table, int64_t ld_table,
+                                      int64_t max_pages, const int64_t* lengths, int64_t max_length, float scale,
+                                      int accumulate, void* out, int64_t o_sb, int64_t o_sh, void* workspace,
+                                      int64_t workspace_bytes, int32_t* err, hipStream_t stream) {
+  return paged_attention("cortex_paged_attention", pages, B, heads, q, q_sb, q_sh, block_table, ld_table, 0, max_pages,
+                         lengths, max_length, scale, accumulate, out, o_sb, o_sh, workspace, workspace_bytes, err, stream);
+}
+
+extern "C" int cortex_paged_attention_tables(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q,
+                                             int64_t q_sb, int64_t q_sh, const int32_t* block_tables, int64_t ld_table,
+                                             int64_t table_sh, int64_t max_pages, const int64_t* lengths,
+                                             int64_t max_length, float scale, int accumulate, void* out, int64_t o_sb,
+                                             int64_t o_sh, void* workspace, int64_t workspace_bytes, int32_t* err,
+                                             hipStream_t stream) {
+  const char* who = "cortex_paged_attention_tables";
+  CORTEX_CHECK_ARG(table_sh >= 0 && (!pages || pages->kv_heads <= 1 || table_sh >= max_pages),
+                   "%s: rows of the block tables overlap", who);
+  return paged_attention(who, pages, B, heads, q, q_sb, q_sh, block_tables, ld_table, table_sh, max_pages, lengths,
+                         max_length, scale, accumulate, out, o_sb, o_sh, workspace, workspace_bytes, err, stream);
 }

@@ -24,10 +24,10 @@ struct KvPages {
   int32_t shift;      // log2(page_size)
   int64_t max_slots;  // max_pages * page_size
 
-  // page of slot j of sequence b, or -1
-  __device__ __forceinline__ int page_of(int64_t b, int64_t j) const {
+  // page of slot j of sequence b, or -1; `at`: where the rows of a table by key heads begin for this head
+  __device__ __forceinline__ int page_of(int64_t b, int64_t j, int64_t at = 0) const {
     if (j < 0 || j >= max_slots) return -1;
-    const int p = table[b * ld_table + (j >> shift)];
+    const int p = table[b * ld_table + at + (j >> shift)];
     return (uint32_t)p < (uint32_t)num_pages ? p : -1;
   }
   __device__ __forceinline__ int row_of(int64_t j) const { return (int)(j & ((1ll << shift) - 1)); }

@@ -527,6 +527,7 @@ typedef struct cortex_kv_pages {
   float* v_scale;
   float* weight;
   int32_t* position;
+  void* bounds; /* read by cortex_kv_copy_pages, cortex_kv_block_bounds and cortex_kv_select alone */
 } cortex_kv_pages;
 
 /* The rows of n_tokens new tokens into the pages of B sequences.  k, v (n_tokens, kv_heads, head_dim)
@@ -584,6 +585,60 @@ int cortex_kv_evict_plan(const cortex_kv_pages* pages, int64_t B, const int32_t*
 int cortex_kv_evict_apply(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
                           int64_t max_pages, const int32_t* dst, const int32_t* src, int64_t cap,
                           const int32_t* counts, int32_t* err, hipStream_t stream);
+
+/* cortex_paged_attention with a row of the block table for each key head: entry (b, h, i) at
+ * b * ld_table + h * table_sh + i, table_sh >= max_pages; lengths[b] slots of each of them.  The workspace is
+ * cortex_paged_attention_workspace_bytes, too. */
+int cortex_paged_attention_tables(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb,
+                                  int64_t q_sh, const int32_t* block_tables, int64_t ld_table, int64_t table_sh,
+                                  int64_t max_pages, const int64_t* lengths, int64_t max_length, float scale,
+                                  int accumulate, void* out, int64_t o_sb, int64_t o_sh, void* workspace,
+                                  int64_t workspace_bytes, int32_t* err, hipStream_t stream);
+
+/* Page src[i] of `from` into page dst[i] of `to`, for i < n: key and value rows and, where the pools have them, scales,
+ * weight, position and bounds.  `to` may be `from`; other pools share no memory with it.  No page may be
+ * twice in dst, nor in dst and (of one pool) in src at another i.  A pair with an id outside its pool is skipped. */
+int cortex_kv_copy_pages(const cortex_kv_pages* from, const cortex_kv_pages* to, int64_t n, const int32_t* src,
+                         const int32_t* dst, int32_t* err, hipStream_t stream);
+
+/* bounds (num_pages, kv_heads, 2, head_dim), contiguous, in the keys' dtype (f32 for int8 pages): the largest and the
+ * smallest value of a page's keys in every dim, NaN where a key has one.  Written for the pages that hold a slot of
+ * [since[b], lengths[b]) (since NULL: 0), from all rows of the page below lengths[b].  max_length as above; max_new:
+ * how many slots [since[b], lengths[b]) has at most (negative: unknown; more are right, but slower). */
+int cortex_kv_block_bounds(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
+                           int64_t max_pages, const int64_t* lengths, int64_t max_length, const int64_t* since,
+                           int64_t max_new, int32_t* err, hipStream_t stream);
+
+/* The pages of a sequence that a query may find its largest scores in, per key head.  Block i of a sequence is page i of
+ * its table; its score is the largest of
+ *   sum_d max(q_d max_d, q_d min_d) = max(q, 0) . max + min(q, 0) . min   (bounds max, min)
+ * over the query heads of the key head, summed in 64 bits and rounded to 32.  Kept are the first `first` and the last
+ * `recent` (>= 1) blocks and then those with the largest scores (a NaN before every number, a block without a page last,
+ * equal ones by the lower block), `count` in all or as many as there are.
+ * table (B, kv_heads, keep) int32, keep = min(count, ceil(max_length / page_size)): the pages kept, in the order of the
+ * blocks, -1 behind them; new_lengths[b]: the slots in use in them (the same for every key head: the last block, which
+ * alone may be in use in part, is always kept), 0 for a malformed negative length.  workspace:
+ * cortex_kv_select_workspace_bytes for the call's own max_length, given as the length that it stands for; 16-byte aligned. */
+int64_t cortex_kv_select_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t max_length, int64_t count);
+int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb, int64_t q_sh,
+                     const int32_t* block_table, int64_t ld_table, int64_t max_pages, const int64_t* lengths,
+                     int64_t max_length, int64_t count, int64_t first, int64_t recent, int32_t* table,
+                     int64_t* new_lengths, void* workspace, int64_t workspace_bytes, int32_t* err, hipStream_t stream);
+
+/* Queries (T, heads, dim) and keys (T, kv_heads, dim), f32 or bf16, element (t, h, d) at t * st + h * sh + d, rows 16-byte
+ * aligned: with norm != 0 every row x / sqrt(mean(x^2) + eps) (times its gain (dim), f32 or bf16, where given), then
+ * turned by position:
+ *   angle of pair p = positions[t * p_st + axes[p] * p_sa] * inv_freq[p]   (the product in 64 bits; axes NULL: 0)
+ *   (y_i, y_j) = (x_i cos - x_j sin, x_j cos + x_i sin),  (i, j) = (p, p + pairs), interleaved: (2 p, 2 p + 1)
+ * dims past 2 * pairs are not turned.  All in fp32, rounded once.  dim: a multiple of 8 up to 256, pairs a multiple of 8.
+ * A pair whose axis is outside [0, n_axes) is not turned and ORs bit 3 (value 8) into *err (when given).  An output
+ * may be its own input and overlaps nothing else. */
+int cortex_qk_norm_rope(int64_t T, int64_t heads, int64_t kv_heads, int64_t dim, int dtype, const void* q, int64_t q_st,
+                        int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const int64_t* positions, int64_t p_st,
+                        int64_t p_sa, int64_t n_axes, int64_t pairs, const float* inv_freq, const int32_t* axes,
+                        int interleaved, int norm, float eps, const void* q_gain, const void* k_gain, int gain_dtype,
+                        void* q_out, int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh,
+                        int32_t* err, hipStream_t stream);
 
 /* Host page table of the event page cache (no device work; not thread-safe, one caller per
  * table).  Replaces the Python bookkeeping of StreamingKVCache with the same policy
