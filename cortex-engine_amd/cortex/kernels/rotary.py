@@ -30,25 +30,36 @@ def rotary_frequencies(dims: int, *, base: float = 10000.0, device: str | torch.
     return (base ** (-2.0 * p / dims)).to(device=device, dtype=torch.float32)
 
 
-def _row(t: torch.Tensor, es: int) -> torch.Tensor:
-    """Rows that vector loads take: as given, or copied."""
-    if t.stride(2) != 1 or (t.data_ptr() | t.stride(0) * es | t.stride(1) * es) & 15:
+def _rows(t: torch.Tensor, es: int) -> tuple[torch.Tensor, int, int]:
+    """Rows that vector loads take, as given or copied, and the strides of their tokens and heads."""
+    if t.is_contiguous():
+        if t.data_ptr() & 15:
+            t = t.clone()
+        _, heads, dim = t.shape
+        return t, heads * dim, dim
+    st, sh, unit = t.stride()
+    if unit != 1 or (t.data_ptr() | st * es | sh * es) & 15:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        st, sh, _ = t.stride()
+    return t, st, sh
 
 
-def _result(x: torch.Tensor, out: torch.Tensor | None, es: int, name: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.shape != x.shape or out.dtype is not x.dtype:
-        raise ValueError(f"{name} must be a {tuple(x.shape)} {x.dtype} tensor, got {tuple(out.shape)} {out.dtype}")
-    if x.numel() == 0:
-        return out
-    if out.stride(2) != 1 or (out.data_ptr() | out.stride(0) * es | out.stride(1) * es) & 15:
-        raise ValueError(f"the rows of {name} must be contiguous and 16-byte aligned")
-    if _own_overlap(out):
-        raise ValueError(f"{name} may not overlap itself (an expanded tensor)")
-    return out
+def _check_out(out: tuple[torch.Tensor, torch.Tensor], q: torch.Tensor, k: torch.Tensor, es: int) -> None:
+    for i, (y, own, x) in enumerate(((out[0], q, k), (out[1], k, q))):
+        if y.shape != own.shape or y.dtype is not own.dtype:
+            raise ValueError(f"out[{i}] must be a {tuple(own.shape)} {own.dtype} tensor, got {tuple(y.shape)} {y.dtype}")
+        if y.numel() == 0:
+            continue
+        st, sh, unit = y.stride()
+        if unit != 1 or (y.data_ptr() | st * es | sh * es) & 15:
+            raise ValueError(f"the rows of out[{i}] must be contiguous and 16-byte aligned")
+        if _own_overlap(y):
+            raise ValueError(f"out[{i}] may not overlap itself (an expanded tensor)")
+        same = y.data_ptr() == own.data_ptr() and y.stride() == own.stride()
+        if (not same and _overlap(y, own)) or (x.numel() and _overlap(y, x)):
+            raise ValueError("a result may be its own input, and overlaps no other")
+    if out[0].numel() and out[1].numel() and _overlap(*out):
+        raise ValueError("the results may not overlap each other")
 
 
 def _gain(t: torch.Tensor | None, dim: int, name: str) -> torch.Tensor | None:
@@ -80,27 +91,31 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     (int32, never cleared here).  ``out``: where the results go; each may be its own input (in place) and overlaps no
     other tensor of the call."""
     idx = q.get_device()
-    if q.is_cuda and idx != _get_device():
+    given = [t for t in (axes, q_gain, k_gain, err_flag) if t is not None]
+    if out is not None:
+        given += out
+    if idx < 0 or k.get_device() != idx or positions.get_device() != idx or inv_freq.get_device() != idx or any(
+            [t.get_device() != idx for t in given]):
+        nat.require_gpu(q, k, positions, inv_freq, *given, what=_WHAT)
+    if idx != _get_device():
         with torch.cuda.device(idx):
             return qk_norm_rope(q, k, positions, inv_freq, axes=axes, interleaved=interleaved, eps=eps, q_gain=q_gain,
                                 k_gain=k_gain, out=out, err_flag=err_flag)
-    q_out, k_out = (None, None) if out is None else out
-    device = nat.require_gpu(q, k, positions, inv_freq, axes, q_gain, k_gain, q_out, k_out, err_flag, what=_WHAT)
-    if any(t is not None and t.requires_grad for t in (q, k, inv_freq, q_gain, k_gain, q_out, k_out)):
+    if q.requires_grad or k.requires_grad or inv_freq.requires_grad or any([t.requires_grad for t in given]):
         _no_grad(_WHAT)
     if forward_ad._current_level >= 0:
-        _no_tangent(_WHAT, q, k, inv_freq, q_gain, k_gain, q_out, k_out)
-    dtype = q.dtype
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or k.dtype is not dtype:
-        raise ValueError(f"q and k must be (T, heads, head_dim) of one dtype, got {tuple(q.shape)} {dtype} and "
-                         f"{tuple(k.shape)} {k.dtype}")
+        _no_tangent(_WHAT, q, k, inv_freq, *given)
+    shape, k_shape, dtype = q.shape, k.shape, q.dtype
+    if len(shape) != 3 or len(k_shape) != 3 or shape[0] != k_shape[0] or shape[2] != k_shape[2] or k.dtype is not dtype:
+        raise ValueError(f"q and k must be (T, heads, head_dim) of one dtype, got {tuple(shape)} {dtype} and "
+                         f"{tuple(k_shape)} {k.dtype}")
     if dtype is torch.bfloat16:
         code, es = nat.BF16, 2
     elif dtype is torch.float32:
         code, es = nat.F32, 4
     else:
         raise ValueError(f"rows of dtype {dtype} are not supported (bfloat16 or float32)")
-    T, heads, dim = q.shape
+    T, heads, dim = shape
     if dim % 8 or not 8 <= dim <= 256:
         raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {dim}")
     if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
@@ -108,43 +123,43 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     pairs = inv_freq.shape[0]
     if pairs % 8 or 2 * pairs > dim:
         raise ValueError(f"{pairs} pairs: a multiple of 8 up to half of the head_dim {dim} is needed")
-    if positions.dtype is not torch.int64 or positions.dim() not in (1, 2) or positions.shape[0] != T:
-        raise ValueError(f"positions must be ({T},) or ({T}, axes) int64, got {tuple(positions.shape)} {positions.dtype}")
-    if positions.dim() == 1:
+    at = positions.shape
+    if positions.dtype is not torch.int64 or len(at) not in (1, 2) or at[0] != T:
+        raise ValueError(f"positions must be ({T},) or ({T}, axes) int64, got {tuple(at)} {positions.dtype}")
+    if len(at) == 1:
         p_st, p_sa, n_axes = positions.stride(0), 0, 1
     else:
-        (p_st, p_sa), n_axes = positions.stride(), positions.shape[1]
-    if n_axes < 1:
-        raise ValueError("positions need one axis at least")
+        (p_st, p_sa), n_axes = positions.stride(), at[1]
+        if n_axes < 1:
+            raise ValueError("positions need one axis at least")
     if axes is not None and (axes.dtype is not torch.int32 or axes.shape != (pairs,) or not axes.is_contiguous()):
         raise ValueError(f"axes must be a contiguous ({pairs},) int32 tensor")
+    gain_code = nat.F32
     if eps is None:
         if q_gain is not None or k_gain is not None:
             raise ValueError("gains belong to the norm: give eps")
     elif not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    elif q_gain is not None or k_gain is not None:
+        q_gain, k_gain = _gain(q_gain, dim, "q_gain"), _gain(k_gain, dim, "k_gain")
+        if q_gain is not None and k_gain is not None and q_gain.dtype is not k_gain.dtype:
+            raise ValueError(f"q_gain and k_gain of different dtypes: {q_gain.dtype} and {k_gain.dtype}")
+        gain_code = nat.code((k_gain if q_gain is None else q_gain).dtype)
     if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
         raise ValueError("err_flag must be one int32")
-    q_gain, k_gain = _gain(q_gain, dim, "q_gain"), _gain(k_gain, dim, "k_gain")
-    if q_gain is not None and k_gain is not None and q_gain.dtype is not k_gain.dtype:
-        raise ValueError(f"q_gain and k_gain of different dtypes: {q_gain.dtype} and {k_gain.dtype}")
-    gain_code = nat.F32 if any(g is not None and g.dtype is torch.float32 for g in (q_gain, k_gain)) else nat.BF16
-    q_out, k_out = _result(q, q_out, es, "out[0]"), _result(k, k_out, es, "out[1]")
-    if out is not None:
-        for y, own, x in ((q_out, q, k), (k_out, k, q)):
-            if y.numel() == 0:
-                continue
-            same = y.data_ptr() == own.data_ptr() and y.stride() == own.stride()
-            if (not same and own.numel() and _overlap(y, own)) or (x.numel() and _overlap(y, x)):
-                raise ValueError("a result may be its own input, and overlaps no other")
-        if q_out.numel() and k_out.numel() and _overlap(q_out, k_out):
-            raise ValueError("the results may not overlap each other")
-    q, k = _row(q, es), _row(k, es)
-    nat.call("cortex_qk_norm_rope", T, heads, k.shape[1], dim, code, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-             k.stride(0), k.stride(1), positions.data_ptr(), p_st, p_sa, n_axes, pairs, inv_freq.data_ptr(), nat.ptr(axes),
-             interleaved, eps is not None, 0.0 if eps is None else eps, nat.ptr(q_gain), nat.ptr(k_gain), gain_code,
-             q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1),
-             nat.ptr(err_flag), nat.stream_of(device))
+    if out is None:
+        q_out, k_out = q.new_empty(shape), k.new_empty(k_shape)
+        yt, yh, zt, zh = heads * dim, dim, k_shape[1] * dim, dim
+    else:
+        _check_out(out, q, k, es)
+        q_out, k_out = out
+        (yt, yh, _), (zt, zh, _) = q_out.stride(), k_out.stride()
+    q, st, sh = _rows(q, es)
+    k, kt, kh = _rows(k, es)
+    nat.call("cortex_qk_norm_rope", T, heads, k_shape[1], dim, code, q.data_ptr(), st, sh, k.data_ptr(), kt, kh,
+             positions.data_ptr(), p_st, p_sa, n_axes, pairs, inv_freq.data_ptr(), nat.ptr(axes), interleaved,
+             eps is not None, 0.0 if eps is None else eps, nat.ptr(q_gain), nat.ptr(k_gain), gain_code, q_out.data_ptr(), yt,
+             yh, k_out.data_ptr(), zt, zh, nat.ptr(err_flag), nat.stream_of(q_out.device))
     return q_out, k_out
 
 
