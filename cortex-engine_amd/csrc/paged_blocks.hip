@@ -116,6 +116,46 @@ __device__ __forceinline__ float most_of(float a, float b) { return __builtin_el
 __device__ __forceinline__ float least_of(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 
 constexpr int KB_AHEAD = 4;  // rows in flight a lane
+constexpr int KB_PER_CU = 32;  // workgroups (16 sequences of 1000 .. 15001 int8 keys, 4 heads x 128: 8 a CU 24.2 us, 16 21.8, 32 and 64 21.0)
+
+// What two lanes have of the same dims, joined: the lanes of the lower half (of every 32, of every 64) go on with a, the
+// others with b.
+template <int SPAN, class F>
+__device__ __forceinline__ float halves(float a, float b, F f) {
+  if constexpr (SPAN == 64) {
+    const auto u = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return f(__uint_as_float(u[0]), __uint_as_float(u[1]));
+  } else {
+    const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return f(__uint_as_float(u[0]), __uint_as_float(u[1]));
+  }
+}
+
+// x[0 .. N): N dims of a row in each of 64 / lanes groups of lanes.  Joined over the groups, the first N / 4 (32 lanes a row:
+// N / 2) hold dims N / 2 (lane / 32) + N / 4 (lane / 16 % 2) .. (N / 2 (lane / 32) ..).
+template <int N, class F>
+__device__ __forceinline__ void join_groups(float (&x)[N], int lanes, F f) {
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) x[e] = halves<64>(x[e], x[e + N / 2], f);
+  if (lanes > 16) return;
+#pragma unroll
+  for (int e = 0; e < N / 4; ++e) x[e] = halves<32>(x[e], x[e + N / 4], f);
+#pragma unroll
+  for (int e = 0; e < N / 4; ++e) {
+    if (lanes <= 8) x[e] = f(x[e], dpp_mov<0x128>(x[e]));
+    if (lanes <= 4) x[e] = f(x[e], __shfl_xor(x[e], 4, 64));
+    if (lanes <= 2) x[e] = f(x[e], dpp_mov<0x4E>(x[e]));
+    if (lanes <= 1) x[e] = f(x[e], dpp_mov<0xB1>(x[e]));
+  }
+}
+
+template <class O, int N>
+__device__ __forceinline__ void store_bounds(O* to, const float* f) {
+  O v[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = from_f32<O>(f[e]);
+  __builtin_memcpy(__builtin_assume_aligned(to, N * sizeof(O)), v, sizeof(v));
+}
 
 // A wavefront takes a (page, key head) at a time: `lanes` lanes a row, 16 bytes each, the groups of lanes joined at the end.
 template <class P>
@@ -130,25 +170,32 @@ __global__ __launch_bounds__(256) void kv_bounds_kernel(BoundsArgs a) {
   if (!ok && chunk == 0 && threadIdx.x == 0) kv_flag(a.err);
   const int64_t begin = a.since ? min(max(a.since[b], (int64_t)0), n) : 0;
   if (begin == n) return;
-  const int first = (int)(begin >> p.shift), blocks = (int)((n - 1) >> p.shift) + 1 - first;
-  const int groups = 64 / a.lanes, group = lane / a.lanes, d = (lane % a.lanes) * N;
+  const int end = (int)((n - 1) >> p.shift) + 1;
+  const int group = lane / a.lanes, groups = 64 / a.lanes, d = (lane & (a.lanes - 1)) * N;
   const bool in = d < p.head_dim;
-  const int64_t items = (int64_t)blocks * p.kv_heads;
-  for (int64_t i = (int64_t)chunk * 4 + wid; i < items; i += (int64_t)a.chunks * 4) {
-    const int block = (int)(i / p.kv_heads), h = (int)(i - (int64_t)block * p.kv_heads);
-    const int64_t j = (int64_t)(first + block) << p.shift;
-    const int page = p.page_of(b, j);
-    if (page < 0) {
+  // blocks and heads of this wavefront: `step` further are `blocks` blocks and `heads` heads
+  const int step = a.chunks * 4, blocks = step / p.kv_heads, heads = step - blocks * p.kv_heads;
+  const int i0 = chunk * 4 + wid;
+  int block = (int)(begin >> p.shift) + i0 / p.kv_heads, h = i0 % p.kv_heads;
+  int page = block < end ? p.page_of(b, (int64_t)block << p.shift) : -1;
+  while (block < end) {
+    const int64_t j = (int64_t)block << p.shift;
+    const int now = page, head = h;
+    h += heads;
+    block += blocks + (h >= p.kv_heads ? 1 : 0);
+    h -= h >= p.kv_heads ? p.kv_heads : 0;
+    if (block < end) page = p.page_of(b, (int64_t)block << p.shift);
+    if (now < 0) {
       if (lane == 0) kv_flag(a.err);
       continue;
     }
     const int used = (int)min(n - j, 1ll << p.shift);
-    const char* k = reinterpret_cast<const char*>(p.k) + (page * p.k_page + h * p.k_head + (in ? d : 0)) * ES;
-    const float* scale = ES == 1 ? p.k_scale + p.scalar_at(page, h, 0) : nullptr;
+    const char* k = reinterpret_cast<const char*>(p.k) + (now * p.k_page + head * p.k_head + (in ? d : 0)) * ES;
+    const float* scale = ES == 1 ? p.k_scale + p.scalar_at(now, head, 0) : nullptr;
     float most[N], least[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) most[e] = -INFINITY, least[e] = INFINITY;
-    for (int r = group; r < used; r += groups * KB_AHEAD) {
+    for (int r = group; r - group < used; r += groups * KB_AHEAD) {
       i32x4 x[KB_AHEAD];
       float s[KB_AHEAD];
 #pragma unroll
@@ -169,25 +216,19 @@ __global__ __launch_bounds__(256) void kv_bounds_kernel(BoundsArgs a) {
         }
       }
     }
-    for (int o = a.lanes; o < 64; o <<= 1)
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        most[e] = most_of(most[e], __shfl_xor(most[e], o, 64));
-        least[e] = least_of(least[e], __shfl_xor(least[e], o, 64));
+    join_groups<N>(most, a.lanes, most_of);
+    join_groups<N>(least, a.lanes, least_of);
+    // (lanes of 16 that hold the same: the first of them)
+    if (in && (a.lanes >= 16 || (lane & 15) < a.lanes)) {
+      O* to = reinterpret_cast<O*>(a.bounds) + ((int64_t)now * p.kv_heads + head) * 2 * p.head_dim + d + (lane >> 5) * (N / 2);
+      if (ES == 4 && a.lanes > 16) {
+        store_bounds<O, N / 2>(to, most);
+        store_bounds<O, N / 2>(to + p.head_dim, least);
+      } else {
+        to += (lane >> 4 & 1) * (N / 4);
+        store_bounds<O, N / 4>(to, most);
+        store_bounds<O, N / 4>(to + p.head_dim, least);
       }
-    if (group == 0 && in) {
-      O out[2][N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) out[0][e] = from_f32<O>(most[e]), out[1][e] = from_f32<O>(least[e]);
-      O* to = reinterpret_cast<O*>(a.bounds) + ((int64_t)page * p.kv_heads + h) * 2 * p.head_dim + d;
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int x = 0; x < (int)(N * sizeof(O) / 16); ++x) {
-          i32x4 w;
-          __builtin_memcpy(&w, reinterpret_cast<const char*>(out[y]) + 16 * x, 16);
-          reinterpret_cast<i32x4*>(to + y * p.head_dim)[x] = w;
-        }
     }
   }
 }
@@ -209,11 +250,10 @@ struct SelectArgs {
   int32_t* err;
   uint32_t* rank;  // workspace: (B, kv_heads, ld)
   int64_t ld;
-  int tiles;       // of 16 blocks a (sequence, key head) at most
 };
 
-// Ranks: 0 for a block without a page, then by score, NaN above every number, then the blocks that are always kept.
-constexpr uint32_t KEPT = 0xffffffffu, NOT_A_NUMBER = 0xfffffffeu;
+// Ranks: 1 for a block without a page, then by score, NaN above every number.  (0: not a candidate.)
+constexpr uint32_t NO_PAGE = 1u, NOT_A_NUMBER = 0xffffffffu;
 __device__ __forceinline__ uint32_t rank_of(float score) {
   if (score != score) return NOT_A_NUMBER;
   const uint32_t u = __float_as_uint(score + 0.0f);  // -0 and 0 are equal
@@ -224,84 +264,404 @@ __device__ __forceinline__ int blocks_of(const SelectArgs& a, int64_t n) {
   return (int)((n + (1ll << a.p.shift) - 1) >> a.p.shift);
 }
 
-// The ranks of 16 blocks a wavefront.  The sums are in 64 bits and rounded to 32 once: which blocks are chosen does not
-// depend on an order of sums.  v_mfma_f64_4x4x4 multiplies four 4 x 4 tiles: lane 16 g + r loads eight dims 8 (4 c + g) ..
-// of the bounds of block r and of the query of head r % 4, and gets the sum of block 4 ((l % 16) / 4) + l / 16 and
-// head l % 4.  DHP: head_dim rounded up to 32.
-template <class O, class Q, int DHP>
-__global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a) {
-  constexpr int NC = DHP / 32;
-  const KvPages& p = a.p;
-  const int lane = threadIdx.x & 63, wid = wave_uniform((int)threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  const int64_t w = (int64_t)blockIdx.x * 4 + wid;
-  const int bh = (int)(w / a.tiles), tile = (int)(w - (int64_t)bh * a.tiles);
-  if (bh >= a.B * p.kv_heads) return;
-  const int b = bh / p.kv_heads, h = bh - b * p.kv_heads;
-  bool ok = true;
-  const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
-  const int blocks = blocks_of(a, n);
-  if (blocks <= a.count || tile * 16 >= blocks) return;  // (all of them are kept)
-  const int block = min(tile * 16 + r, blocks - 1);
-  const int page = p.page_of(b, (int64_t)block << p.shift);
-  if (page < 0 && g == 0) kv_flag(a.err);
-  const O* bounds = reinterpret_cast<const O*>(a.bounds) + ((int64_t)max(page, 0) * p.kv_heads + h) * 2 * p.head_dim;
-  double key[2][NC][8];
+// The ranks of tiles of 16 blocks, a tile a wavefront.  The sums are in 64 bits and rounded to 32 once: which blocks are
+// chosen does not depend on an order of sums.  v_mfma_f64_4x4x4 multiplies four 4 x 4 tiles: lane 16 g + r takes eight dims
+// 8 (4 c + g) .. of the bounds of block r and of the query of head r % 4, and gets the sum of block 4 ((l % 16) / 4) + l / 16
+// and head l % 4.  The bounds come from memory into registers; the queries, max(q, 0) and min(q, 0) in 64 bits, are made
+// once a workgroup while its first bounds are on their way, into LDS: converted at each use they are half of the work.
+// DHP: head_dim rounded up to 64; NG: fours of query heads at a time.
+template <class O, class Q, int DHP, int NG>
+struct Scores {
+  static constexpr int NC = DHP / 32, HEADS = 4 * NG;
+  static constexpr int LD = DHP + 2;  // of a head in LDS: the four heads of a read are in different banks
+  struct Bounds {
+    O x[2][NC][8];
+  };
+  struct Query {
+    double x[2][HEADS][LD];
+  };
+
+  // query heads i .. of a key head (the last one again where there are no more)
+  template <int THREADS>
+  static __device__ __forceinline__ void load_query(const SelectArgs& a, Query& to, int64_t b, int h, int i) {
+    for (int at = threadIdx.x * 4; at < HEADS * DHP; at += THREADS * 4) {
+      const int j = at / DHP, d = at % DHP;
+      Q x[4] = {};
+      if (d < a.p.head_dim)
+        __builtin_memcpy(x, __builtin_assume_aligned(reinterpret_cast<const Q*>(a.q) + b * a.q_sb +
+                                                     (int64_t)(h * a.group + min(i + j, a.group - 1)) * a.q_sh + d, 4 * sizeof(Q)), sizeof(x));
 #pragma unroll
-  for (int y = 0; y < 2; ++y)
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = 8 * (4 * c + g);
-      O x[8] = {};
-      if (d < p.head_dim) __builtin_memcpy(x, __builtin_assume_aligned(bounds + y * p.head_dim + d, 16), sizeof(x));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) key[y][c][e] = (double)to_f32(x[e]);
-    }
-  uint32_t best = 0;
-  for (int i0 = 0; i0 < a.group; i0 += 4) {
-    const Q* q = reinterpret_cast<const Q*>(a.q) + b * a.q_sb + (int64_t)(h * a.group + min(i0 + (r & 3), a.group - 1)) * a.q_sh;
-    double sum = 0.0;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = 8 * (4 * c + g);
-      Q x[8] = {};
-      if (d < p.head_dim) __builtin_memcpy(x, __builtin_assume_aligned(q + d, 16), sizeof(x));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4; ++e) {  // (a NaN is in the first)
         const float f = to_f32(x[e]);
-        // (a NaN reaches the sum by the first)
-        sum = __builtin_amdgcn_mfma_f64_4x4x4f64(key[0][c][e], (double)(f < 0.0f ? 0.0f : f), sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_f64_4x4x4f64(key[1][c][e], (double)(f < 0.0f ? f : 0.0f), sum, 0, 0, 0);
+        to.x[0][j][d + e] = (double)(f < 0.0f ? 0.0f : f);
+        to.x[1][j][d + e] = (double)(f < 0.0f ? f : 0.0f);
       }
     }
-    best = max(best, rank_of((float)sum));
   }
-  best = max(best, (uint32_t)__shfl_xor((int)best, 1, 64));
-  best = max(best, (uint32_t)__shfl_xor((int)best, 2, 64));
-  // this lane's score is of block 4 (r / 4) + g; its lookup was of block r
-  const int mine = tile * 16 + 4 * (r >> 2) + g;
-  const int its_page = __shfl(page, 4 * (r >> 2) + g, 64);
-  if ((r & 3) == 0 && mine < blocks) {
-    if (its_page < 0) best = 0;
-    if (mine < a.first || mine >= blocks - a.recent) best = KEPT;
-    a.rank[(int64_t)bh * a.ld + mine] = best;
-  }
-}
-
-__device__ __forceinline__ int scan64(int v, int lane) {  // inclusive
+  static __device__ __forceinline__ void load_bounds(const SelectArgs& a, Bounds& to, int page, int h, int g) {
+    const O* src = reinterpret_cast<const O*>(a.bounds) + ((int64_t)max(page, 0) * a.p.kv_heads + h) * 2 * a.p.head_dim;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = 8 * (4 * c + g);
+        __builtin_memcpy(to.x[y][c], __builtin_assume_aligned(src + y * a.p.head_dim + (d < a.p.head_dim ? d : 0), 16),
+                         sizeof(to.x[y][c]));
+      }
   }
+  // (the dims behind head_dim, whose query is 0, were loaded from others, which need not be finite)
+  static __device__ __forceinline__ void cut(const SelectArgs& a, Bounds& to, int g) {
+    if (a.p.head_dim == DHP) return;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (8 * (4 * c + g) >= a.p.head_dim) __builtin_memset(to.x[0][c], 0, sizeof(to.x[0][c])), __builtin_memset(to.x[1][c], 0, sizeof(to.x[1][c]));
+  }
+  // Two values, converted where they are used: all at once, ahead of the products, they would take up to 256 registers.
+  static __device__ __forceinline__ void two(const O* x, double (&f)[2]) {
+    uint32_t w[sizeof(O) / 2];
+    __builtin_memcpy(w, x, 2 * sizeof(O));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(O) / 2); ++i) asm volatile("" : "+v"(w[i]));
+    if constexpr (sizeof(O) == 2)
+      f[0] = (double)__uint_as_float(w[0] << 16), f[1] = (double)__uint_as_float(w[0] & 0xffff0000u);
+    else
+      f[0] = (double)__uint_as_float(w[0]), f[1] = (double)__uint_as_float(w[1]);
+  }
+  // the largest rank over the heads of block 4 (r / 4) + g
+  static __device__ __forceinline__ uint32_t rank(const Bounds& k, const Query& q, int r, int g) {
+    constexpr int PARTS = NG == 1 ? 4 : 1;  // sums that do not wait for each other (of the heads and halves, too)
+    double sum[NG][2][PARTS] = {};
+    // the queries of four dims, read a step ahead
+    auto read = [&](double2 (&f)[NG][2][2], int step) {
+#pragma unroll
+      for (int y = 0; y < NG; ++y)
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            f[y][z][i] = *reinterpret_cast<const double2*>(&q.x[z][4 * y + (r & 3)][8 * (4 * (step >> 1) + g) + 4 * (step & 1) + 2 * i]);
+    };
+    double2 f[2][NG][2][2];
+    read(f[0], 0);
+#pragma unroll
+    for (int step = 0; step < 2 * NC; ++step) {
+      if (step + 1 < 2 * NC) read(f[(step + 1) & 1], step + 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = step >> 1, e = 4 * (step & 1) + 2 * i;
+        double bound[2][2];
+        two(&k.x[0][c][e], bound[0]), two(&k.x[1][c][e], bound[1]);
+#pragma unroll
+        for (int y = 0; y < NG; ++y)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const double2 v = f[step & 1][y][z][i];
+            double& s0 = sum[y][z][(2 * i) % PARTS];
+            s0 = __builtin_amdgcn_mfma_f64_4x4x4f64(bound[z][0], v.x, s0, 0, 0, 0);
+            double& s1 = sum[y][z][(2 * i + 1) % PARTS];
+            s1 = __builtin_amdgcn_mfma_f64_4x4x4f64(bound[z][1], v.y, s1, 0, 0, 0);
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint32_t best = 0;
+#pragma unroll
+    for (int y = 0; y < NG; ++y) {
+      double all = 0.0;
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) all += sum[y][z][i];
+      best = max(best, rank_of((float)all));
+    }
+    best = max(best, (uint32_t)__shfl_xor((int)best, 1, 64));
+    return max(best, (uint32_t)__shfl_xor((int)best, 2, 64));
+  }
+
+  // Ranks of the tiles first, first + step .. up to `tiles` of a (sequence, key head) into rank_out[]: 0 for the blocks that
+  // are always kept and, to the end of a tile, for those that are not there.  All threads of the workgroup call it.
+  template <int THREADS>
+  static __device__ __forceinline__ void run(const SelectArgs& a, Query& q, int b, int h, int blocks, int first, int step,
+                                             int tiles, int lane, uint32_t* rank_out) {
+    const int r = lane & 15, g = lane >> 4;
+    auto page_at = [&](int t) { return a.p.page_of(b, (int64_t)min(16 * t + r, blocks - 1) << a.p.shift); };
+    for (int i = 0; i < a.group; i += HEADS) {
+      Bounds now, next;
+      int page = page_at(first), next_page = page_at(first + step);
+      if (first < tiles) load_bounds(a, now, page, h, g);
+      if (i > 0) __syncthreads();
+      load_query<THREADS>(a, q, b, h, i);
+      __syncthreads();
+      if (first >= tiles) continue;
+      auto put = [&](int t) {
+        cut(a, now, g);
+        uint32_t best = rank(now, q, r, g);
+        if (page < 0 && g == 0) kv_flag(a.err);
+        const int mine = 16 * t + 4 * (r >> 2) + g;
+        if (__shfl(page, 4 * (r >> 2) + g, 64) < 0) best = NO_PAGE;
+        if (mine < a.first || mine >= blocks - a.recent) best = 0;
+        if ((r & 3) == 0) rank_out[mine] = i > 0 ? max(best, rank_out[mine]) : best;
+      };
+      int t = first;
+      for (; t + step < tiles; t += step) {  // (the last tile apart: nothing to load beside it)
+        const int page_after = page_at(t + 2 * step);
+        load_bounds(a, next, next_page, h, g);
+        put(t);
+        now = next;
+        page = next_page;
+        next_page = page_after;
+      }
+      put(t);
+    }
+  }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_0(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+// Sums over this lane and those before it.
+__device__ __forceinline__ int scan64(int v) {
+  v += dpp_or_0<0x111, 0xF>(v);
+  v += dpp_or_0<0x112, 0xF>(v);
+  v += dpp_or_0<0x114, 0xF>(v);
+  v += dpp_or_0<0x118, 0xF>(v);
+  v += dpp_or_0<0x142, 0xA>(v);  // the last lane of a row of 16 to the row behind it
+  v += dpp_or_0<0x143, 0xC>(v);  // and of the first half to the second
   return v;
 }
+__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
+  auto more = [](uint32_t p, int q) { return max(p, (uint32_t)q); };
+  x = more(x, dpp_or_0<0x111, 0xF>((int)x));
+  x = more(x, dpp_or_0<0x112, 0xF>((int)x));
+  x = more(x, dpp_or_0<0x114, 0xF>((int)x));
+  x = more(x, dpp_or_0<0x118, 0xF>((int)x));
+  x = more(x, dpp_or_0<0x142, 0xA>((int)x));
+  x = more(x, dpp_or_0<0x143, 0xC>((int)x));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
 
-constexpr int SL_THREADS = 256;
+constexpr int PK_FEW = 64;  // ranks that are compared with each other
 
-// The `count` largest ranks of a (sequence, key head) by a radix selection of a byte a round, and their pages in the
-// order of the blocks.
-__global__ __launch_bounds__(SL_THREADS) void kv_select_kernel(SelectArgs a) {
+template <int WAVES>
+struct PickShared {
+  int hist[64 * WAVES];
+  uint32_t most[WAVES], least[WAVES];
+  int part[WAVES], part2[WAVES];
+  int picked[3], few;
+  uint2 list[PK_FEW];
+};
+
+// Flags before this thread's, and of all threads.
+template <int WAVES, int N>
+__device__ __forceinline__ int before_of(const bool (&flag)[N], int* part, int lane, int wid, int* total) {
+  int mine = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint64_t m = __ballot(flag[i]);
+    mine += __popcll(m & ((1ull << lane) - 1));
+    all += __popcll(m);
+  }
+  if (lane == 0) part[wid] = all;
+  __syncthreads();
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wid) mine += part[w];
+    sum += part[w];
+  }
+  *total = sum;
+  return mine;
+}
+
+// The pages of the a.count blocks to keep, in their order, from the ranks of KPT consecutive blocks a thread (0: always
+// kept, or not there).  The ranks are counted in as many bins as there are threads, even parts of their range; the bin
+// that holds the last one kept is found from the counts, and its ranks, where they are few, are compared with each other
+// by every wavefront for itself.  Where they are many the bin is cut into bins again.
+template <int WAVES, int KPT>
+__device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[KPT], int blocks, const int32_t* pages,
+                                     int32_t* out, PickShared<WAVES>& s) {
+  constexpr int BINS = 64 * WAVES;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, i0 = tid * KPT;
+  int need = a.count - a.first - a.recent, total;
+  bool keep[KPT], open[KPT];  // open: not decided yet
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    open[i] = need > 0 && key[i] != 0;
+    keep[i] = i0 + i < blocks && (i0 + i < a.first || i0 + i >= blocks - a.recent);
+  }
+  while (need > 0) {  // (the same for all threads)
+    uint32_t most = 0, least = 0;  // the largest rank, and of the inverted ranks
+#pragma unroll
+    for (int i = 0; i < KPT; ++i)
+      if (open[i]) most = max(most, key[i]), least = max(least, ~key[i]);
+    most = wave_most(most), least = wave_most(least);
+    if (lane == 0) s.most[wid] = most, s.least[wid] = least;
+    s.hist[tid] = 0;
+    if (tid == 0) s.few = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) most = max(most, s.most[w]), least = max(least, s.least[w]);
+    const uint32_t low = ~least, range = most - low;
+    if (range == 0) {  // one rank for all: the lower blocks
+      int before = before_of<WAVES, KPT>(open, s.part, lane, wid, &total);
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) {
+        keep[i] = keep[i] || (open[i] && before < need);
+        before += open[i];
+      }
+      break;
+    }
+    // (conversion, product and truncation keep the order)
+    const float scale = (float)BINS / ((float)range + 1.0f);
+    int bin[KPT];
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      bin[i] = min((int)((float)(key[i] - low) * scale), BINS - 1);
+      if (open[i]) atomicAdd(&s.hist[bin[i]], 1);
+    }
+    __syncthreads();
+    const int mine = s.hist[BINS - 1 - tid], upto = scan64(mine);
+    if (lane == 63) s.part2[wid] = upto;
+    __syncthreads();
+    int before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      if (w < wid) before += s.part2[w];
+    if (before < need && before + mine >= need) s.picked[0] = BINS - 1 - tid, s.picked[1] = before, s.picked[2] = mine;
+    __syncthreads();
+    const int last = s.picked[0], many = s.picked[2];
+    need -= s.picked[1];
+    const bool whole = need == many;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      keep[i] = keep[i] || (open[i] && (whole ? bin[i] >= last : bin[i] > last));
+      open[i] = open[i] && !whole && bin[i] == last;
+    }
+    if (whole) break;
+    if (many > PK_FEW) continue;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i)
+      if (open[i]) s.list[atomicAdd(&s.few, 1)] = make_uint2(key[i], (uint32_t)(i0 + i));
+    __syncthreads();
+    const uint2 own = lane < many ? s.list[lane] : make_uint2(0, 0);
+    int above = 0;  // those before this one: of higher rank, or of the same and a lower block
+    for (int i = 0; i < many; ++i) {
+      const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)own.x, i), y = (uint32_t)__builtin_amdgcn_readlane((int)own.y, i);
+      above += x > own.x || (x == own.x && y < own.y);
+    }
+    const int at = __builtin_ctzll(__ballot(lane < many && above == need - 1));
+    const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)own.x, at), y = (uint32_t)__builtin_amdgcn_readlane((int)own.y, at);
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) keep[i] = keep[i] || (open[i] && (key[i] > x || (key[i] == x && (uint32_t)(i0 + i) <= y)));
+    break;
+  }
+  __syncthreads();
+  int to = before_of<WAVES, KPT>(keep, s.part, lane, wid, &total);
+#pragma unroll
+  for (int i = 0; i < KPT; ++i)
+    if (keep[i]) {
+      if (to < a.keep) out[to] = pages[i0 + i];
+      ++to;
+    }
+}
+
+// What a selection writes beside the pages chosen; true where all blocks are kept and nothing is left to do.
+__device__ __forceinline__ bool begin_select(const SelectArgs& a, int b, int h, int64_t n, bool ok, int blocks,
+                                             const int32_t* pages, int32_t* out) {
+  const int tid = threadIdx.x, kept = min(blocks, a.keep);
+  if (h == 0 && tid == 0) {
+    if (!ok) kv_flag(a.err);
+    a.new_lengths[b] = n - ((int64_t)(blocks - kept) << a.p.shift);
+  }
+  for (int i = kept + tid; i < a.keep; i += blockDim.x) out[i] = -1;
+  if (blocks > a.count) return false;
+  for (int i = tid; i < blocks; i += blockDim.x) {
+    out[i] = pages[i];
+    if ((uint32_t)pages[i] >= (uint32_t)a.p.num_pages) kv_flag(a.err);
+  }
+  return true;
+}
+
+// Ranks and selection in one: a workgroup a (sequence, key head) of up to KPT * THREADS blocks.
+template <class O, class Q, int DHP, int NG, int THREADS, int KPT>
+__global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  typedef Scores<O, Q, DHP, NG> S;
+  __shared__ __attribute__((aligned(16))) uint32_t rank[THREADS * KPT];
+  __shared__ __attribute__((aligned(16))) typename S::Query query;
+  __shared__ __attribute__((aligned(16))) PickShared<WAVES> s;
+  const int b = blockIdx.x / a.p.kv_heads, h = blockIdx.x - b * a.p.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, wid = wave_uniform(tid >> 6);
+  bool ok = true;
+  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
+  const int blocks = blocks_of(a, n);
+  const int32_t* pages = a.p.table + b * a.p.ld_table;
+  int32_t* out = a.table + (int64_t)blockIdx.x * a.keep;
+  if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
+  const int tiles = (blocks + 15) >> 4;
+  S::template run<THREADS>(a, query, b, h, blocks, wid, WAVES, tiles, lane, rank);
+  __syncthreads();
+  uint32_t key[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; i += 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(rank + tid * KPT + i);
+    key[i] = x.x, key[i + 1] = x.y, key[i + 2] = x.z, key[i + 3] = x.w;
+  }
+#pragma unroll
+  for (int i = 0; i < KPT; ++i)
+    if (tid * KPT + i >= tiles * 16) key[i] = 0;  // (behind the last tile nothing was written)
+  pick<WAVES, KPT>(a, key, blocks, pages, out, s);
+}
+
+// Tiles a wavefront where there are few and where there are many, from RK_MANY a CU on (us, 1 / 4: 8 units of 2048 blocks
+// 13.7 / 18.6, 128 42.7 / 42.8, 512 158 / 135)
+constexpr int RK_MORE = 4, RK_MANY = 64;
+
+// The ranks alone: `per` tiles of a (sequence, key head) a workgroup.
+template <class O, class Q, int DHP, int NG>
+__global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a, int per) {
+  typedef Scores<O, Q, DHP, NG> S;
+  __shared__ __attribute__((aligned(16))) typename S::Query query;
+  const int lane = threadIdx.x & 63, wid = wave_uniform((int)threadIdx.x >> 6);
+  const int units = a.B * a.p.kv_heads, chunk = blockIdx.x / units, bh = blockIdx.x - chunk * units;
+  const int b = bh / a.p.kv_heads, h = bh - b * a.p.kv_heads;
+  bool ok = true;
+  const int blocks = blocks_of(a, a.p.length_of(a.lengths, b, a.max_length, &ok));
+  const int tiles = min((blocks + 15) >> 4, per * (chunk + 1));
+  if (blocks <= a.count || per * chunk >= tiles) return;  // (all of them are kept, or there are none for this workgroup)
+  S::template run<256>(a, query, b, h, blocks, per * chunk + wid, 4, tiles, lane, a.rank + (int64_t)bh * a.ld);
+}
+
+// The selection from ranks in the workspace.
+template <int THREADS, int KPT>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(SelectArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ __attribute__((aligned(16))) PickShared<WAVES> s;
+  const int b = blockIdx.x / a.p.kv_heads, h = blockIdx.x - b * a.p.kv_heads;
+  const int tid = threadIdx.x;
+  bool ok = true;
+  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
+  const int blocks = blocks_of(a, n);
+  const int32_t* pages = a.p.table + b * a.p.ld_table;
+  int32_t* out = a.table + (int64_t)blockIdx.x * a.keep;
+  if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
+  const uint32_t* rank = a.rank + (int64_t)blockIdx.x * a.ld;
+  const int end = (blocks + 15) & ~15;  // (behind the last tile nothing was written)
+  uint32_t key[KPT];
+#pragma unroll
+  for (int i = 0; i < KPT; i += 4) {
+    uint4 x = {0, 0, 0, 0};
+    if (tid * KPT + i < end) x = *reinterpret_cast<const uint4*>(rank + tid * KPT + i);
+    key[i] = x.x, key[i + 1] = x.y, key[i + 2] = x.z, key[i + 3] = x.w;
+  }
+  pick<WAVES, KPT>(a, key, blocks, pages, out, s);
+}
+
+constexpr int SL_THREADS = 1024, SL_KEYS = 16;  // of the largest selection that keeps its ranks in registers
+
+// The selection of more blocks than that: a radix selection of a byte a round, the ranks read again in each.
+__global__ __launch_bounds__(SL_THREADS) void kv_select_long_kernel(SelectArgs a) {
   constexpr int WAVES = SL_THREADS / 64;
   __shared__ __attribute__((aligned(16))) int hist[256];
   __shared__ int part[2][WAVES];
@@ -311,37 +671,29 @@ __global__ __launch_bounds__(SL_THREADS) void kv_select_kernel(SelectArgs a) {
   const int b = blockIdx.x / p.kv_heads, h = blockIdx.x - b * p.kv_heads;
   bool ok = true;
   const int64_t n = p.length_of(a.lengths, b, a.max_length, &ok);
-  const int blocks = blocks_of(a, n), kept = min(blocks, a.keep);
+  const int blocks = blocks_of(a, n);
   const int32_t* pages = p.table + b * p.ld_table;
   int32_t* out = a.table + (int64_t)blockIdx.x * a.keep;
-  if (h == 0 && tid == 0) {
-    if (!ok) kv_flag(a.err);
-    a.new_lengths[b] = n - ((int64_t)(blocks - kept) << p.shift);
-  }
-  for (int i = kept + tid; i < a.keep; i += SL_THREADS) out[i] = -1;
-  if (blocks <= a.count) {
-    for (int i = tid; i < blocks; i += SL_THREADS) {
-      out[i] = pages[i];
-      if ((uint32_t)pages[i] >= (uint32_t)p.num_pages) kv_flag(a.err);
-    }
-    return;
-  }
+  if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
   const uint32_t* rank = a.rank + (int64_t)blockIdx.x * a.ld;
   uint32_t found = 0;
-  int need = a.count;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    hist[tid] = 0;
+  int need = a.count - a.first - a.recent;
+  bool whole = need == 0;
+  if (whole) found = 0xffffffffu;
+  for (int shift = 24; shift >= 0 && !whole; shift -= 8) {
+    __syncthreads();
+    if (tid < 256) hist[tid] = 0;
     __syncthreads();
     for (int i = tid; i < blocks; i += SL_THREADS) {
       const uint32_t x = rank[i];
-      if (shift == 24 || (x >> (shift + 8)) == (found >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255], 1);
+      if (x != 0 && (shift == 24 || (x >> (shift + 8)) == (found >> (shift + 8)))) atomicAdd(&hist[(x >> shift) & 255], 1);
     }
     __syncthreads();
     if (wid == 0) {  // lane l has the bins 252 - 4 l .. 255 - 4 l
       const int4 c = *reinterpret_cast<const int4*>(&hist[252 - 4 * lane]);
       const int many[4] = {c.w, c.z, c.y, c.x};  // the largest ranks first
       const int sum = (c.x + c.y) + (c.z + c.w);
-      int before = scan64(sum, lane) - sum;
+      int before = scan64(sum) - sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (before < need && before + many[i] >= need)  // (one bin of one lane)
@@ -352,42 +704,23 @@ __global__ __launch_bounds__(SL_THREADS) void kv_select_kernel(SelectArgs a) {
     __syncthreads();
     found |= (uint32_t)picked[0] << shift;
     need -= picked[1];
-    if (need == picked[2]) break;  // (all that share the bytes found are kept; every thread sees the same)
-    __syncthreads();
+    whole = need == picked[2];  // all that share the bytes found are kept
   }
-  // ranks above `found`, and of those equal to it in the bytes found the first `need`: in the order of the blocks
+  // ranks above `found`, and of those equal to it the first `need`: in the order of the blocks
   int at = 0, tie = 0;
-  const bool whole = need == picked[2];
+  const bool none = a.count == a.first + a.recent;
   for (int i0 = 0; i0 < blocks; i0 += SL_THREADS) {
     const int i = i0 + tid;
     const uint32_t x = i < blocks ? rank[i] : 0;
-    const bool there = i < blocks, above = there && (whole ? x >= found : x > found), equal = there && !whole && x == found;
-    const uint64_t ties = __ballot(equal);
-    __syncthreads();
-    if (lane == 0) part[0][wid] = __popcll(ties);
-    __syncthreads();
-    int before = tie, sum = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wid) before += part[0][w];
-      sum += part[0][w];
-    }
-    before += __popcll(ties & ((1ull << lane) - 1));
+    bool keep[1] = {i < blocks && (i < a.first || i >= blocks - a.recent)}, equal[1] = {!whole && x != 0 && x == found};
+    keep[0] = keep[0] || (!none && x != 0 && (whole ? x >= found : x > found));
+    int sum;
+    int before = tie + before_of<WAVES, 1>(equal, part[0], lane, wid, &sum);
     tie += sum;
-    const bool keep = above || (equal && before < need);
-    const uint64_t all = __ballot(keep);
-    if (lane == 0) part[1][wid] = __popcll(all);
-    __syncthreads();
-    int to = at;
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wid) to += part[1][w];
-      sum += part[1][w];
-    }
-    to += __popcll(all & ((1ull << lane) - 1));
+    keep[0] = keep[0] || (equal[0] && before < need);
+    const int to = at + before_of<WAVES, 1>(keep, part[1], lane, wid, &sum);
     at += sum;
-    if (keep && to < kept) out[to] = pages[i];
+    if (keep[0] && to < a.keep) out[to] = pages[i];
   }
 }
 
@@ -461,7 +794,7 @@ extern "C" int cortex_kv_block_bounds(const cortex_kv_pages* pages, int64_t B, c
     if (touched < blocks) blocks = touched;
   }
   if (blocks == 0) blocks = 1;
-  const int64_t need = cdiv(blocks * pages->kv_heads, 4), share = cdiv((int64_t)cu_count() * 64, B);
+  const int64_t need = cdiv(blocks * pages->kv_heads, 4), share = cdiv((int64_t)cu_count() * KB_PER_CU, B);
   a.chunks = (int)(need < share ? need : share);
   CORTEX_CHECK_ARG(B <= 0xffffffffLL / 256 / a.chunks, "%s: %lld sequences are too many for one call", who, (long long)B);
   const dim3 grid((unsigned)(B * a.chunks)), block(256);
@@ -486,16 +819,52 @@ int64_t rank_ld(const cortex_kv_pages* pages, int64_t most, int64_t count) {
   return blocks <= count ? 0 : cdiv(blocks, 16) * 16;
 }
 
-template <class O, class Q>
-void launch_rank(const SelectArgs& a, unsigned grid, hipStream_t stream) {
-  if (a.p.head_dim <= 32)
-    hipLaunchKernelGGL((kv_rank_kernel<O, Q, 32>), dim3(grid), dim3(256), 0, stream, a);
-  else if (a.p.head_dim <= 64)
-    hipLaunchKernelGGL((kv_rank_kernel<O, Q, 64>), dim3(grid), dim3(256), 0, stream, a);
-  else if (a.p.head_dim <= 96)
-    hipLaunchKernelGGL((kv_rank_kernel<O, Q, 96>), dim3(grid), dim3(256), 0, stream, a);
+// Ranks and selection in one launch, or in two: one workgroup a (sequence, key head) has the long ones for itself, but two
+// launches begin twice.  us in a graph, blocks 64 / 128 / 256 / 512 / 1024 of 32 query on 8 key heads x 128 in bf16, in
+// one launch of 512 threads, of 256 threads and in two:
+//     8 units    7.8  9.3 13.2 18.4 26.9     8.5 11.4 15.1 20.8 32.4     9.3 10.4 11.1 11.3  9.9
+//   128 units    8.2  9.9 14.0 19.9 29.8     9.0 11.9 15.5 24.4 37.6     9.8 11.3 12.9 18.8 26.7
+//   256 units    8.3  9.8 14.9 21.8 32.4     9.2 11.9 18.0 25.7 39.9     9.9 12.5 18.1 26.6 39.5
+//  1024 units   28.7 37.2 53.9 74.9  130    21.0 28.3 39.5 61.2  128    17.6 27.8 41.6 70.1  149
+constexpr int FUSED_ALWAYS = 128, FUSED_KEYS = 4;  // blocks of any number of units; consecutive blocks a thread
+enum class Form { two, one_256, one_512 };
+Form select_form(int64_t units, int64_t ld) {
+  const int64_t cus = cu_count();
+  if (ld > 512 * FUSED_KEYS || (ld > FUSED_ALWAYS && 4 * units < 3 * cus)) return Form::two;
+  return units > cus && ld <= 256 * FUSED_KEYS ? Form::one_256 : Form::one_512;
+}
+
+template <class O, class Q, int DHP, int NG>
+int launch_select(const SelectArgs& a, hipStream_t stream) {
+  const int64_t n = (int64_t)a.B * a.p.kv_heads;
+  const dim3 units((unsigned)n);
+  const Form form = select_form(n, a.ld);
+  if (form != Form::two) {
+    if (form == Form::one_256)
+      hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, 256, FUSED_KEYS>), units, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, 512, FUSED_KEYS>), units, dim3(512), 0, stream, a);
+    CORTEX_CHECK_LAUNCH("kv_rank_select_kernel");
+    return OK;
+  }
+  const int per_wave = n * a.ld / 16 >= RK_MANY * cu_count() ? RK_MORE : 1, chunks = (int)cdiv(a.ld, 64 * per_wave);
+  hipLaunchKernelGGL((kv_rank_kernel<O, Q, DHP, NG>), dim3((unsigned)(n * chunks)), dim3(256), 0, stream, a, 4 * per_wave);
+  CORTEX_CHECK_LAUNCH("kv_rank_kernel");
+  if (a.ld <= 1024)
+    hipLaunchKernelGGL((kv_select_kernel<256, 4>), units, dim3(256), 0, stream, a);
+  else if (a.ld <= 4096)
+    hipLaunchKernelGGL((kv_select_kernel<1024, 4>), units, dim3(1024), 0, stream, a);
+  else if (a.ld <= SL_THREADS * SL_KEYS)
+    hipLaunchKernelGGL((kv_select_kernel<SL_THREADS, SL_KEYS>), units, dim3(SL_THREADS), 0, stream, a);
   else
-    hipLaunchKernelGGL((kv_rank_kernel<O, Q, 128>), dim3(grid), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv_select_long_kernel, units, dim3(SL_THREADS), 0, stream, a);
+  CORTEX_CHECK_LAUNCH("kv_select_kernel");
+  return OK;
+}
+template <class O, class Q>
+int launch_select(const SelectArgs& a, hipStream_t stream) {
+  if (a.p.head_dim <= 64) return a.group <= 4 ? launch_select<O, Q, 64, 1>(a, stream) : launch_select<O, Q, 64, 4>(a, stream);
+  return a.group <= 4 ? launch_select<O, Q, 128, 1>(a, stream) : launch_select<O, Q, 128, 4>(a, stream);
 }
 
 }  // namespace
@@ -504,7 +873,8 @@ void launch_rank(const SelectArgs& a, unsigned grid, hipStream_t stream) {
 extern "C" int64_t cortex_kv_select_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t max_length,
                                                     int64_t count) {
   if (!pages || pages->page_size < 1 || pages->kv_heads < 1 || B < 0 || max_length < 0 || count < 0) return 0;
-  return B * pages->kv_heads * rank_ld(pages, max_length, count) * 4;
+  const int64_t units = B * pages->kv_heads, ld = rank_ld(pages, max_length, count);
+  return select_form(units, ld) == Form::two ? units * ld * 4 : 0;
 }
 
 extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb,
@@ -531,14 +901,14 @@ extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t
   const int64_t blocks = most_blocks(pages, a.max_length), ld = rank_ld(pages, a.max_length, count);
   const int64_t keep = count < blocks ? count : blocks;
   CORTEX_CHECK_ARG(table || keep == 0, "%s: null table", who);
-  CORTEX_CHECK_ARG((workspace || ld == 0) && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
+  const int64_t need = cortex_kv_select_workspace_bytes(pages, B, a.max_length, count);
+  CORTEX_CHECK_ARG((workspace || need == 0) && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
   // (a launch has fewer than 2^32 threads)
-  CORTEX_CHECK_ARG(B <= 0xffffffffLL / SL_THREADS / pages->kv_heads &&
-                       (ld == 0 || B * pages->kv_heads <= 0xffffff00LL / 64 / (ld / 16)),
+  CORTEX_CHECK_ARG(B <= 0xffffffffLL / 1024 / pages->kv_heads &&
+                       (ld == 0 || B * pages->kv_heads <= 0xffffffffLL / 256 / cdiv(ld, 64)),
                    "%s: %lld sequences of up to %lld blocks are too much for one call", who, (long long)B, (long long)blocks);
-  if (workspace_bytes < B * pages->kv_heads * ld * 4) {
-    set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
-              (long long)(B * pages->kv_heads * ld * 4));
+  if (workspace_bytes < need) {
+    set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
     return E_WORKSPACE;
   }
   a.bounds = pages->bounds;
@@ -558,18 +928,12 @@ extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t
   a.err = err;
   a.rank = reinterpret_cast<uint32_t*>(workspace);
   a.ld = ld;
-  a.tiles = (int)(ld / 16);
-  if (ld > 0) {
-    const unsigned grid = (unsigned)cdiv(B * pages->kv_heads * a.tiles, 4);
-    if (pages->dtype == DT_F32)
-      launch_rank<float, float>(a, grid, stream);
-    else if (pages->dtype == DT_BF16)
-      launch_rank<bf16, bf16>(a, grid, stream);
-    else
-      launch_rank<float, bf16>(a, grid, stream);
-    CORTEX_CHECK_LAUNCH("kv_rank_kernel");
+  if (ld == 0) {  // all blocks are kept
+    hipLaunchKernelGGL((kv_select_kernel<256, 4>), dim3((unsigned)(B * pages->kv_heads)), dim3(256), 0, stream, a);
+    CORTEX_CHECK_LAUNCH("kv_select_kernel");
+    return OK;
   }
-  hipLaunchKernelGGL(kv_select_kernel, dim3((unsigned)(B * pages->kv_heads)), dim3(SL_THREADS), 0, stream, a);
-  CORTEX_CHECK_LAUNCH("kv_select_kernel");
-  return OK;
+  if (pages->dtype == DT_F32) return launch_select<float, float>(a, stream);
+  if (pages->dtype == DT_BF16) return launch_select<bf16, bf16>(a, stream);
+  return launch_select<float, bf16>(a, stream);
 }
