@@ -46,8 +46,8 @@ class KVPages:
     (num_pages, kv_heads, 2, head_dim), optional, in the dtype of ``k`` (fp32 for int8 pages): the largest and the smallest
     value of a page's keys in every dim, as ``kv_block_bounds`` last left them.  The tensors of an object do not change."""
 
-    __slots__ = ("k", "v", *_PER_ROW, "bounds", "num_pages", "kv_heads", "page_size", "head_dim", "device", "index", "query_dtype",
-                 "_struct", "ref")
+    __slots__ = ("k", "v", *_PER_ROW, "bounds", "num_pages", "kv_heads", "page_size", "head_dim", "device", "index",
+                 "query_dtype", "_struct", "ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, *, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None, weight: torch.Tensor | None = None,
@@ -451,8 +451,8 @@ def kv_copy_pages(pages: KVPages, src: torch.Tensor, dst: torch.Tensor, *, into:
         _elsewhere("kv_copy_pages", pages, src, dst, to.k, err_flag)
     if (src.dtype is not torch.int32 or dst.dtype is not torch.int32 or src.dim() != 1 or dst.shape != src.shape
             or not src.is_contiguous() or not dst.is_contiguous()):
-        raise ValueError(f"src and dst must be contiguous int32 tensors of one length, got {tuple(src.shape)} {src.dtype} and "
-                         f"{tuple(dst.shape)} {dst.dtype}")
+        raise ValueError(f"src and dst must be contiguous int32 tensors of one length, got {tuple(src.shape)} {src.dtype} "
+                         f"and {tuple(dst.shape)} {dst.dtype}")
     if err_flag is not None and (err_flag.dtype is not torch.int32 or err_flag.numel() != 1):
         raise ValueError("kv_copy_pages: err_flag must be one int32")
     if into is not None:
