@@ -852,6 +852,8 @@ int launch_select(const SelectArgs& a, hipStream_t stream) {
   CORTEX_CHECK_LAUNCH("kv_rank_kernel");
   if (a.ld <= 1024)
     hipLaunchKernelGGL((kv_select_kernel<256, 4>), units, dim3(256), 0, stream, a);
+  else if (a.ld <= 2048)
+    hipLaunchKernelGGL((kv_select_kernel<512, 4>), units, dim3(512), 0, stream, a);
   else if (a.ld <= 4096)
     hipLaunchKernelGGL((kv_select_kernel<1024, 4>), units, dim3(1024), 0, stream, a);
   else if (a.ld <= SL_THREADS * SL_KEYS)

@@ -42,18 +42,15 @@ def select64(table, bounds, q, n, page, count, first, recent, num_pages):
     blocks = -(-n // page)
     if blocks <= count:
         return list(range(blocks))
-    rank = []
-    for i in range(blocks):
-        p = int(table[i])
-        score = -np.inf
-        if 0 <= p < num_pages:
-            with np.errstate(invalid="ignore", over="ignore"):
-                up, down = np.where(q < 0, 0.0, q), np.where(q < 0, q, 0.0)
-                each = (up * bounds[p, 0] + down * bounds[p, 1]).sum(-1).astype(np.float32)
-            score = np.inf if np.isnan(each).any() else each.max()
-            rank.append((2 if np.isnan(each).any() else 1, 0.0 if np.isnan(each).any() else float(score)))
-        else:
-            rank.append((0, 0.0))
+    ids = np.asarray(table[:blocks], dtype=np.int64)
+    there = (ids >= 0) & (ids < num_pages)
+    rows = bounds[np.where(there, ids, 0)]
+    with np.errstate(invalid="ignore", over="ignore"):
+        up, down = np.where(q < 0, 0.0, q), np.where(q < 0, q, 0.0)
+        each = np.stack([(u * rows[:, 0] + d * rows[:, 1]).sum(-1) for u, d in zip(up, down)], 1).astype(np.float32)
+    lost = np.isnan(each).any(1)
+    score = np.where(lost, 0.0, np.where(np.isnan(each), 0.0, each).max(1))
+    rank = [(2 if n else 1, float(x)) if t else (0, 0.0) for t, n, x in zip(there.tolist(), lost.tolist(), score.tolist())]
     always = [i < first or i >= blocks - recent for i in range(blocks)]
     order = sorted(range(blocks), key=lambda i: (not always[i], -rank[i][0], -rank[i][1], i))
     return sorted(order[:count])

@@ -298,6 +298,30 @@ def test_selection_of_many_blocks(lens):
         check_selection(c, q, count)
 
 
+@pytest.mark.parametrize("batch,kv_heads,dim,blocks", [(3, 1, 16, 100), (70, 4, 48, 60), (300, 1, 128, 130), (50, 4, 32, 1030),
+                                                       (200, 1, 16, 1500), (110, 1, 16, 2500), (24, 2, 64, 300), (2, 2, 64, 2049)])
+@pytest.mark.parametrize("dtype,heads", [("bf16", 1), ("fp32", 5), ("int8", 3)])
+def test_selection_of_few_and_many_sequences(dtype, heads, batch, kv_heads, dim, blocks):
+    """The one launch of 256 and of 512 threads, the two, with one and with four tiles a wavefront: on either side of
+    where one takes over from the other."""
+    from types import SimpleNamespace
+
+    from cortex.kernels.paged_kv import KVPages
+
+    g = torch.Generator().manual_seed(batch + blocks)
+    c = SimpleNamespace(kv_heads=kv_heads, page=8, width=blocks, num=blocks + 40)
+    c.lens = [8 * blocks - 8 * (37 * b % blocks) - b % 8 for b in range(batch)]
+    c.table = torch.stack([torch.randperm(c.num, generator=g)[:blocks] for _ in range(batch)]).int()
+    c.pages = KVPages.allocate(c.num, kv_heads, 8, dim, DTYPES[dtype], DEV, bounded=True)
+    edge = torch.randn(c.num, kv_heads, 2, dim, generator=g)
+    c.gb = c.pages.bounds
+    c.gb.copy_(torch.stack([edge.amax(2), edge.amin(2)], 2).to(c.gb.dtype))
+    c.block_table, c.lengths = c.table.to(DEV), torch.tensor(c.lens, device=DEV)
+    q = torch.randn(batch, heads * kv_heads, dim, generator=g).to(c.pages.query_dtype)
+    for count in (3, blocks // 3):
+        check_selection(c, q, count)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_selection_ties(dtype):
     """Scores of few different values, of one value, and of both zeros: equal ones by the lower block."""
