@@ -308,8 +308,8 @@ class PagedKVCache:
         return src.shape[0]
 
     def resize(self, num_pages: int) -> int:
-        """Pools of ``num_pages`` pages instead; returns how many pages got another place, those past the end of smaller
-        pools.  MemoryError, and nothing changed, where the pages in use are more, or where the device has no room for the
+        """Pools of ``num_pages`` pages instead (``layers`` are other objects then); returns how many pages got another
+        place, those past the end of smaller pools.  MemoryError, and nothing changed, where the pages in use are more, or where the device has no room for the
         new pools beside the old ones.  Every layer must have the rows of the tokens of sessions that move; batches made
         before no longer hold for these."""
         if num_pages < 1:

@@ -284,7 +284,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     """``softmax_{j < lengths[b]}(scale * q . k_j) v_j`` of one query a sequence: ``q`` (B, heads, head_dim) in
     ``pages.query_dtype`` with ``heads`` a multiple of the key heads (query head h reads key head
     ``h // (heads // kv_heads)``), ``scale`` ``head_dim ** -0.5`` by default.  A sequence of length 0 gives 0.
-    ``block_table``: also a contiguous (B, kv_heads, max_pages), a row of pages for each key head (``paged_block_select``).
+    ``block_table``: also a contiguous (B, kv_heads, max_pages), a row of pages for each key head (``paged_block_select``);
+    with ``accumulate`` no page twice in a row.
 
     ``accumulate`` adds to ``pages.weight`` the softmax weight that each key received, summed over the query heads
     of its key head; no two sequences of the call may then share a page.  ``out`` may not overlap ``q`` or itself.
@@ -363,7 +364,8 @@ def kv_block_bounds(pages: KVPages, block_table: torch.Tensor, lengths: torch.Te
                     since: torch.Tensor | None = None, max_new: int | None = None, max_length: int | None = None,
                     err_flag: torch.Tensor | None = None) -> None:
     """Writes ``pages.bounds`` of the pages that hold a slot of ``[since[b], lengths[b])`` (``since`` (B,) int64, by default
-    0: all pages in use), each from all of its keys below ``lengths[b]``; NaN in the dims where a key has one.
+    0: all pages in use), each from all of its keys below ``lengths[b]``; NaN in the dims where a key has one.  Sequences of
+    the call may share pages that all of them use in full.
 
     Append, eviction and everything else that writes keys leaves the bounds as they were: call this behind it, after an
     append with the lengths before it as ``since``.  ``max_new``: a bound of ``lengths - since`` known on the host, which

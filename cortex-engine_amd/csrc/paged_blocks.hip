@@ -780,7 +780,7 @@ extern "C" int cortex_kv_block_bounds(const cortex_kv_pages* pages, int64_t B, c
   if (int rc = kv_check(who, pages, B, block_table, ld_table, max_pages, &a.p)) return rc;
   if (int rc = check_bounds(who, pages)) return rc;
   a.max_length = max_length < 0 || max_length > a.p.max_slots ? a.p.max_slots : max_length;
-  if (B == 0 || a.max_length == 0) return OK;
+  if (B == 0) return OK;
   CORTEX_CHECK_ARG(lengths, "%s: null lengths", who);
   a.bounds = pages->bounds;
   a.lengths = lengths;

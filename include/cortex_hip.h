@@ -603,7 +603,8 @@ int cortex_kv_copy_pages(const cortex_kv_pages* from, const cortex_kv_pages* to,
 
 /* bounds (num_pages, kv_heads, 2, head_dim), contiguous, in the keys' dtype (f32 for int8 pages): the largest and the
  * smallest value of a page's keys in every dim, NaN where a key has one.  Written for the pages that hold a slot of
- * [since[b], lengths[b]) (since NULL: 0), from all rows of the page below lengths[b].  max_length as above; max_new:
+ * [since[b], lengths[b]) (since NULL: 0), from all rows of the page below lengths[b]; sequences may share pages that all of
+ * them use in full.  max_length as above; max_new:
  * how many slots [since[b], lengths[b]) has at most (negative: unknown; more are right, but slower). */
 int cortex_kv_block_bounds(const cortex_kv_pages* pages, int64_t B, const int32_t* block_table, int64_t ld_table,
                            int64_t max_pages, const int64_t* lengths, int64_t max_length, const int64_t* since,

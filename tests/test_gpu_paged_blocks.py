@@ -231,6 +231,13 @@ def test_bounds_with_malformed_pages_and_lengths():
     for i in range(2):
         want[int(c.table[0][i])] = c.bounds64(0, i, 12)
     assert flag.item() == 4 and torch.equal(c.gb.cpu(), want.to(c.gb.dtype))
+    for kw in ({"max_length": 0}, {"max_length": 0, "since": c.lengths[:1] * 0, "max_new": 0}):
+        flag.zero_()
+        kv_block_bounds(c.pages, c.block_table[:1], c.lengths[:1], err_flag=flag, **kw)
+        assert flag.item() == 4
+    flag.zero_()
+    kv_block_bounds(c.pages, c.block_table[:1, :0], c.lengths[:1] * 0, err_flag=flag)
+    assert flag.item() == 0 and torch.equal(c.gb.cpu(), want.to(c.gb.dtype))
 
 
 # ------------------------------------------------------------------------------- selection
@@ -300,7 +307,7 @@ def test_selection_of_many_blocks(lens):
 
 @pytest.mark.parametrize("batch,kv_heads,dim,blocks", [(3, 1, 16, 100), (70, 4, 48, 60), (300, 1, 128, 130), (50, 4, 32, 1030),
                                                        (200, 1, 16, 1500), (110, 1, 16, 2500), (24, 2, 64, 300), (2, 2, 64, 2049)])
-@pytest.mark.parametrize("dtype,heads", [("bf16", 1), ("fp32", 5), ("int8", 3)])
+@pytest.mark.parametrize("dtype,heads", [("bf16", 1), ("fp32", 5), ("int8", 3), ("bf16", 18)])
 def test_selection_of_few_and_many_sequences(dtype, heads, batch, kv_heads, dim, blocks):
     """The one launch of 256 and of 512 threads, the two, with one and with four tiles a wavefront: on either side of
     where one takes over from the other."""

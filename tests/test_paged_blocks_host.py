@@ -101,8 +101,7 @@ def test_refused_bounds():
     refused(bounds(pages(bounds=None)), "aligned bounds")
     refused(bounds(pages(bounds=8)), "aligned bounds")
     refused(bounds(pages(kv_heads=65535), B=1 << 24, ld=1, width=1), "too many")
-    accepted(bounds(pages(), most=0))
-    accepted(bounds(pages(), table=None, ld=0, width=0))
+    accepted(bounds(pages(), B=0, most=0))
 
 
 def test_refused_selections():
