@@ -91,17 +91,23 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     (int32, never cleared here).  ``out``: where the results go; each may be its own input (in place) and overlaps no
     other tensor of the call."""
     idx = q.get_device()
-    given = [t for t in (axes, q_gain, k_gain, err_flag) if t is not None]
-    if out is not None:
-        given += out
-    if idx < 0 or k.get_device() != idx or positions.get_device() != idx or inv_freq.get_device() != idx or any(
-            [t.get_device() != idx for t in given]):
+    given = ()
+    if axes is not None or eps is not None or err_flag is not None or out is not None:
+        given = [t for t in (axes, q_gain, k_gain, err_flag) if t is not None]
+        if out is not None:
+            given += out
+    elsewhere = idx < 0 or k.get_device() != idx or positions.get_device() != idx or inv_freq.get_device() != idx
+    wants_grad = q.requires_grad or k.requires_grad or inv_freq.requires_grad
+    for t in given:
+        elsewhere = elsewhere or t.get_device() != idx
+        wants_grad = wants_grad or t.requires_grad
+    if elsewhere:
         nat.require_gpu(q, k, positions, inv_freq, *given, what=_WHAT)
     if idx != _get_device():
         with torch.cuda.device(idx):
             return qk_norm_rope(q, k, positions, inv_freq, axes=axes, interleaved=interleaved, eps=eps, q_gain=q_gain,
                                 k_gain=k_gain, out=out, err_flag=err_flag)
-    if q.requires_grad or k.requires_grad or inv_freq.requires_grad or any([t.requires_grad for t in given]):
+    if wants_grad:
         _no_grad(_WHAT)
     if forward_ad._current_level >= 0:
         _no_tangent(_WHAT, q, k, inv_freq, *given)

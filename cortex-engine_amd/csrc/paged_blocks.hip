@@ -479,7 +479,7 @@ __device__ __forceinline__ int before_of(const bool (&flag)[N], int* part, int l
 // that holds the last one kept is found from the counts, and its ranks, where they are few, are compared with each other
 // by every wavefront for itself.  Where they are many the bin is cut into bins again.
 template <int WAVES, int KPT>
-__device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[KPT], int blocks, const int32_t* pages,
+__device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[KPT], int blocks, const int32_t (&page)[KPT],
                                      int32_t* out, PickShared<WAVES>& s) {
   constexpr int BINS = 64 * WAVES;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, i0 = tid * KPT;
@@ -561,9 +561,20 @@ __device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[
 #pragma unroll
   for (int i = 0; i < KPT; ++i)
     if (keep[i]) {
-      if (to < a.keep) out[to] = pages[i0 + i];
+      if (to < a.keep) out[to] = page[i];
       ++to;
     }
+}
+
+// The pages of this thread's blocks, loaded before it is known which of them are there.
+template <int KPT>
+__device__ __forceinline__ void load_pages(const SelectArgs& a, const int32_t* pages, int32_t (&page)[KPT]) {
+  const int width = (int)(a.p.max_slots >> a.p.shift);
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int at = threadIdx.x * KPT + i;
+    page[i] = at < width ? pages[at] : -1;
+  }
 }
 
 // What a selection writes beside the pages chosen; true where all blocks are kept and nothing is left to do.
@@ -600,6 +611,8 @@ __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   int32_t* out = a.table + (int64_t)blockIdx.x * a.keep;
   if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
   const int tiles = (blocks + 15) >> 4;
+  int32_t page[KPT];
+  load_pages(a, pages, page);
   S::template run<THREADS>(a, query, b, h, blocks, wid, WAVES, tiles, lane, rank);
   __syncthreads();
   uint32_t key[KPT];
@@ -611,7 +624,7 @@ __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
 #pragma unroll
   for (int i = 0; i < KPT; ++i)
     if (tid * KPT + i >= tiles * 16) key[i] = 0;  // (behind the last tile nothing was written)
-  pick<WAVES, KPT>(a, key, blocks, pages, out, s);
+  pick<WAVES, KPT>(a, key, blocks, page, out, s);
 }
 
 // Tiles a wavefront where there are few and where there are many, from RK_MANY a CU on (us, 1 / 4: 8 units of 2048 blocks
@@ -640,22 +653,27 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(SelectArgs a) {
   __shared__ __attribute__((aligned(16))) PickShared<WAVES> s;
   const int b = blockIdx.x / a.p.kv_heads, h = blockIdx.x - b * a.p.kv_heads;
   const int tid = threadIdx.x;
-  bool ok = true;
-  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
-  const int blocks = blocks_of(a, n);
-  const int32_t* pages = a.p.table + b * a.p.ld_table;
-  int32_t* out = a.table + (int64_t)blockIdx.x * a.keep;
-  if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
+  // ranks and pages beside the length that says which of them count
   const uint32_t* rank = a.rank + (int64_t)blockIdx.x * a.ld;
-  const int end = (blocks + 15) & ~15;  // (behind the last tile nothing was written)
   uint32_t key[KPT];
 #pragma unroll
   for (int i = 0; i < KPT; i += 4) {
     uint4 x = {0, 0, 0, 0};
-    if (tid * KPT + i < end) x = *reinterpret_cast<const uint4*>(rank + tid * KPT + i);
+    if (tid * KPT + i < a.ld) x = *reinterpret_cast<const uint4*>(rank + tid * KPT + i);
     key[i] = x.x, key[i + 1] = x.y, key[i + 2] = x.z, key[i + 3] = x.w;
   }
-  pick<WAVES, KPT>(a, key, blocks, pages, out, s);
+  const int32_t* pages = a.p.table + b * a.p.ld_table;
+  int32_t page[KPT];
+  load_pages(a, pages, page);
+  bool ok = true;
+  const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
+  const int blocks = blocks_of(a, n);
+  int32_t* out = a.table + (int64_t)blockIdx.x * a.keep;
+  if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i)
+    if (tid * KPT + i >= ((blocks + 15) & ~15)) key[i] = 0;  // (behind the last tile nothing was written)
+  pick<WAVES, KPT>(a, key, blocks, page, out, s);
 }
 
 constexpr int SL_THREADS = 1024, SL_KEYS = 16;  // of the largest selection that keeps its ranks in registers
@@ -826,7 +844,7 @@ int64_t rank_ld(const cortex_kv_pages* pages, int64_t most, int64_t count) {
 //   128 units    8.2  9.9 14.0 19.9 29.8     9.0 11.9 15.5 24.4 37.6     9.8 11.3 12.9 18.8 26.7
 //   256 units    8.3  9.8 14.9 21.8 32.4     9.2 11.9 18.0 25.7 39.9     9.9 12.5 18.1 26.6 39.5
 //  1024 units   28.7 37.2 53.9 74.9  130    21.0 28.3 39.5 61.2  128    17.6 27.8 41.6 70.1  149
-constexpr int FUSED_ALWAYS = 128, FUSED_KEYS = 4;  // blocks of any number of units; consecutive blocks a thread
+constexpr int FUSED_ALWAYS = 192, FUSED_KEYS = 4;  // blocks of any number of units; consecutive blocks a thread
 enum class Form { two, one_256, one_512 };
 Form select_form(int64_t units, int64_t ld) {
   const int64_t cus = cu_count();
