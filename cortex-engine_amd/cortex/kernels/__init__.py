@@ -4,6 +4,7 @@ Modules keep the reference's import paths and signatures:
 ``cortex.kernels.tokenizer`` (fused_tokenizer), ``cortex.kernels.sparse_xattn``
 (sparse_cross_attention, build_temporal_block_mask) and
 ``cortex.kernels.fused_rmsnorm`` (rms_norm_linear), plus ``cortex.kernels.pack``
-(device-side ragged-event pack), ``cortex.kernels.ops`` (functional layer) and
-``cortex.kernels.paged_kv`` (keys and values in pages: append, attention, eviction).
+(device-side ragged-event pack), ``cortex.kernels.ops`` (functional layer),
+``cortex.kernels.paged_kv`` (keys and values in pages: append, attention, selection, eviction, copies)
+and ``cortex.kernels.rotary`` (norms of queries and keys with their rotation by position).
 """

@@ -14,6 +14,9 @@
 //           one byte permute per register, and product j gives the dims {r E + j}.
 // K's registers are free after the scores and V's after the output: the next tile's loads are issued there.
 //
+// A key head may have a row of the table of its own (pages selected for its queries): one length for all heads, so the split
+// below holds as it is.
+//
 // Split over the length: all tiles of all (sequence, key head) units are laid end to end and cut into equal shares, one a
 // workgroup, from the lengths on the device (a replayed graph follows them, ragged batches need no plan, and the grid
 // is one workgroup per slot of the card).  A unit cut by a share leaves its running (m, l, sum p v) in the workspace, at

@@ -44,7 +44,8 @@ struct CopyArgs {
 constexpr int CP_AHEAD = 4;  // rows in flight, keys and values of each
 
 // `lanes` lanes a row, 16 bytes of the key and of the value each; the arrays by row lie in the order of a page's
-// (head, row) and are copied 16 bytes at a time.
+// (head, row) and are copied 16 bytes at a time.  Bound by HBM: 2053 pages of 16 rows x 8 heads x 128 in bf16 with weight and
+// position, 273 MB read and written, 57.8 us among other calls, 4.7 TB/s; one page 2.5.
 __global__ __launch_bounds__(256) void kv_copy_pages_kernel(CopyArgs a) {
   const int tid = threadIdx.x;
   const int64_t i = blockIdx.x / a.parts;
@@ -158,6 +159,9 @@ __device__ __forceinline__ void store_bounds(O* to, const float* f) {
 }
 
 // A wavefront takes a (page, key head) at a time: `lanes` lanes a row, 16 bytes each, the groups of lanes joined at the end.
+// 16 sequences of 1000 .. 15001 int8 keys, 4 heads x 128, 84 MB: 20.8 us, 4.0 TB/s.  A value takes a conversion, a product with
+// its row's scale and half of a three-operand maximum and minimum each, about as long as its bytes; joined by shuffles it was
+// 24.6.  The last page of 32 sequences: 3.9 us, the chain length -> table -> rows.
 template <class P>
 __global__ __launch_bounds__(256) void kv_bounds_kernel(BoundsArgs a) {
   constexpr int ES = sizeof(P), N = 16 / ES;
@@ -594,7 +598,9 @@ __device__ __forceinline__ bool begin_select(const SelectArgs& a, int b, int h, 
   return true;
 }
 
-// Ranks and selection in one: a workgroup a (sequence, key head) of up to KPT * THREADS blocks.
+// Ranks and selection in one: a workgroup a (sequence, key head) of up to KPT * THREADS blocks.  32 sequences of 10 .. 501
+// blocks, 32 query on 8 key heads x 128 in bf16, 33 MB: 17.2 us.  Of that about 7 are the 64-bit products of the longest
+// sequences, whose wavefronts have four tiles each where the mean is two, and 2.6 the selection; 38 blocks of 8 heads x 64: 6.2.
 template <class O, class Q, int DHP, int NG, int THREADS, int KPT>
 __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
@@ -631,7 +637,8 @@ __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
 // 13.7 / 18.6, 128 42.7 / 42.8, 512 158 / 135)
 constexpr int RK_MORE = 4, RK_MANY = 64;
 
-// The ranks alone: `per` tiles of a (sequence, key head) a workgroup.
+// The ranks alone: `per` tiles of a (sequence, key head) a workgroup.  2048 blocks of 32 query on 8 key heads x 128, 8.4 MB: 6.7 us,
+// the chain length -> table -> bounds -> products of one tile.
 template <class O, class Q, int DHP, int NG>
 __global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a, int per) {
   typedef Scores<O, Q, DHP, NG> S;
@@ -646,7 +653,7 @@ __global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a, int per) {
   S::template run<256>(a, query, b, h, blocks, per * chunk + wid, 4, tiles, lane, a.rank + (int64_t)bh * a.ld);
 }
 
-// The selection from ranks in the workspace.
+// The selection from ranks in the workspace.  2048 blocks: 5.8 us, a launch and the rounds between its barriers.
 template <int THREADS, int KPT>
 __global__ __launch_bounds__(THREADS) void kv_select_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
@@ -837,13 +844,13 @@ int64_t rank_ld(const cortex_kv_pages* pages, int64_t most, int64_t count) {
   return blocks <= count ? 0 : cdiv(blocks, 16) * 16;
 }
 
-// Ranks and selection in one launch, or in two: one workgroup a (sequence, key head) has the long ones for itself, but two
-// launches begin twice.  us in a graph, blocks 64 / 128 / 256 / 512 / 1024 of 32 query on 8 key heads x 128 in bf16, in
-// one launch of 512 threads, of 256 threads and in two:
-//     8 units    7.8  9.3 13.2 18.4 26.9     8.5 11.4 15.1 20.8 32.4     9.3 10.4 11.1 11.3  9.9
-//   128 units    8.2  9.9 14.0 19.9 29.8     9.0 11.9 15.5 24.4 37.6     9.8 11.3 12.9 18.8 26.7
-//   256 units    8.3  9.8 14.9 21.8 32.4     9.2 11.9 18.0 25.7 39.9     9.9 12.5 18.1 26.6 39.5
-//  1024 units   28.7 37.2 53.9 74.9  130    21.0 28.3 39.5 61.2  128    17.6 27.8 41.6 70.1  149
+// Ranks and selection in one launch, or in two: one workgroup has all blocks of a (sequence, key head), but two launches
+// begin twice.  us in a graph, 64 / 128 / 192 / 256 / 512 / 1024 blocks of 32 query on 8 key heads x 128 in bf16:
+//               512 threads                    256 threads                    two launches
+//     8 units    7.6  9.5 11.0 13.3 17.9 26.7   7.6 10.4 12.5 14.0 19.8 31.6   9.7 10.6 11.3 11.6 11.7 11.9
+//   128 units    7.9  9.7 11.8 13.9 19.4 29.2   8.0 10.9 12.8 14.7 21.3 33.6  10.2 11.4 13.1 13.2 18.2 26.1
+//   256 units    8.0  9.8 11.8 14.6 21.3 31.8   8.0 11.0 12.9 15.2 22.3 35.3  10.1 12.8 14.2 18.0 26.4 37.1
+//  1024 units   28.6 36.4 44.4 53.3 75.3  129  17.2 25.9 33.2 39.2 61.9  123  17.7 27.8 34.6 39.0 61.8  127
 constexpr int FUSED_ALWAYS = 192, FUSED_KEYS = 4;  // blocks of any number of units; consecutive blocks a thread
 enum class Form { two, one_256, one_512 };
 Form select_form(int64_t units, int64_t ld) {
