@@ -533,6 +533,8 @@ __device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[
     for (int w = 0; w < WAVES; ++w)
       if (w < wid) before += s.part2[w];
     if (before < need && before + mine >= need) s.picked[0] = BINS - 1 - tid, s.picked[1] = before, s.picked[2] = mine;
+    // (fewer ranks than are needed: lengths that were written to during the call; all of them, so that the rounds end)
+    if (tid == BINS - 1 && before + mine < need) s.picked[0] = 0, s.picked[1] = need - mine, s.picked[2] = mine;
     __syncthreads();
     const int last = s.picked[0], many = s.picked[2];
     need -= s.picked[1];
@@ -725,6 +727,8 @@ __global__ __launch_bounds__(SL_THREADS) void kv_select_long_kernel(SelectArgs a
           picked[0] = 255 - 4 * lane - i, picked[1] = before, picked[2] = many[i];
         before += many[i];
       }
+      // (fewer ranks than are needed: lengths that were written to during the call)
+      if (lane == 63 && before < need) picked[0] = 0, picked[1] = need - many[3], picked[2] = many[3];
     }
     __syncthreads();
     found |= (uint32_t)picked[0] << shift;
@@ -925,9 +929,16 @@ extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t
   const int64_t es = pages->dtype == DT_F32 ? 4 : 2;
   CORTEX_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_sb * es) % 16 == 0 && (q_sh * es) % 16 == 0,
                    "%s: query rows must be 16-byte aligned", who);
+  // what the call writes is read by no workgroup of it
+  auto meet = [](const void* x, int64_t n, const void* y, int64_t m) {
+    return x && y && (uintptr_t)x < (uintptr_t)y + (uintptr_t)m && (uintptr_t)y < (uintptr_t)x + (uintptr_t)n;
+  };
   const int64_t blocks = most_blocks(pages, a.max_length), ld = rank_ld(pages, a.max_length, count);
   const int64_t keep = count < blocks ? count : blocks;
   CORTEX_CHECK_ARG(table || keep == 0, "%s: null table", who);
+  CORTEX_CHECK_ARG(!meet(new_lengths, 8 * B, lengths, 8 * B), "%s: new_lengths may not be lengths, nor overlap them", who);
+  CORTEX_CHECK_ARG(max_pages == 0 || !meet(table, 4 * B * pages->kv_heads * keep, block_table, 4 * ((B - 1) * ld_table + max_pages)),
+                   "%s: table may not overlap the block table", who);
   const int64_t need = cortex_kv_select_workspace_bytes(pages, B, a.max_length, count);
   CORTEX_CHECK_ARG((workspace || need == 0) && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
   // (a launch has fewer than 2^32 threads)

@@ -36,7 +36,7 @@ def bounds(p, B=2, table=P, ld=3, width=3, lengths=P, most=48, since=None, new=-
 
 
 def select(p, B=2, heads=4, q=P, sb=256, sh=64, table=P, ld=300, width=300, lengths=P, most=4800, count=8, first=1, recent=1,
-           out=P, after=P, ws=P, ws_bytes=1 << 40):
+           out=4 * V, after=2 * V, ws=P, ws_bytes=1 << 40):
     return ("cortex_kv_select", ref(p), B, heads, q, sb, sh, table, ld, width, lengths, most, count, first, recent, out, after,
             ws, ws_bytes, None, None)
 
@@ -115,12 +115,16 @@ def test_refused_selections():
     refused(select(pages(), q=None), "null pointer")
     refused(select(pages(), after=None), "null pointer")
     refused(select(pages(), out=None), "null table")
+    for after in (P, P + 8, P - 8):
+        refused(select(pages(), after=after), "overlap")
+    refused(select(pages(), out=P + 2396), "overlap")
+    refused(select(pages(), out=2 * V, table=2 * V + 4), "overlap")
     refused(select(pages(), q=8), "16-byte")
     refused(select(pages(), sb=252), "16-byte")
     refused(select(pages(), ws=None), "workspace")
     refused(select(pages(), ws=8), "workspace")
     refused(select(pages(), ws_bytes=64), "needed", rc=-4)
-    refused(select(pages(kv_heads=65535, head_dim=64), heads=65535, B=1 << 12), "too much")
+    refused(select(pages(kv_heads=65535, head_dim=64), heads=65535, B=1 << 12, out=1 << 60), "too much")
     lib = nat.load()
     size = lib.cortex_kv_select_workspace_bytes
     assert size(ref(pages()), 2, 4800, 8) == 2 * 2 * 304 * 4
