@@ -268,11 +268,14 @@ __device__ __forceinline__ int blocks_of(const SelectArgs& a, int64_t n) {
   return (int)((n + (1ll << a.p.shift) - 1) >> a.p.shift);
 }
 
-// The ranks of tiles of 16 blocks, a tile a wavefront.  The sums are in 64 bits and rounded to 32 once: which blocks are
-// chosen does not depend on an order of sums.  v_mfma_f64_4x4x4 multiplies four 4 x 4 tiles: lane 16 g + r takes eight dims
+// The ranks of tiles of 16 blocks, a tile a wavefront.  The sums are in 64 bits, in one order for every form of the launch, and
+// rounded to 32 once; those of bf16 products are exact as long as the terms lie within 2^29 of each other.  So neither the
+// batch nor the launch decides which blocks are chosen, and another order of sums would not.  v_mfma_f64_4x4x4 multiplies four 4 x 4 tiles: lane 16 g + r takes eight dims
 // 8 (4 c + g) .. of the bounds of block r and of the query of head r % 4, and gets the sum of block 4 ((l % 16) / 4) + l / 16
 // and head l % 4.  The bounds come from memory into registers; the queries, max(q, 0) and min(q, 0) in 64 bits, are made
 // once a workgroup while its first bounds are on their way, into LDS: converted at each use they are half of the work.
+// Matrix and vector instructions add up here, from whichever wavefront they come (20 cycles a product of a wavefront, 20 + 17
+// with four vector instructions beside it): 64 products and as many unpackings and conversions a tile of 128 dims take 1900.
 // DHP: head_dim rounded up to 64; NG: fours of query heads at a time.
 template <class O, class Q, int DHP, int NG>
 struct Scores {
