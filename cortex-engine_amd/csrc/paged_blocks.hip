@@ -450,58 +450,66 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t x) {
 
 constexpr int PK_FEW = 64;  // ranks that are compared with each other
 
-template <int WAVES>
+template <int WAVES, int KPT>
 struct PickShared {
   int hist[64 * WAVES];
   uint32_t most[WAVES], least[WAVES];
-  int part[WAVES], part2[WAVES];
+  int part[KPT * WAVES], part2[WAVES];
   int picked[3], few;
   uint2 list[PK_FEW];
 };
 
-// Flags before this thread's, and of all threads.
+// How many flags there are before each of this thread's: flag i of thread t is the (i * threads + t)-th.  Returns how many
+// there are in all; flags from `rounds` rounds on are not looked at.
 template <int WAVES, int N>
-__device__ __forceinline__ int before_of(const bool (&flag)[N], int* part, int lane, int wid, int* total) {
-  int mine = 0, all = 0;
+__device__ __forceinline__ int before_of(const bool (&flag)[N], int (&before)[N], int rounds, int* part, int lane, int wid) {
+  uint64_t m[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint64_t m = __ballot(flag[i]);
-    mine += __popcll(m & ((1ull << lane) - 1));
-    all += __popcll(m);
-  }
-  if (lane == 0) part[wid] = all;
+  for (int i = 0; i < N; ++i)
+    if (i < rounds) {
+      m[i] = __ballot(flag[i]);
+      if (lane == 0) part[i * WAVES + wid] = __popcll(m[i]);
+    }
   __syncthreads();
   int sum = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < wid) mine += part[w];
-    sum += part[w];
-  }
-  *total = sum;
-  return mine;
+  for (int i = 0; i < N; ++i)
+    if (i < rounds) {
+      before[i] = sum + __popcll(m[i] & ((1ull << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const int v = part[i * WAVES + w];
+        if (w < wid) before[i] += v;
+        sum += v;
+      }
+    }
+  return sum;
 }
 
-// The pages of the a.count blocks to keep, in their order, from the ranks of KPT consecutive blocks a thread (0: always
+// The pages of the a.count blocks to keep, in their order, from the ranks of the blocks tid, tid + threads .. (0: always
 // kept, or not there).  The ranks are counted in as many bins as there are threads, even parts of their range; the bin
 // that holds the last one kept is found from the counts, and its ranks, where they are few, are compared with each other
 // by every wavefront for itself.  Where they are many the bin is cut into bins again.
 template <int WAVES, int KPT>
 __device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[KPT], int blocks, const int32_t (&page)[KPT],
-                                     int32_t* out, PickShared<WAVES>& s) {
+                                     int32_t* out, PickShared<WAVES, KPT>& s) {
   constexpr int BINS = 64 * WAVES;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, i0 = tid * KPT;
-  int need = a.count - a.first - a.recent, total;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int rounds = (blocks + BINS - 1) / BINS;
+  int need = a.count - a.first - a.recent;
   bool keep[KPT], open[KPT];  // open: not decided yet
+  int before[KPT];
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
+    const int at = i * BINS + tid;
     open[i] = need > 0 && key[i] != 0;
-    keep[i] = i0 + i < blocks && (i0 + i < a.first || i0 + i >= blocks - a.recent);
+    keep[i] = at < blocks && (at < a.first || at >= blocks - a.recent);
   }
   while (need > 0) {  // (the same for all threads)
     uint32_t most = 0, least = 0;  // the largest rank, and of the inverted ranks
 #pragma unroll
     for (int i = 0; i < KPT; ++i)
-      if (open[i]) most = max(most, key[i]), least = max(least, ~key[i]);
+      if (i < rounds && open[i]) most = max(most, key[i]), least = max(least, ~key[i]);
     most = wave_most(most), least = wave_most(least);
     if (lane == 0) s.most[wid] = most, s.least[wid] = least;
     s.hist[tid] = 0;
@@ -511,12 +519,9 @@ __device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[
     for (int w = 0; w < WAVES; ++w) most = max(most, s.most[w]), least = max(least, s.least[w]);
     const uint32_t low = ~least, range = most - low;
     if (range == 0) {  // one rank for all: the lower blocks
-      int before = before_of<WAVES, KPT>(open, s.part, lane, wid, &total);
+      before_of<WAVES, KPT>(open, before, rounds, s.part, lane, wid);
 #pragma unroll
-      for (int i = 0; i < KPT; ++i) {
-        keep[i] = keep[i] || (open[i] && before < need);
-        before += open[i];
-      }
+      for (int i = 0; i < KPT; ++i) keep[i] = keep[i] || (i < rounds && open[i] && before[i] < need);
       break;
     }
     // (conversion, product and truncation keep the order)
@@ -525,19 +530,19 @@ __device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       bin[i] = min((int)((float)(key[i] - low) * scale), BINS - 1);
-      if (open[i]) atomicAdd(&s.hist[bin[i]], 1);
+      if (i < rounds && open[i]) atomicAdd(&s.hist[bin[i]], 1);
     }
     __syncthreads();
     const int mine = s.hist[BINS - 1 - tid], upto = scan64(mine);
     if (lane == 63) s.part2[wid] = upto;
     __syncthreads();
-    int before = upto - mine;
+    int above = upto - mine;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w)
-      if (w < wid) before += s.part2[w];
-    if (before < need && before + mine >= need) s.picked[0] = BINS - 1 - tid, s.picked[1] = before, s.picked[2] = mine;
+      if (w < wid) above += s.part2[w];
+    if (above < need && above + mine >= need) s.picked[0] = BINS - 1 - tid, s.picked[1] = above, s.picked[2] = mine;
     // (fewer ranks than are needed: lengths that were written to during the call; all of them, so that the rounds end)
-    if (tid == BINS - 1 && before + mine < need) s.picked[0] = 0, s.picked[1] = need - mine, s.picked[2] = mine;
+    if (tid == BINS - 1 && above + mine < need) s.picked[0] = 0, s.picked[1] = need - mine, s.picked[2] = mine;
     __syncthreads();
     const int last = s.picked[0], many = s.picked[2];
     need -= s.picked[1];
@@ -551,37 +556,35 @@ __device__ __forceinline__ void pick(const SelectArgs& a, const uint32_t (&key)[
     if (many > PK_FEW) continue;
 #pragma unroll
     for (int i = 0; i < KPT; ++i)
-      if (open[i]) s.list[atomicAdd(&s.few, 1)] = make_uint2(key[i], (uint32_t)(i0 + i));
+      if (i < rounds && open[i]) s.list[atomicAdd(&s.few, 1)] = make_uint2(key[i], (uint32_t)(i * BINS + tid));
     __syncthreads();
     const uint2 own = lane < many ? s.list[lane] : make_uint2(0, 0);
-    int above = 0;  // those before this one: of higher rank, or of the same and a lower block
+    int ahead = 0;  // those before this one: of higher rank, or of the same and a lower block
     for (int i = 0; i < many; ++i) {
       const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)own.x, i), y = (uint32_t)__builtin_amdgcn_readlane((int)own.y, i);
-      above += x > own.x || (x == own.x && y < own.y);
+      ahead += x > own.x || (x == own.x && y < own.y);
     }
-    const int at = __builtin_ctzll(__ballot(lane < many && above == need - 1));
+    const int at = __builtin_ctzll(__ballot(lane < many && ahead == need - 1));
     const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)own.x, at), y = (uint32_t)__builtin_amdgcn_readlane((int)own.y, at);
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) keep[i] = keep[i] || (open[i] && (key[i] > x || (key[i] == x && (uint32_t)(i0 + i) <= y)));
+    for (int i = 0; i < KPT; ++i)
+      keep[i] = keep[i] || (open[i] && (key[i] > x || (key[i] == x && (uint32_t)(i * BINS + tid) <= y)));
     break;
   }
   __syncthreads();
-  int to = before_of<WAVES, KPT>(keep, s.part, lane, wid, &total);
+  before_of<WAVES, KPT>(keep, before, rounds, s.part, lane, wid);
 #pragma unroll
   for (int i = 0; i < KPT; ++i)
-    if (keep[i]) {
-      if (to < a.keep) out[to] = page[i];
-      ++to;
-    }
+    if (i < rounds && keep[i] && before[i] < a.keep) out[before[i]] = page[i];
 }
 
 // The pages of this thread's blocks, loaded before it is known which of them are there.
-template <int KPT>
+template <int THREADS, int KPT>
 __device__ __forceinline__ void load_pages(const SelectArgs& a, const int32_t* pages, int32_t (&page)[KPT]) {
   const int width = (int)(a.p.max_slots >> a.p.shift);
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const int at = threadIdx.x * KPT + i;
+    const int at = i * THREADS + threadIdx.x;
     page[i] = at < width ? pages[at] : -1;
   }
 }
@@ -612,7 +615,7 @@ __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   typedef Scores<O, Q, DHP, NG> S;
   __shared__ __attribute__((aligned(16))) uint32_t rank[THREADS * KPT];
   __shared__ __attribute__((aligned(16))) typename S::Query query;
-  __shared__ __attribute__((aligned(16))) PickShared<WAVES> s;
+  __shared__ __attribute__((aligned(16))) PickShared<WAVES, KPT> s;
   const int b = blockIdx.x / a.p.kv_heads, h = blockIdx.x - b * a.p.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wid = wave_uniform(tid >> 6);
   bool ok = true;
@@ -623,18 +626,13 @@ __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
   const int tiles = (blocks + 15) >> 4;
   int32_t page[KPT];
-  load_pages(a, pages, page);
+  load_pages<THREADS>(a, pages, page);
   S::template run<THREADS>(a, query, b, h, blocks, wid, WAVES, tiles, lane, rank);
   __syncthreads();
   uint32_t key[KPT];
 #pragma unroll
-  for (int i = 0; i < KPT; i += 4) {
-    const uint4 x = *reinterpret_cast<const uint4*>(rank + tid * KPT + i);
-    key[i] = x.x, key[i + 1] = x.y, key[i + 2] = x.z, key[i + 3] = x.w;
-  }
-#pragma unroll
-  for (int i = 0; i < KPT; ++i)
-    if (tid * KPT + i >= tiles * 16) key[i] = 0;  // (behind the last tile nothing was written)
+  for (int i = 0; i < KPT; ++i)  // (behind the last tile nothing was written)
+    key[i] = i * THREADS + tid < tiles * 16 ? rank[i * THREADS + tid] : 0;
   pick<WAVES, KPT>(a, key, blocks, page, out, s);
 }
 
@@ -662,21 +660,17 @@ __global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a, int per) {
 template <int THREADS, int KPT>
 __global__ __launch_bounds__(THREADS) void kv_select_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
-  __shared__ __attribute__((aligned(16))) PickShared<WAVES> s;
+  __shared__ __attribute__((aligned(16))) PickShared<WAVES, KPT> s;
   const int b = blockIdx.x / a.p.kv_heads, h = blockIdx.x - b * a.p.kv_heads;
   const int tid = threadIdx.x;
   // ranks and pages beside the length that says which of them count
   const uint32_t* rank = a.rank + (int64_t)blockIdx.x * a.ld;
   uint32_t key[KPT];
 #pragma unroll
-  for (int i = 0; i < KPT; i += 4) {
-    uint4 x = {0, 0, 0, 0};
-    if (tid * KPT + i < a.ld) x = *reinterpret_cast<const uint4*>(rank + tid * KPT + i);
-    key[i] = x.x, key[i + 1] = x.y, key[i + 2] = x.z, key[i + 3] = x.w;
-  }
+  for (int i = 0; i < KPT; ++i) key[i] = i * THREADS + tid < a.ld ? rank[i * THREADS + tid] : 0;
   const int32_t* pages = a.p.table + b * a.p.ld_table;
   int32_t page[KPT];
-  load_pages(a, pages, page);
+  load_pages<THREADS>(a, pages, page);
   bool ok = true;
   const int64_t n = a.p.length_of(a.lengths, b, a.max_length, &ok);
   const int blocks = blocks_of(a, n);
@@ -684,7 +678,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(SelectArgs a) {
   if (begin_select(a, b, h, n, ok, blocks, pages, out)) return;
 #pragma unroll
   for (int i = 0; i < KPT; ++i)
-    if (tid * KPT + i >= ((blocks + 15) & ~15)) key[i] = 0;  // (behind the last tile nothing was written)
+    if (i * THREADS + tid >= ((blocks + 15) & ~15)) key[i] = 0;  // (behind the last tile nothing was written)
   pick<WAVES, KPT>(a, key, blocks, page, out, s);
 }
 
@@ -746,12 +740,12 @@ __global__ __launch_bounds__(SL_THREADS) void kv_select_long_kernel(SelectArgs a
     const uint32_t x = i < blocks ? rank[i] : 0;
     bool keep[1] = {i < blocks && (i < a.first || i >= blocks - a.recent)}, equal[1] = {!whole && x != 0 && x == found};
     keep[0] = keep[0] || (!none && x != 0 && (whole ? x >= found : x > found));
-    int sum;
-    int before = tie + before_of<WAVES, 1>(equal, part[0], lane, wid, &sum);
-    tie += sum;
-    keep[0] = keep[0] || (equal[0] && before < need);
-    const int to = at + before_of<WAVES, 1>(keep, part[1], lane, wid, &sum);
-    at += sum;
+    int before[1];
+    const int ties = before_of<WAVES, 1>(equal, before, 1, part[0], lane, wid);
+    keep[0] = keep[0] || (equal[0] && tie + before[0] < need);
+    tie += ties;
+    const int kept = before_of<WAVES, 1>(keep, before, 1, part[1], lane, wid), to = at + before[0];
+    at += kept;
     if (keep[0] && to < a.keep) out[to] = pages[i];
   }
 }
@@ -858,7 +852,7 @@ int64_t rank_ld(const cortex_kv_pages* pages, int64_t most, int64_t count) {
 //   128 units    7.9  9.7 11.8 13.9 19.4 29.2   8.0 10.9 12.8 14.7 21.3 33.6  10.2 11.4 13.1 13.2 18.2 26.1
 //   256 units    8.0  9.8 11.8 14.6 21.3 31.8   8.0 11.0 12.9 15.2 22.3 35.3  10.1 12.8 14.2 18.0 26.4 37.1
 //  1024 units   28.6 36.4 44.4 53.3 75.3  129  17.2 25.9 33.2 39.2 61.9  123  17.7 27.8 34.6 39.0 61.8  127
-constexpr int FUSED_ALWAYS = 192, FUSED_KEYS = 4;  // blocks of any number of units; consecutive blocks a thread
+constexpr int FUSED_ALWAYS = 192, FUSED_KEYS = 4;  // blocks of any number of units; blocks a thread
 enum class Form { two, one_256, one_512 };
 Form select_form(int64_t units, int64_t ld) {
   const int64_t cus = cu_count();
@@ -866,6 +860,13 @@ Form select_form(int64_t units, int64_t ld) {
   return units > cus && ld <= 256 * FUSED_KEYS ? Form::one_256 : Form::one_512;
 }
 
+template <class O, class Q, int DHP, int NG, int THREADS>
+void launch_one(const SelectArgs& a, dim3 units, hipStream_t stream) {
+  if (a.ld <= THREADS)  // (the code for one block a thread is shorter: 38 blocks 6.2 -> 5.3 us, up to 501 17.1 -> 16.2)
+    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, 1>), units, dim3(THREADS), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, FUSED_KEYS>), units, dim3(THREADS), 0, stream, a);
+}
 template <class O, class Q, int DHP, int NG>
 int launch_select(const SelectArgs& a, hipStream_t stream) {
   const int64_t n = (int64_t)a.B * a.p.kv_heads;
@@ -873,9 +874,9 @@ int launch_select(const SelectArgs& a, hipStream_t stream) {
   const Form form = select_form(n, a.ld);
   if (form != Form::two) {
     if (form == Form::one_256)
-      hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, 256, FUSED_KEYS>), units, dim3(256), 0, stream, a);
+      launch_one<O, Q, DHP, NG, 256>(a, units, stream);
     else
-      hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, 512, FUSED_KEYS>), units, dim3(512), 0, stream, a);
+      launch_one<O, Q, DHP, NG, 512>(a, units, stream);
     CORTEX_CHECK_LAUNCH("kv_rank_select_kernel");
     return OK;
   }
