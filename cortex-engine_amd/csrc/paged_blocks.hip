@@ -896,10 +896,17 @@ int launch_select(const SelectArgs& a, hipStream_t stream) {
   CORTEX_CHECK_LAUNCH("kv_select_kernel");
   return OK;
 }
+// Fours of query heads at a time: as many as there are, up to 16 heads.  (Eight heads as sixteen: 256 blocks 15.1 us instead of
+// 11.7, int8 18.8 and 13.3; sixteen as twice eight: the same in bf16, fp32 of 64 dims 13.7 instead of 11.9, fp32 bounds of 128 dims
+// 20.0 instead of 19.6 although those spill 47 of 256 registers.)
+template <class O, class Q, int DHP>
+int launch_select(const SelectArgs& a, hipStream_t stream) {
+  if (a.group <= 4) return launch_select<O, Q, DHP, 1>(a, stream);
+  return a.group <= 8 ? launch_select<O, Q, DHP, 2>(a, stream) : launch_select<O, Q, DHP, 4>(a, stream);
+}
 template <class O, class Q>
 int launch_select(const SelectArgs& a, hipStream_t stream) {
-  if (a.p.head_dim <= 64) return a.group <= 4 ? launch_select<O, Q, 64, 1>(a, stream) : launch_select<O, Q, 64, 4>(a, stream);
-  return a.group <= 4 ? launch_select<O, Q, 128, 1>(a, stream) : launch_select<O, Q, 128, 4>(a, stream);
+  return a.p.head_dim <= 64 ? launch_select<O, Q, 64>(a, stream) : launch_select<O, Q, 128>(a, stream);
 }
 
 }  // namespace
