@@ -386,15 +386,16 @@ struct Scores {
   }
 
   // Ranks of the tiles first, first + step .. up to `tiles` of a (sequence, key head) into rank_out[]: 0 for the blocks that
-  // are always kept and, to the end of a tile, for those that are not there.  All threads of the workgroup call it.
-  template <int THREADS>
+  // are always kept and, to the end of a tile, for those that are not there.  All threads of the workgroup call it.  ONE: a
+  // wavefront has one tile at most (shorter code, fewer registers).
+  template <int THREADS, bool ONE>
   static __device__ __forceinline__ void run(const SelectArgs& a, Query& q, int b, int h, int blocks, int first, int step,
                                              int tiles, int lane, uint32_t* rank_out) {
     const int r = lane & 15, g = lane >> 4;
     auto page_at = [&](int t) { return a.p.page_of(b, (int64_t)min(16 * t + r, blocks - 1) << a.p.shift); };
     for (int i = 0; i < a.group; i += HEADS) {
       Bounds now, next;
-      int page = page_at(first), next_page = page_at(first + step);
+      int page = page_at(first), next_page = ONE ? 0 : page_at(first + step);
       if (first < tiles) load_bounds(a, now, page, h, g);
       if (i > 0) __syncthreads();
       load_query<THREADS>(a, q, b, h, i);
@@ -410,7 +411,7 @@ struct Scores {
         if ((r & 3) == 0) rank_out[mine] = i > 0 ? max(best, rank_out[mine]) : best;
       };
       int t = first;
-      for (; t + step < tiles; t += step) {  // (the last tile apart: nothing to load beside it)
+      for (; !ONE && t + step < tiles; t += step) {  // (the last tile apart: nothing to load beside it)
         const int page_after = page_at(t + 2 * step);
         load_bounds(a, next, next_page, h, g);
         put(t);
@@ -609,7 +610,7 @@ __device__ __forceinline__ bool begin_select(const SelectArgs& a, int b, int h, 
 // Ranks and selection in one: a workgroup a (sequence, key head) of up to KPT * THREADS blocks.  32 sequences of 10 .. 501
 // blocks, 32 query on 8 key heads x 128 in bf16, 33 MB: 17.2 us.  Of that about 7 are the 64-bit products of the longest
 // sequences, whose wavefronts have four tiles each where the mean is two, and 2.6 the selection; 38 blocks of 8 heads x 64: 6.2.
-template <class O, class Q, int DHP, int NG, int THREADS, int KPT>
+template <class O, class Q, int DHP, int NG, int THREADS, int KPT, bool ONE>
 __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
   typedef Scores<O, Q, DHP, NG> S;
@@ -627,7 +628,7 @@ __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   const int tiles = (blocks + 15) >> 4;
   int32_t page[KPT];
   load_pages<THREADS>(a, pages, page);
-  S::template run<THREADS>(a, query, b, h, blocks, wid, WAVES, tiles, lane, rank);
+  S::template run<THREADS, ONE>(a, query, b, h, blocks, wid, WAVES, tiles, lane, rank);
   __syncthreads();
   uint32_t key[KPT];
 #pragma unroll
@@ -642,7 +643,7 @@ constexpr int RK_MORE = 4, RK_MANY = 64;
 
 // The ranks alone: `per` tiles of a (sequence, key head) a workgroup.  2048 blocks of 32 query on 8 key heads x 128, 8.4 MB: 6.7 us,
 // the chain length -> table -> bounds -> products of one tile.
-template <class O, class Q, int DHP, int NG>
+template <class O, class Q, int DHP, int NG, bool ONE>
 __global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a, int per) {
   typedef Scores<O, Q, DHP, NG> S;
   __shared__ __attribute__((aligned(16))) typename S::Query query;
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256) void kv_rank_kernel(SelectArgs a, int per) {
   const int blocks = blocks_of(a, a.p.length_of(a.lengths, b, a.max_length, &ok));
   const int tiles = min((blocks + 15) >> 4, per * (chunk + 1));
   if (blocks <= a.count || per * chunk >= tiles) return;  // (all of them are kept, or there are none for this workgroup)
-  S::template run<256>(a, query, b, h, blocks, per * chunk + wid, 4, tiles, lane, a.rank + (int64_t)bh * a.ld);
+  S::template run<256, ONE>(a, query, b, h, blocks, per * chunk + wid, 4, tiles, lane, a.rank + (int64_t)bh * a.ld);
 }
 
 // The selection from ranks in the workspace.  2048 blocks: 5.8 us, a launch and the rounds between its barriers.
@@ -862,10 +863,13 @@ Form select_form(int64_t units, int64_t ld) {
 
 template <class O, class Q, int DHP, int NG, int THREADS>
 void launch_one(const SelectArgs& a, dim3 units, hipStream_t stream) {
-  if (a.ld <= THREADS)  // (the code for one block a thread is shorter: 38 blocks 6.2 -> 5.3 us, up to 501 17.1 -> 16.2)
-    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, 1>), units, dim3(THREADS), 0, stream, a);
+  // (the code for one block a thread is shorter: 38 blocks 6.2 -> 5.3 us, up to 501 17.1 -> 16.2)
+  if (a.ld <= THREADS / 4)
+    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, 1, true>), units, dim3(THREADS), 0, stream, a);
+  else if (a.ld <= THREADS)
+    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, 1, false>), units, dim3(THREADS), 0, stream, a);
   else
-    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, FUSED_KEYS>), units, dim3(THREADS), 0, stream, a);
+    hipLaunchKernelGGL((kv_rank_select_kernel<O, Q, DHP, NG, THREADS, FUSED_KEYS, false>), units, dim3(THREADS), 0, stream, a);
 }
 template <class O, class Q, int DHP, int NG>
 int launch_select(const SelectArgs& a, hipStream_t stream) {
@@ -881,7 +885,10 @@ int launch_select(const SelectArgs& a, hipStream_t stream) {
     return OK;
   }
   const int per_wave = n * a.ld / 16 >= RK_MANY * cu_count() ? RK_MORE : 1, chunks = (int)cdiv(a.ld, 64 * per_wave);
-  hipLaunchKernelGGL((kv_rank_kernel<O, Q, DHP, NG>), dim3((unsigned)(n * chunks)), dim3(256), 0, stream, a, 4 * per_wave);
+  if (per_wave == 1)
+    hipLaunchKernelGGL((kv_rank_kernel<O, Q, DHP, NG, true>), dim3((unsigned)(n * chunks)), dim3(256), 0, stream, a, 4);
+  else
+    hipLaunchKernelGGL((kv_rank_kernel<O, Q, DHP, NG, false>), dim3((unsigned)(n * chunks)), dim3(256), 0, stream, a, 4 * per_wave);
   CORTEX_CHECK_LAUNCH("kv_rank_kernel");
   if (a.ld <= 1024)
     hipLaunchKernelGGL((kv_select_kernel<256, 4>), units, dim3(256), 0, stream, a);
