@@ -608,8 +608,8 @@ __device__ __forceinline__ bool begin_select(const SelectArgs& a, int b, int h, 
 }
 
 // Ranks and selection in one: a workgroup a (sequence, key head) of up to KPT * THREADS blocks.  32 sequences of 10 .. 501
-// blocks, 32 query on 8 key heads x 128 in bf16, 33 MB: 17.2 us.  Of that about 7 are the 64-bit products of the longest
-// sequences, whose wavefronts have four tiles each where the mean is two, and 2.6 the selection; 38 blocks of 8 heads x 64: 6.2.
+// blocks, 32 query on 8 key heads x 128 in bf16, 33 MB: 16.2 us.  Of that about 7 are the 64-bit products of the longest
+// sequences, whose wavefronts have four tiles each where the mean is two, and 2 the selection; 38 blocks of 8 heads x 64: 5.2.
 template <class O, class Q, int DHP, int NG, int THREADS, int KPT, bool ONE>
 __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
@@ -847,12 +847,13 @@ int64_t rank_ld(const cortex_kv_pages* pages, int64_t most, int64_t count) {
 }
 
 // Ranks and selection in one launch, or in two: one workgroup has all blocks of a (sequence, key head), but two launches
-// begin twice.  us in a graph, 64 / 128 / 192 / 256 / 512 / 1024 blocks of 32 query on 8 key heads x 128 in bf16:
-//               512 threads                    256 threads                    two launches
-//     8 units    7.6  9.5 11.0 13.3 17.9 26.7   7.6 10.4 12.5 14.0 19.8 31.6   9.7 10.6 11.3 11.6 11.7 11.9
-//   128 units    7.9  9.7 11.8 13.9 19.4 29.2   8.0 10.9 12.8 14.7 21.3 33.6  10.2 11.4 13.1 13.2 18.2 26.1
-//   256 units    8.0  9.8 11.8 14.6 21.3 31.8   8.0 11.0 12.9 15.2 22.3 35.3  10.1 12.8 14.2 18.0 26.4 37.1
-//  1024 units   28.6 36.4 44.4 53.3 75.3  129  17.2 25.9 33.2 39.2 61.9  123  17.7 27.8 34.6 39.0 61.8  127
+// begin twice.  us in a graph, 64 / 128 / 256 / 512 / 1024 blocks of 32 query on 8 key heads x 128 in bf16:
+//               512 threads               256 threads               two launches
+//     8 units    6.4  8.0 12.3 17.0 27.5   6.7  9.5 13.0 18.2 30.3   9.0 10.1 10.5 10.8 10.0
+//   128 units    6.7  8.4 12.6 18.2 29.3   6.9  9.9 13.4 21.3 34.5   9.3 10.6 12.2 16.2 24.1
+//   192 units    6.7  8.5 12.9 18.8 29.9   7.1  9.9 13.5 21.8 34.9   9.4 11.8 13.5 20.7 29.9
+//   256 units    6.6  8.7 13.5 20.5 31.7   7.0  9.9 14.2 22.3 35.5   9.5 12.0 16.0 23.7 36.8
+//  1024 units   16.0 22.1 48.8 70.6  131  12.0 24.2 37.5 62.3  125  15.7 25.2 38.3 61.5  128
 constexpr int FUSED_ALWAYS = 192, FUSED_KEYS = 4;  // blocks of any number of units; blocks a thread
 enum class Form { two, one_256, one_512 };
 Form select_form(int64_t units, int64_t ld) {
