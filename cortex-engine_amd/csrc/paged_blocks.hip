@@ -160,8 +160,10 @@ __device__ __forceinline__ void store_bounds(O* to, const float* f) {
 
 // A wavefront takes a (page, key head) at a time: `lanes` lanes a row, 16 bytes each, the groups of lanes joined at the end.
 // 16 sequences of 1000 .. 15001 int8 keys, 4 heads x 128, 84 MB: 20.8 us, 4.0 TB/s.  A value takes a conversion, a product with
-// its row's scale and half of a three-operand maximum and minimum each, about as long as its bytes; joined by shuffles it was
-// 24.6.  The last page of 32 sequences: 3.9 us, the chain length -> table -> rows.
+// its row's scale and half of a three-operand maximum and minimum each, about as long as its bytes: 20.3 us with the rows in
+// cache, 15.6 without the arithmetic, 17.6 without the join, 10.2 with neither rows nor arithmetic.  The next page loaded while
+// one is joined takes 184 registers: 32 us.  Joined by shuffles it was 24.6.
+// The last page of 32 sequences: 3.9 us, the chain length -> table -> rows.
 template <class P>
 __global__ __launch_bounds__(256) void kv_bounds_kernel(BoundsArgs a) {
   constexpr int ES = sizeof(P), N = 16 / ES;
