@@ -41,8 +41,8 @@ class KVBatch(NamedTuple):
     """Sessions of a step as the operators take them (device tensors): ``block_table`` (B, pages) int32, the slots in use
     before the step's tokens (``before``) and with them (``lengths``), ``offsets`` (B + 1,) of the tokens (None: one a
     session), their ``positions``, and on the host ``tokens`` and ``max_length``.  It holds until one of its sessions is
-    cut, dropped, forked or moved; ``append`` and ``attend`` refuse it from then on.  ``filled``: the layers that have its tokens' rows;
-    ``needs``: the same of every batch whose rows some layer lacked when this one was made, its own among them."""
+    cut, dropped, forked or moved; ``append`` and ``attend`` refuse it from then on.  ``filled``: the layers that have its
+    tokens' rows; ``needs``: the same of every batch whose rows some layer lacked when this one was made, its own among them."""
 
     sessions: tuple[str, ...]
     block_table: torch.Tensor
@@ -309,9 +309,9 @@ class PagedKVCache:
 
     def resize(self, num_pages: int) -> int:
         """Pools of ``num_pages`` pages instead (``layers`` are other objects then); returns how many pages got another
-        place, those past the end of smaller pools.  MemoryError, and nothing changed, where the pages in use are more, or where the device has no room for the
-        new pools beside the old ones.  Every layer must have the rows of the tokens of sessions that move; batches made
-        before no longer hold for these."""
+        place, those past the end of smaller pools.  MemoryError, and nothing changed, where the pages in use are more, or
+        where the device has no room for the new pools beside the old ones.  Every layer must have the rows of the tokens of
+        sessions that move; batches made before no longer hold for these."""
         if num_pages < 1:
             raise ValueError("num_pages must be >= 1")
         src = np.flatnonzero(self._users > 0).astype(np.int32)

@@ -394,8 +394,9 @@ def paged_block_select(q: torch.Tensor, pages: KVPages, block_table: torch.Tenso
     """Up to ``count`` pages of each sequence and key head that ``q`` (B, heads, head_dim) may find its largest scores in,
     as a table that ``paged_attention`` takes.
 
-    A page's score is the largest ``sum_d max(q_d max_d, q_d min_d)`` (``pages.bounds``) over the query heads of the key
-    head, which no ``q . k`` of the page exceeds; it is summed in 64 bits and rounded to 32.  The ``first`` and the last
+    A page's score is the largest ``sum_d max(q_d, 0) max_d + min(q_d, 0) min_d`` (``pages.bounds``) over the query heads of
+    the key head, which no ``q . k`` of the page exceeds; it is summed in 64 bits and rounded to 32, and NaN where a bound is,
+    or where an infinite one meets a 0.  The ``first`` and the last
     ``recent`` (>= 1) pages of a sequence are always kept (``first + recent <= count``), then those with the largest scores:
     a NaN before every number, a page id outside the pool last, equal scores by the lower page of the sequence.  Sequences
     of up to ``count`` pages keep all of them.  (Scores stand for ``scale > 0`` in the attention.)  ``max_length`` and

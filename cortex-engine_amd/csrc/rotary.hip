@@ -207,7 +207,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < NU; ++j)
-            if (there && in[j]) *reinterpret_cast<i32x4*>(y + j * d_step) = packed(f + j * CE, X());
+      if (there && in[j]) *reinterpret_cast<i32x4*>(y + j * d_step) = packed(f + j * CE, X());
     const bool wrap = (r += dr) >= o.heads;
     r -= wrap ? o.heads : 0;
     k += dk + (wrap ? 1 : 0);

@@ -613,7 +613,8 @@ int cortex_kv_block_bounds(const cortex_kv_pages* pages, int64_t B, const int32_
 /* The pages of a sequence that a query may find its largest scores in, per key head.  Block i of a sequence is page i of
  * its table; its score is the largest of
  *   sum_d max(q_d max_d, q_d min_d) = max(q, 0) . max + min(q, 0) . min   (bounds max, min)
- * over the query heads of the key head, summed in 64 bits and rounded to 32.  Kept are the first `first` and the last
+ * over the query heads of the key head, summed in 64 bits and rounded to 32 (by the second form: 0 times an infinite bound
+ * is NaN).  Kept are the first `first` and the last
  * `recent` (>= 1) blocks and then those with the largest scores (a NaN before every number, a block without a page last,
  * equal ones by the lower block), `count` in all or as many as there are.
  * table (B, kv_heads, keep) int32, keep = min(count, ceil(max_length / page_size)): the pages kept, in the order of the
