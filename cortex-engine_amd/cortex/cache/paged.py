@@ -81,11 +81,12 @@ class PagedKVCache:
         if num_pages < 1 or layers < 1:
             raise ValueError("num_pages and layers must be >= 1")
         self.num_pages, self.page_size, self.tracked, self.bounded = num_pages, page_size, tracked, bounded
-        self._shape, self._kind = (kv_heads, page_size, head_dim, dtype, device), {"tracked": tracked}
+        shape, self._kind = (kv_heads, page_size, head_dim, dtype), {"tracked": tracked}
         if bounded:
             self._kind["bounded"] = True
-        self.layers = [KVPages.allocate(num_pages, *self._shape, **self._kind) for _ in range(layers)]
+        self.layers = [KVPages.allocate(num_pages, *shape, device, **self._kind) for _ in range(layers)]
         self.device = self.layers[0].device
+        self._shape = (*shape, self.device)  # ("cuda" alone is whatever device is current)
         self._free = list(range(num_pages - 1, -1, -1))
         self._users = np.zeros(num_pages, dtype=np.int32)  # sessions that have a page
         self._sessions: OrderedDict[str, _Session] = OrderedDict()  # least recently used first

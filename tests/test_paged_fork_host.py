@@ -227,6 +227,22 @@ def test_pools_of_another_size(host):
     consistent(cache)
 
 
+def test_pools_of_another_size_stay_on_their_device(host, monkeypatch):
+    """The device that the cache was made on, whatever device is current by then."""
+    allocate, where = paged.KVPages.allocate, []
+
+    def follow(num_pages, kv_heads, page_size, head_dim, dtype, device, **kw):
+        where.append(device)
+        return allocate(num_pages, kv_heads, page_size, head_dim, dtype, device, **kw)
+
+    monkeypatch.setattr(paged.KVPages, "allocate", follow)
+    cache = PagedKVCache(10, 1, 16, page_size=8, layers=2, device="cuda")
+    grow(cache, "a", 20)
+    assert where == ["cuda"] * 2
+    cache.resize(12)
+    assert where[2:] == [cache.device] * 2 and cache.device.type == "cpu"  # (where the stand-ins' pools are)
+
+
 @pytest.mark.parametrize("what", ["fork", "compact", "resize"])
 def test_what_fails_changes_nothing(host, monkeypatch, what):
     cache = PagedKVCache(12, 1, 16, page_size=8)
