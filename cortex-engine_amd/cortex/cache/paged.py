@@ -72,6 +72,10 @@ class _Session:
         self.pending: list[set[int]] = []  # ``filled`` of the batches whose rows some layer may lack
 
 
+class _NoRoom(MemoryError, torch.OutOfMemoryError):
+    """What ``resize`` raises where the device has no room: its own promise, and the kind of every other allocation."""
+
+
 class PagedKVCache:
     """Pages of keys and values for named sessions, ``layers`` pools that share one block table."""
 
@@ -311,8 +315,8 @@ class PagedKVCache:
     def resize(self, num_pages: int) -> int:
         """Pools of ``num_pages`` pages instead (``layers`` are other objects then); returns how many pages got another
         place, those past the end of smaller pools.  MemoryError, and nothing changed, where the pages in use are more, or
-        where the device has no room for the new pools beside the old ones.  Every layer must have the rows of the tokens of
-        sessions that move; batches made before no longer hold for these."""
+        where the device has no room for the new pools beside the old ones (a torch.OutOfMemoryError too, then).  Every layer
+        must have the rows of the tokens of sessions that move; batches made before no longer hold for these."""
         if num_pages < 1:
             raise ValueError("num_pages must be >= 1")
         src = np.flatnonzero(self._users > 0).astype(np.int32)
@@ -324,8 +328,14 @@ class PagedKVCache:
         moved = self._moved(place)
         self._not_captured()
         self._enter()
-        layers = [KVPages.allocate(num_pages, *self._shape, **self._kind) for _ in self.layers]
-        at = self._ids(src, place[src]) if src.shape[0] else ()
+        layers = []
+        try:
+            layers = [KVPages.allocate(num_pages, *self._shape, **self._kind) for _ in self.layers]
+            at = self._ids(src, place[src]) if src.shape[0] else ()
+        except torch.OutOfMemoryError as e:
+            layers.clear()  # (what was allocated does not live as long as the error)
+            raise _NoRoom(f"no room on {self.device} for {num_pages} pages beside the {self.num_pages} there are: "
+                          f"{e}") from e.with_traceback(None)
         self._rename(place, moved, num_pages)
         for old, new in zip(self.layers, layers):
             if at:

@@ -275,6 +275,26 @@ def test_what_fails_changes_nothing(host, monkeypatch, what):
     consistent(cache)
 
 
+@pytest.mark.parametrize("where", ["pools", "ids"])
+def test_no_room_for_other_pools_is_a_memory_error(host, monkeypatch, where):
+    """As for pages in use that are too many; torch's own error, which callers of other operators expect, too."""
+    cache = PagedKVCache(10, 1, 16, page_size=8, layers=2)
+    batch = grow(cache, "a", 20)
+    before, layers, users = state(cache), list(cache.layers), cache._users.copy()
+
+    def none_left(*args, **kw):
+        raise torch.OutOfMemoryError("out of memory")
+
+    for error in (MemoryError, torch.OutOfMemoryError):
+        with monkeypatch.context() as m, pytest.raises(error, match="no room"):
+            m.setattr(*((paged.KVPages, "allocate") if where == "pools" else (PagedKVCache, "_upload")), none_left)
+            cache.resize(1 << 20)
+    assert state(cache) == before and cache.layers == layers and (cache._users == users).all() and cache.num_pages == 10
+    cache.attend(batch, rows(1))
+    assert cache.resize(20) == 0
+    consistent(cache)
+
+
 def test_bounds_follow_appends_and_evictions(host):
     cache = PagedKVCache(20, 1, 16, page_size=8, layers=2, tracked=True, bounded=True)
     first = cache.extend(["a"], [20])
