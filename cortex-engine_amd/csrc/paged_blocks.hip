@@ -950,26 +950,60 @@ extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t
   const int64_t es = pages->dtype == DT_F32 ? 4 : 2;
   CORTEX_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_sb * es) % 16 == 0 && (q_sh * es) % 16 == 0,
                    "%s: query rows must be 16-byte aligned", who);
-  // what the call writes is read by no workgroup of it
-  auto meet = [](const void* x, int64_t n, const void* y, int64_t m) {
-    return x && y && (uintptr_t)x < (uintptr_t)y + (uintptr_t)m && (uintptr_t)y < (uintptr_t)x + (uintptr_t)n;
-  };
   const int64_t blocks = most_blocks(pages, a.max_length), ld = rank_ld(pages, a.max_length, count);
   const int64_t keep = count < blocks ? count : blocks;
-  CORTEX_CHECK_ARG(table || keep == 0, "%s: null table", who);
-  CORTEX_CHECK_ARG(!meet(new_lengths, 8 * B, lengths, 8 * B), "%s: new_lengths may not be lengths, nor overlap them", who);
-  CORTEX_CHECK_ARG(max_pages == 0 || !meet(table, 4 * B * pages->kv_heads * keep, block_table, 4 * ((B - 1) * ld_table + max_pages)),
-                   "%s: table may not overlap the block table", who);
-  const int64_t need = cortex_kv_select_workspace_bytes(pages, B, a.max_length, count);
-  CORTEX_CHECK_ARG((workspace || need == 0) && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
-  // (a launch has fewer than 2^32 threads)
+  // (a launch has fewer than 2^32 threads; and the sizes of what the call writes fit 64 bits then)
   CORTEX_CHECK_ARG(B <= 0xffffffffLL / 1024 / pages->kv_heads &&
                        (ld == 0 || B * pages->kv_heads <= 0xffffffffLL / 256 / cdiv(ld, 64)),
                    "%s: %lld sequences of up to %lld blocks are too much for one call", who, (long long)B, (long long)blocks);
+  CORTEX_CHECK_ARG(table || keep == 0, "%s: null table", who);
+  // what the call writes is read by no workgroup of it, and written once
+  struct Rows {  // `n` of `size` bytes, from one to the next `pitch` >= 0
+    const char* name;
+    __int128 at, n, pitch, size;
+  };
+  auto whole = [](const char* name, const void* p, __int128 size) {
+    return Rows{name, (__int128)(uintptr_t)p, p && size > 0, 0, size};
+  };
+  auto strided = [](const char* name, const void* p, int64_t n, __int128 pitch, __int128 size) {
+    const __int128 at = (uintptr_t)p;
+    return pitch < 0 ? Rows{name, at + (n - 1) * pitch, n, -pitch, size} : Rows{name, at, n, pitch, size};
+  };
+  auto meet = [](const Rows& x, const Rows& one) {
+    if (x.n == 0 || one.n == 0) return false;
+    const __int128 past = one.at - x.at - x.size;  // the first row that ends behind one's begin
+    const __int128 i = past < 0 ? 0 : x.pitch == 0 ? x.n : past / x.pitch + 1;
+    return i < x.n && x.at + i * x.pitch < one.at + one.size;
+  };
+  auto queries = [&] {  // rows of the larger stride; the other one within them
+    const __int128 sb = (__int128)q_sb * es, sh = (__int128)q_sh * es, b = sb < 0 ? -sb : sb, h = sh < 0 ? -sh : sh;
+    const bool by_b = b >= h;
+    const __int128 in = by_b ? (heads - 1) * sh : (B - 1) * sb, dims = pages->head_dim * es;
+    const char* at = reinterpret_cast<const char*>(q) + (int64_t)(in < 0 ? in : 0);
+    return strided("the queries", at, by_b ? B : heads, by_b ? sb : sh, (in < 0 ? -in : in) + dims);
+  };
+  const int64_t need = cortex_kv_select_workspace_bytes(pages, B, a.max_length, count);
+  const Rows read[] = {
+      whole("lengths", lengths, 8 * B),
+      strided("the block table", block_table, max_pages ? B : 0, B > 1 ? (__int128)ld_table * 4 : 0, 4 * max_pages), queries(),
+      whole("the bounds", pages->bounds, (__int128)pages->num_pages * pages->kv_heads * 2 * pages->head_dim * bound_bytes_of(pages))};
+  const Rows made[] = {whole("new_lengths", new_lengths, 8 * B), whole("table", table, 4 * B * pages->kv_heads * keep),
+                       whole("the workspace", workspace, need)};
+  auto check_apart = [&](int i) {
+    for (const Rows& x : read)
+      CORTEX_CHECK_ARG(!meet(x, made[i]), "%s: %s may not overlap %s", who, made[i].name, x.name);
+    for (int j = 0; j < i; ++j)
+      CORTEX_CHECK_ARG(!meet(made[j], made[i]), "%s: %s may not overlap %s", who, made[i].name, made[j].name);
+    return OK;
+  };
+  if (int rc = check_apart(0)) return rc;
+  if (int rc = check_apart(1)) return rc;
+  CORTEX_CHECK_ARG((workspace || need == 0) && (uintptr_t)workspace % 16 == 0, "%s: null or unaligned workspace", who);
   if (workspace_bytes < need) {
     set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes, (long long)need);
     return E_WORKSPACE;
   }
+  if (int rc = check_apart(2)) return rc;
   a.bounds = pages->bounds;
   a.B = (int)B;
   a.heads = (int)heads;

@@ -619,8 +619,9 @@ int cortex_kv_block_bounds(const cortex_kv_pages* pages, int64_t B, const int32_
  * equal ones by the lower block), `count` in all or as many as there are.
  * table (B, kv_heads, keep) int32, keep = min(count, ceil(max_length / page_size)): the pages kept, in the order of the
  * blocks, -1 behind them; new_lengths[b]: the slots in use in them (the same for every key head: the last block, which
- * alone may be in use in part, is always kept), 0 for a malformed negative length; neither may overlap what is read.  workspace:
- * cortex_kv_select_workspace_bytes for the call's own max_length, given as the length that it stands for; 16-byte aligned. */
+ * alone may be in use in part, is always kept), 0 for a malformed negative length.  workspace:
+ * cortex_kv_select_workspace_bytes for the call's own max_length, given as the length that it stands for; 16-byte aligned.
+ * table, new_lengths and the workspace that the call needs overlap neither each other nor lengths, block_table, q or bounds. */
 int64_t cortex_kv_select_workspace_bytes(const cortex_kv_pages* pages, int64_t B, int64_t max_length, int64_t count);
 int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t heads, const void* q, int64_t q_sb, int64_t q_sh,
                      const int32_t* block_table, int64_t ld_table, int64_t max_pages, const int64_t* lengths,

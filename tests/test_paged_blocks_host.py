@@ -132,6 +132,38 @@ def test_refused_selections():
     assert size(None, 2, 4800, 8) == 0 and size(ref(pages()), -1, 4800, 8) == 0 and size(ref(pages()), 2, -1, 8) == 0
 
 
+def test_selections_whose_tensors_meet():
+    """Workgroups write while others still read: an output or the workspace that overlaps what is read, or another of them,
+    is refused, at its first byte and at its last one."""
+    # 4 pages of 2 heads x 64 in bf16, 2 sequences of up to 300 blocks, 4 query heads, 8 blocks kept
+    size = {"q": 2 * (256 + 3 * 64 + 64), "table": 4 * 600, "lengths": 16, "bounds": 4 * 2 * 2 * 64 * 2, "out": 4 * 2 * 2 * 8,
+            "after": 16, "ws": 4 * 2 * 2 * 304}
+    places = {name: (i + 2) * V for i, name in enumerate(size)}
+
+    def with_places(**kw):
+        at = {**places, **kw}
+        bounds = at.pop("bounds")
+        return select(pages(bounds=bounds), **at)
+
+    for written in ("after", "out", "ws"):
+        for other in size:
+            if other == written:
+                continue
+            for at in (places[other], places[other] + size[other] - 16, places[other] - size[written] + 16):
+                refused(with_places(**{written: at}), "overlap")
+    # the sizes that this goes by do not wrap around
+    refused(with_places(B=1 << 40, ld=1 << 40), "too much")
+    # rows far apart: each of them, from either end, and what lies between them is nobody's
+    far = 1 << 40
+    for place in (places["table"], places["table"] + far):
+        refused(with_places(ld=far // 4, after=place), "overlap the block table")
+    refused(with_places(ld=1 << 62, after=places["table"] + 1184), "overlap the block table")
+    for sb, sh in ((far // 2, 64), (64, far // 2), (-far // 2, 64), (64, -far // 2), (-far // 2, -64)):
+        refused(with_places(q=1 << 44, sb=sb, sh=sh, after=(1 << 44) + 2 * (sb + sh)), "overlap the queries")
+    for kw in ({"ld": far // 4, "after": places["table"] + far // 2}, {"sb": far // 2, "after": places["q"] + far // 2}):
+        refused(with_places(ws=None, **kw), "workspace")  # (past the outputs, to what is refused next)
+
+
 def test_refused_tables_by_key_head():
     refused(tables(pages(), sh=299), "overlap")
     refused(tables(pages(), sh=-1), "overlap")
