@@ -215,9 +215,12 @@ class PagedKVCache:
         them: ``layer`` must have the rows of all of them by then (``append``), also of batches before this one (where
         one of those is given up, its sessions have to be dropped).  ``accumulate``: by default where the pages are
         tracked.  ``blocks``: attend to that many pages of a session at most, of each key head those that the largest scores
-        may be in, the first ``first`` and the last ``recent`` among them (``paged_block_select``; a bounded cache)."""
+        may be in, the first ``first`` and the last ``recent`` among them (``paged_block_select``; a bounded cache, and a
+        ``scale`` above 0)."""
         if blocks is not None and not self.bounded:
             raise ValueError("a selection of pages needs bounded=True")
+        if blocks is not None and scale is not None and not scale > 0:
+            raise ValueError(f"a selection of pages, which goes by the largest q . k, needs a scale above 0, got {scale}")
         if any(layer % len(self.layers) not in filled for filled in batch.needs):
             raise RuntimeError(f"some slots of the batch's sessions have no rows in layer {layer}: append them first")
         self._enter(batch)

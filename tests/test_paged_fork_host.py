@@ -332,6 +332,20 @@ def test_bounds_follow_appends_and_evictions(host):
         plain.attend(batch, rows(1), blocks=2)
 
 
+def test_a_selection_needs_a_scale_above_zero(host):
+    """Pages are ranked by bounds of q . k: with a scale that turns or levels the scores they say nothing."""
+    cache = PagedKVCache(20, 1, 16, page_size=8, bounded=True)
+    batch = grow(cache, "a", 20)
+    for scale in (-0.125, 0.0, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            cache.attend(batch, rows(1), scale=scale, blocks=2)
+        cache.attend(batch, rows(1), scale=scale)
+    assert not host.of("select")
+    cache.attend(batch, rows(1), scale=0.125, blocks=2)
+    cache.attend(batch, rows(1), blocks=2)
+    assert len(host.of("select")) == 2
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_random_steps_keep_pages_apart(host, seed):
     """What each session's slots hold, carried through every copy: no step of one session changes another's."""
