@@ -40,9 +40,10 @@ from cortex.kernels.paged_kv import (KVPages, kv_block_bounds, kv_copy_pages, kv
 class KVBatch(NamedTuple):
     """Sessions of a step as the operators take them (device tensors): ``block_table`` (B, pages) int32, the slots in use
     before the step's tokens (``before``) and with them (``lengths``), ``offsets`` (B + 1,) of the tokens (None: one a
-    session), their ``positions``, and on the host ``tokens`` and ``max_length``.  It holds until one of its sessions is
-    cut, dropped, forked or moved; ``append`` and ``attend`` refuse it from then on.  ``filled``: the layers that have its
-    tokens' rows; ``needs``: the same of every batch whose rows some layer lacked when this one was made, its own among them."""
+    session), their ``positions``, and on the host ``tokens``, ``max_length`` and ``max_new``, the most tokens of a session.
+    It holds until one of its sessions is cut, dropped, forked or moved; ``append`` and ``attend`` refuse it from then on.
+    ``filled``: the layers that have its tokens' rows; ``needs``: the same of every batch whose rows some layer lacked when
+    this one was made, its own among them."""
 
     sessions: tuple[str, ...]
     block_table: torch.Tensor
@@ -58,6 +59,7 @@ class KVBatch(NamedTuple):
     stream: torch.cuda.Stream  # that its tensors were made on
     filled: set[int]
     needs: tuple[set[int], ...]
+    max_new: int
 
 
 class _Session:
@@ -178,7 +180,8 @@ class PagedKVCache:
         return KVBatch(names, parts[4].view(torch.int32)[:table.size].view(B, width), parts[0], parts[1],
                        parts[3] if ragged else None, parts[2], positions.shape[0],
                        int((before + new).max()) if B else 0, tuple(held), tuple(s.version for s in held), self._epoch,
-                       self._stream, filled, tuple({id(f): f for s in held for f in s.pending}.values()))
+                       self._stream, filled, tuple({id(f): f for s in held for f in s.pending}.values()),
+                       int(new.max()) if B else 0)
 
     def batch(self, session_ids) -> KVBatch:
         """The sessions as they stand, without new tokens (KeyError: an unknown one)."""
@@ -204,8 +207,8 @@ class PagedKVCache:
         pages = self.layers[layer]
         paged_kv_append(pages, k, v, batch.block_table, batch.before, offsets=batch.offsets, positions=batch.positions)
         if self.bounded:
-            kv_block_bounds(pages, batch.block_table, batch.lengths, since=batch.before,
-                            max_new=1 if batch.offsets is None else batch.tokens, max_length=batch.max_length)
+            kv_block_bounds(pages, batch.block_table, batch.lengths, since=batch.before, max_new=batch.max_new,
+                            max_length=batch.max_length)
         batch.filled.add(at)
 
     def attend(self, batch: KVBatch, q: torch.Tensor, layer: int = 0, *, scale: float | None = None,

@@ -332,6 +332,17 @@ def test_bounds_follow_appends_and_evictions(host):
         plain.attend(batch, rows(1), blocks=2)
 
 
+def test_bounds_of_ragged_steps_are_sized_by_the_longest(host):
+    """What one session got at most, not all of them together: the launch has that many workgroups for each."""
+    cache = PagedKVCache(60, 1, 16, page_size=8, bounded=True)
+    for counts, most in (([20, 1, 7], 20), ([0, 3, 30], 30), ([1, 1, 1], 1), (None, 1), ([0, 0, 0], 0)):
+        batch = cache.extend(["a", "b", "c"], counts)
+        cache.append(batch, rows(batch.tokens), rows(batch.tokens))
+        assert host.of("bounds")[-1][2]["max_new"] == most
+    cache.append(cache.extend([]), rows(0), rows(0))
+    assert host.of("bounds")[-1][2]["max_new"] == 0
+
+
 def test_a_selection_needs_a_scale_above_zero(host):
     """Pages are ranked by bounds of q . k: with a scale that turns or levels the scores they say nothing."""
     cache = PagedKVCache(20, 1, 16, page_size=8, bounded=True)
