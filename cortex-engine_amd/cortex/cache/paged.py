@@ -356,20 +356,23 @@ class PagedKVCache:
         the end of the free list as it is once they are gone, the last one first."""
         missing, victims, back = total - len(self._free), [], []
         if missing > 0:
-            left = self._users.copy()
-            for name, s in self._sessions.items():
-                if len(back) >= missing:
-                    break
-                if name not in keep and s.used:
-                    pages = s.pages[:s.used]
-                    left[pages] -= 1
-                    free = pages[left[pages] == 0].tolist()
-                    victims.append((name, pages))
-                    back += free
+            gone, users = [], self._users
+            try:  # the counts as they are once these are gone, and back again: a copy would be one of all pages
+                for name, s in self._sessions.items():
+                    if len(back) >= missing:
+                        break
+                    if name not in keep and s.used:
+                        pages = s.pages[:s.used]
+                        gone.append((name, pages))
+                        users[pages] -= 1
+                        back += pages[users[pages] == 0].tolist()
+                # (not those whose pages others keep)
+                victims = [name for name, pages in gone if (users[pages] == 0).any()]
+            finally:
+                for _, pages in gone:
+                    users[pages] += 1
             if len(back) < missing:
                 raise MemoryError(f"{missing - len(back)} pages short of {total} (of {self.num_pages} in all)")
-            # (not those whose pages others keep)
-            victims = [name for name, pages in victims if (left[pages] == 0).any()]
         taken = back[::-1][:total]
         return victims, taken + self._free[len(self._free) - (total - len(taken)):][::-1]
 

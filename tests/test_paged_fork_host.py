@@ -148,6 +148,28 @@ def test_who_gives_way_for_a_fork(host):
     consistent(cache)
 
 
+def test_who_gives_way_is_found_without_a_look_at_every_page(host):
+    """A cache that is full lets sessions go at every step: that goes by their pages, however large the pools are."""
+
+    class Users(np.ndarray):
+        def copy(self, *args, **kw):
+            raise AssertionError("the counts of all pages were copied")
+
+    cache = PagedKVCache(6, 1, 16, page_size=8)
+    cache._users = cache._users.view(Users)
+    grow(cache, "old", 9)
+    grow(cache, "twin", 16)
+    cache.fork("twin", ["other"])
+    cache.extend(["old"], [0])
+    users = np.array(cache._users)
+    with pytest.raises(MemoryError):
+        cache.extend(["new"], [8 * 7])
+    assert (cache._users == users).all() and cache.sessions == ["twin", "other", "old"]
+    cache.extend(["new"], [8 * 3])
+    assert cache.sessions == ["old", "new"]
+    consistent(cache)
+
+
 def test_compaction(host):
     cache = PagedKVCache(12, 1, 16, page_size=8, layers=2)
     for name in "abcd":
