@@ -37,6 +37,11 @@ from cortex.kernels.paged_kv import (KVPages, kv_block_bounds, kv_copy_pages, kv
                                      paged_block_select, paged_kv_append)
 
 
+# Rows of a call of kv_copy_pages.  A workgroup takes 32 rows or more and a page 8 or more, so that these are at most 2^21 + 2^23
+# workgroups; a launch has fewer than 2^24.
+_COPY_ROWS = 1 << 26
+
+
 class KVBatch(NamedTuple):
     """Sessions of a step as the operators take them (device tensors): ``block_table`` (B, pages) int32, the slots in use
     before the step's tokens (``before``) and with them (``lengths``), ``offsets`` (B + 1,) of the tokens (None: one a
@@ -300,7 +305,7 @@ class PagedKVCache:
             f.used, f.length, f.seen = s.used, s.length, s.seen
         if at:
             for pages in self.layers:
-                kv_copy_pages(pages, *at)
+                self._copy(pages, *at)
 
     def compact(self) -> int:
         """Moves pages so that those in use are the first ``pages_used`` of the pools; returns how many moved.  Every layer
@@ -315,7 +320,7 @@ class PagedKVCache:
         at = self._ids(src, place[src])
         self._rename(place, moved, self.num_pages)
         for pages in self.layers:
-            kv_copy_pages(pages, *at)
+            self._copy(pages, *at)
         return src.shape[0]
 
     def resize(self, num_pages: int) -> int:
@@ -345,7 +350,7 @@ class PagedKVCache:
         self._rename(place, moved, num_pages)
         for old, new in zip(self.layers, layers):
             if at:
-                kv_copy_pages(old, *at, into=new)
+                self._copy(old, *at, into=new)
         self.layers = layers
         return past.shape[0]
 
@@ -388,6 +393,11 @@ class PagedKVCache:
         flat[:, :n] = ids
         (dev,) = self._upload([flat.reshape(-1).view(np.int64)])
         return [t[:n] for t in dev.view(torch.int32).view(flat.shape)]
+
+    def _copy(self, pages: KVPages, src: torch.Tensor, dst: torch.Tensor, into: KVPages | None = None) -> None:
+        n = max(1, _COPY_ROWS // (self._shape[0] * self.page_size))
+        for i in range(0, src.shape[0], n):
+            kv_copy_pages(pages, src[i:i + n], dst[i:i + n], into=into)
 
     def _filled(self, names) -> None:
         for n in names:

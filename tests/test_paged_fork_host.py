@@ -249,6 +249,33 @@ def test_pools_of_another_size(host):
     consistent(cache)
 
 
+@pytest.mark.parametrize("what", ["fork", "compact", "resize"])
+def test_more_pages_than_one_launch_takes(host, monkeypatch, what):
+    """The copies come after the tables were rewritten: pages that are too many for a launch go in several."""
+    monkeypatch.setattr(paged, "_COPY_ROWS", 5 * 8)
+    cache = PagedKVCache(40, 1, 16, page_size=8, layers=2, tracked=True)
+    grow(cache, "a", 8 * 13)
+    grow(cache, "b", 8 * 13)
+    a, b = (cache._sessions[n].pages[:13].tolist() for n in "ab")
+    if what == "fork":
+        cache.fork("b", ["c"])
+        want = list(zip(b, cache._sessions["c"].pages[:13].tolist()))
+    elif what == "compact":
+        cache.evict_session("a")
+        cache.compact()
+        want = list(zip(b, cache._sessions["b"].pages[:13].tolist()))
+    else:
+        cache.resize(80)
+        want = list(zip(a + b, a + b))
+    copies = host.of("copy")
+    assert all(len(src) == len(dst) <= 5 for _, src, dst, _ in copies)
+    for layer in (0, 1):
+        half = copies[len(copies) // 2 * layer:len(copies) // 2 * (layer + 1)]
+        assert len({id(pages) for pages, *_ in half}) == 1
+        assert sorted(p for _, src, dst, _ in half for p in zip(src, dst)) == sorted(want)
+    consistent(cache)
+
+
 def test_pools_of_another_size_stay_on_their_device(host, monkeypatch):
     """The device that the cache was made on, whatever device is current by then."""
     allocate, where = paged.KVPages.allocate, []
