@@ -7,7 +7,8 @@
 // with (i, j) = (p, p + pairs) or (2 p, 2 p + 1); dims past the pairs are only normed.  Everything between the load of a
 // row and its store is in fp32, rounded once.
 //
-// The angle is the product in 64 bits: at position 2^20 a product in 32 is off by up to 0.06 rad.  It is reduced to
+// The angle is the product in 64 bits: at position 2^20 a product in 32 is off by up to 0.06 rad.  That of a position and a
+// frequency of 24 bits is exact up to 2^29; further out it is rounded, by up to 2^-53 of it (1.2e-4 rad at 2^40).  It is reduced to
 // [-pi/4, pi/4] and a quadrant in 64 bits, so that sine and cosine are those of a small fp32 argument.  The angles of a token are
 // the same for all its heads: a workgroup computes them once, into LDS.
 #include <hip/hip_runtime.h>

@@ -631,7 +631,8 @@ int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t heads, con
 /* Queries (T, heads, dim) and keys (T, kv_heads, dim), f32 or bf16, element (t, h, d) at t * st + h * sh + d, rows 16-byte
  * aligned: with norm != 0 every row x / sqrt(mean(x^2) + eps) (times its gain (dim), f32 or bf16, where given), then
  * turned by position:
- *   angle of pair p = positions[t * p_st + axes[p] * p_sa] * inv_freq[p]   (the product in 64 bits; axes NULL: 0)
+ *   angle of pair p = positions[t * p_st + axes[p] * p_sa] * inv_freq[p]   (the product rounded to 64 bits: exact up to
+ *     positions of 2^29, off by at most 2^-53 of it further out; axes NULL: 0)
  *   (y_i, y_j) = (x_i cos - x_j sin, x_j cos + x_i sin),  (i, j) = (p, p + pairs), interleaved: (2 p, 2 p + 1)
  * dims past 2 * pairs are not turned.  All in fp32, rounded once.  dim: a multiple of 8 up to 256, pairs a multiple of 8.
  * A pair whose axis is outside [0, n_axes) is not turned and ORs bit 3 (value 8) into *err (when given).  An output

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -85,6 +87,32 @@ def test_far_positions(far):
     c.positions[:4, 0] = torch.tensor([0, far, -far, far - 1])
     for eps in (None, 1e-5):
         c.check(c.run(eps=eps), eps=eps)
+
+
+PI = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+@pytest.mark.parametrize("far", [1 << 20, 1 << 29, 1 << 31, 1 << 40, (1 << 53) - 1])
+def test_far_positions_by_exact_angles(far):
+    """Angles as fractions, without the rounding of the product: up to 2^29 (29 bits times 24) there is none, further out
+    the angle is off by half a unit of the 64-bit product, at most 2^-53 of it, times |x_i| + |x_j| in the result."""
+    c = Case(40, 1, 1, 64, 32, torch.float32, far=far, seed=6, gains=False)
+    c.positions[:4, 0] = torch.tensor([far, -far, far - 1, far // 3])
+    angle = [[int(p) * Fraction(float(f)) for f in c.inv_freq] for p in c.positions[:, 0]]
+    product = c.positions.double() * c.inv_freq.double()
+    apart = [[float(abs(a - Fraction(float(x)))) for a, x in zip(r, s)] for r, s in zip(angle, product)]
+    off = torch.tensor(apart, dtype=torch.float64)
+    assert (off == 0).all() if far <= 1 << 29 else (off <= 2.0 ** -53 * product.abs()).all() and off.any()
+    small = torch.tensor([[float(a - round(a / (2 * PI)) * 2 * PI) for a in r] for r in angle], dtype=torch.float64)[:, None]
+    for x, y in zip((c.q, c.k), c.run(eps=None)):
+        u, v = x.double()[..., :32], x.double()[..., 32:]
+        cos, sin = small.cos(), small.sin()
+        want = torch.cat([u * cos - v * sin, v * cos + u * sin], -1)
+        near = torch.cat([u.abs() * cos.abs() + v.abs() * sin.abs(), v.abs() * cos.abs() + u.abs() * sin.abs()], -1)
+        size = torch.cat([u.abs() + v.abs()] * 2, -1)
+        # (2^-50: the reduced angle and its functions in 64 bits here)
+        tol = rope_bound(want, near, size, 64, False, torch.float32) + (torch.cat([off, off], -1)[:, None] + 2.0 ** -50) * size
+        assert ((y.double().cpu() - want).abs() <= tol).all(), far
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
