@@ -82,7 +82,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     ``q`` (T, heads, head_dim), ``k`` (T, kv_heads, head_dim) bf16 or fp32, any strides (views of a joint projection);
     ``head_dim`` a multiple of 8 up to 256.  With ``eps`` a row becomes ``x / sqrt(mean(x ** 2) + eps)``, times
     ``q_gain`` / ``k_gain`` (head_dim,) where given; without it rows are only rotated.  Squares are summed in fp32:
-    ``sum(x ** 2)`` is to stay below 2^127.
+    ``sum(x ** 2)`` is to stay below 2^127, and ``mean(x ** 2) + eps`` from 2^-110 up (a row of zeros without eps is NaN).
 
     Pair p turns by ``positions[t, axes[p]] * inv_freq[p]`` (fp32 frequencies, the product rounded to 64 bits: exact up to
     positions of 2^29, further out off by at most 2^-53 of the angle, 2.4e-7 rad at 2^31 and 1.2e-4 at 2^40 where the

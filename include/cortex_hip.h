@@ -634,7 +634,7 @@ int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t heads, con
  *   angle of pair p = positions[t * p_st + axes[p] * p_sa] * inv_freq[p]   (the product rounded to 64 bits: exact up to
  *     positions of 2^29, off by at most 2^-53 of it further out; axes NULL: 0)
  *   (y_i, y_j) = (x_i cos - x_j sin, x_j cos + x_i sin),  (i, j) = (p, p + pairs), interleaved: (2 p, 2 p + 1)
- * dims past 2 * pairs are not turned.  All in fp32, rounded once.  dim: a multiple of 8 up to 256, pairs a multiple of 8.
+ * dims past 2 * pairs are not turned.  All in fp32, rounded once (sum(x^2) below 2^127, mean(x^2) + eps from 2^-110 up).  dim: a multiple of 8 up to 256, pairs a multiple of 8.
  * A pair whose axis is outside [0, n_axes) is not turned and ORs bit 3 (value 8) into *err (when given).  An output
  * may be its own input and overlaps nothing else. */
 int cortex_qk_norm_rope(int64_t T, int64_t heads, int64_t kv_heads, int64_t dim, int dtype, const void* q, int64_t q_st,

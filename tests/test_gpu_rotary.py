@@ -194,6 +194,17 @@ def test_values_at_the_ends(dtype):
     assert got[7, 1].isnan().all() and got[8].isfinite().all()  # 0 / 0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [2.0 ** -53, 1.0, 2.0 ** 59])
+def test_rows_at_either_end_without_eps(dtype, size):
+    """Squares are summed in fp32: a mean from 2^-110 up loses nothing to numbers below the normal ones (256 squares that
+    are off by 2^-150 each: 2^-40 of their sum), and sums below 2^127 have room."""
+    c = Case(30, 2, 2, 256, 32, DTYPES[dtype], seed=11)
+    c.q, c.k = (x / x.double().square().mean(-1, keepdim=True).sqrt() * size for x in (c.q, c.k))
+    c.q, c.k = c.q.to(c.dtype), c.k.to(c.dtype)
+    c.check(c.run(eps=0.0), eps=0.0)
+
+
 def test_axes_that_are_not_there():
     """Such pairs are not turned, and the flag says so."""
     c = Case(20, 2, 2, 64, 32, torch.float32, axes=3)
