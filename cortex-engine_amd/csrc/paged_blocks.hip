@@ -163,6 +163,7 @@ __device__ __forceinline__ void store_bounds(O* to, const float* f) {
 // its row's scale and half of a three-operand maximum and minimum each, about as long as its bytes: 20.3 us with the rows in
 // cache, 15.6 without the arithmetic, 17.6 without the join, 10.2 with neither rows nor arithmetic.  The next page loaded while
 // one is joined takes 184 registers: 32 us.  Joined by shuffles it was 24.6.
+// The same keys in bf16, and in fp32 with 64 dims, 139 MB: 23.5 and 23.3 us, 5.9 TB/s.
 // The last page of 32 sequences: 3.9 us, the chain length -> table -> rows.
 template <class P>
 __global__ __launch_bounds__(256) void kv_bounds_kernel(BoundsArgs a) {
@@ -610,8 +611,10 @@ __device__ __forceinline__ bool begin_select(const SelectArgs& a, int b, int h, 
 }
 
 // Ranks and selection in one: a workgroup a (sequence, key head) of up to KPT * THREADS blocks.  32 sequences of 10 .. 501
-// blocks, 32 query on 8 key heads x 128 in bf16, 33 MB: 16.2 us.  Of that about 7 are the 64-bit products of the longest
-// sequences, whose wavefronts have four tiles each where the mean is two, and 2 the selection; 38 blocks of 8 heads x 64: 5.2.
+// blocks, 32 query on 8 key heads x 128 in bf16, 33 MB: 16.4 us; 13.5 with ranks that take no product or conversion (by count
+// those are 6.3 us of the longest sequences' CUs, whose wavefronts have four tiles each where the mean is two; the loads beside them
+// are not faster), 14.8 without the selection.  The same blocks of int8 pages, 66 MB, 22.6 us; 12 heads of 64 in fp32, 50 MB, 21.9;
+// 38 blocks of 8 heads x 64 in bf16 5.0.
 template <class O, class Q, int DHP, int NG, int THREADS, int KPT, bool ONE>
 __global__ __launch_bounds__(THREADS) void kv_rank_select_kernel(SelectArgs a) {
   constexpr int WAVES = THREADS / 64;
@@ -687,7 +690,8 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(SelectArgs a) {
 
 constexpr int SL_THREADS = 1024, SL_KEYS = 16;  // of the largest selection that keeps its ranks in registers
 
-// The selection of more blocks than that: a radix selection of a byte a round, the ranks read again in each.
+// The selection of more blocks than that: a radix selection of a byte a round, the ranks read again in each.  20,000 blocks of 8
+// key heads: 53.5 us beside 20.3 for the ranks (82 MB); 8192 by the one above 26.2 beside 10.4.
 __global__ __launch_bounds__(SL_THREADS) void kv_select_long_kernel(SelectArgs a) {
   constexpr int WAVES = SL_THREADS / 64;
   __shared__ __attribute__((aligned(16))) int hist[256];
@@ -856,6 +860,12 @@ int64_t rank_ld(const cortex_kv_pages* pages, int64_t most, int64_t count) {
 //   192 units    6.7  8.5 12.9 18.8 29.9   7.1  9.9 13.5 21.8 34.9   9.4 11.8 13.5 20.7 29.9
 //   256 units    6.6  8.7 13.5 20.5 31.7   7.0  9.9 14.2 22.3 35.5   9.5 12.0 16.0 23.7 36.8
 //  1024 units   16.0 22.1 48.8 70.6  131  12.0 24.2 37.5 62.3  125  15.7 25.2 38.3 61.5  128
+// The rule goes by units and blocks alone.  Where a tile costs less than in this form one launch would go further, where it
+// costs more less far (128 / 192 / 256 blocks, 512 threads against two launches):
+//   one query head a key head, 64 dims in bf16    8 units  6.0  6.9  8.2 /  8.0  8.6  8.7   128 units  6.2  7.5  8.6 /  8.4  9.9 10.6
+//   the same in fp32                             12 units  6.3  7.9  9.4 /  8.5  8.9  9.3   120 units  6.7  8.4  9.9 /  8.7 10.4 10.9
+//   eight heads, 128 dims in int8                 8 units 10.6 13.5 17.1 / 11.8 12.1 12.2   128 units 11.3 14.9 18.1 / 12.4 14.7 15.5
+//   sixteen, 128 dims in bf16                     8 units 12.4 15.6 18.7 / 12.7 13.2 11.6   128 units 13.0 16.3 19.3 / 13.5 16.4 16.5
 constexpr int FUSED_ALWAYS = 192, FUSED_KEYS = 4;  // blocks of any number of units; blocks a thread
 enum class Form { two, one_256, one_512 };
 Form select_form(int64_t units, int64_t ld) {
@@ -893,6 +903,9 @@ int launch_select(const SelectArgs& a, hipStream_t stream) {
   else
     hipLaunchKernelGGL((kv_rank_kernel<O, Q, DHP, NG, false>), dim3((unsigned)(n * chunks)), dim3(256), 0, stream, a, 4 * per_wave);
   CORTEX_CHECK_LAUNCH("kv_rank_kernel");
+  // The smallest that holds the ranks; the next one instead, ranks and selection of 8 units (us): 1024 blocks 10.1 -> 11.2, 2048
+  // 12.4 -> 13.9, 4096 16.7 -> 27.6.  Ranks read again in each round instead of held: 16,384 blocks whose scores differ by
+  // little 47.7 -> 72.0, that are all alike 49 -> 93, but with independent bounds 56.1 -> 53.1, and 9000 of those 43.7 -> 34.3
   if (a.ld <= 1024)
     hipLaunchKernelGGL((kv_select_kernel<256, 4>), units, dim3(256), 0, stream, a);
   else if (a.ld <= 2048)

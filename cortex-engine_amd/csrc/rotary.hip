@@ -96,8 +96,9 @@ __device__ __forceinline__ float row_sum(float v, int lanes) {
 //
 // Bound by HBM for many tokens: 16,801 tokens of 32 + 8 heads x 128 in bf16, 344 MB, 71 us, 4.8 TB/s (with eight values a lane,
 // whose partners then come through LDS, and four rows at once instead of the next one ahead 168 us; non-temporal stores
-// 66.5, but 31 instead of 17 us where only 32 bytes lie side by side).  4999 tokens of 12 + 12 heads x 64 in fp32, 62 MB, 17.2 us:
-// the loads, angles and first rows of the one round of workgroups come first.  One token: 3.3 us.
+// 66.5, but 31 instead of 17 us where only 32 bytes lie side by side).  4999 tokens of 12 + 12 heads x 64 in fp32, 62 MB, 16.6 us:
+// the loads, angles and first rows of the one round of workgroups come first.  64 tokens of 32 + 8 heads x 128: 4.7 us, one
+// token 3.2.
 template <class X, bool NORM, bool INTER>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
   constexpr int CE = 16 / sizeof(X), NU = 16 / CE;  // values of a unit, units a lane
