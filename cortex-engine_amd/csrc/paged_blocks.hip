@@ -978,8 +978,7 @@ extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t
   auto whole = [](const char* name, const void* p, __int128 size) {
     return Rows{name, (__int128)(uintptr_t)p, p && size > 0, 0, size};
   };
-  auto strided = [](const char* name, const void* p, int64_t n, __int128 pitch, __int128 size) {
-    const __int128 at = (uintptr_t)p;
+  auto strided = [](const char* name, __int128 at, int64_t n, __int128 pitch, __int128 size) {
     return pitch < 0 ? Rows{name, at + (n - 1) * pitch, n, -pitch, size} : Rows{name, at, n, pitch, size};
   };
   auto meet = [](const Rows& x, const Rows& one) {
@@ -992,13 +991,12 @@ extern "C" int cortex_kv_select(const cortex_kv_pages* pages, int64_t B, int64_t
     const __int128 sb = (__int128)q_sb * es, sh = (__int128)q_sh * es, b = sb < 0 ? -sb : sb, h = sh < 0 ? -sh : sh;
     const bool by_b = b >= h;
     const __int128 in = by_b ? (heads - 1) * sh : (B - 1) * sb, dims = pages->head_dim * es;
-    const char* at = reinterpret_cast<const char*>(q) + (int64_t)(in < 0 ? in : 0);
-    return strided("the queries", at, by_b ? B : heads, by_b ? sb : sh, (in < 0 ? -in : in) + dims);
+    return strided("the queries", (__int128)(uintptr_t)q + (in < 0 ? in : 0), by_b ? B : heads, by_b ? sb : sh, (in < 0 ? -in : in) + dims);
   };
   const int64_t need = cortex_kv_select_workspace_bytes(pages, B, a.max_length, count);
   const Rows read[] = {
       whole("lengths", lengths, 8 * B),
-      strided("the block table", block_table, max_pages ? B : 0, B > 1 ? (__int128)ld_table * 4 : 0, 4 * max_pages), queries(),
+      strided("the block table", (uintptr_t)block_table, max_pages ? B : 0, B > 1 ? (__int128)ld_table * 4 : 0, 4 * max_pages), queries(),
       whole("the bounds", pages->bounds, (__int128)pages->num_pages * pages->kv_heads * 2 * pages->head_dim * bound_bytes_of(pages))};
   const Rows made[] = {whole("new_lengths", new_lengths, 8 * B), whole("table", table, 4 * B * pages->kv_heads * keep),
                        whole("the workspace", workspace, need)};

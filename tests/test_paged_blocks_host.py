@@ -160,6 +160,8 @@ def test_selections_whose_tensors_meet():
     refused(with_places(ld=1 << 62, after=places["table"] + 1184), "overlap the block table")
     for sb, sh in ((far // 2, 64), (64, far // 2), (-far // 2, 64), (64, -far // 2), (-far // 2, -64)):
         refused(with_places(q=1 << 44, sb=sb, sh=sh, after=(1 << 44) + 2 * (sb + sh)), "overlap the queries")
+    refused(with_places(sb=64, sh=1 << 61, q=1 << 44, after=(1 << 44) + 2 * 64), "overlap the queries")
+    refused(with_places(sb=64, sh=-(1 << 61), q=1 << 44, after=(1 << 44) + 2 * 64), "overlap the queries")
     for kw in ({"ld": far // 4, "after": places["table"] + far // 2}, {"sb": far // 2, "after": places["q"] + far // 2}):
         refused(with_places(ws=None, **kw), "workspace")  # (past the outputs, to what is refused next)
 
