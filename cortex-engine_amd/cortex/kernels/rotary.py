@@ -86,10 +86,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
 
     Pair p turns by ``positions[t, axes[p]] * inv_freq[p]`` (fp32 frequencies, the product rounded to 64 bits: exact up to
     positions of 2^29, further out off by at most 2^-53 of the angle, 2.4e-7 rad at 2^31 and 1.2e-4 at 2^40 where the
-    frequency is 1): dims p and p + pairs, or 2p and 2p + 1 where ``interleaved``.  ``inv_freq`` (pairs,) with pairs a multiple of 8; the dims past
-    2 * pairs are not turned.  ``positions`` (T,) or (T, n) int64 of any strides, below 2^53 in amount; ``axes`` (pairs,)
-    int32, by default axis 0 for every pair.  A pair whose axis is not there is not turned and sets bit 3 of ``err_flag``
-    (int32, never cleared here).  ``out``: where the results go; each may be its own input (in place) and overlaps no
+    frequency is 1): dims p and p + pairs, or 2p and 2p + 1 where ``interleaved``.  ``inv_freq`` (pairs,) with pairs a
+    multiple of 8; the dims past 2 * pairs are not turned.  ``positions`` (T,) or (T, n) int64 of any strides, below 2^53 in
+    amount; ``axes`` (pairs,) int32, by default axis 0 for every pair.  A pair whose axis is not there is not turned and
+    sets bit 3 of ``err_flag`` (int32, never cleared here).  ``out``: where the results go; each may be its own input (in place) and overlaps no
     other tensor of the call."""
     idx = q.get_device()
     given = ()
