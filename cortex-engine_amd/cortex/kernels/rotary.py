@@ -89,8 +89,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     frequency is 1): dims p and p + pairs, or 2p and 2p + 1 where ``interleaved``.  ``inv_freq`` (pairs,) with pairs a
     multiple of 8; the dims past 2 * pairs are not turned.  ``positions`` (T,) or (T, n) int64 of any strides, below 2^53 in
     amount; ``axes`` (pairs,) int32, by default axis 0 for every pair.  A pair whose axis is not there is not turned and
-    sets bit 3 of ``err_flag`` (int32, never cleared here).  ``out``: where the results go; each may be its own input (in place) and overlaps no
-    other tensor of the call."""
+    sets bit 3 of ``err_flag`` (int32, never cleared here).  ``out``: where the results go; each may be its own input (in
+    place) and overlaps no other tensor of the call."""
     idx = q.get_device()
     given = ()
     if axes is not None or eps is not None or err_flag is not None or out is not None:
