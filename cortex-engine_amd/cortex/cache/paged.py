@@ -37,8 +37,8 @@ from cortex.kernels.paged_kv import (KVPages, kv_block_bounds, kv_copy_pages, kv
                                      paged_block_select, paged_kv_append)
 
 
-# Rows of a call of kv_copy_pages.  A workgroup takes 32 rows or more and a page 8 or more, so that these are at most 2^21 + 2^23
-# workgroups; a launch has fewer than 2^24.
+# Rows of a call of kv_copy_pages.  A workgroup takes 32 rows or more and a page 8 or more, so that these are at most
+# 2^21 + 2^23 workgroups; a launch has fewer than 2^24.
 _COPY_ROWS = 1 << 26
 
 
